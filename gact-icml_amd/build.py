@@ -12,10 +12,12 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc", "gact_hip.hip")
+LAYERS_SRC = os.path.join(HERE, "csrc", "layers.hip")         # linked into the same library
 PROBE_SRC = os.path.join(HERE, "csrc", "stream_probe.hip")   # compute-free traffic probes for bench.py
 HDR = os.path.join(ROOT, "include", "gact_hip.h")
 OUT_DIR = os.path.join(HERE, "gact", "lib")
@@ -29,7 +31,6 @@ HIPCC_FLAGS = [
     "--offload-arch=gfx950",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     # every floating-point operation in the kernels is meant literally (the one FMA is spelled out)
     "-ffp-contract=off",
     # keep the compiler from forming packed-FP32 instructions
@@ -59,7 +60,7 @@ def up_to_date():
         if torch_mark() not in f.read():     # built for another torch
             return False
     t = min(os.path.getmtime(p) for p in built)
-    return all(os.path.getmtime(p) <= t for p in (SRC, PROBE_SRC, TORCH_SRC, HDR, os.path.abspath(__file__)))
+    return all(os.path.getmtime(p) <= t for p in (SRC, LAYERS_SRC, PROBE_SRC, TORCH_SRC, HDR, os.path.abspath(__file__)))
 
 
 def torch_mark():
@@ -91,9 +92,20 @@ def build(force=False, extra=()):
     if not force and up_to_date():
         return OUT
     os.makedirs(OUT_DIR, exist_ok=True)
-    cmd = [hipcc()] + HIPCC_FLAGS + list(extra) + ["-I", os.path.join(ROOT, "include"), "-o", OUT, SRC]
-    subprocess.run(cmd, check=True)
-    subprocess.run([hipcc()] + HIPCC_FLAGS + ["-o", PROBE_OUT, PROBE_SRC], check=True)
+    include = ["-I", os.path.join(ROOT, "include")]
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, "gact_hip.o"), os.path.join(tmp, "layers.o")]
+        jobs = [[hipcc()] + HIPCC_FLAGS + list(extra) + include + ["-c", "-o", o, src] for o, src in zip(objects, (SRC, LAYERS_SRC))]
+        jobs.append([hipcc()] + HIPCC_FLAGS + ["-shared", "-o", PROBE_OUT, PROBE_SRC])
+        running = [(job, subprocess.Popen(job)) for job in jobs]       # side by side: each is one compiler on one core
+        for job, process in running:
+            if process.wait() != 0:
+                for _, other in running:
+                    if other.poll() is None:
+                        other.kill()
+                        other.wait()
+                raise subprocess.CalledProcessError(process.returncode, job)
+        subprocess.run([hipcc(), "--offload-arch=gfx950", "-fPIC", "-shared", "-o", OUT] + objects, check=True)
     subprocess.run(torch_command(), check=True)
     return OUT
 

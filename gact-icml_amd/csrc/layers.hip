@@ -1,0 +1,1405 @@
+// Layers that train on 8-bit checkpoints, for MI355X (gfx950): checkpoints of rows, layer norm, linear layers with bias, activation
+// and residual in the product's epilogue, and the products of the backward pass, one of which reads the checkpoint's codes.
+//
+// A checkpoint of a matrix of T holds every row in groups of 256 columns, the last one shorter.  Per group: the minimum and a scale,
+// both float, scale = float(255 / (double(max - min) + 2e-6)); per value: code = rint(max(fma(x - min, scale, 0.5) - 0.5, 0)).
+// That is the 8-bit code of gact_quantize on the values widened to float, rounded to nearest (GACT_NOISE_CONST).
+// A code stands for code / scale + min, computed as fma(code, 1 / scale, min): one division per group and not one per value, which
+// differs from the quotient by a rounding of float.
+//
+// Compiled with -ffp-contract=off: every operation is the one it spells.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "gact_hip.h"
+
+namespace {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+constexpr int kGroup = 256;
+constexpr int kVec = 8;   // columns of a lane's piece
+
+// ---- eight consecutive columns ----
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[kVec]) {
+  if constexpr (std::is_same<T, float>::value) {
+    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = a[e], v[e + 4] = b[e];
+  } else {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    const T8 a = *(const T8*)p;
+#pragma unroll
+    for (int e = 0; e < kVec; e++) v[e] = (float)a[e];
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[kVec]) {
+  if constexpr (std::is_same<T, float>::value) {
+    *(f32x4*)p = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4*)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    T8 a;
+#pragma unroll
+    for (int e = 0; e < kVec; e++) a[e] = (T)v[e];
+    *(T8*)p = a;
+  }
+}
+// the same of a row of which `n` columns are left; WHOLE: n is 0 or at least 8 and the address a multiple of 16 bytes
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void load_cols(const T* p, int64_t n, float (&v)[kVec], float fill = 0.0f) {
+  if (WHOLE) {
+    if (n > 0) {
+      load8(p, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; e++) v[e] = fill;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kVec; e++) v[e] = e < n ? (float)p[e] : fill;
+  }
+}
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void store_cols(T* p, int64_t n, const float (&v)[kVec]) {
+  if (WHOLE) {
+    if (n > 0) store8(p, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kVec; e++)
+      if (e < n) p[e] = (T)v[e];
+  }
+}
+
+// ---- reductions over 2^n neighbouring lanes, the result in each of them ----
+template <int CTRL>
+__device__ __forceinline__ float row_rotated(float v) {
+  const int b = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, b, CTRL, 0xf, 0xf, false));
+}
+struct Sum {
+  static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+struct Least {
+  static __device__ __forceinline__ float of(float a, float b) { return __builtin_fminf(a, b); }
+};
+struct Most {
+  static __device__ __forceinline__ float of(float a, float b) { return __builtin_fmaxf(a, b); }
+};
+template <typename OP, int LANES>
+__device__ __forceinline__ float over_lanes(float v) {
+  static_assert(LANES >= 16 && LANES <= 64, "rows of 16 lanes");
+  v = OP::of(v, row_rotated<0x128>(v));
+  v = OP::of(v, row_rotated<0x124>(v));
+  v = OP::of(v, row_rotated<0x122>(v));
+  v = OP::of(v, row_rotated<0x121>(v));
+  if (LANES >= 32) v = OP::of(v, __shfl_xor(v, 16));
+  if (LANES >= 64) v = OP::of(v, __shfl_xor(v, 32));
+  return v;
+}
+
+// ---- the checkpoint's arithmetic ----
+__device__ __forceinline__ float scale_of(float lo, float hi) { return (float)(255.0 / ((double)(hi - lo) + 2e-6)); }
+// [0, 255] and rounded to nearest even by the conversion itself; a NaN becomes 0
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d, float lo, float scale) {
+  uint32_t w = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(a - lo, scale, 0.5f) - 0.5f, 0, 0);
+  w = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(b - lo, scale, 0.5f) - 0.5f, 1, w);
+  w = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(c - lo, scale, 0.5f) - 0.5f, 2, w);
+  return __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(d - lo, scale, 0.5f) - 0.5f, 3, w);
+}
+__device__ __forceinline__ float code_at(uint32_t w, int e) { return (float)(uint8_t)(w >> (8 * e)); }
+__device__ __forceinline__ void eight_values(u32x2 w, float inv, float lo, float (&v)[kVec]) {
+#pragma unroll
+  for (int e = 0; e < kVec; e++) v[e] = __builtin_fmaf(code_at(w[e >> 2], e & 3), inv, lo);
+}
+
+// ---- activations: act(z) and act'(z) ----
+enum { ACT_NONE = GACT_ACT_NONE, ACT_GELU = GACT_ACT_GELU, ACT_GELU_TANH = GACT_ACT_GELU_TANH, ACT_SILU = GACT_ACT_SILU };
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+// the normal distribution's cumulative function and exp(-z^2/2)
+__device__ __forceinline__ void normal_cdf(float z, float& cdf, float& e) {
+  e = expf(-0.5f * z * z);
+  cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+}
+__device__ __forceinline__ float activated(float z, int act) {
+  switch (act) {
+    case ACT_GELU: {
+      float cdf, e;
+      normal_cdf(z, cdf, e);
+      return z * cdf;
+    }
+    case ACT_GELU_TANH: return z * sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));   // 0.5 (1 + tanh u) = sigmoid(2 u)
+    case ACT_SILU: return z * sigmoid(z);
+    default: return z;
+  }
+}
+__device__ __forceinline__ float slope(float z, int act) {
+  switch (act) {
+    case ACT_GELU: {
+      float cdf, e;
+      normal_cdf(z, cdf, e);
+      return cdf + z * e * 0.39894228040143268f;
+    }
+    case ACT_GELU_TANH: {
+      const float s = sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
+      return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
+    }
+    case ACT_SILU: {
+      const float s = sigmoid(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    default: return 1.0f;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Checkpoints of rows.  32 lanes own a group: one 16-byte piece each (float: two), its minimum and maximum over the half wave.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int groups,
+                                                         uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale,
+                                                         float* __restrict__ mn) {
+  const int64_t unit = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int64_t row = unit / groups;
+  const int g = (int)(unit - row * groups), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int col = g * kGroup + lane * kVec, n = cols - col;
+  float v[kVec];
+  load_cols<T, WHOLE>(x + row * ldx + col, n, v);
+  float lo = __builtin_inff(), hi = -__builtin_inff();
+#pragma unroll
+  for (int e = 0; e < kVec; e++)
+    if (e < n) lo = __builtin_fminf(lo, v[e]), hi = __builtin_fmaxf(hi, v[e]);
+  lo = over_lanes<Least, 32>(lo);
+  hi = over_lanes<Most, 32>(hi);
+  const float s = scale_of(lo, hi);
+  if (n > 0) {
+    const u32x2 w = {four_codes(v[0], v[1], v[2], v[3], lo, s), four_codes(v[4], v[5], v[6], v[7], lo, s)};
+    *(u32x2*)(codes + row * ldc + col) = w;
+  }
+  if (lane == 0) {
+    scale[unit] = s;
+    mn[unit] = lo;
+  }
+}
+
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void restore_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scale,
+                                                      const float* __restrict__ mn, int64_t rows, int cols, int groups,
+                                                      T* __restrict__ out) {
+  const int64_t unit = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int64_t row = unit / groups;
+  const int g = (int)(unit - row * groups), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int col = g * kGroup + lane * kVec, n = cols - col;
+  if (n <= 0) return;
+  float v[kVec];
+  eight_values(*(const u32x2*)(codes + row * ldc + col), 1.0f / scale[unit], mn[unit], v);
+  store_cols<T, WHOLE>(out + row * cols + col, n, v);
+}
+
+// rows copied to a stride that the products can load 16 bytes at a time from, the columns behind the last one zero
+template <typename T>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, T* __restrict__ out,
+                                                       int ldo) {
+  const int per = ldo / kVec;
+  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = unit / per;
+  if (row >= rows) return;
+  const int col = (int)(unit - row * per) * kVec;
+  float v[kVec];
+  load_cols<T, false>(x + row * ldx + col, cols - col, v);
+  store8(out + row * ldo + col, v);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Layer norm.  LPR threads own a row and hold it in registers: NC pieces of 8 columns each, LPR * 8 columns apart, so that a group
+// of 256 columns is one piece of 32 neighbouring threads (LPR 16: two pieces of 16).  LPR up to 64: 256 / LPR rows per workgroup;
+// above: a workgroup of LPR threads per row.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <int LPR>
+struct RowShape {
+  static constexpr int kThreads = LPR <= 64 ? 256 : LPR;
+  static constexpr int kRows = kThreads / LPR;            // rows at a time
+  static constexpr int kWaves = LPR <= 64 ? 1 : LPR / 64;   // waves of a row
+  static constexpr int kSpan = LPR * kVec;                // columns of a piece
+};
+// the sum of v over the threads of a row; `turn` tells apart the buffers of consecutive sums
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v, float* shared, int turn) {
+  v = over_lanes<Sum, (LPR < 64 ? LPR : 64)>(v);
+  if constexpr (RowShape<LPR>::kWaves > 1) {
+    constexpr int W = RowShape<LPR>::kWaves;
+    float* at = shared + (turn & 1) * W;
+    if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w++) v += at[w];
+  }
+  return v;
+}
+
+template <typename T, int LPR, int NC, bool WHOLE>
+__global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_forward_kernel(
+    const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias, int64_t rows, int cols, float eps,
+    T* __restrict__ y, uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale, float* __restrict__ mn,
+    float* __restrict__ stats) {
+  using Shape = RowShape<LPR>;
+  __shared__ float shared[2 * Shape::kWaves];
+  const int lane = threadIdx.x % LPR;
+  const int64_t row = (int64_t)blockIdx.x * Shape::kRows + threadIdx.x / LPR;
+  if (Shape::kRows > 1 && row >= rows) return;
+  float v[NC][kVec];
+  const T* in = x + row * ldx;
+#pragma unroll
+  for (int c = 0; c < NC; c++) {
+    const int col = c * Shape::kSpan + lane * kVec;
+    load_cols<T, WHOLE>(in + col, cols - col, v[c]);
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; c++)
+#pragma unroll
+    for (int e = 0; e < kVec; e++) sum += v[c][e];
+  const float mean = row_sum<LPR>(sum, shared, 0) / (float)cols;
+  sum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; c++) {
+    const int left = cols - (c * Shape::kSpan + lane * kVec);
+#pragma unroll
+    for (int e = 0; e < kVec; e++) {
+      const float d = e < left ? v[c][e] - mean : 0.0f;
+      sum += d * d;
+    }
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<LPR>(sum, shared, 1) / (float)cols + eps);
+  if (stats && lane == 0) {
+    stats[2 * row] = mean;
+    stats[2 * row + 1] = rstd;
+  }
+  const int groups = (cols + kGroup - 1) / kGroup;
+  constexpr int PAIR = LPR == 16 && NC > 1 ? 2 : 1;   // pieces of a group
+  constexpr int GLANES = LPR < 32 ? 16 : 32;
+#pragma unroll
+  for (int c0 = 0; c0 < NC; c0 += PAIR) {
+    if (codes) {
+      float lo = __builtin_inff(), hi = -__builtin_inff();
+#pragma unroll
+      for (int c = c0; c < c0 + PAIR; c++) {
+        const int left = cols - (c * Shape::kSpan + lane * kVec);
+#pragma unroll
+        for (int e = 0; e < kVec; e++)
+          if (e < left) lo = __builtin_fminf(lo, v[c][e]), hi = __builtin_fmaxf(hi, v[c][e]);
+      }
+      lo = over_lanes<Least, GLANES>(lo);
+      hi = over_lanes<Most, GLANES>(hi);
+      const float s = scale_of(lo, hi);
+#pragma unroll
+      for (int c = c0; c < c0 + PAIR; c++) {
+        const int col = c * Shape::kSpan + lane * kVec;
+        if (col < cols)
+          *(u32x2*)(codes + row * ldc + col) = u32x2{four_codes(v[c][0], v[c][1], v[c][2], v[c][3], lo, s),
+                                                     four_codes(v[c][4], v[c][5], v[c][6], v[c][7], lo, s)};
+      }
+      const int col = c0 * Shape::kSpan + lane * kVec;
+      if (lane % GLANES == 0 && col < cols) {
+        scale[row * groups + col / kGroup] = s;
+        mn[row * groups + col / kGroup] = lo;
+      }
+    }
+#pragma unroll
+    for (int c = c0; c < c0 + PAIR; c++) {
+      const int col = c * Shape::kSpan + lane * kVec;
+      float w[kVec], b[kVec];
+      if (weight)
+        load_cols<T, WHOLE>(weight + col, cols - col, w);
+      else
+        for (int e = 0; e < kVec; e++) w[e] = 1.0f;
+      if (bias)
+        load_cols<T, WHOLE>(bias + col, cols - col, b);
+      else
+        for (int e = 0; e < kVec; e++) b[e] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kVec; e++) w[e] = __builtin_fmaf((v[c][e] - mean) * rstd, w[e], b[e]);
+      store_cols<T, WHOLE>(y + row * cols + col, cols - col, w);
+    }
+  }
+}
+
+// xh = (value - mean) rstd, g = dy w: dx = rstd (g - mean(g) - xh mean(g xh)); a thread adds up dy xh and dy of its columns over the
+// rows it sees, a workgroup writes one row of partial sums.
+template <typename T, int LPR, int NC, bool WHOLE>
+__global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_backward_kernel(
+    const T* __restrict__ dy, int64_t lddy, const T* __restrict__ weight, const uint8_t* __restrict__ codes, int64_t ldc,
+    const float* __restrict__ scale, const float* __restrict__ mn, const float* __restrict__ stats, int64_t rows, int cols,
+    T* __restrict__ dx, float* __restrict__ partial) {
+  using Shape = RowShape<LPR>;
+  __shared__ float shared[4 * Shape::kWaves];
+  constexpr int kFold = LPR < 64 ? 64 / LPR : 1;        // rows of a wave
+  constexpr int kAcross = LPR <= 64 ? 4 : 1;             // waves whose partial sums a workgroup adds up
+  __shared__ float folded[kAcross > 1 ? 64 * kVec * kAcross : 1];
+  const int lane = threadIdx.x % LPR;
+  const int groups = (cols + kGroup - 1) / kGroup;
+  float w[NC][kVec], dw[NC][kVec], db[NC][kVec];
+#pragma unroll
+  for (int c = 0; c < NC; c++) {
+    const int col = c * Shape::kSpan + lane * kVec;
+    if (weight)
+      load_cols<T, WHOLE>(weight + col, cols - col, w[c]);
+    else
+      for (int e = 0; e < kVec; e++) w[c][e] = 1.0f;
+#pragma unroll
+    for (int e = 0; e < kVec; e++) dw[c][e] = db[c][e] = 0.0f;
+  }
+  int turn = 0;
+  for (int64_t first = (int64_t)blockIdx.x * Shape::kRows; first < rows; first += (int64_t)gridDim.x * Shape::kRows) {
+    const int64_t row = first + threadIdx.x / LPR;
+    const bool there = Shape::kRows == 1 || row < rows;
+    const int64_t at = there ? row : rows - 1;
+    const float mean = stats[2 * at], rstd = stats[2 * at + 1];
+    float g[NC][kVec], xh[NC][kVec];
+    float sum_g = 0.0f, sum_gx = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      const int col = c * Shape::kSpan + lane * kVec;
+      const int64_t left = there ? cols - col : 0;
+      load_cols<T, WHOLE>(dy + at * lddy + col, left, g[c]);
+#pragma unroll
+      for (int e = 0; e < kVec; e++) xh[c][e] = 0.0f;
+      if (left > 0) {
+        const int64_t group = at * groups + col / kGroup;
+        eight_values(*(const u32x2*)(codes + at * ldc + col), 1.0f / scale[group], mn[group], xh[c]);
+#pragma unroll
+        for (int e = 0; e < kVec; e++) xh[c][e] = WHOLE || e < left ? (xh[c][e] - mean) * rstd : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < kVec; e++) {
+        const float gx = g[c][e] * xh[c][e];
+        dw[c][e] += gx;
+        db[c][e] += g[c][e];
+        g[c][e] *= w[c][e];
+        sum_g += g[c][e];
+        sum_gx += g[c][e] * xh[c][e];
+      }
+    }
+    const float mg = row_sum<LPR>(sum_g, shared, turn) / (float)cols;
+    const float mgx = row_sum<LPR>(sum_gx, shared + 2 * Shape::kWaves, turn) / (float)cols;
+    turn ^= 1;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      const int col = c * Shape::kSpan + lane * kVec;
+#pragma unroll
+      for (int e = 0; e < kVec; e++) g[c][e] = rstd * (g[c][e] - mg - xh[c][e] * mgx);
+      store_cols<T, WHOLE>(dx + at * cols + col, there ? cols - col : 0, g[c]);
+    }
+  }
+  if (!partial) return;
+  // rows of the wave first (lanes LPR apart own the same columns), then the workgroup's waves
+#pragma unroll
+  for (int c = 0; c < NC; c++) {
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+      float (&s)[kVec] = which ? db[c] : dw[c];
+#pragma unroll
+      for (int e = 0; e < kVec; e++) {
+        if (kFold >= 4) s[e] += __shfl_xor(s[e], 16);
+        if (kFold >= 2) s[e] += __shfl_xor(s[e], 32);
+      }
+      float* out = partial + ((int64_t)blockIdx.x * 2 + which) * cols;
+      const int col = c * Shape::kSpan + lane * kVec;
+      if constexpr (kAcross > 1) {
+        const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
+        __syncthreads();
+        if (l < LPR)
+#pragma unroll
+          for (int e = 0; e < kVec; e++) folded[(wave * kVec + e) * 64 + l] = s[e];
+        __syncthreads();
+        if (wave == 0 && l < LPR)
+#pragma unroll
+          for (int e = 0; e < kVec; e++)
+            if (col + e < cols)
+              out[col + e] = folded[e * 64 + l] + folded[(kVec + e) * 64 + l] + folded[(2 * kVec + e) * 64 + l] + folded[(3 * kVec + e) * 64 + l];
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; e++)
+          if (col + e < cols) out[col + e] = s[e];
+      }
+    }
+  }
+}
+
+// out[c] = sum of partial[p][c]; `stride` values from one partial row to the next.  16 waves per 64 columns.
+template <typename T>
+__global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict__ partial, int count, int64_t stride, int cols,
+                                                        T* __restrict__ out0, T* __restrict__ out1) {
+  __shared__ float shared[16][64];
+  const int col = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+  const float* in = partial + (int64_t)blockIdx.y * cols;
+  float s = 0.0f;
+  if (col < cols)
+    for (int p = wave; p < count; p += 16) s += in[p * stride + col];
+  shared[wave][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (wave == 0 && col < cols) {
+    s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; w++) s += shared[w][threadIdx.x];
+    T* out = blockIdx.y ? out1 : out0;
+    if (out) out[col] = (T)s;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// dz = dy act'(z) from the checkpoint of z, and the column sums of dz before they are rounded.  A thread owns 8 columns and walks
+// down `per` rows; without codes (no activation) dz is dy, copied to the products' stride where `dz` is given.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void activation_backward_kernel(const T* __restrict__ dy, int64_t lddy, const uint8_t* __restrict__ codes,
+                                                                  int64_t ldc, const float* __restrict__ scale,
+                                                                  const float* __restrict__ mn, int act, int64_t rows, int cols, int per,
+                                                                  T* __restrict__ dz, int64_t lddz, float* __restrict__ partial) {
+  __shared__ float shared[4][32][kVec + 1];
+  const int lane = threadIdx.x & 31, strip = threadIdx.x >> 5;     // 8 rows at a time
+  const int col = (int)blockIdx.x * kGroup + lane * kVec;
+  const int groups = (cols + kGroup - 1) / kGroup;
+  const int64_t first = (int64_t)blockIdx.y * per, last = first + per < rows ? first + per : rows;
+  const int64_t left = cols - col;
+  float sum[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; e++) sum[e] = 0.0f;
+  if (left > 0 || (dz && col < lddz)) {
+    for (int64_t row = first + strip; row < last; row += 8) {
+      float g[kVec], z[kVec];
+      load_cols<T, WHOLE>(dy + row * lddy + col, left, g);
+      if (codes && left > 0) {
+        const int64_t group = row * groups + blockIdx.x;
+        eight_values(*(const u32x2*)(codes + row * ldc + col), 1.0f / scale[group], mn[group], z);
+#pragma unroll
+        for (int e = 0; e < kVec; e++) g[e] = WHOLE || e < left ? g[e] * slope(z[e], act) : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < kVec; e++) sum[e] += g[e];
+      if (dz) store8(dz + row * lddz + col, g);
+    }
+  }
+  if (!partial) return;
+  // strips 2i and 2i + 1 share a wave
+#pragma unroll
+  for (int e = 0; e < kVec; e++) sum[e] += __shfl_xor(sum[e], 32);
+  if ((strip & 1) == 0)
+#pragma unroll
+    for (int e = 0; e < kVec; e++) shared[strip >> 1][lane][e] = sum[e];
+  __syncthreads();
+  const int c = (int)threadIdx.x;   // 256 columns
+  if ((int)blockIdx.x * kGroup + c < cols) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) s += shared[w][c / kVec][c % kVec];
+    partial[(int64_t)blockIdx.y * cols + (int)blockIdx.x * kGroup + c] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Products.  out[i][j] = sum over r of A(i, r) B(j, r), each operand in one of two layouts: rows of it contiguous along r (x and W of
+// the forward pass, dz of dx), or contiguous along i or j, one memory row per r (W of dx; dz and the checkpoint of dW).
+//
+// A workgroup owns a tile of BM x BN and walks along r in steps of 128 bytes of T, two tiles of each operand in LDS: the next one
+// arrives straight from memory (16 bytes a lane, no registers) while the present one is multiplied.  A checkpoint's codes pass
+// through registers, where they become values of T.  A lane's fragment is 8 values along r of 16-bit types (one 16x16x32 product) or 4 floats
+// (four 16x16x4 products).  Operands contiguous along r are read 16 bytes at a time, the others through the transposing LDS read (16-bit) or
+// value by value (float).  LDS is addressed so that neither kind of read meets a bank twice: contiguous rows of 128 bytes permute
+// their eight 16-byte pieces by the row's number, the others their blocks of 16 columns.
+//
+// B supplies the matrix instruction's rows and A its columns, so that a lane holds four consecutive j of one i.
+// ---------------------------------------------------------------------------------------------------------------------------------
+[[maybe_unused]] constexpr uint32_t kNowhere = 0x80000000u;   // beyond every window: such a load gives zero
+
+struct ProductArgs {
+  const void* a;
+  const void* b;
+  int64_t lda, ldb;
+  int rows, cols;          // of the output
+  int64_t depth;           // values along r
+  void* out;
+  int64_t ldo;
+  // a checkpoint as B
+  const float* b_scale;
+  const float* b_min;
+  int b_groups;
+  // the forward pass
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  int act;
+  uint8_t* codes;
+  int64_t ldc;
+  float* scale;
+  float* mn;
+  // tiles
+  int tiles_i, tiles_j, splits;
+  int64_t per_split;       // depth of a split, a multiple of the step
+  bool wide;               // output rows take stores of four values
+};
+
+template <typename T>
+struct Mma {
+  static constexpr int kStep = 128 / (int)sizeof(T);       // values along r of a step
+  static constexpr int kBlock = 16 * (int)sizeof(T);        // bytes of 16 columns
+  using Frag = std::conditional_t<std::is_same<T, bf16>::value, bf16x8, std::conditional_t<std::is_same<T, f16>::value, f16x8, f32x4>>;
+  static __device__ __forceinline__ f32x4 run(Frag a, Frag b, f32x4 c) {
+    if constexpr (std::is_same<T, bf16>::value) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    if constexpr (std::is_same<T, f16>::value) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int t = 0; t < 4; t++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], b[t], c, 0, 0, 0);
+    }
+    return c;
+  }
+  // by which a tile row's blocks of 16 columns are permuted: the rows that one read touches lie in different banks
+  static __device__ __forceinline__ uint32_t block_turn(uint32_t r) {
+    return sizeof(T) == 2 ? ((r & 3) | (((r >> 3) & 1) << 2)) : ((r >> 2) & 3);
+  }
+};
+
+// what is left of an operand from a tile's corner on, as a buffer that loads beyond it give zero from
+struct Window {
+  const char* base;
+  int64_t left;
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
+    const int64_t n = left <= 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : left;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)n, 0x00020000);
+  }
+  __device__ __forceinline__ void advance(int64_t bytes) {
+    base += bytes;
+    left -= bytes;
+  }
+};
+
+// Loads a tile of COUNT rows (contiguous along r) or COUNT columns (strided) into LDS: an instruction of a wave fills 1 KB.
+template <typename T, int COUNT, bool STRIDED, int WAVES>
+struct TileLoad {
+  static constexpr int kLoads = COUNT * 128 / 1024 / WAVES;
+  static constexpr int kEsz = (int)sizeof(T);
+  static_assert(kLoads >= 1, "a wave takes at least one load");
+  Window window;
+  int64_t step;
+  uint32_t at[kLoads];
+  // up to the end of the piece: a window drops a value of 16 bits whose neighbour in the word lies beyond it
+  static __device__ __forceinline__ int64_t whole(int64_t n) { return (n + 16 / kEsz - 1) / (16 / kEsz) * (16 / kEsz); }
+  int piece, left;     // contiguous: the lane's first value along r, and the values that are left from the step on
+  int wave;
+  __device__ __forceinline__ void start(const void* p, int64_t ld, int i0, int count, int64_t depth, int64_t r0, int w, int lane) {
+    wave = w;
+    if (STRIDED) {
+      constexpr int W = COUNT * kEsz, RPL = 1024 / W, BLK = Mma<T>::kBlock;
+      window.base = (const char*)p + (r0 * ld + i0) * kEsz;
+      window.left = ((depth - 1 - r0) * ld + whole(count) - i0) * kEsz;
+      if (depth <= r0) window.left = 0;
+      step = (int64_t)Mma<T>::kStep * ld * kEsz;
+#pragma unroll
+      for (int q = 0; q < kLoads; q++) {
+        const uint32_t r = (wave * kLoads + q) * RPL + lane * 16 / W, within = lane * 16 % W;
+        at[q] = r * (uint32_t)(ld * kEsz) + ((within / BLK) ^ Mma<T>::block_turn(r)) * BLK + within % BLK;
+      }
+    } else {
+      window.base = (const char*)p + (i0 * ld + r0) * kEsz;
+      window.left = ((count - 1 - i0) * ld + whole(depth) - r0) * kEsz;
+      step = 128;
+      piece = ((lane & 7) ^ (lane >> 3)) * (16 / kEsz);
+      left = (int)(depth - r0 < 0x7fffffff ? depth - r0 : 0x7fffffff);
+#pragma unroll
+      for (int q = 0; q < kLoads; q++) at[q] = ((wave * kLoads + q) * 8 + (lane >> 3)) * (uint32_t)(ld * kEsz) + piece * kEsz;
+    }
+  }
+  __device__ __forceinline__ void issue(lds_u8* tile) {
+#ifdef __HIP_DEVICE_COMPILE__   // the host pass knows no loads of 16 bytes into LDS and drops the kernels without a word
+    const __amdgpu_buffer_rsrc_t rsrc = window.rsrc();
+    const bool beyond = !STRIDED && piece >= left;
+#pragma unroll
+    for (int q = 0; q < kLoads; q++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(tile + (wave * kLoads + q) * 1024), 16,
+                                               beyond ? kNowhere : at[q], 0, 0, 0);
+#endif
+    window.advance(step);
+    left -= Mma<T>::kStep;
+  }
+};
+
+// Codes of a checkpoint, one memory row per r, as a strided tile of values: 16 codes of a row are one piece, a block of the tile.
+template <typename T, int COUNT, int WAVES>
+struct CodeLoad {
+  static constexpr int kPieces = Mma<T>::kStep * COUNT / 16 / (WAVES * 64);
+  static_assert(kPieces >= 1, "a thread takes at least one piece");
+  const uint8_t* codes;
+  const float* scale;
+  const float* mn;
+  int64_t ld, r;       // r: the step's first row
+  int64_t depth;
+  int groups, thread;
+  int j0;
+  u32x4 held[kPieces];
+  float s[kPieces], lo[kPieces];
+  __device__ __forceinline__ void start(const ProductArgs& p, int first, int64_t r0, int64_t end, int t) {
+    codes = (const uint8_t*)p.b;
+    scale = p.b_scale;
+    mn = p.b_min;
+    ld = p.ldb;
+    r = r0;
+    depth = end;
+    groups = p.b_groups;
+    thread = t;
+    j0 = first;
+  }
+  __device__ __forceinline__ void fetch() {
+#pragma unroll
+    for (int q = 0; q < kPieces; q++) {
+      const int piece = thread + q * WAVES * 64;
+      const int64_t row = r + piece / (COUNT / 16);
+      const int col = j0 + piece % (COUNT / 16) * 16;
+      held[q] = u32x4{0, 0, 0, 0};
+      s[q] = 1.0f;
+      lo[q] = 0.0f;
+      if (row < depth && col < ld) {
+        held[q] = *(const u32x4*)(codes + row * ld + col);
+        const int64_t g = row * groups + col / kGroup;
+        if (col / kGroup < groups) {
+          s[q] = scale[g];
+          lo[q] = mn[g];
+        }
+      }
+    }
+    r += Mma<T>::kStep;
+  }
+  __device__ __forceinline__ void put(lds_u8* tile) {
+#pragma unroll
+    for (int q = 0; q < kPieces; q++) {
+      const int piece = thread + q * WAVES * 64;
+      const uint32_t row = piece / (COUNT / 16), block = piece % (COUNT / 16);
+      const float inv = 1.0f / s[q];
+      lds_u8* to = tile + row * (COUNT * (int)sizeof(T)) + (block ^ Mma<T>::block_turn(row)) * Mma<T>::kBlock;
+      if constexpr (sizeof(T) == 2) {
+        typedef T T8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          T8 v;
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[e] = (T)__builtin_fmaf(code_at(held[q][2 * h + (e >> 2)], e & 3), inv, lo[q]);
+          *(__attribute__((address_space(3))) T8*)(to + 16 * h) = v;
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 4; h++) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(code_at(held[q][h], e), inv, lo[q]);
+          *(__attribute__((address_space(3))) f32x4*)(to + 16 * h) = v;
+        }
+      }
+    }
+  }
+};
+
+// Fragments of 16 rows (contiguous) or columns (strided) of a tile: `at` of a lane for k step kk, then immediate offsets.
+template <typename T, int COUNT, bool STRIDED>
+struct TileRead {
+  using Frag = typename Mma<T>::Frag;
+  static constexpr int W = COUNT * (int)sizeof(T), BLK = Mma<T>::kBlock;
+  static __device__ __forceinline__ Frag get(const lds_u8* tile, int first, int kk, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    if constexpr (!STRIDED) {
+      return *(const __attribute__((address_space(3))) Frag*)(tile + first * 128 + i * 128 + (((kk * 4 + g) ^ (i & 7)) * 16));
+    } else if constexpr (sizeof(T) == 2) {
+      const uint32_t turn = (i >> 2) | ((g & 1) << 2);
+      const lds_u8* p = tile + (g * 8 + (i >> 2)) * W + (((first / 16) ^ turn) * BLK) + (i & 3) * 8 + kk * 32 * W;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * W));
+      return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const lds_u8* p = tile + (kk * 16 + 4 * g) * W + (((first / 16) ^ g) * BLK) + i * 4;
+      f32x4 v;
+#pragma unroll
+      for (int t = 0; t < 4; t++) v[t] = *(const __attribute__((address_space(3))) float*)(p + t * W);
+      return v;
+    }
+  }
+};
+
+// Workgroups go to the 8 XCDs in turn: each XCD gets a run of consecutive tiles, and a run walks down `kTall` tile rows before it
+// moves to the next tile column, so that the tiles that an XCD works on at a time share rows of A and B in its L2.
+constexpr int kTall = 8;
+__device__ __forceinline__ void tile_of(uint32_t b, const ProductArgs& p, int& ti, int& tj, int& split) {
+  const uint32_t nb = gridDim.x, even = nb / 8, more = nb % 8, xcd = b % 8, k = b / 8;
+  uint32_t t = xcd * even + (xcd < more ? xcd : more) + k;
+  const uint32_t tiles = p.tiles_i * p.tiles_j;
+  split = t / tiles;
+  t -= split * tiles;
+  const uint32_t band = kTall * p.tiles_j, which = t / band, in = t - which * band;
+  const uint32_t tall = (uint32_t)p.tiles_i - which * kTall < kTall ? p.tiles_i - which * kTall : kTall;
+  ti = which * kTall + in % tall;
+  tj = in / tall;
+}
+
+enum { B_ROWS = 0, B_STRIDED = 1, B_CODES = 2 };
+
+template <typename T, int BM, int BN, int WI, int WJ, bool A_STRIDED, int B_KIND>
+__global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
+  constexpr int WAVES = WI * WJ, MI = BM / WI / 16, NJ = BN / WJ / 16;
+  constexpr int KK = 2;      // fragments along r of a step
+  constexpr bool FORWARD = B_KIND == B_ROWS;
+  __shared__ __attribute__((aligned(1024))) uint8_t memory[2 * (BM + BN) * 128];
+  lds_u8* lds = (lds_u8*)memory;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wi = wave / WJ, wj = wave % WJ;
+  int ti, tj, split;
+  tile_of(blockIdx.x, p, ti, tj, split);
+  const int i0 = ti * BM, j0 = tj * BN;
+  const int64_t r0 = split * p.per_split, end = r0 + p.per_split < p.depth ? r0 + p.per_split : p.depth;
+  const int steps = (int)((end - r0 + Mma<T>::kStep - 1) / Mma<T>::kStep);
+
+  TileLoad<T, BM, A_STRIDED, WAVES> a;
+  a.start(p.a, p.lda, i0, p.rows, end, r0, wave, lane);
+  std::conditional_t<B_KIND == B_CODES, CodeLoad<T, BN, WAVES>, TileLoad<T, BN, B_KIND == B_STRIDED, WAVES>> b;
+  if constexpr (B_KIND == B_CODES)
+    b.start(p, j0, r0, end, threadIdx.x);
+  else
+    b.start(p.b, p.ldb, j0, p.cols, end, r0, wave, lane);
+
+  f32x4 acc[MI][NJ];
+#pragma unroll
+  for (int m = 0; m < MI; m++)
+#pragma unroll
+    for (int n = 0; n < NJ; n++) acc[m][n] = f32x4{0, 0, 0, 0};
+
+  constexpr int BUF = (BM + BN) * 128;
+  a.issue(lds);
+  if constexpr (B_KIND == B_CODES) {
+    b.fetch();
+    b.put(lds + BM * 128);
+    b.fetch();
+  } else {
+    b.issue(lds + BM * 128);
+  }
+  for (int t = 0; t < steps; t++) {
+    __builtin_amdgcn_s_waitcnt(0);      // this step's tiles are there, for all waves
+    __syncthreads();
+    lds_u8* now = lds + (t & 1) * BUF;
+    lds_u8* next = lds + ((t + 1) & 1) * BUF;
+    if (t + 1 < steps) {
+      a.issue(next);
+      if constexpr (B_KIND == B_CODES) {
+        b.put(next + BM * 128);
+        b.fetch();
+      } else {
+        b.issue(next + BM * 128);
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++) {
+      typename Mma<T>::Frag fa[MI], fb[NJ];
+#pragma unroll
+      for (int m = 0; m < MI; m++) fa[m] = TileRead<T, BM, A_STRIDED>::get(now, wi * (BM / WI) + m * 16, kk, lane);
+#pragma unroll
+      for (int n = 0; n < NJ; n++) fb[n] = TileRead<T, BN, B_KIND != B_ROWS>::get(now + BM * 128, wj * (BN / WJ) + n * 16, kk, lane);
+#pragma unroll
+      for (int m = 0; m < MI; m++)
+#pragma unroll
+        for (int n = 0; n < NJ; n++) acc[m][n] = Mma<T>::run(fb[n], fa[m], acc[m][n]);
+    }
+  }
+
+  const int i_lane = i0 + wi * (BM / WI) + (lane & 15);
+  const int j_lane = j0 + wj * (BN / WJ) + (lane >> 4) * 4;
+  if constexpr (FORWARD) {
+    const T* bias = (const T*)p.bias;
+#pragma unroll
+    for (int n = 0; n < NJ; n++) {
+      const int j = j_lane + n * 16;
+      f32x4 v = {0, 0, 0, 0};
+      if (bias)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = j + e < p.cols ? (float)bias[j + e] : 0.0f;
+#pragma unroll
+      for (int m = 0; m < MI; m++) acc[m][n] += v;
+    }
+    if constexpr (BN == kGroup) {
+      if (p.codes) {
+        // a tile's row is one group: least and most of the wave's columns, then over the waves side by side
+        __shared__ float ends[2][WJ][BM];
+#pragma unroll
+        for (int m = 0; m < MI; m++) {
+          float lo = __builtin_inff(), hi = -__builtin_inff();
+#pragma unroll
+          for (int n = 0; n < NJ; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (j_lane + n * 16 + e < p.cols) lo = __builtin_fminf(lo, acc[m][n][e]), hi = __builtin_fmaxf(hi, acc[m][n][e]);
+          lo = __builtin_fminf(lo, __shfl_xor(lo, 16));
+          hi = __builtin_fmaxf(hi, __shfl_xor(hi, 16));
+          lo = __builtin_fminf(lo, __shfl_xor(lo, 32));
+          hi = __builtin_fmaxf(hi, __shfl_xor(hi, 32));
+          if (lane < 16) {
+            const int at = wi * (BM / WI) + m * 16 + lane;
+            ends[0][wj][at] = lo;
+            ends[1][wj][at] = hi;
+          }
+        }
+        __syncthreads();
+        const int groups = p.tiles_j;
+#pragma unroll
+        for (int m = 0; m < MI; m++) {
+          const int at = wi * (BM / WI) + m * 16 + (lane & 15), i = i0 + at;
+          float lo = ends[0][0][at], hi = ends[1][0][at];
+#pragma unroll
+          for (int w = 1; w < WJ; w++) lo = __builtin_fminf(lo, ends[0][w][at]), hi = __builtin_fmaxf(hi, ends[1][w][at]);
+          const float s = scale_of(lo, hi);
+          if (i < p.rows) {
+            if (wj == 0 && lane < 16) {
+              p.scale[(int64_t)i * groups + tj] = s;
+              p.mn[(int64_t)i * groups + tj] = lo;
+            }
+#pragma unroll
+            for (int n = 0; n < NJ; n++) {
+              const int j = j_lane + n * 16;
+              if (j < p.cols)
+                *(uint32_t*)(p.codes + i * p.ldc + j) = four_codes(acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3], lo, s);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MI; m++) {
+      const int64_t i = i_lane + m * 16;
+      if (i >= p.rows) continue;
+      T* out = (T*)p.out + i * p.ldo;
+      const T* residual = p.residual ? (const T*)p.residual + i * p.ldr : nullptr;
+#pragma unroll
+      for (int n = 0; n < NJ; n++) {
+        const int j = j_lane + n * 16;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        f32x4 v = acc[m][n];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = activated(v[e], p.act);
+        if (p.wide) {
+          if (j < p.cols) {
+            if (residual) {
+              const T4 r = *(const T4*)(residual + j);
+#pragma unroll
+              for (int e = 0; e < 4; e++) v[e] += (float)r[e];
+            }
+            T4 o;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = (T)v[e];
+            *(T4*)(out + j) = o;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (j + e < p.cols) out[j + e] = (T)(residual ? v[e] + (float)residual[j + e] : v[e]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int m = 0; m < MI; m++) {
+      const int64_t i = i_lane + m * 16;
+      if (i >= p.rows) continue;
+#pragma unroll
+      for (int n = 0; n < NJ; n++) {
+        const int j = j_lane + n * 16;
+        if (p.splits > 1) {     // partial sums, in float
+          float* out = (float*)p.out + ((int64_t)split * p.rows + i) * p.ldo;
+          if (j < p.cols) *(f32x4*)(out + j) = acc[m][n];
+        } else if (p.wide) {
+          typedef T T4 __attribute__((ext_vector_type(4)));
+          T4 o;
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[e] = (T)acc[m][n][e];
+          if (j < p.cols) *(T4*)((T*)p.out + i * p.ldo + j) = o;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (j + e < p.cols) ((T*)p.out)[i * p.ldo + j + e] = (T)acc[m][n][e];
+        }
+      }
+    }
+  }
+}
+
+// the splits' partial sums [splits][rows][ldp] added up, in order
+template <typename T>
+__global__ __launch_bounds__(256) void join_splits_kernel(const float* __restrict__ partial, int splits, int64_t rows, int cols, int ldp,
+                                                          T* __restrict__ out) {
+  const int per = ldp / 4;
+  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = unit / per;
+  const int col = (int)(unit - row * per) * 4;
+  if (row >= rows) return;
+  f32x4 v = *(const f32x4*)(partial + row * ldp + col);
+  for (int s = 1; s < splits; s++) v += *(const f32x4*)(partial + (s * rows + row) * ldp + col);
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (col + e < cols) out[row * cols + col + e] = (T)v[e];
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// The forward product of a few rows (up to 64): the weights are read once, straight into the matrix instruction's fragments, by
+// workgroups of 16 output columns whose waves share the depth; their sums meet in LDS.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <typename T, bool WHOLE>
+__device__ __forceinline__ typename Mma<T>::Frag fragment_of(const T* row, int64_t k, int64_t depth) {
+  using Frag = typename Mma<T>::Frag;
+  constexpr int N = 16 / (int)sizeof(T);
+  Frag f;
+  if (WHOLE) {
+    if (k < depth) return *(const Frag*)(row + k);
+#pragma unroll
+    for (int e = 0; e < N; e++) f[e] = (T)0.0f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e++) f[e] = k + e < depth ? row[k + e] : (T)0.0f;
+  }
+  return f;
+}
+template <typename T, int MT, int WAVES, bool WHOLE>
+__global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(ProductArgs p) {
+  constexpr int SPAN = 4 * 16 / (int)sizeof(T);      // values along r of a fragment step of the wave
+  __shared__ f32x4 shared[WAVES][MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int j0 = blockIdx.x * 16;
+  const int j = j0 + i < p.cols ? j0 + i : p.cols - 1;
+  const T* w = (const T*)p.b + j * p.ldb;
+  const T* x[MT];
+  f32x4 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    const int row = m * 16 + i < p.rows ? m * 16 + i : p.rows - 1;
+    x[m] = (const T*)p.a + row * p.lda;
+    acc[m] = f32x4{0, 0, 0, 0};
+  }
+  constexpr int UNROLL = 4;
+  for (int64_t k0 = (int64_t)wave * SPAN * UNROLL; k0 < p.depth; k0 += (int64_t)WAVES * SPAN * UNROLL) {
+    typename Mma<T>::Frag fw[UNROLL], fx[UNROLL][MT];
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) {
+      const int64_t k = k0 + u * SPAN + g * (16 / (int)sizeof(T));
+      fw[u] = fragment_of<T, WHOLE>(w, k, p.depth);
+#pragma unroll
+      for (int m = 0; m < MT; m++) fx[u][m] = fragment_of<T, WHOLE>(x[m], k, p.depth);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+      for (int m = 0; m < MT; m++) acc[m] = Mma<T>::run(fw[u], fx[u][m], acc[m]);
+  }
+#pragma unroll
+  for (int m = 0; m < MT; m++) shared[wave][m][lane] = acc[m];
+  __syncthreads();
+  for (int m = wave; m < MT; m += WAVES) {
+    f32x4 v = shared[0][m][lane];
+#pragma unroll
+    for (int s = 1; s < WAVES; s++) v += shared[s][m][lane];
+    const int row = m * 16 + i;
+    if (row >= p.rows) continue;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int c = j0 + g * 4 + e;
+      if (c >= p.cols) continue;
+      float o = v[e] + (p.bias ? (float)((const T*)p.bias)[c] : 0.0f);
+      o = activated(o, p.act);
+      if (p.residual) o += (float)((const T*)p.residual)[row * p.ldr + c];
+      ((T*)p.out)[row * p.ldo + c] = (T)o;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Host side of the ABI
+// ---------------------------------------------------------------------------------------------------------------------------------
+inline void fresh_launch() { (void)hipGetLastError(); }
+inline int launch_status() { return hipGetLastError() == hipSuccess ? GACT_OK : GACT_ELAUNCH; }
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+inline int size_of(int dtype) { return dtype == GACT_F32 ? 4 : 2; }
+inline bool known(int dtype) { return dtype == GACT_F32 || dtype == GACT_F16 || dtype == GACT_BF16; }
+inline bool blocks_fit(int64_t blocks) { return blocks > 0 && blocks <= 0x7fffffff; }
+constexpr int64_t kMostCols = GACT_LAYER_MAX_COLS;
+
+// rows that every lane's piece lies whole and aligned in
+inline bool whole_rows(const void* p, int dtype, int64_t cols, int64_t ld) {
+  return aligned16(p) && cols % kVec == 0 && ld * size_of(dtype) % 16 == 0;
+}
+inline bool codes_fit(const void* codes, int64_t cols, int64_t ldc) { return aligned16(codes) && ldc % 16 == 0 && ldc >= cols; }
+
+template <typename F>
+int with_type(int dtype, F&& f) {
+  switch (dtype) {
+    case GACT_F32: return f(float{});
+    case GACT_F16: return f(f16{});
+    default: return f(bf16{});
+  }
+}
+
+template <typename T, bool WHOLE, typename F>
+int with_row_shape(int64_t cols, F&& f) {
+  using std::integral_constant;
+  if (cols <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  if (cols <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+  if (cols <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  if (cols <= 1024) return f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  if (cols <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  if (cols <= 4096) return f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  if (cols <= 8192) return f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  return f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+}
+// workgroups of a layer norm's backward pass: each leaves one row of partial sums
+inline int64_t norm_blocks(int64_t rows, int64_t cols) {
+  const int64_t at_a_time = cols <= 128 ? 16 : cols <= 256 ? 8 : cols <= 1024 ? 4 : 1;
+  const int64_t needed = (rows + at_a_time - 1) / at_a_time;
+  return needed < 1024 ? needed : 1024;
+}
+inline int64_t strip_rows(int64_t rows, int64_t cols) {   // rows of a workgroup of the activation's backward pass
+  const int64_t across = (cols + kGroup - 1) / kGroup;
+  int64_t per = (rows * across + 2047) / 2048;
+  per = (per + 7) / 8 * 8;
+  if (per < 8) per = 8;
+  while ((rows + per - 1) / per > 65535) per *= 2;
+  return per;
+}
+
+template <typename T>
+int sum_rows(const float* partial, int64_t count, int64_t stride, int64_t cols, int parts, void* out0, void* out1, hipStream_t s) {
+  hipLaunchKernelGGL((sum_rows_kernel<T>), dim3((unsigned)((cols + 63) / 64), (unsigned)parts), dim3(1024), 0, s, partial, (int)count,
+                     stride, (int)cols, (T*)out0, (T*)out1);
+  return launch_status();
+}
+
+struct Tiles {
+  int bm, bn, splits;
+  int64_t per_split;
+};
+constexpr int kComputeUnits = 256;
+
+template <typename T, int BM, int BN, int WI, int WJ, bool AS, int BK>
+int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s) {
+  p.tiles_i = (p.rows + BM - 1) / BM;
+  p.tiles_j = (p.cols + BN - 1) / BN;
+  p.splits = splits;
+  p.per_split = per_split;
+  const int64_t blocks = (int64_t)p.tiles_i * p.tiles_j * splits;
+  if (!blocks_fit(blocks)) return GACT_ELIMIT;
+  auto kernel = product_kernel<T, BM, BN, WI, WJ, AS, BK>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(WI * WJ * 64), 0, s, p);
+  return launch_status();
+}
+
+// how a backward product is cut: the tile, and the parts of its depth where the tiles alone leave compute units idle
+inline Tiles tiles_of(int dtype, int64_t rows, int64_t cols, int64_t depth) {
+  Tiles t = {128, 128, 1, 0};
+  const int64_t step = 128 / size_of(dtype);
+  if (dtype != GACT_F32 && ((rows + 255) / 256) * ((cols + 255) / 256) >= kComputeUnits) t.bm = t.bn = 256;
+  const int64_t tiles = ((rows + t.bm - 1) / t.bm) * ((cols + t.bn - 1) / t.bn);
+  const int64_t steps = (depth + step - 1) / step;
+  int64_t splits = tiles >= 2 * kComputeUnits ? 1 : 2 * kComputeUnits / tiles;
+  if (splits > steps / 8) splits = steps / 8;
+  if (splits > 64) splits = 64;
+  if (splits < 1) splits = 1;
+  const int64_t per = (steps + splits - 1) / splits;
+  t.splits = (int)((steps + per - 1) / per);
+  t.per_split = per * step;
+  return t;
+}
+inline int64_t padded4(int64_t cols) { return (cols + 3) / 4 * 4; }
+
+template <typename T, bool AS, int BK>
+int backward_product(ProductArgs& p, int dtype, void* workspace, hipStream_t s) {
+  const Tiles t = tiles_of(dtype, p.rows, p.cols, p.depth);
+  void* out = p.out;
+  if (t.splits > 1) {
+    if (!workspace || !aligned16(workspace)) return GACT_EALIGN;
+    p.out = workspace;
+    p.ldo = padded4(p.cols);
+  }
+  int rc;
+  if constexpr (sizeof(T) == 2) {
+    rc = t.bm == 256 ? launch_product<T, 256, 256, 2, 4, AS, BK>(p, t.splits, t.per_split, s)
+                     : launch_product<T, 128, 128, 2, 2, AS, BK>(p, t.splits, t.per_split, s);
+  } else {
+    rc = launch_product<T, 128, 128, 2, 2, AS, BK>(p, t.splits, t.per_split, s);
+  }
+  if (rc != GACT_OK || t.splits == 1) return rc;
+  const int64_t blocks = ((int64_t)p.rows * (p.ldo / 4) + 255) / 256;
+  if (!blocks_fit(blocks)) return GACT_ELIMIT;
+  hipLaunchKernelGGL((join_splits_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, (const float*)workspace, t.splits, (int64_t)p.rows,
+                     p.cols, (int)p.ldo, (T*)out);
+  return launch_status();
+}
+
+inline bool layer_sizes(int64_t rows, int64_t a, int64_t b) {
+  return rows >= 0 && rows <= GACT_LAYER_MAX_ROWS && a > 0 && a <= kMostCols && b > 0 && b <= kMostCols;
+}
+// operands that the products load 16 bytes at a time
+inline bool operand_fits(const void* p, int64_t ld, int dtype, int64_t cols) {
+  return aligned16(p) && ld * size_of(dtype) % 16 == 0 && ld >= cols && ld <= 4 * kMostCols && cols * size_of(dtype) % 16 == 0;
+}
+}  // namespace
+
+extern "C" {
+
+int gact_checkpoint(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* codes, int64_t ldc, float* scale, float* mn,
+                    void* stream) {
+  if (!known(dtype) || !layer_sizes(rows, cols, 1) || (ldx < cols && rows > 1)) return GACT_EINVAL;
+  if (rows == 0) return GACT_OK;
+  if (!x || !codes || !scale || !mn) return GACT_EINVAL;
+  if (!codes_fit(codes, cols, ldc)) return GACT_EALIGN;
+  const int64_t groups = (cols + kGroup - 1) / kGroup, blocks = (rows * groups + 7) / 8;
+  if (!blocks_fit(blocks)) return GACT_ELIMIT;
+  fresh_launch();
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    auto kernel = whole_rows(x, dtype, cols, ldx) ? checkpoint_kernel<T, true> : checkpoint_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, (int)cols, ldx, (int)groups,
+                       (uint8_t*)codes, ldc, scale, mn);
+    return launch_status();
+  });
+}
+
+int gact_restore(const void* codes, int64_t ldc, const float* scale, const float* mn, int dtype, int64_t rows, int64_t cols, void* out,
+                 void* stream) {
+  if (!known(dtype) || !layer_sizes(rows, cols, 1)) return GACT_EINVAL;
+  if (rows == 0) return GACT_OK;
+  if (!codes || !scale || !mn || !out) return GACT_EINVAL;
+  if (!codes_fit(codes, cols, ldc) || !aligned16(out)) return GACT_EALIGN;
+  const int64_t groups = (cols + kGroup - 1) / kGroup, blocks = (rows * groups + 7) / 8;
+  if (!blocks_fit(blocks)) return GACT_ELIMIT;
+  fresh_launch();
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    auto kernel = whole_rows(out, dtype, cols, cols) ? restore_kernel<T, true> : restore_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)codes, ldc, scale, mn, rows,
+                       (int)cols, (int)groups, (T*)out);
+    return launch_status();
+  });
+}
+
+int gact_pad_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* out, int64_t ldo, void* stream) {
+  if (!known(dtype) || !layer_sizes(rows, cols, 1) || (ldx < cols && rows > 1)) return GACT_EINVAL;
+  if (rows == 0) return GACT_OK;
+  if (!x || !out) return GACT_EINVAL;
+  if (!aligned16(out) || ldo % kVec || ldo < cols || ldo > kMostCols + kVec) return GACT_EALIGN;
+  const int64_t blocks = (rows * (ldo / kVec) + 255) / 256;
+  if (!blocks_fit(blocks)) return GACT_ELIMIT;
+  fresh_launch();
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, (int)cols, ldx,
+                       (T*)out, (int)ldo);
+    return launch_status();
+  });
+}
+
+int gact_norm_forward(const void* x, int64_t ldx, const void* weight, const void* bias, int dtype, int64_t rows, int64_t cols, float eps,
+                      void* y, void* codes, int64_t ldc, float* scale, float* mn, float* stats, void* stream) {
+  if (!known(dtype) || !layer_sizes(rows, cols, 1) || cols > GACT_NORM_MAX_COLS || (ldx < cols && rows > 1)) return GACT_EINVAL;
+  if (rows == 0) return GACT_OK;
+  if (!x || !y || (codes && (!scale || !mn || !stats))) return GACT_EINVAL;
+  if (codes && !codes_fit(codes, cols, ldc)) return GACT_EALIGN;
+  fresh_launch();
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const bool whole = whole_rows(x, dtype, cols, ldx) && whole_rows(y, dtype, cols, cols) && aligned16(weight) && aligned16(bias);
+    auto run = [&](auto lpr, auto nc, auto w) {
+      constexpr int LPR = decltype(lpr)::value, NC = decltype(nc)::value;
+      const int64_t blocks = (rows + RowShape<LPR>::kRows - 1) / RowShape<LPR>::kRows;
+      if (!blocks_fit(blocks)) return GACT_ELIMIT;
+      hipLaunchKernelGGL((norm_forward_kernel<T, LPR, NC, decltype(w)::value>), dim3((unsigned)blocks), dim3(RowShape<LPR>::kThreads), 0,
+                         (hipStream_t)stream, (const T*)x, ldx, (const T*)weight, (const T*)bias, rows, (int)cols, eps, (T*)y,
+                         (uint8_t*)codes, ldc, scale, mn, stats);
+      return launch_status();
+    };
+    return whole ? with_row_shape<T, true>(cols, [&](auto l, auto n) { return run(l, n, std::true_type{}); })
+                 : with_row_shape<T, false>(cols, [&](auto l, auto n) { return run(l, n, std::false_type{}); });
+  });
+}
+
+int64_t gact_norm_workspace_bytes(int64_t rows, int64_t cols) {
+  return rows <= 0 || cols <= 0 ? 0 : norm_blocks(rows, cols) * 2 * cols * (int64_t)sizeof(float);
+}
+
+int gact_norm_backward(const void* dy, int64_t lddy, const void* weight, const void* codes, int64_t ldc, const float* scale,
+                       const float* mn, const float* stats, int dtype, int64_t rows, int64_t cols, void* dx, void* dweight, void* dbias,
+                       float* workspace, void* stream) {
+  if (!known(dtype) || !layer_sizes(rows, cols, 1) || rows == 0 || cols > GACT_NORM_MAX_COLS || (lddy < cols && rows > 1)) return GACT_EINVAL;
+  if (!dy || !codes || !scale || !mn || !stats || !dx) return GACT_EINVAL;
+  const bool sums = dweight || dbias;
+  if (sums && !workspace) return GACT_EINVAL;
+  if (!codes_fit(codes, cols, ldc)) return GACT_EALIGN;
+  fresh_launch();
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const bool whole = whole_rows(dy, dtype, cols, lddy) && whole_rows(dx, dtype, cols, cols) && aligned16(weight);
+    const int64_t blocks = norm_blocks(rows, cols);
+    auto run = [&](auto lpr, auto nc, auto w) {
+      constexpr int LPR = decltype(lpr)::value, NC = decltype(nc)::value;
+      hipLaunchKernelGGL((norm_backward_kernel<T, LPR, NC, decltype(w)::value>), dim3((unsigned)blocks), dim3(RowShape<LPR>::kThreads), 0,
+                         (hipStream_t)stream, (const T*)dy, lddy, (const T*)weight, (const uint8_t*)codes, ldc, scale, mn, stats, rows,
+                         (int)cols, (T*)dx, sums ? workspace : nullptr);
+      return launch_status();
+    };
+    const int rc = whole ? with_row_shape<T, true>(cols, [&](auto l, auto n) { return run(l, n, std::true_type{}); })
+                         : with_row_shape<T, false>(cols, [&](auto l, auto n) { return run(l, n, std::false_type{}); });
+    if (rc != GACT_OK || !sums) return rc;
+    return sum_rows<T>(workspace, blocks, 2 * cols, cols, 2, dweight, dbias, (hipStream_t)stream);
+  });
+}
+
+int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
+                int activation, int dtype, int64_t rows, int64_t inner, int64_t outer, void* y, void* codes, int64_t ldc, float* scale,
+                float* mn, void* stream) {
+  if (!known(dtype) || !layer_sizes(rows, inner, outer) || activation < GACT_ACT_NONE || activation > GACT_ACT_SILU) return GACT_EINVAL;
+  if (rows == 0) return GACT_OK;
+  if (!x || !weight || !y || (codes && (!scale || !mn)) || (residual && ldr < outer && rows > 1)) return GACT_EINVAL;
+  if (codes && !codes_fit(codes, outer, ldc)) return GACT_EALIGN;
+  const bool few = !codes && rows <= GACT_LINEAR_FEW_ROWS;
+  const bool whole = operand_fits(x, ldx, dtype, inner) && operand_fits(weight, ldw, dtype, inner);
+  if (!whole && !few) return GACT_EALIGN;
+  ProductArgs p = {};
+  p.a = x;
+  p.b = weight;
+  p.lda = ldx;
+  p.ldb = ldw;
+  p.rows = (int)rows;
+  p.cols = (int)outer;
+  p.depth = inner;
+  p.out = y;
+  p.ldo = outer;
+  p.bias = bias;
+  p.residual = residual;
+  p.ldr = ldr;
+  p.act = activation;
+  p.codes = (uint8_t*)codes;
+  p.ldc = ldc;
+  p.scale = scale;
+  p.mn = mn;
+  const int four = 4 * size_of(dtype);
+  p.wide = outer % 4 == 0 && (uintptr_t)y % four == 0 && (!residual || ((uintptr_t)residual % four == 0 && ldr % 4 == 0));
+  fresh_launch();
+  hipStream_t s = (hipStream_t)stream;
+  return with_type(dtype, [&](auto zero) -> int {
+    using T = decltype(zero);
+    if (few) {
+      auto run = [&](auto mt, auto waves) {
+        constexpr int MT = decltype(mt)::value, W = decltype(waves)::value;
+        auto kernel = whole ? few_rows_kernel<T, MT, W, true> : few_rows_kernel<T, MT, W, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((outer + 15) / 16)), dim3(W * 64), 0, s, p);
+        return launch_status();
+      };
+      using std::integral_constant;
+      if (rows <= 16) return run(integral_constant<int, 1>{}, integral_constant<int, 8>{});
+      if (rows <= 32) return run(integral_constant<int, 2>{}, integral_constant<int, 8>{});
+      return run(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    }
+    const int64_t step = 128 / (int)sizeof(T), depth = (inner + step - 1) / step * step;
+    if constexpr (sizeof(T) == 2)
+      if (((rows + 255) / 256) * ((outer + 255) / 256) >= kComputeUnits)
+        return launch_product<T, 256, 256, 2, 4, false, B_ROWS>(p, 1, depth, s);
+    if (codes) return launch_product<T, 128, 256, 2, 4, false, B_ROWS>(p, 1, depth, s);
+    return launch_product<T, 128, 128, 2, 2, false, B_ROWS>(p, 1, depth, s);
+  });
+}
+
+int64_t gact_activation_workspace_bytes(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  const int64_t per = strip_rows(rows, cols);
+  return (rows + per - 1) / per * cols * (int64_t)sizeof(float);
+}
+
+int gact_activation_backward(const void* dy, int64_t lddy, const void* codes, int64_t ldc, const float* scale, const float* mn,
+                             int activation, int dtype, int64_t rows, int64_t cols, void* dz, int64_t lddz, void* dbias, float* workspace,
+                             void* stream) {
+  if (!known(dtype) || !layer_sizes(rows, cols, 1) || rows == 0 || (lddy < cols && rows > 1)) return GACT_EINVAL;
+  if (activation < GACT_ACT_NONE || activation > GACT_ACT_SILU || (activation != GACT_ACT_NONE && !codes)) return GACT_EINVAL;
+  if (!dy || (codes && (!scale || !mn)) || (dbias && !workspace) || (!dz && !dbias)) return GACT_EINVAL;
+  if ((codes && !codes_fit(codes, cols, ldc)) || (dz && (!aligned16(dz) || lddz % kVec || lddz < cols || lddz >= cols + kVec))) return GACT_EALIGN;
+  const int64_t per = strip_rows(rows, cols), strips = (rows + per - 1) / per;
+  fresh_launch();
+  return with_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    auto kernel = whole_rows(dy, dtype, cols, lddy) ? activation_backward_kernel<T, true> : activation_backward_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((cols + kGroup - 1) / kGroup), (unsigned)strips), dim3(256), 0, (hipStream_t)stream,
+                       (const T*)dy, lddy, (const uint8_t*)codes, ldc, scale, mn, activation, rows, (int)cols, (int)per, (T*)dz, lddz,
+                       dbias ? workspace : nullptr);
+    const int rc = launch_status();
+    if (rc != GACT_OK || !dbias) return rc;
+    return sum_rows<T>(workspace, strips, cols, cols, 1, dbias, nullptr, (hipStream_t)stream);
+  });
+}
+
+int64_t gact_product_workspace_bytes(int dtype, int64_t rows, int64_t cols, int64_t depth) {
+  if (!known(dtype) || rows <= 0 || cols <= 0 || depth <= 0) return 0;
+  const Tiles t = tiles_of(dtype, rows, cols, depth);
+  return t.splits == 1 ? 0 : t.splits * rows * padded4(cols) * (int64_t)sizeof(float);
+}
+
+int gact_product(const void* a, int64_t lda, const void* b, int64_t ldb, int dtype, int64_t rows, int64_t depth, int64_t cols, void* out,
+                 void* workspace, void* stream) {
+  if (!known(dtype) || !layer_sizes(rows, depth, cols)) return GACT_EINVAL;
+  if (rows == 0) return GACT_OK;
+  if (!a || !b || !out) return GACT_EINVAL;
+  const int64_t padded = (cols * size_of(dtype) + 15) / 16 * 16 / size_of(dtype);
+  if (!operand_fits(a, lda, dtype, (depth * size_of(dtype) + 15) / 16 * 16 / size_of(dtype)) || !operand_fits(b, ldb, dtype, padded)) return GACT_EALIGN;
+  ProductArgs p = {};
+  p.a = a;
+  p.b = b;
+  p.lda = lda;
+  p.ldb = ldb;
+  p.rows = (int)rows;
+  p.cols = (int)cols;
+  p.depth = depth;
+  p.out = out;
+  p.ldo = cols;
+  p.wide = cols % 4 == 0 && (uintptr_t)out % (4 * size_of(dtype)) == 0;
+  fresh_launch();
+  return with_type(dtype, [&](auto zero) { return backward_product<decltype(zero), false, B_STRIDED>(p, dtype, workspace, (hipStream_t)stream); });
+}
+
+int gact_checkpoint_product(const void* grad, int64_t ldg, const void* codes, int64_t ldc, const float* scale, const float* mn, int dtype,
+                            int64_t rows, int64_t outer, int64_t inner, void* out, void* workspace, void* stream) {
+  if (!known(dtype) || !layer_sizes(rows, outer, inner) || rows == 0) return GACT_EINVAL;
+  if (!grad || !codes || !scale || !mn || !out) return GACT_EINVAL;
+  const int64_t padded = (outer * size_of(dtype) + 15) / 16 * 16 / size_of(dtype);
+  if (!operand_fits(grad, ldg, dtype, padded) || !codes_fit(codes, inner, ldc)) return GACT_EALIGN;
+  ProductArgs p = {};
+  p.a = grad;
+  p.b = codes;
+  p.lda = ldg;
+  p.ldb = ldc;
+  p.rows = (int)outer;
+  p.cols = (int)inner;
+  p.depth = rows;
+  p.out = out;
+  p.ldo = inner;
+  p.b_scale = scale;
+  p.b_min = mn;
+  p.b_groups = (int)((inner + kGroup - 1) / kGroup);
+  p.wide = inner % 4 == 0 && (uintptr_t)out % (4 * size_of(dtype)) == 0;
+  fresh_launch();
+  return with_type(dtype, [&](auto zero) { return backward_product<decltype(zero), true, B_CODES>(p, dtype, workspace, (hipStream_t)stream); });
+}
+
+}  // extern "C"

@@ -41,7 +41,7 @@ class BatchEntry(ctypes.Structure):
     ]
 
 
-_vp, _i32, _i64, _u64, _f64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_double
+_vp, _i32, _i64, _u64, _f32, _f64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_float, ctypes.c_double
 
 # name -> (restype, argtypes); exactly the entry points include/gact_hip.h declares
 SIGNATURES = {
@@ -70,6 +70,18 @@ SIGNATURES = {
     "gact_dequantize_batched_types": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp]),
     "gact_dequantize_batched_to": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp]),
     "gact_quantize_batched_static": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "gact_checkpoint": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "gact_restore": (_i32, [_vp, _i64, _vp, _vp, _i32, _i64, _i64, _vp, _vp]),
+    "gact_pad_rows": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "gact_norm_forward": (_i32, [_vp, _i64, _vp, _vp, _i32, _i64, _i64, _f32, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "gact_norm_workspace_bytes": (_i64, [_i64, _i64]),
+    "gact_norm_backward": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "gact_linear": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp]),
+    "gact_activation_workspace_bytes": (_i64, [_i64, _i64]),
+    "gact_activation_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i32, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "gact_product_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64]),
+    "gact_product": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "gact_checkpoint_product": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
 }
 
 

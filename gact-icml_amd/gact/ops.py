@@ -15,6 +15,7 @@ import torch
 from .conf import config
 from .cpp_extension import _abi
 from .cpp_extension import quantization as ext_quantization
+from .layers import Checkpoint, op_checkpoint, op_checkpoint_product, op_layer_norm, op_linear, op_restore  # noqa: F401
 
 
 # the raw HIP stream torch currently launches on for a device (what _abi.stream_of wraps), bound once: these two

@@ -222,6 +222,68 @@ int gact_quantize_batched_static(gact_batch_entry* table, const int32_t* bits, i
                                  int64_t capacity, int noise_mode, int dtypes, void* packed_arena,
                                  void* scale_arena, void* min_arena, int64_t* verdict, void* stream);
 
+/* ---- Layers that train on 8-bit checkpoints.  No counterpart in the reference, whose layers save whole tensors through the hooks. ----
+ *
+ * A checkpoint of a matrix [rows, cols] of any element type: codes (one byte each, rows `ldc` bytes apart, ldc a multiple of 16
+ * and at least cols, 16-byte aligned), and a float scale and minimum per row and group of 256 columns, [rows, ceil(cols/256)], the last
+ * group of a row being shorter.  Codes, scale and minimum are those of gact_quantize of the values widened to float at 8 bit with
+ * GACT_NOISE_CONST (equal to it where 256 divides cols); a code stands for code / scale + min.
+ * `ld...` are elements from one row to the next.  Rows up to GACT_LAYER_MAX_ROWS, columns up to GACT_LAYER_MAX_COLS. */
+#define GACT_LAYER_MAX_ROWS 0x40000000
+#define GACT_LAYER_MAX_COLS 262144
+#define GACT_NORM_MAX_COLS 16384
+#define GACT_LINEAR_FEW_ROWS 64
+#define GACT_ACT_NONE 0
+#define GACT_ACT_GELU 1      /* z Phi(z)                                            */
+#define GACT_ACT_GELU_TANH 2 /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))     */
+#define GACT_ACT_SILU 3      /* z / (1 + exp(-z))                                    */
+
+/* x [rows, cols] -> its checkpoint, and back to values of `dtype` in a contiguous [rows, cols] (16-byte aligned). */
+int gact_checkpoint(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* codes, int64_t ldc, float* scale, float* mn,
+                    void* stream);
+int gact_restore(const void* codes, int64_t ldc, const float* scale, const float* mn, int dtype, int64_t rows, int64_t cols, void* out,
+                 void* stream);
+
+/* x [rows, cols] copied to rows `ldo` apart (a multiple of 8, 16-byte aligned), columns behind the last one zero: what the products below
+ * take of matrices whose rows are no whole 16-byte pieces. */
+int gact_pad_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, void* out, int64_t ldo, void* stream);
+
+/* Layer norm over the last dimension, cols <= GACT_NORM_MAX_COLS: y = (x - mean) / sqrt(var + eps) weight + bias (either may be null),
+ * y contiguous.  With `codes`: also the checkpoint of x, and mean and 1 / sqrt(var + eps) of each row in stats [rows, 2]. */
+int gact_norm_forward(const void* x, int64_t ldx, const void* weight, const void* bias, int dtype, int64_t rows, int64_t cols, float eps,
+                      void* y, void* codes, int64_t ldc, float* scale, float* mn, float* stats, void* stream);
+/* Its backward pass from the checkpoint: dx (contiguous), and dweight and dbias where they are not null, which need `workspace`
+ * (gact_norm_workspace_bytes(), float aligned).  rows > 0. */
+int64_t gact_norm_workspace_bytes(int64_t rows, int64_t cols);
+int gact_norm_backward(const void* dy, int64_t lddy, const void* weight, const void* codes, int64_t ldc, const float* scale,
+                       const float* mn, const float* stats, int dtype, int64_t rows, int64_t cols, void* dx, void* dweight, void* dbias,
+                       float* workspace, void* stream);
+
+/* y [rows, outer] = act(x [rows, inner] weight [outer, inner]^T + bias) + residual, y contiguous; bias and residual may be null.  With
+ * `codes`: also the checkpoint of z = x weight^T + bias.  x and weight: 16-byte aligned rows of whole 16-byte pieces (else
+ * GACT_EALIGN), except for up to GACT_LINEAR_FEW_ROWS rows without codes. */
+int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
+                int activation, int dtype, int64_t rows, int64_t inner, int64_t outer, void* y, void* codes, int64_t ldc, float* scale,
+                float* mn, void* stream);
+
+/* dz [rows, cols] = dy act'(z) with z from its checkpoint (codes null and activation GACT_ACT_NONE: dz = dy), rows lddz apart (cols rounded up to a
+ * multiple of 8, the columns behind the last one zero); dbias [cols] = the column sums of dz before rounding, through `workspace`
+ * (gact_activation_workspace_bytes()).  Either output may be null.  rows > 0. */
+int64_t gact_activation_workspace_bytes(int64_t rows, int64_t cols);
+int gact_activation_backward(const void* dy, int64_t lddy, const void* codes, int64_t ldc, const float* scale, const float* mn,
+                             int activation, int dtype, int64_t rows, int64_t cols, void* dz, int64_t lddz, void* dbias, float* workspace,
+                             void* stream);
+
+/* out [rows, cols] = a [rows, depth] b [depth, cols], and out [outer, inner] = grad [rows, outer]^T times the values, rounded to `dtype`, of a
+ * checkpoint [rows, inner] (rows > 0); out contiguous.  Operands: 16-byte aligned rows of whole 16-byte pieces, `ld` leaving room for the
+ * last one; what lies behind the last column of `a` up to its piece's end must be zero.  workspace: gact_product_workspace_bytes()
+ * of (rows, cols, depth), or (outer, inner, rows); 16-byte aligned. */
+int64_t gact_product_workspace_bytes(int dtype, int64_t rows, int64_t cols, int64_t depth);
+int gact_product(const void* a, int64_t lda, const void* b, int64_t ldb, int dtype, int64_t rows, int64_t depth, int64_t cols, void* out,
+                 void* workspace, void* stream);
+int gact_checkpoint_product(const void* grad, int64_t ldg, const void* codes, int64_t ldc, const float* scale, const float* mn, int dtype,
+                            int64_t rows, int64_t outer, int64_t inner, void* out, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
