@@ -19,6 +19,7 @@ namespace {
 
 typedef _Float16 f16;
 typedef __bf16 bf16;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -130,37 +131,65 @@ __device__ __forceinline__ void eight_values(u32x2 w, float inv, float lo, float
 
 // ---- activations: act(z) and act'(z) ----
 enum { ACT_NONE = GACT_ACT_NONE, ACT_GELU = GACT_ACT_GELU, ACT_GELU_TANH = GACT_ACT_GELU_TANH, ACT_SILU = GACT_ACT_SILU };
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
-// the normal distribution's cumulative function and exp(-z^2/2)
-__device__ __forceinline__ void normal_cdf(float z, float& cdf, float& e) {
-  e = expf(-0.5f * z * z);
-  cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+// Exact to float's rounding for float; for 16-bit types, whose own rounding is at least 2^-12, the hardware's exponential and reciprocal and a
+// polynomial: 1 - Phi(|z|) = exp(-z^2/2) q(t), t = 1 / (1 + 0.425 |z| / sqrt 2), q of degree 6 fitted to erfc over [0, 9.5] (relative error 1e-5,
+// absolute error of Phi 4.3e-7).  In the epilogue of a product the library's erfc takes as long as the product of 1024 columns.
+template <bool EXACT>
+__device__ __forceinline__ float sigmoid(float x) {
+  if (EXACT) return 1.0f / (1.0f + expf(-x));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
 }
+// the normal distribution's cumulative function and exp(-z^2/2)
+template <bool EXACT>
+__device__ __forceinline__ void normal_cdf(float z, float& cdf, float& e) {
+  if (EXACT) {
+    e = expf(-0.5f * z * z);
+    cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+    return;
+  }
+  e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fabsf(z), 0.30052038200428270f, 1.0f));
+  float q = __builtin_fmaf(t, -0.079363826f, 0.2208909465f);
+  q = __builtin_fmaf(t, q, -0.02224172415f);
+  q = __builtin_fmaf(t, q, 0.1470668855f);
+  q = __builtin_fmaf(t, q, 0.113310361f);
+  q = __builtin_fmaf(t, q, 0.120337111f);
+  q = t * e * q;
+  cdf = z < 0.0f ? q : 1.0f - q;
+}
+template <bool EXACT>
 __device__ __forceinline__ float activated(float z, int act) {
   switch (act) {
     case ACT_GELU: {
       float cdf, e;
-      normal_cdf(z, cdf, e);
+      normal_cdf<EXACT>(z, cdf, e);
       return z * cdf;
     }
-    case ACT_GELU_TANH: return z * sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));   // 0.5 (1 + tanh u) = sigmoid(2 u)
-    case ACT_SILU: return z * sigmoid(z);
+    case ACT_GELU_TANH: return z * sigmoid<EXACT>(1.5957691216057308f * (z + 0.044715f * z * z * z));   // 0.5 (1 + tanh u) = sigmoid(2 u)
+    case ACT_SILU: return z * sigmoid<EXACT>(z);
     default: return z;
   }
 }
+template <typename T, int ACT>
+__device__ __forceinline__ f32x4 activated4(f32x4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = activated<std::is_same<T, float>::value>(v[e], ACT);
+  return v;
+}
+template <bool EXACT>
 __device__ __forceinline__ float slope(float z, int act) {
   switch (act) {
     case ACT_GELU: {
       float cdf, e;
-      normal_cdf(z, cdf, e);
+      normal_cdf<EXACT>(z, cdf, e);
       return cdf + z * e * 0.39894228040143268f;
     }
     case ACT_GELU_TANH: {
-      const float s = sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
+      const float s = sigmoid<EXACT>(1.5957691216057308f * (z + 0.044715f * z * z * z));
       return s + z * s * (1.0f - s) * 1.5957691216057308f * (1.0f + 0.134145f * z * z);
     }
     case ACT_SILU: {
-      const float s = sigmoid(z);
+      const float s = sigmoid<EXACT>(z);
       return s * (1.0f + z * (1.0f - s));
     }
     default: return 1.0f;
@@ -491,7 +520,7 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __res
         const int64_t group = row * groups + blockIdx.x;
         eight_values(*(const u32x2*)(codes + row * ldc + col), 1.0f / scale[group], mn[group], z);
 #pragma unroll
-        for (int e = 0; e < kVec; e++) g[e] = WHOLE || e < left ? g[e] * slope(z[e], act) : 0.0f;
+        for (int e = 0; e < kVec; e++) g[e] = WHOLE || e < left ? g[e] * slope<std::is_same<T, float>::value>(z[e], act) : 0.0f;
       }
 #pragma unroll
       for (int e = 0; e < kVec; e++) sum[e] += g[e];
@@ -554,7 +583,7 @@ struct ProductArgs {
   // tiles
   int tiles_i, tiles_j, splits;
   int64_t per_split;       // depth of a split, a multiple of the step
-  bool wide;               // output rows take stores of four values
+  bool wide;               // output rows, and the residual's, are whole 16-byte pieces
 };
 
 template <typename T>
@@ -628,13 +657,18 @@ struct TileLoad {
     }
   }
   __device__ __forceinline__ void issue(lds_u8* tile) {
-#ifdef __HIP_DEVICE_COMPILE__   // the host pass knows no loads of 16 bytes into LDS and drops the kernels without a word
+#ifdef __HIP_DEVICE_COMPILE__
     const __amdgpu_buffer_rsrc_t rsrc = window.rsrc();
     const bool beyond = !STRIDED && piece >= left;
+    // buffer_load_dwordx4 with its destination in LDS (M0: the wave's first byte there).  It writes no register.  As asm, because the compiler
+    // waits for every such load that it knows of before it reads LDS through the transposing read, whichever tile that lies in;
+    // the product waits for them itself, before the barrier that gives a tile free.
 #pragma unroll
     for (int q = 0; q < kLoads; q++)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(tile + (wave * kLoads + q) * 1024), 16,
-                                               beyond ? kNowhere : at[q], 0, 0, 0);
+      asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                   :
+                   : "v"(beyond ? kNowhere : at[q]), "s"(rsrc), "{m0}"((uint32_t)(uintptr_t)(tile + (wave * kLoads + q) * 1024))
+                   : "memory");
 #endif
     window.advance(step);
     left -= Mma<T>::kStep;
@@ -645,53 +679,49 @@ struct TileLoad {
 template <typename T, int COUNT, int WAVES>
 struct CodeLoad {
   static constexpr int kPieces = Mma<T>::kStep * COUNT / 16 / (WAVES * 64);
+  static constexpr int kAcross = COUNT / 16, kApart = WAVES * 64 / kAcross;     // pieces of a row; rows between a thread's pieces
   static_assert(kPieces >= 1, "a thread takes at least one piece");
-  const uint8_t* codes;
-  const float* scale;
-  const float* mn;
-  int64_t ld, r;       // r: the step's first row
-  int64_t depth;
-  int groups, thread;
-  int j0;
+  Window codes, scale, mn;
+  int64_t step, stat_step;
+  uint32_t at, stat_at, apart, stat_apart;    // of the thread's first piece, and to the next one
+  int left, held_left, thread;                // rows from the next step on, and from the one that is held on
   u32x4 held[kPieces];
   float s[kPieces], lo[kPieces];
-  __device__ __forceinline__ void start(const ProductArgs& p, int first, int64_t r0, int64_t end, int t) {
-    codes = (const uint8_t*)p.b;
-    scale = p.b_scale;
-    mn = p.b_min;
-    ld = p.ldb;
-    r = r0;
-    depth = end;
-    groups = p.b_groups;
+  __device__ __forceinline__ void start(const ProductArgs& p, int j0, int64_t r0, int64_t end, int t) {
     thread = t;
-    j0 = first;
+    left = (int)(end - r0 < 0x7fffffff ? end - r0 : 0x7fffffff);
+    const int row = t / kAcross, col = t % kAcross * 16, groups = p.b_groups;
+    codes.base = (const char*)p.b + r0 * p.ldb + j0;
+    codes.left = (end - r0) * p.ldb - j0;
+    scale.base = (const char*)(p.b_scale + r0 * groups + j0 / kGroup);
+    mn.base = (const char*)(p.b_min + r0 * groups + j0 / kGroup);
+    scale.left = mn.left = ((end - r0) * groups - j0 / kGroup) * 4;
+    step = Mma<T>::kStep * p.ldb;
+    stat_step = Mma<T>::kStep * groups * 4;
+    at = row * (uint32_t)p.ldb + col;
+    stat_at = (row * groups + (j0 % kGroup + col) / kGroup) * 4;
+    apart = kApart * (uint32_t)p.ldb;
+    stat_apart = kApart * groups * 4;
   }
   __device__ __forceinline__ void fetch() {
+    held_left = left;
+    const __amdgpu_buffer_rsrc_t c = codes.rsrc(), f = scale.rsrc(), m = mn.rsrc();
 #pragma unroll
     for (int q = 0; q < kPieces; q++) {
-      const int piece = thread + q * WAVES * 64;
-      const int64_t row = r + piece / (COUNT / 16);
-      const int col = j0 + piece % (COUNT / 16) * 16;
-      held[q] = u32x4{0, 0, 0, 0};
-      s[q] = 1.0f;
-      lo[q] = 0.0f;
-      if (row < depth && col < ld) {
-        held[q] = *(const u32x4*)(codes + row * ld + col);
-        const int64_t g = row * groups + col / kGroup;
-        if (col / kGroup < groups) {
-          s[q] = scale[g];
-          lo[q] = mn[g];
-        }
-      }
+      held[q] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(c, (int)(at + q * apart), 0, 0));
+      s[q] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(f, (int)(stat_at + q * stat_apart), 0, 0));
+      lo[q] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(m, (int)(stat_at + q * stat_apart), 0, 0));
     }
-    r += Mma<T>::kStep;
+    codes.advance(step);
+    scale.advance(stat_step);
+    mn.advance(stat_step);
+    left -= Mma<T>::kStep;
   }
   __device__ __forceinline__ void put(lds_u8* tile) {
 #pragma unroll
     for (int q = 0; q < kPieces; q++) {
-      const int piece = thread + q * WAVES * 64;
-      const uint32_t row = piece / (COUNT / 16), block = piece % (COUNT / 16);
-      const float inv = 1.0f / s[q];
+      const uint32_t row = thread / kAcross + q * kApart, block = thread % kAcross;
+      const float inv = (int)row < held_left ? 1.0f / s[q] : 0.0f;      // rows behind the last one: zeros
       lds_u8* to = tile + row * (COUNT * (int)sizeof(T)) + (block ^ Mma<T>::block_turn(row)) * Mma<T>::kBlock;
       if constexpr (sizeof(T) == 2) {
         typedef T T8 __attribute__((ext_vector_type(8)));
@@ -740,205 +770,340 @@ struct TileRead {
   }
 };
 
-// Workgroups go to the 8 XCDs in turn: each XCD gets a run of consecutive tiles, and a run walks down `kTall` tile rows before it
-// moves to the next tile column, so that the tiles that an XCD works on at a time share rows of A and B in its L2.
+// Workgroups go to the 8 XCDs in turn: each XCD has a run of consecutive tiles, which its workgroups take side by side, and a run walks
+// down `kTall` tile rows before it moves to the next tile column, so that the tiles that an XCD works on at a time share rows of A and
+// B in its L2.
 constexpr int kTall = 8;
-__device__ __forceinline__ void tile_of(uint32_t b, const ProductArgs& p, int& ti, int& tj, int& split) {
-  const uint32_t nb = gridDim.x, even = nb / 8, more = nb % 8, xcd = b % 8, k = b / 8;
-  uint32_t t = xcd * even + (xcd < more ? xcd : more) + k;
+struct Tile {
+  int i, j, split;
+};
+__device__ __forceinline__ bool tile_of(const ProductArgs& p, int turn, Tile& t) {
+  const uint32_t total = (uint32_t)p.tiles_i * p.tiles_j * p.splits, xcd = blockIdx.x % 8;
+  const uint32_t mine = total / 8 + (xcd < total % 8), beside = gridDim.x / 8 + (xcd < gridDim.x % 8);
+  const uint32_t k = blockIdx.x / 8 + turn * beside;
+  if (k >= mine) return false;
+  uint32_t at = xcd * (total / 8) + (xcd < total % 8 ? xcd : total % 8) + k;
   const uint32_t tiles = p.tiles_i * p.tiles_j;
-  split = t / tiles;
-  t -= split * tiles;
-  const uint32_t band = kTall * p.tiles_j, which = t / band, in = t - which * band;
+  t.split = at / tiles;
+  at -= t.split * tiles;
+  const uint32_t band = kTall * p.tiles_j, which = at / band, in = at - which * band;
   const uint32_t tall = (uint32_t)p.tiles_i - which * kTall < kTall ? p.tiles_i - which * kTall : kTall;
-  ti = which * kTall + in % tall;
-  tj = in / tall;
+  t.i = which * kTall + in % tall;
+  t.j = in / tall;
+  return true;
+}
+
+// A lane holds four consecutive columns of blocks n and n + 1 of a row; lanes 16 apart the columns beside them.  Afterwards it holds eight
+// consecutive columns of block n + (g & 1), from column 8 (g >> 1) on, g = lane / 16.  The same again undoes it.
+__device__ __forceinline__ void swap_rows16(uint32_t& a, uint32_t& b) {
+#ifdef __HIP_DEVICE_COMPILE__
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+#endif
+}
+__device__ __forceinline__ void swap_rows32(uint32_t& a, uint32_t& b) {
+#ifdef __HIP_DEVICE_COMPILE__
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+#endif
+}
+template <typename T>
+__device__ __forceinline__ u32x2 rounded4(f32x4 v) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 o;
+#pragma unroll
+  for (int e = 0; e < 4; e++) o[e] = (T)v[e];
+  return __builtin_bit_cast(u32x2, o);
+}
+template <typename T>
+__device__ __forceinline__ f32x4 widened4(uint32_t a, uint32_t b) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  const T4 o = __builtin_bit_cast(T4, u32x2{a, b});
+  return f32x4{(float)o[0], (float)o[1], (float)o[2], (float)o[3]};
 }
 
 enum { B_ROWS = 0, B_STRIDED = 1, B_CODES = 2 };
 
-template <typename T, int BM, int BN, int WI, int WJ, bool A_STRIDED, int B_KIND>
+template <typename T, int BM, int BN, int WI, int WJ, bool A_STRIDED, int B_KIND, int ACT, bool CODES>
 __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
-  constexpr int WAVES = WI * WJ, MI = BM / WI / 16, NJ = BN / WJ / 16;
-  constexpr int KK = 2;      // fragments along r of a step
+  constexpr int WAVES = WI * WJ, MI = BM / WI / 16, MH = MI / 2, NJ = BN / WJ / 16;
   constexpr bool FORWARD = B_KIND == B_ROWS;
-  __shared__ __attribute__((aligned(1024))) uint8_t memory[2 * (BM + BN) * 128];
-  lds_u8* lds = (lds_u8*)memory;
+  using Frag = typename Mma<T>::Frag;
+  // two objects, so that the compiler can tell a read of one from the loads that fill the other and does not wait for those
+  __shared__ __attribute__((aligned(1024))) uint8_t even[(BM + BN) * 128];
+  __shared__ __attribute__((aligned(1024))) uint8_t odd[(BM + BN) * 128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
-  int ti, tj, split;
-  tile_of(blockIdx.x, p, ti, tj, split);
-  const int i0 = ti * BM, j0 = tj * BN;
-  const int64_t r0 = split * p.per_split, end = r0 + p.per_split < p.depth ? r0 + p.per_split : p.depth;
-  const int steps = (int)((end - r0 + Mma<T>::kStep - 1) / Mma<T>::kStep);
+  int steps;
 
   TileLoad<T, BM, A_STRIDED, WAVES> a;
-  a.start(p.a, p.lda, i0, p.rows, end, r0, wave, lane);
   std::conditional_t<B_KIND == B_CODES, CodeLoad<T, BN, WAVES>, TileLoad<T, BN, B_KIND == B_STRIDED, WAVES>> b;
-  if constexpr (B_KIND == B_CODES)
-    b.start(p, j0, r0, end, threadIdx.x);
-  else
-    b.start(p.b, p.ldb, j0, p.cols, end, r0, wave, lane);
+  auto fill = [&](lds_u8* tile) __attribute__((always_inline)) {
+    a.issue(tile);
+    if constexpr (B_KIND == B_CODES) {
+      b.put(tile + BM * 128);
+      b.fetch();
+    } else {
+      b.issue(tile + BM * 128);
+    }
+  };
+  // the tile's bias, asked for ahead of the tiles (a load waits for those before it) and put into LDS when the tile begins
+  __shared__ float biases[2][FORWARD ? BN : 1];
+  float own_bias = 0.0f;
+  auto begin = [&](const Tile& tile) __attribute__((always_inline)) {
+    if constexpr (FORWARD) {
+      const int j = tile.j * BN + (int)threadIdx.x;
+      own_bias = 0.0f;
+      if (p.bias && threadIdx.x < BN && j < p.cols) own_bias = (float)((const T*)p.bias)[j];
+    }
+    const int64_t r0 = tile.split * p.per_split, end = r0 + p.per_split < p.depth ? r0 + p.per_split : p.depth;
+    steps = (int)((end - r0 + Mma<T>::kStep - 1) / Mma<T>::kStep);
+    a.start(p.a, p.lda, tile.i * BM, p.rows, end, r0, wave, lane);
+    if constexpr (B_KIND == B_CODES) {
+      b.start(p, tile.j * BN, r0, end, threadIdx.x);
+      b.fetch();
+    } else {
+      b.start(p.b, p.ldb, tile.j * BN, p.cols, end, r0, wave, lane);
+    }
+    fill((lds_u8*)even);
+    if (steps > 1) fill((lds_u8*)odd);
+  };
 
   f32x4 acc[MI][NJ];
+  // s_waitcnt's operands: for the loads, and for all but the newest stores of a tile
+  constexpr int kStores = MI * NJ / (sizeof(T) == 2 ? 2 : 1);
+  constexpr int kLoads = 15 << 8 | 7 << 4, kBehindStores = (kStores & 15) | (kStores >> 4) << 14 | kLoads;
+  static_assert(kStores < 64, "s_waitcnt counts to 63");
+  auto meet = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  };
+  // A step is four phases: (first, second half of the fragments along r) x (upper, lower half of the wave's rows).  Each phase
+  // multiplies what was read from LDS in the phase before and reads for the next; B's fragments are replaced one by one as soon as their
+  // last product is under way, which leaves the registers to the sums.  After the third phase nothing is left to read of
+  // the present tiles: once every wave is there and the next tiles have arrived, the present ones' memory takes those after the next.
+  Frag fa[2][MH], fb[NJ];
+  auto read_a = [&](const lds_u8* tile, int kk, int half, Frag (&f)[MH]) __attribute__((always_inline)) {
 #pragma unroll
-  for (int m = 0; m < MI; m++)
+    for (int m = 0; m < MH; m++) f[m] = TileRead<T, BM, A_STRIDED>::get(tile, wi * (BM / WI) + (half * MH + m) * 16, kk, lane);
+  };
+  auto read_b = [&](const lds_u8* tile, int kk, int n) __attribute__((always_inline)) {
+    fb[n] = TileRead<T, BN, B_KIND != B_ROWS>::get(tile + BM * 128, wj * (BN / WJ) + n * 16, kk, lane);
+  };
+  auto multiply = [&](const Frag (&x)[MH], int half, int n) __attribute__((always_inline)) {
 #pragma unroll
-    for (int n = 0; n < NJ; n++) acc[m][n] = f32x4{0, 0, 0, 0};
-
-  constexpr int BUF = (BM + BN) * 128;
-  a.issue(lds);
-  if constexpr (B_KIND == B_CODES) {
-    b.fetch();
-    b.put(lds + BM * 128);
-    b.fetch();
-  } else {
-    b.issue(lds + BM * 128);
-  }
-  for (int t = 0; t < steps; t++) {
-    __builtin_amdgcn_s_waitcnt(0);      // this step's tiles are there, for all waves
-    __syncthreads();
-    lds_u8* now = lds + (t & 1) * BUF;
-    lds_u8* next = lds + ((t + 1) & 1) * BUF;
-    if (t + 1 < steps) {
-      a.issue(next);
-      if constexpr (B_KIND == B_CODES) {
-        b.put(next + BM * 128);
-        b.fetch();
-      } else {
-        b.issue(next + BM * 128);
-      }
-    }
+    for (int m = 0; m < MH; m++) acc[half * MH + m][n] = Mma<T>::run(fb[n], x[m], acc[half * MH + m][n]);
+  };
+  auto step = [&](lds_u8* now, lds_u8* next, int t) __attribute__((always_inline)) {
+    read_a(now, 0, 1, fa[1]);
 #pragma unroll
-    for (int kk = 0; kk < KK; kk++) {
-      typename Mma<T>::Frag fa[MI], fb[NJ];
-#pragma unroll
-      for (int m = 0; m < MI; m++) fa[m] = TileRead<T, BM, A_STRIDED>::get(now, wi * (BM / WI) + m * 16, kk, lane);
-#pragma unroll
-      for (int n = 0; n < NJ; n++) fb[n] = TileRead<T, BN, B_KIND != B_ROWS>::get(now + BM * 128, wj * (BN / WJ) + n * 16, kk, lane);
-#pragma unroll
-      for (int m = 0; m < MI; m++)
-#pragma unroll
-        for (int n = 0; n < NJ; n++) acc[m][n] = Mma<T>::run(fb[n], fa[m], acc[m][n]);
-    }
-  }
-
-  const int i_lane = i0 + wi * (BM / WI) + (lane & 15);
-  const int j_lane = j0 + wj * (BN / WJ) + (lane >> 4) * 4;
-  if constexpr (FORWARD) {
-    const T* bias = (const T*)p.bias;
+    for (int n = 0; n < NJ; n++) multiply(fa[0], 0, n);
+    __builtin_amdgcn_sched_barrier(0);
+    read_a(now, 1, 0, fa[0]);
 #pragma unroll
     for (int n = 0; n < NJ; n++) {
-      const int j = j_lane + n * 16;
-      f32x4 v = {0, 0, 0, 0};
-      if (bias)
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = j + e < p.cols ? (float)bias[j + e] : 0.0f;
-#pragma unroll
-      for (int m = 0; m < MI; m++) acc[m][n] += v;
+      multiply(fa[1], 1, n);
+      read_b(now, 1, n);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (BN == kGroup) {
-      if (p.codes) {
-        // a tile's row is one group: least and most of the wave's columns, then over the waves side by side
-        __shared__ float ends[2][WJ][BM];
+    read_a(now, 1, 1, fa[1]);
+#pragma unroll
+    for (int n = 0; n < NJ; n++) multiply(fa[0], 0, n);
+    __builtin_amdgcn_sched_barrier(0);
+    if (t > 0) __builtin_amdgcn_s_waitcnt(kLoads);      // a tile's first two steps were waited for before it began
+    meet();
+    // behind a tile's last step these read what is there and nobody uses it
+    read_a(next, 0, 0, fa[0]);
+    if (t + 2 < steps) fill(now);
+#pragma unroll
+    for (int n = 0; n < NJ; n++) {
+      multiply(fa[1], 1, n);
+      read_b(next, 0, n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  lds_u8* const first = (lds_u8*)even;
+  lds_u8* const second = (lds_u8*)odd;
+
+  // A workgroup takes tile after tile.  The next one's first two steps are asked for before the present one's results are stored, and
+  // the stores of a whole tile go on while the next one is multiplied.
+  Tile tile;
+  if (!tile_of(p, 0, tile)) return;
+  begin(tile);
+  __builtin_amdgcn_s_waitcnt(kLoads);
+  for (int turn = 1;; turn++) {
+    if (FORWARD && threadIdx.x < BN) biases[turn & 1][threadIdx.x] = own_bias;
+    meet();
+#pragma unroll
+    for (int m = 0; m < MI; m++)
+#pragma unroll
+      for (int n = 0; n < NJ; n++) acc[m][n] = f32x4{0, 0, 0, 0};
+    read_a(first, 0, 0, fa[0]);
+#pragma unroll
+    for (int n = 0; n < NJ; n++) read_b(first, 0, n);
+    for (int t = 0; t < steps; t += 2) {
+      step(first, second, t);
+      if (t + 1 < steps) step(second, first, t + 1);
+    }
+    const Tile done = tile;
+    const bool more = tile_of(p, turn, tile);
+    if (more) begin(tile);
+    __builtin_amdgcn_sched_barrier(0);
+
+    const int i0 = done.i * BM, j0 = done.j * BN;
+    int l = lane;       // the addresses below are made here, not before the loop, where they would take registers from it
+    asm volatile("" : "+v"(l));
+    const int i_lane = i0 + wi * (BM / WI) + (l & 15);
+    const int j_wave = j0 + wj * (BN / WJ);
+    const int j_lane = j_wave + (l >> 4) * 4;
+    const bool whole = i0 + BM <= p.rows && j0 + BN <= p.cols;
+    if constexpr (FORWARD) {
+#pragma unroll
+      for (int n = 0; n < NJ; n++) {
+        const f32x4 v = *(const f32x4*)&biases[turn & 1][wj * (BN / WJ) + n * 16 + (l >> 4) * 4];
+#pragma unroll
+        for (int m = 0; m < MI; m++) acc[m][n] += v;
+      }
+      if constexpr (CODES) {
+        static_assert(BN == kGroup, "a tile's row is one group");
+        {
+          // a tile's row is one group: least and most of the wave's columns, then over the waves side by side; one thread per row
+          // makes the scale
+          __shared__ float ends[2][WJ][BM];
+          __shared__ f32x2 ready[BM];
+#pragma unroll
+          for (int m = 0; m < MI; m++) {
+            float lo = __builtin_inff(), hi = -__builtin_inff();
+#pragma unroll
+            for (int n = 0; n < NJ; n++)
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                if (whole || j_lane + n * 16 + e < p.cols) lo = __builtin_fminf(lo, acc[m][n][e]), hi = __builtin_fmaxf(hi, acc[m][n][e]);
+            lo = __builtin_fminf(lo, __shfl_xor(lo, 16));
+            hi = __builtin_fmaxf(hi, __shfl_xor(hi, 16));
+            lo = __builtin_fminf(lo, __shfl_xor(lo, 32));
+            hi = __builtin_fmaxf(hi, __shfl_xor(hi, 32));
+            if (l < 16) {
+              const int at = wi * (BM / WI) + m * 16 + l;
+              ends[0][wj][at] = lo;
+              ends[1][wj][at] = hi;
+            }
+          }
+          meet();
+          if (threadIdx.x < BM) {
+            const int at = threadIdx.x;
+            float lo = ends[0][0][at], hi = ends[1][0][at];
+#pragma unroll
+            for (int w = 1; w < WJ; w++) lo = __builtin_fminf(lo, ends[0][w][at]), hi = __builtin_fmaxf(hi, ends[1][w][at]);
+            const float s = scale_of(lo, hi);
+            ready[at] = f32x2{s, lo};
+            if (i0 + at < p.rows) {
+              const int64_t g = (int64_t)(i0 + at) * p.tiles_j + done.j;
+              p.scale[g] = s;
+              p.mn[g] = lo;
+            }
+          }
+          meet();
+#pragma unroll
+          for (int m = 0; m < MI; m++) {
+            const int at = wi * (BM / WI) + m * 16 + (l & 15);
+            const f32x2 r = ready[at];
+            uint32_t c[NJ];
+#pragma unroll
+            for (int n = 0; n < NJ; n++) c[n] = four_codes(acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3], r[1], r[0]);
+            uint8_t* out = p.codes + (int64_t)(i0 + at) * p.ldc;
+            if (whole) {
+              static_assert(NJ == 4, "16 bytes of a lane are four blocks' codes");
+              swap_rows16(c[0], c[1]);
+              swap_rows16(c[2], c[3]);
+              swap_rows32(c[0], c[2]);
+              swap_rows32(c[1], c[3]);
+              *(u32x4*)(out + j_wave + (l >> 4) * 16) = u32x4{c[0], c[1], c[2], c[3]};
+            } else if (i0 + at < p.rows) {
+#pragma unroll
+              for (int n = 0; n < NJ; n++)
+                if (j_lane + n * 16 < p.cols) *(uint32_t*)(out + j_lane + n * 16) = c[n];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    }
+    const bool partial = !FORWARD && p.splits > 1;
+    {
+      if (partial || (p.wide && sizeof(T) == 4)) {      // 16 bytes are the four columns that a lane holds
 #pragma unroll
         for (int m = 0; m < MI; m++) {
-          float lo = __builtin_inff(), hi = -__builtin_inff();
+          const int64_t i = i_lane + m * 16;
+          float* out = (float*)p.out + (partial ? (int64_t)done.split * p.rows + i : i) * p.ldo + j_lane;
+          const float* residual = FORWARD && p.residual ? (const float*)p.residual + i * p.ldr + j_lane : nullptr;
 #pragma unroll
           for (int n = 0; n < NJ; n++)
+            if (whole || (i < p.rows && j_lane + n * 16 < p.cols)) {
+              f32x4 v = activated4<T, ACT>(acc[m][n]);
+              if (FORWARD && residual) v += *(const f32x4*)(residual + n * 16);
+              *(f32x4*)(out + n * 16) = v;
+            }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else if (p.wide) {
+        if constexpr (sizeof(T) == 2) {
+          const int j_eight = j_wave + ((l >> 4) & 1) * 16 + (l >> 5) * 8;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              if (j_lane + n * 16 + e < p.cols) lo = __builtin_fminf(lo, acc[m][n][e]), hi = __builtin_fmaxf(hi, acc[m][n][e]);
-          lo = __builtin_fminf(lo, __shfl_xor(lo, 16));
-          hi = __builtin_fmaxf(hi, __shfl_xor(hi, 16));
-          lo = __builtin_fminf(lo, __shfl_xor(lo, 32));
-          hi = __builtin_fmaxf(hi, __shfl_xor(hi, 32));
-          if (lane < 16) {
-            const int at = wi * (BM / WI) + m * 16 + lane;
-            ends[0][wj][at] = lo;
-            ends[1][wj][at] = hi;
+          for (int m = 0; m < MI; m++) {
+            const int64_t i = i_lane + m * 16;
+            T* out = (T*)p.out + i * p.ldo + j_eight;
+            const T* residual = FORWARD && p.residual ? (const T*)p.residual + i * p.ldr + j_eight : nullptr;
+#pragma unroll
+            for (int n = 0; n < NJ; n += 2) {
+              const bool there = whole || (i < p.rows && j_eight + n * 16 < p.cols);
+              f32x4 v0 = activated4<T, ACT>(acc[m][n]), v1 = activated4<T, ACT>(acc[m][n + 1]);
+              if (FORWARD && residual) {
+                u32x4 r = {0, 0, 0, 0};
+                if (there) r = *(const u32x4*)(residual + n * 16);
+                uint32_t r0 = r[0], r1 = r[1], r2 = r[2], r3 = r[3];
+                swap_rows16(r0, r2);
+                swap_rows16(r1, r3);
+                v0 += widened4<T>(r0, r1);
+                v1 += widened4<T>(r2, r3);
+              }
+              const u32x2 a0 = rounded4<T>(v0), a1 = rounded4<T>(v1);
+              uint32_t r0 = a0[0], r1 = a0[1], r2 = a1[0], r3 = a1[1];
+              swap_rows16(r0, r2);
+              swap_rows16(r1, r3);
+              if (there) *(u32x4*)(out + n * 16) = u32x4{r0, r1, r2, r3};
+            }
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
-        __syncthreads();
-        const int groups = p.tiles_j;
+      } else {
 #pragma unroll
         for (int m = 0; m < MI; m++) {
-          const int at = wi * (BM / WI) + m * 16 + (lane & 15), i = i0 + at;
-          float lo = ends[0][0][at], hi = ends[1][0][at];
+          const int64_t i = i_lane + m * 16;
+          if (i >= p.rows) continue;
 #pragma unroll
-          for (int w = 1; w < WJ; w++) lo = __builtin_fminf(lo, ends[0][w][at]), hi = __builtin_fmaxf(hi, ends[1][w][at]);
-          const float s = scale_of(lo, hi);
-          if (i < p.rows) {
-            if (wj == 0 && lane < 16) {
-              p.scale[(int64_t)i * groups + tj] = s;
-              p.mn[(int64_t)i * groups + tj] = lo;
-            }
+          for (int n = 0; n < NJ; n++) {
+            const f32x4 v = activated4<T, ACT>(acc[m][n]);
 #pragma unroll
-            for (int n = 0; n < NJ; n++) {
-              const int j = j_lane + n * 16;
-              if (j < p.cols)
-                *(uint32_t*)(p.codes + i * p.ldc + j) = four_codes(acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3], lo, s);
+            for (int e = 0; e < 4; e++) {
+              const int j = j_lane + n * 16 + e;
+              if (j >= p.cols) continue;
+              ((T*)p.out)[i * p.ldo + j] = (T)(FORWARD && p.residual ? v[e] + (float)((const T*)p.residual)[i * p.ldr + j] : v[e]);
             }
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
-#pragma unroll
-    for (int m = 0; m < MI; m++) {
-      const int64_t i = i_lane + m * 16;
-      if (i >= p.rows) continue;
-      T* out = (T*)p.out + i * p.ldo;
-      const T* residual = p.residual ? (const T*)p.residual + i * p.ldr : nullptr;
-#pragma unroll
-      for (int n = 0; n < NJ; n++) {
-        const int j = j_lane + n * 16;
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        f32x4 v = acc[m][n];
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = activated(v[e], p.act);
-        if (p.wide) {
-          if (j < p.cols) {
-            if (residual) {
-              const T4 r = *(const T4*)(residual + j);
-#pragma unroll
-              for (int e = 0; e < 4; e++) v[e] += (float)r[e];
-            }
-            T4 o;
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = (T)v[e];
-            *(T4*)(out + j) = o;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (j + e < p.cols) out[j + e] = (T)(residual ? v[e] + (float)residual[j + e] : v[e]);
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int m = 0; m < MI; m++) {
-      const int64_t i = i_lane + m * 16;
-      if (i >= p.rows) continue;
-#pragma unroll
-      for (int n = 0; n < NJ; n++) {
-        const int j = j_lane + n * 16;
-        if (p.splits > 1) {     // partial sums, in float
-          float* out = (float*)p.out + ((int64_t)split * p.rows + i) * p.ldo;
-          if (j < p.cols) *(f32x4*)(out + j) = acc[m][n];
-        } else if (p.wide) {
-          typedef T T4 __attribute__((ext_vector_type(4)));
-          T4 o;
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[e] = (T)acc[m][n][e];
-          if (j < p.cols) *(T4*)((T*)p.out + i * p.ldo + j) = o;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (j + e < p.cols) ((T*)p.out)[i * p.ldo + j + e] = (T)acc[m][n][e];
-        }
-      }
-    }
+    if (!more) return;
+    // the next tile's first loads are older than this tile's stores, every one of which every wave has made of a whole tile
+    if (whole && (partial || p.wide))
+      __builtin_amdgcn_s_waitcnt(kBehindStores);
+    else
+      __builtin_amdgcn_s_waitcnt(kLoads);
   }
 }
 
@@ -1022,7 +1187,7 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(ProductArgs p) {
       const int c = j0 + g * 4 + e;
       if (c >= p.cols) continue;
       float o = v[e] + (p.bias ? (float)((const T*)p.bias)[c] : 0.0f);
-      o = activated(o, p.act);
+      o = activated<std::is_same<T, float>::value>(o, p.act);
       if (p.residual) o += (float)((const T*)p.residual)[row * p.ldr + c];
       ((T*)p.out)[row * p.ldo + c] = (T)o;
     }
@@ -1095,27 +1260,50 @@ struct Tiles {
 };
 constexpr int kComputeUnits = 256;
 
-template <typename T, int BM, int BN, int WI, int WJ, bool AS, int BK>
+template <typename T, int BM, int BN, int WI, int WJ, bool AS, int BK, int ACT = ACT_NONE, bool CODES = false>
 int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s) {
   p.tiles_i = (p.rows + BM - 1) / BM;
   p.tiles_j = (p.cols + BN - 1) / BN;
   p.splits = splits;
   p.per_split = per_split;
-  const int64_t blocks = (int64_t)p.tiles_i * p.tiles_j * splits;
-  if (!blocks_fit(blocks)) return GACT_ELIMIT;
-  auto kernel = product_kernel<T, BM, BN, WI, WJ, AS, BK>;
+  const int64_t tiles = (int64_t)p.tiles_i * p.tiles_j * splits;
+  if (!blocks_fit(tiles)) return GACT_ELIMIT;
+  constexpr int kSlots = kComputeUnits * (BM * BN <= 128 * 128 ? 2 : 1);      // workgroups that the card holds at a time
+  const int64_t blocks = tiles < kSlots ? tiles : kSlots;
+  auto kernel = product_kernel<T, BM, BN, WI, WJ, AS, BK, ACT, CODES>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(WI * WJ * 64), 0, s, p);
   return launch_status();
+}
+
+template <typename T, int ACT>
+int forward_product(ProductArgs& p, hipStream_t s) {
+  const int64_t step = 128 / (int)sizeof(T), depth = (p.depth + step - 1) / step * step;
+  const bool large = sizeof(T) == 2 && (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256) >= kComputeUnits;
+  // the pre-activation's codes need a whole group of columns in a tile; without an activation nobody asks for them
+  if constexpr (ACT != ACT_NONE) {
+    if (p.codes) {
+      if constexpr (sizeof(T) == 2)
+        if (large) return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
+      return launch_product<T, 128, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
+    }
+  }
+  if constexpr (sizeof(T) == 2)
+    if (large) return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT>(p, 1, depth, s);
+  return launch_product<T, 128, 128, 2, 2, false, B_ROWS, ACT>(p, 1, depth, s);
 }
 
 // how a backward product is cut: the tile, and the parts of its depth where the tiles alone leave compute units idle
 inline Tiles tiles_of(int dtype, int64_t rows, int64_t cols, int64_t depth) {
   Tiles t = {128, 128, 1, 0};
   const int64_t step = 128 / size_of(dtype);
-  if (dtype != GACT_F32 && ((rows + 255) / 256) * ((cols + 255) / 256) >= kComputeUnits) t.bm = t.bn = 256;
+  int64_t slots = 2 * kComputeUnits;
+  if (dtype != GACT_F32 && ((rows + 255) / 256) * ((cols + 255) / 256) >= kComputeUnits / 4) {
+    t.bm = t.bn = 256;
+    slots = kComputeUnits;
+  }
   const int64_t tiles = ((rows + t.bm - 1) / t.bm) * ((cols + t.bn - 1) / t.bn);
   const int64_t steps = (depth + step - 1) / step;
-  int64_t splits = tiles >= 2 * kComputeUnits ? 1 : 2 * kComputeUnits / tiles;
+  int64_t splits = tiles >= slots ? 1 : slots / tiles;
   if (splits > steps / 8) splits = steps / 8;
   if (splits > 64) splits = 64;
   if (splits < 1) splits = 1;
@@ -1273,7 +1461,7 @@ int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
                 float* mn, void* stream) {
   if (!known(dtype) || !layer_sizes(rows, inner, outer) || activation < GACT_ACT_NONE || activation > GACT_ACT_SILU) return GACT_EINVAL;
   if (rows == 0) return GACT_OK;
-  if (!x || !weight || !y || (codes && (!scale || !mn)) || (residual && ldr < outer && rows > 1)) return GACT_EINVAL;
+  if (!x || !weight || !y || (codes && (!scale || !mn || activation == GACT_ACT_NONE)) || (residual && ldr < outer && rows > 1)) return GACT_EINVAL;
   if (codes && !codes_fit(codes, outer, ldc)) return GACT_EALIGN;
   const bool few = !codes && rows <= GACT_LINEAR_FEW_ROWS;
   const bool whole = operand_fits(x, ldx, dtype, inner) && operand_fits(weight, ldw, dtype, inner);
@@ -1296,8 +1484,7 @@ int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
   p.ldc = ldc;
   p.scale = scale;
   p.mn = mn;
-  const int four = 4 * size_of(dtype);
-  p.wide = outer % 4 == 0 && (uintptr_t)y % four == 0 && (!residual || ((uintptr_t)residual % four == 0 && ldr % 4 == 0));
+  p.wide = whole_rows(y, dtype, outer, outer) && (!residual || whole_rows(residual, dtype, outer, ldr));
   fresh_launch();
   hipStream_t s = (hipStream_t)stream;
   return with_type(dtype, [&](auto zero) -> int {
@@ -1314,12 +1501,12 @@ int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
       if (rows <= 32) return run(integral_constant<int, 2>{}, integral_constant<int, 8>{});
       return run(integral_constant<int, 4>{}, integral_constant<int, 8>{});
     }
-    const int64_t step = 128 / (int)sizeof(T), depth = (inner + step - 1) / step * step;
-    if constexpr (sizeof(T) == 2)
-      if (((rows + 255) / 256) * ((outer + 255) / 256) >= kComputeUnits)
-        return launch_product<T, 256, 256, 2, 4, false, B_ROWS>(p, 1, depth, s);
-    if (codes) return launch_product<T, 128, 256, 2, 4, false, B_ROWS>(p, 1, depth, s);
-    return launch_product<T, 128, 128, 2, 2, false, B_ROWS>(p, 1, depth, s);
+    switch (activation) {
+      case GACT_ACT_GELU: return forward_product<T, ACT_GELU>(p, s);
+      case GACT_ACT_GELU_TANH: return forward_product<T, ACT_GELU_TANH>(p, s);
+      case GACT_ACT_SILU: return forward_product<T, ACT_SILU>(p, s);
+      default: return forward_product<T, ACT_NONE>(p, s);
+    }
   });
 }
 
@@ -1373,7 +1560,7 @@ int gact_product(const void* a, int64_t lda, const void* b, int64_t ldb, int dty
   p.depth = depth;
   p.out = out;
   p.ldo = cols;
-  p.wide = cols % 4 == 0 && (uintptr_t)out % (4 * size_of(dtype)) == 0;
+  p.wide = whole_rows(out, dtype, cols, cols);
   fresh_launch();
   return with_type(dtype, [&](auto zero) { return backward_product<decltype(zero), false, B_STRIDED>(p, dtype, workspace, (hipStream_t)stream); });
 }
@@ -1397,7 +1584,7 @@ int gact_checkpoint_product(const void* grad, int64_t ldg, const void* codes, in
   p.b_scale = scale;
   p.b_min = mn;
   p.b_groups = (int)((inner + kGroup - 1) / kGroup);
-  p.wide = inner % 4 == 0 && (uintptr_t)out % (4 * size_of(dtype)) == 0;
+  p.wide = whole_rows(out, dtype, inner, inner);
   fresh_launch();
   return with_type(dtype, [&](auto zero) { return backward_product<decltype(zero), true, B_CODES>(p, dtype, workspace, (hipStream_t)stream); });
 }

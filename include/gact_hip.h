@@ -260,7 +260,7 @@ int gact_norm_backward(const void* dy, int64_t lddy, const void* weight, const v
                        float* workspace, void* stream);
 
 /* y [rows, outer] = act(x [rows, inner] weight [outer, inner]^T + bias) + residual, y contiguous; bias and residual may be null.  With
- * `codes`: also the checkpoint of z = x weight^T + bias.  x and weight: 16-byte aligned rows of whole 16-byte pieces (else
+ * `codes` (and an activation): also the checkpoint of z = x weight^T + bias.  x and weight: 16-byte aligned rows of whole 16-byte pieces (else
  * GACT_EALIGN), except for up to GACT_LINEAR_FEW_ROWS rows without codes. */
 int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
                 int activation, int dtype, int64_t rows, int64_t inner, int64_t outer, void* y, void* codes, int64_t ldc, float* scale,
