@@ -23,6 +23,8 @@ HDR = os.path.join(ROOT, "include", "gact_hip.h")
 OUT_DIR = os.path.join(HERE, "gact", "lib")
 OUT = os.path.join(OUT_DIR, "libgact_hip.so")
 TORCH_SRC = os.path.join(HERE, "csrc", "torch_ops.cpp")
+TORCH_LAYERS_SRC = os.path.join(HERE, "csrc", "torch_layers.cpp")
+TORCH_HDR = os.path.join(HERE, "csrc", "torch_layers.h")
 TORCH_OUT = os.path.join(OUT_DIR, "gact_torch.so")
 PROBE_OUT = os.path.join(OUT_DIR, "libgact_probe.so")
 
@@ -60,7 +62,7 @@ def up_to_date():
         if torch_mark() not in f.read():     # built for another torch
             return False
     t = min(os.path.getmtime(p) for p in built)
-    return all(os.path.getmtime(p) <= t for p in (SRC, LAYERS_SRC, PROBE_SRC, TORCH_SRC, HDR, os.path.abspath(__file__)))
+    return all(os.path.getmtime(p) <= t for p in (SRC, LAYERS_SRC, PROBE_SRC, TORCH_SRC, TORCH_LAYERS_SRC, TORCH_HDR, HDR, os.path.abspath(__file__)))
 
 
 def torch_mark():
@@ -84,7 +86,7 @@ def torch_command():
     for path in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", path]
     # libtorch.so itself stays out: it would pull in every library torch was built with
-    return cmd + ["-o", TORCH_OUT, TORCH_SRC, "-L", OUT_DIR, "-l:libgact_hip.so", "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10",
+    return cmd + ["-o", TORCH_OUT, TORCH_SRC, TORCH_LAYERS_SRC, "-L", OUT_DIR, "-l:libgact_hip.so", "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10",
                   "-lc10_hip", "-Wl,-rpath,$ORIGIN"]
 
 

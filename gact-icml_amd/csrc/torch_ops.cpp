@@ -31,6 +31,7 @@
 #include <vector>
 
 #include "gact_hip.h"
+#include "torch_layers.h"
 
 namespace {
 
@@ -551,10 +552,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "gact_torch", "The operators' host 
 
 }  // namespace
 
+bool gact_torch_ordinary() { return ordinary_call(); }
+at::Tensor gact_torch_empty(c10::IntArrayRef shape, at::ScalarType dtype, c10::Device device) { return make(shape, dtype, device); }
+
 PyMODINIT_FUNC PyInit_gact_torch(void) {
   static const char built_with[] = "torch " GACT_TORCH_VERSION;   // the build looks for it in the library
   PyObject* const m = PyModule_Create(&module);
-  if (m && PyModule_AddStringConstant(m, "torch_version", built_with + 6) < 0) {
+  if (m && (PyModule_AddStringConstant(m, "torch_version", built_with + 6) < 0 || PyModule_AddFunctions(m, gact_layer_methods) < 0)) {
     Py_DECREF(m);
     return nullptr;
   }
