@@ -61,25 +61,39 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[kVec]) {
     *(T8*)p = a;
   }
 }
-// the same of a row of which `n` columns are left; WHOLE: n is 0 or at least 8 and the address a multiple of 16 bytes
+// the same of a row of which `n` columns are left; WHOLE: n is 0 or at least 8 and the address a multiple of 16 bytes.  Otherwise whole
+// pieces are still one access, at whatever address (value by value a layer norm of 771 halves takes twice as long).
+template <typename T>
+struct Loose {
+  typedef T Eight __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
 template <typename T, bool WHOLE>
-__device__ __forceinline__ void load_cols(const T* p, int64_t n, float (&v)[kVec], float fill = 0.0f) {
+__device__ __forceinline__ void load_cols(const T* p, int64_t n, float (&v)[kVec]) {
   if (WHOLE) {
     if (n > 0) {
       load8(p, v);
     } else {
 #pragma unroll
-      for (int e = 0; e < kVec; e++) v[e] = fill;
+      for (int e = 0; e < kVec; e++) v[e] = 0.0f;
     }
+  } else if (n >= kVec) {
+    const typename Loose<T>::Eight a = *(const typename Loose<T>::Eight*)p;
+#pragma unroll
+    for (int e = 0; e < kVec; e++) v[e] = (float)a[e];
   } else {
 #pragma unroll
-    for (int e = 0; e < kVec; e++) v[e] = e < n ? (float)p[e] : fill;
+    for (int e = 0; e < kVec; e++) v[e] = e < n ? (float)p[e] : 0.0f;
   }
 }
 template <typename T, bool WHOLE>
 __device__ __forceinline__ void store_cols(T* p, int64_t n, const float (&v)[kVec]) {
   if (WHOLE) {
     if (n > 0) store8(p, v);
+  } else if (n >= kVec) {
+    typename Loose<T>::Eight a;
+#pragma unroll
+    for (int e = 0; e < kVec; e++) a[e] = (T)v[e];
+    *(typename Loose<T>::Eight*)p = a;
   } else {
 #pragma unroll
     for (int e = 0; e < kVec; e++)
@@ -116,6 +130,41 @@ __device__ __forceinline__ float over_lanes(float v) {
 
 // ---- the checkpoint's arithmetic ----
 __device__ __forceinline__ float scale_of(float lo, float hi) { return (float)(255.0 / ((double)(hi - lo) + 2e-6)); }
+// scales of K groups, of which every row of 16 lanes holds the ends: lane k divides for group k, one division for all of them
+template <int LANE>
+__device__ __forceinline__ float row_broadcast(float v) {
+  const int b = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, b, 0x150 + LANE, 0xf, 0xf, false));
+}
+template <int K, int AT = 0>
+__device__ __forceinline__ void broadcast_all(float mine, float (&s)[K]) {
+  if constexpr (AT < K) {
+    s[AT] = row_broadcast<AT>(mine);
+    broadcast_all<K, AT + 1>(mine, s);
+  }
+}
+template <int K>
+__device__ __forceinline__ void scales_of(const float (&lo)[K], const float (&hi)[K], float (&s)[K]) {
+  static_assert(K <= 16, "a row has 16 lanes");
+  float l = lo[0], h = hi[0];
+#pragma unroll
+  for (int k = 1; k < K; k++) {
+    const bool mine = (threadIdx.x & 15) == k;
+    l = mine ? lo[k] : l;
+    h = mine ? hi[k] : h;
+  }
+  const float q = scale_of(l, h);
+  if (K == 1)
+    s[0] = q;
+  else
+    broadcast_all<K>(q, s);
+}
+// 1 / scale: the hardware's reciprocal and one step of Newton's, within a unit in the last place; NaN for a scale of zero (a range that
+// overflowed), which stands for nothing
+__device__ __forceinline__ float inverse_of(float scale) {
+  const float r = __builtin_amdgcn_rcpf(scale);
+  return __builtin_fmaf(__builtin_fmaf(-scale, r, 1.0f), r, r);
+}
 // [0, 255] and rounded to nearest even by the conversion itself; a NaN becomes 0
 __device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d, float lo, float scale) {
   uint32_t w = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(a - lo, scale, 0.5f) - 0.5f, 0, 0);
@@ -238,7 +287,7 @@ __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* __restrict_
   const int col = g * kGroup + lane * kVec, n = cols - col;
   if (n <= 0) return;
   float v[kVec];
-  eight_values(*(const u32x2*)(codes + row * ldc + col), 1.0f / scale[unit], mn[unit], v);
+  eight_values(*(const u32x2*)(codes + row * ldc + col), inverse_of(scale[unit]), mn[unit], v);
   store_cols<T, WHOLE>(out + row * cols + col, n, v);
 }
 
@@ -261,9 +310,9 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const T* __restrict__ x, 
 // of 256 columns is one piece of 32 neighbouring threads (LPR 16: two pieces of 16).  LPR up to 64: 256 / LPR rows per workgroup;
 // above: a workgroup of LPR threads per row.
 // ---------------------------------------------------------------------------------------------------------------------------------
-template <int LPR>
+template <int LPR, int THREADS = 256>
 struct RowShape {
-  static constexpr int kThreads = LPR <= 64 ? 256 : LPR;
+  static constexpr int kThreads = LPR <= 64 ? THREADS : LPR;
   static constexpr int kRows = kThreads / LPR;            // rows at a time
   static constexpr int kWaves = LPR <= 64 ? 1 : LPR / 64;   // waves of a row
   static constexpr int kSpan = LPR * kVec;                // columns of a piece
@@ -284,107 +333,163 @@ __device__ __forceinline__ float row_sum(float v, float* shared, int turn) {
   return v;
 }
 
-template <typename T, int LPR, int NC, bool WHOLE>
+// U consecutive rows at a time: their loads are on the way together, and their scales are one division (see scales_of).
+template <typename T, int LPR, int NC, int U, bool WHOLE>
 __global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_forward_kernel(
-    const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias, int64_t rows, int cols, float eps,
-    T* __restrict__ y, uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale, float* __restrict__ mn,
+    const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias, int64_t rows, int cols, float per_col,
+    float eps, T* __restrict__ y, uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale, float* __restrict__ mn,
     float* __restrict__ stats) {
   using Shape = RowShape<LPR>;
   __shared__ float shared[2 * Shape::kWaves];
   const int lane = threadIdx.x % LPR;
-  const int64_t row = (int64_t)blockIdx.x * Shape::kRows + threadIdx.x / LPR;
-  if (Shape::kRows > 1 && row >= rows) return;
-  float v[NC][kVec];
-  const T* in = x + row * ldx;
+  const int64_t row0 = ((int64_t)blockIdx.x * Shape::kRows + threadIdx.x / LPR) * U;
+  if (Shape::kRows > 1 && row0 >= rows) return;
+  const int there = U == 1 || rows - row0 >= U ? U : (int)(rows - row0);      // of the U rows
+  float v[U][NC][kVec];
 #pragma unroll
-  for (int c = 0; c < NC; c++) {
-    const int col = c * Shape::kSpan + lane * kVec;
-    load_cols<T, WHOLE>(in + col, cols - col, v[c]);
-  }
-  float sum = 0.0f;
+  for (int u = 0; u < U; u++)
 #pragma unroll
-  for (int c = 0; c < NC; c++)
-#pragma unroll
-    for (int e = 0; e < kVec; e++) sum += v[c][e];
-  const float mean = row_sum<LPR>(sum, shared, 0) / (float)cols;
-  sum = 0.0f;
-#pragma unroll
-  for (int c = 0; c < NC; c++) {
-    const int left = cols - (c * Shape::kSpan + lane * kVec);
-#pragma unroll
-    for (int e = 0; e < kVec; e++) {
-      const float d = e < left ? v[c][e] - mean : 0.0f;
-      sum += d * d;
+    for (int c = 0; c < NC; c++) {
+      const int col = c * Shape::kSpan + lane * kVec;
+      load_cols<T, WHOLE>(x + (row0 + (u < there ? u : 0)) * ldx + col, cols - col, v[u][c]);
     }
-  }
-  const float rstd = 1.0f / sqrtf(row_sum<LPR>(sum, shared, 1) / (float)cols + eps);
-  if (stats && lane == 0) {
-    stats[2 * row] = mean;
-    stats[2 * row + 1] = rstd;
-  }
-  const int groups = (cols + kGroup - 1) / kGroup;
-  constexpr int PAIR = LPR == 16 && NC > 1 ? 2 : 1;   // pieces of a group
-  constexpr int GLANES = LPR < 32 ? 16 : 32;
+  float mean[U], rstd[U];
 #pragma unroll
-  for (int c0 = 0; c0 < NC; c0 += PAIR) {
-    if (codes) {
-      float lo = __builtin_inff(), hi = -__builtin_inff();
+  for (int u = 0; u < U; u++) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int e = 0; e < kVec; e++) sum += v[u][c][e];
+    mean[u] = row_sum<LPR>(sum, shared, 2 * u) * per_col;
+    sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      const int left = cols - (c * Shape::kSpan + lane * kVec);
+#pragma unroll
+      for (int e = 0; e < kVec; e++) {
+        const float d = (WHOLE ? 0 : e) < left ? v[u][c][e] - mean[u] : 0.0f;
+        sum = __builtin_fmaf(d, d, sum);
+      }
+    }
+    rstd[u] = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<LPR>(sum, shared, 2 * u + 1), per_col, eps));
+  }
+  if (stats && lane == 0)
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (u < there) *(f32x2*)(stats + 2 * (row0 + u)) = f32x2{mean[u], rstd[u]};
+  if (codes) {
+    constexpr int PAIR = LPR == 16 && NC > 1 ? 2 : 1;   // pieces of a group
+    constexpr int GLANES = LPR < 32 ? 16 : 32, K = U * (NC / PAIR);
+    const int groups = (cols + kGroup - 1) / kGroup;
+    float lo[K], hi[K], s[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      const int u = k / (NC / PAIR), c0 = k % (NC / PAIR) * PAIR;
+      lo[k] = __builtin_inff();
+      hi[k] = -__builtin_inff();
 #pragma unroll
       for (int c = c0; c < c0 + PAIR; c++) {
         const int left = cols - (c * Shape::kSpan + lane * kVec);
 #pragma unroll
         for (int e = 0; e < kVec; e++)
-          if (e < left) lo = __builtin_fminf(lo, v[c][e]), hi = __builtin_fmaxf(hi, v[c][e]);
+          if ((WHOLE ? 0 : e) < left) lo[k] = __builtin_fminf(lo[k], v[u][c][e]), hi[k] = __builtin_fmaxf(hi[k], v[u][c][e]);
       }
-      lo = over_lanes<Least, GLANES>(lo);
-      hi = over_lanes<Most, GLANES>(hi);
-      const float s = scale_of(lo, hi);
+      lo[k] = over_lanes<Least, GLANES>(lo[k]);
+      hi[k] = over_lanes<Most, GLANES>(hi[k]);
+    }
+    scales_of<K>(lo, hi, s);
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      const int u = k / (NC / PAIR), c0 = k % (NC / PAIR) * PAIR;
+      if (u >= there) continue;
 #pragma unroll
       for (int c = c0; c < c0 + PAIR; c++) {
         const int col = c * Shape::kSpan + lane * kVec;
+        const float (&w)[kVec] = v[u][c];
         if (col < cols)
-          *(u32x2*)(codes + row * ldc + col) = u32x2{four_codes(v[c][0], v[c][1], v[c][2], v[c][3], lo, s),
-                                                     four_codes(v[c][4], v[c][5], v[c][6], v[c][7], lo, s)};
+          *(u32x2*)(codes + (row0 + u) * ldc + col) =
+              u32x2{four_codes(w[0], w[1], w[2], w[3], lo[k], s[k]), four_codes(w[4], w[5], w[6], w[7], lo[k], s[k])};
       }
       const int col = c0 * Shape::kSpan + lane * kVec;
       if (lane % GLANES == 0 && col < cols) {
-        scale[row * groups + col / kGroup] = s;
-        mn[row * groups + col / kGroup] = lo;
+        scale[(row0 + u) * groups + col / kGroup] = s[k];
+        mn[(row0 + u) * groups + col / kGroup] = lo[k];
       }
     }
+  }
 #pragma unroll
-    for (int c = c0; c < c0 + PAIR; c++) {
-      const int col = c * Shape::kSpan + lane * kVec;
-      float w[kVec], b[kVec];
-      if (weight)
-        load_cols<T, WHOLE>(weight + col, cols - col, w);
-      else
-        for (int e = 0; e < kVec; e++) w[e] = 1.0f;
-      if (bias)
-        load_cols<T, WHOLE>(bias + col, cols - col, b);
-      else
-        for (int e = 0; e < kVec; e++) b[e] = 0.0f;
+  for (int c = 0; c < NC; c++) {
+    const int col = c * Shape::kSpan + lane * kVec;
+    float w[kVec], b[kVec];
+    if (weight)
+      load_cols<T, WHOLE>(weight + col, cols - col, w);
+    else
+      for (int e = 0; e < kVec; e++) w[e] = 1.0f;
+    if (bias)
+      load_cols<T, WHOLE>(bias + col, cols - col, b);
+    else
+      for (int e = 0; e < kVec; e++) b[e] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < kVec; e++) w[e] = __builtin_fmaf((v[c][e] - mean) * rstd, w[e], b[e]);
-      store_cols<T, WHOLE>(y + row * cols + col, cols - col, w);
+    for (int u = 0; u < U; u++) {
+      float o[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; e++) o[e] = __builtin_fmaf((v[u][c][e] - mean[u]) * rstd[u], w[e], b[e]);
+      if (u < there) store_cols<T, WHOLE>(y + (row0 + u) * cols + col, cols - col, o);
     }
   }
 }
 
 // xh = (value - mean) rstd, g = dy w: dx = rstd (g - mean(g) - xh mean(g xh)); a thread adds up dy xh and dy of its columns over the
-// rows it sees, a workgroup writes one row of partial sums.
+// rows it sees, a workgroup writes one row of partial sums.  While a row is worked on, the next one's loads are on the way.
+constexpr int kNormThreads = 512;   // waves that share a row of partial sums (with 4 of them and twice the workgroups there is twice as much to add up)
+template <int LPR>
+using SharedRows = RowShape<LPR, kNormThreads>;
 template <typename T, int LPR, int NC, bool WHOLE>
-__global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_backward_kernel(
+__global__ __launch_bounds__(SharedRows<LPR>::kThreads) void norm_backward_kernel(
     const T* __restrict__ dy, int64_t lddy, const T* __restrict__ weight, const uint8_t* __restrict__ codes, int64_t ldc,
-    const float* __restrict__ scale, const float* __restrict__ mn, const float* __restrict__ stats, int64_t rows, int cols,
+    const float* __restrict__ scale, const float* __restrict__ mn, const float* __restrict__ stats, int64_t rows, int cols, float per_col,
     T* __restrict__ dx, float* __restrict__ partial) {
-  using Shape = RowShape<LPR>;
+  using Shape = SharedRows<LPR>;
   __shared__ float shared[4 * Shape::kWaves];
   constexpr int kFold = LPR < 64 ? 64 / LPR : 1;        // rows of a wave
-  constexpr int kAcross = LPR <= 64 ? 4 : 1;             // waves whose partial sums a workgroup adds up
+  constexpr int kAcross = LPR <= 64 ? kNormThreads / 64 : 1;             // waves whose partial sums a workgroup adds up
   __shared__ float folded[kAcross > 1 ? 64 * kVec * kAcross : 1];
+  typedef T T8 __attribute__((ext_vector_type(8), aligned(WHOLE ? 16 : sizeof(T))));
+  struct Asked {     // a row on its way
+    T8 dy[NC];
+    u32x2 codes[NC];
+    float scale[NC], lo[NC];
+    f32x2 stats;
+  };
   const int lane = threadIdx.x % LPR;
   const int groups = (cols + kGroup - 1) / kGroup;
+  const int64_t apart = (int64_t)gridDim.x * Shape::kRows;
+  auto ask = [&](int64_t row, Asked& a) __attribute__((always_inline)) {
+    row = row < rows ? row : rows - 1;
+    a.stats = *(const f32x2*)(stats + 2 * row);
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      const int col = c * Shape::kSpan + lane * kVec, left = cols - col;
+      a.dy[c] = T8{};
+      a.codes[c] = u32x2{0, 0};
+      a.scale[c] = 1.0f;
+      a.lo[c] = 0.0f;
+      if (left > 0) {
+        const T* p = dy + row * lddy + col;
+        if (WHOLE || left >= kVec) {
+          a.dy[c] = *(const T8*)p;
+        } else {
+#pragma unroll
+          for (int e = 0; e < kVec; e++)
+            if (e < left) a.dy[c][e] = p[e];
+        }
+        a.codes[c] = *(const u32x2*)(codes + row * ldc + col);
+        a.scale[c] = scale[row * groups + col / kGroup];
+        a.lo[c] = mn[row * groups + col / kGroup];
+      }
+    }
+  };
   float w[NC][kVec], dw[NC][kVec], db[NC][kVec];
 #pragma unroll
   for (int c = 0; c < NC; c++) {
@@ -397,45 +502,44 @@ __global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_backward_kernel(
     for (int e = 0; e < kVec; e++) dw[c][e] = db[c][e] = 0.0f;
   }
   int turn = 0;
-  for (int64_t first = (int64_t)blockIdx.x * Shape::kRows; first < rows; first += (int64_t)gridDim.x * Shape::kRows) {
+  constexpr bool kAhead = NC <= 2;      // with four pieces the registers do not hold a second row
+  Asked next;
+  int64_t first = (int64_t)blockIdx.x * Shape::kRows;
+  if (kAhead) ask(first + threadIdx.x / LPR, next);
+  for (; first < rows; first += apart) {
     const int64_t row = first + threadIdx.x / LPR;
     const bool there = Shape::kRows == 1 || row < rows;
-    const int64_t at = there ? row : rows - 1;
-    const float mean = stats[2 * at], rstd = stats[2 * at + 1];
+    if (!kAhead) ask(row, next);
+    const Asked now = next;
+    if (kAhead && first + apart < rows) ask(row + apart, next);
+    const float mean = now.stats[0], rstd = now.stats[1];
     float g[NC][kVec], xh[NC][kVec];
     float sum_g = 0.0f, sum_gx = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-      const int col = c * Shape::kSpan + lane * kVec;
-      const int64_t left = there ? cols - col : 0;
-      load_cols<T, WHOLE>(dy + at * lddy + col, left, g[c]);
-#pragma unroll
-      for (int e = 0; e < kVec; e++) xh[c][e] = 0.0f;
-      if (left > 0) {
-        const int64_t group = at * groups + col / kGroup;
-        eight_values(*(const u32x2*)(codes + at * ldc + col), 1.0f / scale[group], mn[group], xh[c]);
-#pragma unroll
-        for (int e = 0; e < kVec; e++) xh[c][e] = WHOLE || e < left ? (xh[c][e] - mean) * rstd : 0.0f;
-      }
+      const int left = there ? cols - (c * Shape::kSpan + lane * kVec) : 0;
+      eight_values(now.codes[c], inverse_of(now.scale[c]), now.lo[c], xh[c]);
 #pragma unroll
       for (int e = 0; e < kVec; e++) {
-        const float gx = g[c][e] * xh[c][e];
-        dw[c][e] += gx;
-        db[c][e] += g[c][e];
-        g[c][e] *= w[c][e];
+        const bool in = (WHOLE ? 0 : e) < left;      // columns behind the last one and a row that is not there add nothing
+        const float d = in ? (float)now.dy[c][e] : 0.0f;
+        xh[c][e] = in ? (xh[c][e] - mean) * rstd : 0.0f;
+        dw[c][e] = __builtin_fmaf(d, xh[c][e], dw[c][e]);
+        db[c][e] += d;
+        g[c][e] = d * w[c][e];
         sum_g += g[c][e];
-        sum_gx += g[c][e] * xh[c][e];
+        sum_gx = __builtin_fmaf(g[c][e], xh[c][e], sum_gx);
       }
     }
-    const float mg = row_sum<LPR>(sum_g, shared, turn) / (float)cols;
-    const float mgx = row_sum<LPR>(sum_gx, shared + 2 * Shape::kWaves, turn) / (float)cols;
+    const float mg = row_sum<LPR>(sum_g, shared, turn) * per_col;
+    const float mgx = row_sum<LPR>(sum_gx, shared + 2 * Shape::kWaves, turn) * per_col;
     turn ^= 1;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
       const int col = c * Shape::kSpan + lane * kVec;
 #pragma unroll
-      for (int e = 0; e < kVec; e++) g[c][e] = rstd * (g[c][e] - mg - xh[c][e] * mgx);
-      store_cols<T, WHOLE>(dx + at * cols + col, there ? cols - col : 0, g[c]);
+      for (int e = 0; e < kVec; e++) g[c][e] = rstd * (g[c][e] - __builtin_fmaf(xh[c][e], mgx, mg));
+      store_cols<T, WHOLE>(dx + row * cols + col, there ? cols - col : 0, g[c]);
     }
   }
   if (!partial) return;
@@ -459,11 +563,14 @@ __global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_backward_kernel(
 #pragma unroll
           for (int e = 0; e < kVec; e++) folded[(wave * kVec + e) * 64 + l] = s[e];
         __syncthreads();
-        if (wave == 0 && l < LPR)
+        // a wave per column of the pieces
+        if (l < LPR && c * Shape::kSpan + l * kVec + wave < cols) {
+          static_assert(kAcross == kVec, "eight waves, eight columns");
+          float total = 0.0f;
 #pragma unroll
-          for (int e = 0; e < kVec; e++)
-            if (col + e < cols)
-              out[col + e] = folded[e * 64 + l] + folded[(kVec + e) * 64 + l] + folded[(2 * kVec + e) * 64 + l] + folded[(3 * kVec + e) * 64 + l];
+          for (int from = 0; from < kAcross; from++) total += folded[(from * kVec + wave) * 64 + l];
+          out[c * Shape::kSpan + l * kVec + wave] = total;
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < kVec; e++)
@@ -481,8 +588,18 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
   const int col = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
   const float* in = partial + (int64_t)blockIdx.y * cols;
   float s = 0.0f;
-  if (col < cols)
-    for (int p = wave; p < count; p += 16) s += in[p * stride + col];
+  if (col < cols) {
+    // eight rows' loads at a time: one after the other they would be all latency (1024 partial rows of 1024 columns: 20 us)
+    int p = wave;
+    for (; p + 7 * 16 < count; p += 8 * 16) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) v[u] = in[(int64_t)(p + u * 16) * stride + col];
+#pragma unroll
+      for (int u = 0; u < 8; u++) s += v[u];
+    }
+    for (; p < count; p += 16) s += in[(int64_t)p * stride + col];
+  }
   shared[wave][threadIdx.x & 63] = s;
   __syncthreads();
   if (wave == 0 && col < cols) {
@@ -518,7 +635,7 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __res
       load_cols<T, WHOLE>(dy + row * lddy + col, left, g);
       if (codes && left > 0) {
         const int64_t group = row * groups + blockIdx.x;
-        eight_values(*(const u32x2*)(codes + row * ldc + col), 1.0f / scale[group], mn[group], z);
+        eight_values(*(const u32x2*)(codes + row * ldc + col), inverse_of(scale[group]), mn[group], z);
 #pragma unroll
         for (int e = 0; e < kVec; e++) g[e] = WHOLE || e < left ? g[e] * slope<std::is_same<T, float>::value>(z[e], act) : 0.0f;
       }
@@ -600,9 +717,13 @@ struct Mma {
     }
     return c;
   }
-  // by which a tile row's blocks of 16 columns are permuted: the rows that one read touches lie in different banks
+  // by which the blocks of 16 columns of a tile row of `COUNT` columns are permuted: the rows that one read touches (16-bit: four
+  // neighbours, and those 8 further on; float: every fourth) lie in different banks
+  template <int COUNT>
   static __device__ __forceinline__ uint32_t block_turn(uint32_t r) {
-    return sizeof(T) == 2 ? ((r & 3) | (((r >> 3) & 1) << 2)) : ((r >> 2) & 3);
+    if (sizeof(T) == 4) return (r >> 2) & 3;
+    if (COUNT == 64) return ((r >> 1) & 1) | (((r >> 3) & 1) << 1);      // two rows fill the banks: four blocks each
+    return (r & 3) | (((r >> 3) & 1) << 2);
   }
 };
 
@@ -644,7 +765,7 @@ struct TileLoad {
 #pragma unroll
       for (int q = 0; q < kLoads; q++) {
         const uint32_t r = (wave * kLoads + q) * RPL + lane * 16 / W, within = lane * 16 % W;
-        at[q] = r * (uint32_t)(ld * kEsz) + ((within / BLK) ^ Mma<T>::block_turn(r)) * BLK + within % BLK;
+        at[q] = r * (uint32_t)(ld * kEsz) + ((within / BLK) ^ Mma<T>::template block_turn<COUNT>(r)) * BLK + within % BLK;
       }
     } else {
       window.base = (const char*)p + (i0 * ld + r0) * kEsz;
@@ -678,9 +799,8 @@ struct TileLoad {
 // Codes of a checkpoint, one memory row per r, as a strided tile of values: 16 codes of a row are one piece, a block of the tile.
 template <typename T, int COUNT, int WAVES>
 struct CodeLoad {
-  static constexpr int kPieces = Mma<T>::kStep * COUNT / 16 / (WAVES * 64);
+  static constexpr int kTotal = Mma<T>::kStep * COUNT / 16, kPieces = kTotal > WAVES * 64 ? kTotal / (WAVES * 64) : 1;
   static constexpr int kAcross = COUNT / 16, kApart = WAVES * 64 / kAcross;     // pieces of a row; rows between a thread's pieces
-  static_assert(kPieces >= 1, "a thread takes at least one piece");
   Window codes, scale, mn;
   int64_t step, stat_step;
   uint32_t at, stat_at, apart, stat_apart;    // of the thread's first piece, and to the next one
@@ -718,11 +838,12 @@ struct CodeLoad {
     left -= Mma<T>::kStep;
   }
   __device__ __forceinline__ void put(lds_u8* tile) {
+    if (kTotal < WAVES * 64 && thread >= kTotal) return;      // floats of a small tile: fewer pieces than threads
 #pragma unroll
     for (int q = 0; q < kPieces; q++) {
       const uint32_t row = thread / kAcross + q * kApart, block = thread % kAcross;
-      const float inv = (int)row < held_left ? 1.0f / s[q] : 0.0f;      // rows behind the last one: zeros
-      lds_u8* to = tile + row * (COUNT * (int)sizeof(T)) + (block ^ Mma<T>::block_turn(row)) * Mma<T>::kBlock;
+      const float inv = (int)row < held_left ? inverse_of(s[q]) : 0.0f;      // rows behind the last one: zeros
+      lds_u8* to = tile + row * (COUNT * (int)sizeof(T)) + (block ^ Mma<T>::template block_turn<COUNT>(row)) * Mma<T>::kBlock;
       if constexpr (sizeof(T) == 2) {
         typedef T T8 __attribute__((ext_vector_type(8)));
 #pragma unroll
@@ -755,7 +876,7 @@ struct TileRead {
     if constexpr (!STRIDED) {
       return *(const __attribute__((address_space(3))) Frag*)(tile + first * 128 + i * 128 + (((kk * 4 + g) ^ (i & 7)) * 16));
     } else if constexpr (sizeof(T) == 2) {
-      const uint32_t turn = (i >> 2) | ((g & 1) << 2);
+      const uint32_t turn = Mma<T>::template block_turn<COUNT>(g * 8 + (i >> 2));     // the same in every row that the lane reads
       const lds_u8* p = tile + (g * 8 + (i >> 2)) * W + (((first / 16) ^ turn) * BLK) + (i & 3) * 8 + kk * 32 * W;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * W));
@@ -1204,6 +1325,7 @@ inline int size_of(int dtype) { return dtype == GACT_F32 ? 4 : 2; }
 inline bool known(int dtype) { return dtype == GACT_F32 || dtype == GACT_F16 || dtype == GACT_BF16; }
 inline bool blocks_fit(int64_t blocks) { return blocks > 0 && blocks <= 0x7fffffff; }
 constexpr int64_t kMostCols = GACT_LAYER_MAX_COLS;
+constexpr int kComputeUnits = 256;
 
 // rows that every lane's piece lies whole and aligned in
 inline bool whole_rows(const void* p, int dtype, int64_t cols, int64_t ld) {
@@ -1220,23 +1342,26 @@ int with_type(int dtype, F&& f) {
   }
 }
 
-template <typename T, bool WHOLE, typename F>
+// threads of a row, its pieces per thread, and the rows that a thread of the forward pass takes at a time
+template <typename F>
 int with_row_shape(int64_t cols, F&& f) {
   using std::integral_constant;
-  if (cols <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-  if (cols <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-  if (cols <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  if (cols <= 1024) return f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  if (cols <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-  if (cols <= 4096) return f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  if (cols <= 8192) return f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-  return f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+  if (cols <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  if (cols <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  if (cols <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  if (cols <= 1024) return f(integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+  if (cols <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  if (cols <= 4096) return f(integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
+  if (cols <= 8192) return f(integral_constant<int, 512>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
+  return f(integral_constant<int, 512>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
 }
 // workgroups of a layer norm's backward pass: each leaves one row of partial sums
 inline int64_t norm_blocks(int64_t rows, int64_t cols) {
-  const int64_t at_a_time = cols <= 128 ? 16 : cols <= 256 ? 8 : cols <= 1024 ? 4 : 1;
-  const int64_t needed = (rows + at_a_time - 1) / at_a_time;
-  return needed < 1024 ? needed : 1024;
+  const int64_t at_a_time = cols <= 128 ? kNormThreads / 16 : cols <= 256 ? kNormThreads / 32 : cols <= 1024 ? kNormThreads / 64 : 1;
+  const int64_t needed = (rows + at_a_time - 1) / at_a_time, most = cols <= 4096 ? 512 : 256;
+  if (needed <= kComputeUnits) return needed;
+  const int64_t shared = needed / 8 > kComputeUnits ? needed / 8 : kComputeUnits;     // enough turns to pay for a row of partial sums
+  return shared < most ? shared : most;
 }
 inline int64_t strip_rows(int64_t rows, int64_t cols) {   // rows of a workgroup of the activation's backward pass
   const int64_t across = (cols + kGroup - 1) / kGroup;
@@ -1254,11 +1379,12 @@ int sum_rows(const float* partial, int64_t count, int64_t stride, int64_t cols, 
   return launch_status();
 }
 
+// workgroups of a tile whose LDS (two steps of both operands, and up to 12 KB beside them) a compute unit holds
+constexpr int slots_per_cu(int bm, int bn) { return bm + bn <= 128 ? 4 : bm + bn <= 256 ? 2 : 1; }
 struct Tiles {
   int bm, bn, splits;
   int64_t per_split;
 };
-constexpr int kComputeUnits = 256;
 
 template <typename T, int BM, int BN, int WI, int WJ, bool AS, int BK, int ACT = ACT_NONE, bool CODES = false>
 int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s) {
@@ -1268,7 +1394,7 @@ int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s)
   p.per_split = per_split;
   const int64_t tiles = (int64_t)p.tiles_i * p.tiles_j * splits;
   if (!blocks_fit(tiles)) return GACT_ELIMIT;
-  constexpr int kSlots = kComputeUnits * (BM * BN <= 128 * 128 ? 2 : 1);      // workgroups that the card holds at a time
+  constexpr int kSlots = kComputeUnits * slots_per_cu(BM, BN);      // workgroups that the card holds at a time
   const int64_t blocks = tiles < kSlots ? tiles : kSlots;
   auto kernel = product_kernel<T, BM, BN, WI, WJ, AS, BK, ACT, CODES>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(WI * WJ * 64), 0, s, p);
@@ -1278,33 +1404,37 @@ int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s)
 template <typename T, int ACT>
 int forward_product(ProductArgs& p, hipStream_t s) {
   const int64_t step = 128 / (int)sizeof(T), depth = (p.depth + step - 1) / step * step;
-  const bool large = sizeof(T) == 2 && (int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256) >= kComputeUnits;
+  auto tiles = [&](int bm, int bn) { return (int64_t)((p.rows + bm - 1) / bm) * ((p.cols + bn - 1) / bn); };
+  const bool large = sizeof(T) == 2 && tiles(256, 256) >= kComputeUnits;
   // the pre-activation's codes need a whole group of columns in a tile; without an activation nobody asks for them
   if constexpr (ACT != ACT_NONE) {
     if (p.codes) {
       if constexpr (sizeof(T) == 2)
         if (large) return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
-      return launch_product<T, 128, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
+      if (tiles(128, 256) >= kComputeUnits / 2) return launch_product<T, 128, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
+      return launch_product<T, 64, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
     }
   }
   if constexpr (sizeof(T) == 2)
     if (large) return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT>(p, 1, depth, s);
-  return launch_product<T, 128, 128, 2, 2, false, B_ROWS, ACT>(p, 1, depth, s);
+  if (tiles(128, 128) >= kComputeUnits) return launch_product<T, 128, 128, 2, 2, false, B_ROWS, ACT>(p, 1, depth, s);
+  return launch_product<T, 64, 64, 2, 2, false, B_ROWS, ACT>(p, 1, depth, s);
 }
 
 // how a backward product is cut: the tile, and the parts of its depth where the tiles alone leave compute units idle
 inline Tiles tiles_of(int dtype, int64_t rows, int64_t cols, int64_t depth) {
-  Tiles t = {128, 128, 1, 0};
-  const int64_t step = 128 / size_of(dtype);
-  int64_t slots = 2 * kComputeUnits;
-  if (dtype != GACT_F32 && ((rows + 255) / 256) * ((cols + 255) / 256) >= kComputeUnits / 4) {
+  Tiles t = {64, 64, 1, 0};
+  const int64_t step = 128 / size_of(dtype), steps = (depth + step - 1) / step;
+  auto tiles = [&](int side) { return ((rows + side - 1) / side) * ((cols + side - 1) / side); };
+  // as many workgroups as the card holds, in the largest tiles that leave each at least 8 steps
+  if (dtype != GACT_F32 && tiles(256) * (steps / 8) >= kComputeUnits)
     t.bm = t.bn = 256;
-    slots = kComputeUnits;
-  }
-  const int64_t tiles = ((rows + t.bm - 1) / t.bm) * ((cols + t.bn - 1) / t.bn);
-  const int64_t steps = (depth + step - 1) / step;
-  int64_t splits = tiles >= slots ? 1 : slots / tiles;
-  if (splits > steps / 8) splits = steps / 8;
+  else if (tiles(128) * (steps / 8) >= kComputeUnits)
+    t.bm = t.bn = 128;
+  const int64_t slots = kComputeUnits * slots_per_cu(t.bm, t.bn);
+  int64_t splits = tiles(t.bm) >= slots ? 1 : slots / tiles(t.bm);
+  const int64_t most = steps / (t.bm == 64 ? 4 : 8);
+  if (splits > most) splits = most;
   if (splits > 64) splits = 64;
   if (splits < 1) splits = 1;
   const int64_t per = (steps + splits - 1) / splits;
@@ -1323,13 +1453,11 @@ int backward_product(ProductArgs& p, int dtype, void* workspace, hipStream_t s) 
     p.out = workspace;
     p.ldo = padded4(p.cols);
   }
-  int rc;
-  if constexpr (sizeof(T) == 2) {
-    rc = t.bm == 256 ? launch_product<T, 256, 256, 2, 4, AS, BK>(p, t.splits, t.per_split, s)
-                     : launch_product<T, 128, 128, 2, 2, AS, BK>(p, t.splits, t.per_split, s);
-  } else {
-    rc = launch_product<T, 128, 128, 2, 2, AS, BK>(p, t.splits, t.per_split, s);
-  }
+  int rc = GACT_ESHAPE;
+  if constexpr (sizeof(T) == 2)
+    if (t.bm == 256) rc = launch_product<T, 256, 256, 2, 4, AS, BK>(p, t.splits, t.per_split, s);
+  if (t.bm == 128) rc = launch_product<T, 128, 128, 2, 2, AS, BK>(p, t.splits, t.per_split, s);
+  if (t.bm == 64) rc = launch_product<T, 64, 64, 2, 2, AS, BK>(p, t.splits, t.per_split, s);
   if (rc != GACT_OK || t.splits == 1) return rc;
   const int64_t blocks = ((int64_t)p.rows * (p.ldo / 4) + 255) / 256;
   if (!blocks_fit(blocks)) return GACT_ELIMIT;
@@ -1411,17 +1539,21 @@ int gact_norm_forward(const void* x, int64_t ldx, const void* weight, const void
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     const bool whole = whole_rows(x, dtype, cols, ldx) && whole_rows(y, dtype, cols, cols) && aligned16(weight) && aligned16(bias);
-    auto run = [&](auto lpr, auto nc, auto w) {
-      constexpr int LPR = decltype(lpr)::value, NC = decltype(nc)::value;
-      const int64_t blocks = (rows + RowShape<LPR>::kRows - 1) / RowShape<LPR>::kRows;
-      if (!blocks_fit(blocks)) return GACT_ELIMIT;
-      hipLaunchKernelGGL((norm_forward_kernel<T, LPR, NC, decltype(w)::value>), dim3((unsigned)blocks), dim3(RowShape<LPR>::kThreads), 0,
-                         (hipStream_t)stream, (const T*)x, ldx, (const T*)weight, (const T*)bias, rows, (int)cols, eps, (T*)y,
-                         (uint8_t*)codes, ldc, scale, mn, stats);
-      return launch_status();
-    };
-    return whole ? with_row_shape<T, true>(cols, [&](auto l, auto n) { return run(l, n, std::true_type{}); })
-                 : with_row_shape<T, false>(cols, [&](auto l, auto n) { return run(l, n, std::false_type{}); });
+    return with_row_shape(cols, [&](auto lpr, auto nc, auto at_a_time) {
+      constexpr int LPR = decltype(lpr)::value, NC = decltype(nc)::value, U = decltype(at_a_time)::value;
+      auto run = [&](auto kernel, int u) {
+        const int64_t blocks = (rows + RowShape<LPR>::kRows * u - 1) / (RowShape<LPR>::kRows * u);
+        if (!blocks_fit(blocks)) return GACT_ELIMIT;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(RowShape<LPR>::kThreads), 0, (hipStream_t)stream, (const T*)x, ldx,
+                           (const T*)weight, (const T*)bias, rows, (int)cols, 1.0f / (float)cols, eps, (T*)y, (uint8_t*)codes, ldc, scale, mn,
+                           stats);
+        return launch_status();
+      };
+      // few rows: one at a time, on as many compute units as there are
+      if (U > 1 && rows < (int64_t)kComputeUnits * 4 * RowShape<LPR>::kRows * U)
+        return whole ? run(norm_forward_kernel<T, LPR, NC, 1, true>, 1) : run(norm_forward_kernel<T, LPR, NC, 1, false>, 1);
+      return whole ? run(norm_forward_kernel<T, LPR, NC, U, true>, U) : run(norm_forward_kernel<T, LPR, NC, U, false>, U);
+    });
   });
 }
 
@@ -1442,15 +1574,14 @@ int gact_norm_backward(const void* dy, int64_t lddy, const void* weight, const v
     using T = decltype(zero);
     const bool whole = whole_rows(dy, dtype, cols, lddy) && whole_rows(dx, dtype, cols, cols) && aligned16(weight);
     const int64_t blocks = norm_blocks(rows, cols);
-    auto run = [&](auto lpr, auto nc, auto w) {
+    const int rc = with_row_shape(cols, [&](auto lpr, auto nc, auto) {
       constexpr int LPR = decltype(lpr)::value, NC = decltype(nc)::value;
-      hipLaunchKernelGGL((norm_backward_kernel<T, LPR, NC, decltype(w)::value>), dim3((unsigned)blocks), dim3(RowShape<LPR>::kThreads), 0,
-                         (hipStream_t)stream, (const T*)dy, lddy, (const T*)weight, (const uint8_t*)codes, ldc, scale, mn, stats, rows,
-                         (int)cols, (T*)dx, sums ? workspace : nullptr);
+      auto kernel = whole ? norm_backward_kernel<T, LPR, NC, true> : norm_backward_kernel<T, LPR, NC, false>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(SharedRows<LPR>::kThreads), 0, (hipStream_t)stream, (const T*)dy, lddy,
+                         (const T*)weight, (const uint8_t*)codes, ldc, scale, mn, stats, rows, (int)cols, 1.0f / (float)cols, (T*)dx,
+                         sums ? workspace : nullptr);
       return launch_status();
-    };
-    const int rc = whole ? with_row_shape<T, true>(cols, [&](auto l, auto n) { return run(l, n, std::true_type{}); })
-                         : with_row_shape<T, false>(cols, [&](auto l, auto n) { return run(l, n, std::false_type{}); });
+    });
     if (rc != GACT_OK || !sums) return rc;
     return sum_rows<T>(workspace, blocks, 2 * cols, cols, 2, dweight, dbias, (hipStream_t)stream);
   });
