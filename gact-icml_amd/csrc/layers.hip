@@ -665,12 +665,12 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __res
 // Products.  out[i][j] = sum over r of A(i, r) B(j, r), each operand in one of two layouts: rows of it contiguous along r (x and W of
 // the forward pass, dz of dx), or contiguous along i or j, one memory row per r (W of dx; dz and the checkpoint of dW).
 //
-// A workgroup owns a tile of BM x BN and walks along r in steps of 128 bytes of T, two tiles of each operand in LDS: the next one
-// arrives straight from memory (16 bytes a lane, no registers) while the present one is multiplied.  A checkpoint's codes pass
-// through registers, where they become values of T.  A lane's fragment is 8 values along r of 16-bit types (one 16x16x32 product) or 4 floats
-// (four 16x16x4 products).  Operands contiguous along r are read 16 bytes at a time, the others through the transposing LDS read (16-bit) or
-// value by value (float).  LDS is addressed so that neither kind of read meets a bank twice: contiguous rows of 128 bytes permute
-// their eight 16-byte pieces by the row's number, the others their blocks of 16 columns.
+// A workgroup owns a tile of BM x BN and walks along r in steps of 128 bytes of T, two of which are in LDS: while one is multiplied the next
+// one arrives, straight from memory (16 bytes a lane, no registers).  A checkpoint's codes pass through registers, where they
+// become values of T.  A lane's fragment is 8 values along r of 16-bit types (one 16x16x32 product) or 4 floats (four 16x16x4
+// products).  Operands contiguous along r are read 16 bytes at a time, the others through the transposing LDS read (16-bit) or value by value
+// (float).  LDS is addressed so that neither kind of read meets a bank twice: contiguous rows of 128 bytes permute their eight
+// 16-byte pieces by the row's number, the others their blocks of 16 columns.
 //
 // B supplies the matrix instruction's rows and A its columns, so that a lane holds four consecutive j of one i.
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -729,8 +729,8 @@ struct Mma {
 
 // what is left of an operand from a tile's corner on, as a buffer that loads beyond it give zero from
 struct Window {
-  const char* base;
-  int64_t left;
+  const char* base = nullptr;
+  int64_t left = 0;
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
     const int64_t n = left <= 0 ? 0 : left > 0x7fffffff ? 0x7fffffff : left;
     return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)n, 0x00020000);
@@ -740,27 +740,38 @@ struct Window {
     left -= bytes;
   }
 };
+// buffer_load with its destination in LDS: lane l's BYTES go to `to` + l BYTES (two bytes: 4 l; M0 holds `to`, the same for the wave).  It writes no
+// register.  As asm, because the compiler waits for every such load that it knows of before it reads LDS through the transposing
+// read, whichever memory that reads; the product counts them itself, and waits before the barrier that gives a step's memory free.
+template <int BYTES>
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint32_t offset, lds_u8* to) {
+#ifdef __HIP_DEVICE_COMPILE__
+  static_assert(BYTES == 16 || BYTES == 4 || BYTES == 2, "a quad, a word or half a word, which takes a word of LDS");
+  if constexpr (BYTES == 2)
+    asm volatile("s_nop 0\n\tbuffer_load_ushort %0, %1, 0 offen lds" : : "v"(offset), "s"(rsrc), "{m0}"((uint32_t)(uintptr_t)to) : "memory");
+  else if constexpr (BYTES == 16)
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(offset), "s"(rsrc), "{m0}"((uint32_t)(uintptr_t)to) : "memory");
+  else
+    asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" : : "v"(offset), "s"(rsrc), "{m0}"((uint32_t)(uintptr_t)to) : "memory");
+#endif
+}
 
-// Loads a tile of COUNT rows (contiguous along r) or COUNT columns (strided) into LDS: an instruction of a wave fills 1 KB.
+// Loads a step of COUNT rows (contiguous along r) or COUNT columns (strided) into LDS: an instruction of a wave fills 1 KB.
 template <typename T, int COUNT, bool STRIDED, int WAVES>
 struct TileLoad {
-  static constexpr int kLoads = COUNT * 128 / 1024 / WAVES;
-  static constexpr int kEsz = (int)sizeof(T);
+  static constexpr int kLoads = COUNT * 128 / 1024 / WAVES, kEsz = (int)sizeof(T);
   static_assert(kLoads >= 1, "a wave takes at least one load");
   Window window;
-  int64_t step;
+  int64_t step = 0;
   uint32_t at[kLoads];
+  int piece = 0, left = 0;     // contiguous: the lane's first value along r, and the values that are left from the step on
+  int wave = 0;
   // up to the end of the piece: a window drops a value of 16 bits whose neighbour in the word lies beyond it
   static __device__ __forceinline__ int64_t whole(int64_t n) { return (n + 16 / kEsz - 1) / (16 / kEsz) * (16 / kEsz); }
-  int piece, left;     // contiguous: the lane's first value along r, and the values that are left from the step on
-  int wave;
-  __device__ __forceinline__ void start(const void* p, int64_t ld, int i0, int count, int64_t depth, int64_t r0, int w, int lane) {
+  __device__ __forceinline__ void set_up(int64_t ld, int w, int lane) {
     wave = w;
     if (STRIDED) {
       constexpr int W = COUNT * kEsz, RPL = 1024 / W, BLK = Mma<T>::kBlock;
-      window.base = (const char*)p + (r0 * ld + i0) * kEsz;
-      window.left = ((depth - 1 - r0) * ld + whole(count) - i0) * kEsz;
-      if (depth <= r0) window.left = 0;
       step = (int64_t)Mma<T>::kStep * ld * kEsz;
 #pragma unroll
       for (int q = 0; q < kLoads; q++) {
@@ -768,61 +779,65 @@ struct TileLoad {
         at[q] = r * (uint32_t)(ld * kEsz) + ((within / BLK) ^ Mma<T>::template block_turn<COUNT>(r)) * BLK + within % BLK;
       }
     } else {
-      window.base = (const char*)p + (i0 * ld + r0) * kEsz;
-      window.left = ((count - 1 - i0) * ld + whole(depth) - r0) * kEsz;
       step = 128;
       piece = ((lane & 7) ^ (lane >> 3)) * (16 / kEsz);
-      left = (int)(depth - r0 < 0x7fffffff ? depth - r0 : 0x7fffffff);
 #pragma unroll
       for (int q = 0; q < kLoads; q++) at[q] = ((wave * kLoads + q) * 8 + (lane >> 3)) * (uint32_t)(ld * kEsz) + piece * kEsz;
     }
   }
-  __device__ __forceinline__ void issue(lds_u8* tile) {
-#ifdef __HIP_DEVICE_COMPILE__
-    const __amdgpu_buffer_rsrc_t rsrc = window.rsrc();
-    const bool beyond = !STRIDED && piece >= left;
-    // buffer_load_dwordx4 with its destination in LDS (M0: the wave's first byte there).  It writes no register.  As asm, because the compiler
-    // waits for every such load that it knows of before it reads LDS through the transposing read, whichever tile that lies in;
-    // the product waits for them itself, before the barrier that gives a tile free.
-#pragma unroll
-    for (int q = 0; q < kLoads; q++)
-      asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-                   :
-                   : "v"(beyond ? kNowhere : at[q]), "s"(rsrc), "{m0}"((uint32_t)(uintptr_t)(tile + (wave * kLoads + q) * 1024))
-                   : "memory");
-#endif
+  // from row or column i0 of `count` and value r0 of `depth` on
+  __device__ __forceinline__ void start(const void* p, int64_t ld, int i0, int count, int64_t depth, int64_t r0) {
+    if (STRIDED) {
+      window.base = (const char*)p + (r0 * ld + i0) * kEsz;
+      window.left = ((depth - 1 - r0) * ld + whole(count) - i0) * kEsz;
+    } else {
+      window.base = (const char*)p + (i0 * ld + r0) * kEsz;
+      window.left = ((count - 1 - i0) * ld + whole(depth) - r0) * kEsz;
+      left = (int)(depth - r0 < 0x7fffffff ? depth - r0 : 0x7fffffff);
+    }
+  }
+  __device__ __forceinline__ void stop() { window.left = 0; }
+  // load q of the wave's; after the last one the step is done
+  __device__ __forceinline__ void issue(int q, lds_u8* to) const {
+    load_to_lds<16>(window.rsrc(), !STRIDED && piece >= left ? kNowhere : at[q], to + (wave * kLoads + q) * 1024);
+  }
+  __device__ __forceinline__ void advance() {
     window.advance(step);
     left -= Mma<T>::kStep;
   }
 };
 
-// Codes of a checkpoint, one memory row per r, as a strided tile of values: 16 codes of a row are one piece, a block of the tile.
+// Codes of a checkpoint, one memory row per r, as a strided step of values: 16 codes of a row are one piece, a block of the step.
 template <typename T, int COUNT, int WAVES>
 struct CodeLoad {
   static constexpr int kTotal = Mma<T>::kStep * COUNT / 16, kPieces = kTotal > WAVES * 64 ? kTotal / (WAVES * 64) : 1;
   static constexpr int kAcross = COUNT / 16, kApart = WAVES * 64 / kAcross;     // pieces of a row; rows between a thread's pieces
+  static constexpr int kLoads = 0;            // straight to LDS
   Window codes, scale, mn;
-  int64_t step, stat_step;
-  uint32_t at, stat_at, apart, stat_apart;    // of the thread's first piece, and to the next one
-  int left, held_left, thread;                // rows from the next step on, and from the one that is held on
+  int64_t step = 0, stat_step = 0;
+  uint32_t at = 0, stat_at = 0, apart = 0, stat_apart = 0;    // of the thread's first piece, and to the next one
+  int left = 0, held_left = 0;                                // rows from the next step on, and from the one that is held on
   u32x4 held[kPieces];
   float s[kPieces], lo[kPieces];
-  __device__ __forceinline__ void start(const ProductArgs& p, int j0, int64_t r0, int64_t end, int t) {
-    thread = t;
-    left = (int)(end - r0 < 0x7fffffff ? end - r0 : 0x7fffffff);
-    const int row = t / kAcross, col = t % kAcross * 16, groups = p.b_groups;
-    codes.base = (const char*)p.b + r0 * p.ldb + j0;
-    codes.left = (end - r0) * p.ldb - j0;
-    scale.base = (const char*)(p.b_scale + r0 * groups + j0 / kGroup);
-    mn.base = (const char*)(p.b_min + r0 * groups + j0 / kGroup);
-    scale.left = mn.left = ((end - r0) * groups - j0 / kGroup) * 4;
+  __device__ __forceinline__ void set_up(const ProductArgs& p) {
+    const int t = threadIdx.x, row = t / kAcross, col = t % kAcross * 16, groups = p.b_groups;
     step = Mma<T>::kStep * p.ldb;
-    stat_step = Mma<T>::kStep * groups * 4;
+    stat_step = (int64_t)Mma<T>::kStep * groups * 4;
     at = row * (uint32_t)p.ldb + col;
-    stat_at = (row * groups + (j0 % kGroup + col) / kGroup) * 4;
+    stat_at = row * groups * 4;
     apart = kApart * (uint32_t)p.ldb;
     stat_apart = kApart * groups * 4;
   }
+  __device__ __forceinline__ void start(const ProductArgs& p, int j0, int64_t depth, int64_t r0) {
+    left = (int)(depth - r0 < 0x7fffffff ? depth - r0 : 0x7fffffff);
+    const int groups = p.b_groups;
+    codes.base = (const char*)p.b + r0 * p.ldb + j0;
+    codes.left = (depth - r0) * p.ldb - j0;
+    scale.base = (const char*)(p.b_scale + r0 * groups + j0 / kGroup);      // one group of columns: no tile is wider than one or meets two
+    mn.base = (const char*)(p.b_min + r0 * groups + j0 / kGroup);
+    scale.left = mn.left = ((depth - r0) * groups - j0 / kGroup) * 4;
+  }
+  __device__ __forceinline__ void stop() { codes.left = scale.left = mn.left = 0; }
   __device__ __forceinline__ void fetch() {
     held_left = left;
     const __amdgpu_buffer_rsrc_t c = codes.rsrc(), f = scale.rsrc(), m = mn.rsrc();
@@ -837,36 +852,35 @@ struct CodeLoad {
     mn.advance(stat_step);
     left -= Mma<T>::kStep;
   }
-  __device__ __forceinline__ void put(lds_u8* tile) {
-    if (kTotal < WAVES * 64 && thread >= kTotal) return;      // floats of a small tile: fewer pieces than threads
+  // piece q's values
+  __device__ __forceinline__ void put(int q, lds_u8* tile) const {
+    const int t = threadIdx.x;
+    if (kTotal < WAVES * 64 && t >= kTotal) return;      // floats of a small tile: fewer pieces than threads
+    const uint32_t row = t / kAcross + q * kApart, block = t % kAcross;
+    const float inv = (int)row < held_left ? inverse_of(s[q]) : 0.0f;      // rows behind the last one: zeros
+    lds_u8* to = tile + row * (COUNT * (int)sizeof(T)) + (block ^ Mma<T>::template block_turn<COUNT>(row)) * Mma<T>::kBlock;
+    if constexpr (sizeof(T) == 2) {
+      typedef T T8 __attribute__((ext_vector_type(8)));
 #pragma unroll
-    for (int q = 0; q < kPieces; q++) {
-      const uint32_t row = thread / kAcross + q * kApart, block = thread % kAcross;
-      const float inv = (int)row < held_left ? inverse_of(s[q]) : 0.0f;      // rows behind the last one: zeros
-      lds_u8* to = tile + row * (COUNT * (int)sizeof(T)) + (block ^ Mma<T>::template block_turn<COUNT>(row)) * Mma<T>::kBlock;
-      if constexpr (sizeof(T) == 2) {
-        typedef T T8 __attribute__((ext_vector_type(8)));
+      for (int h = 0; h < 2; h++) {
+        T8 v;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          T8 v;
+        for (int e = 0; e < 8; e++) v[e] = (T)__builtin_fmaf(code_at(held[q][2 * h + (e >> 2)], e & 3), inv, lo[q]);
+        *(__attribute__((address_space(3))) T8*)(to + 16 * h) = v;
+      }
+    } else {
 #pragma unroll
-          for (int e = 0; e < 8; e++) v[e] = (T)__builtin_fmaf(code_at(held[q][2 * h + (e >> 2)], e & 3), inv, lo[q]);
-          *(__attribute__((address_space(3))) T8*)(to + 16 * h) = v;
-        }
-      } else {
+      for (int h = 0; h < 4; h++) {
+        f32x4 v;
 #pragma unroll
-        for (int h = 0; h < 4; h++) {
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(code_at(held[q][h], e), inv, lo[q]);
-          *(__attribute__((address_space(3))) f32x4*)(to + 16 * h) = v;
-        }
+        for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(code_at(held[q][h], e), inv, lo[q]);
+        *(__attribute__((address_space(3))) f32x4*)(to + 16 * h) = v;
       }
     }
   }
 };
 
-// Fragments of 16 rows (contiguous) or columns (strided) of a tile: `at` of a lane for k step kk, then immediate offsets.
+// A lane's fragment of 16 rows (contiguous) or columns (strided) of half kk of a step, from row or column `first` on
 template <typename T, int COUNT, bool STRIDED>
 struct TileRead {
   using Frag = typename Mma<T>::Frag;
@@ -939,6 +953,13 @@ __device__ __forceinline__ u32x2 rounded4(f32x4 v) {
   return __builtin_bit_cast(u32x2, o);
 }
 template <typename T>
+__device__ __forceinline__ float low_value(uint32_t word) {
+  if constexpr (std::is_same<T, float>::value) return __builtin_bit_cast(float, word);
+  if constexpr (std::is_same<T, bf16>::value) return __builtin_bit_cast(float, word << 16);
+  if constexpr (std::is_same<T, f16>::value) return (float)__builtin_bit_cast(f16, (uint16_t)word);
+  return 0.0f;
+}
+template <typename T>
 __device__ __forceinline__ f32x4 widened4(uint32_t a, uint32_t b) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   const T4 o = __builtin_bit_cast(T4, u32x2{a, b});
@@ -950,128 +971,199 @@ enum { B_ROWS = 0, B_STRIDED = 1, B_CODES = 2 };
 template <typename T, int BM, int BN, int WI, int WJ, bool A_STRIDED, int B_KIND, int ACT, bool CODES>
 __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
   constexpr int WAVES = WI * WJ, MI = BM / WI / 16, MH = MI / 2, NJ = BN / WJ / 16;
-  constexpr bool FORWARD = B_KIND == B_ROWS;
+  constexpr bool FORWARD = B_KIND == B_ROWS, CODED = B_KIND == B_CODES;
   using Frag = typename Mma<T>::Frag;
-  // two objects, so that the compiler can tell a read of one from the loads that fill the other and does not wait for those
-  __shared__ __attribute__((aligned(1024))) uint8_t even[(BM + BN) * 128];
-  __shared__ __attribute__((aligned(1024))) uint8_t odd[(BM + BN) * 128];
+  using LoadA = TileLoad<T, BM, A_STRIDED, WAVES>;
+  using LoadB = std::conditional_t<CODED, CodeLoad<T, BN, WAVES>, TileLoad<T, BN, B_KIND == B_STRIDED, WAVES>>;
+  constexpr int kA = BM * 128, kB = BN * 128;
+  __shared__ __attribute__((aligned(1024))) uint8_t memory[2 * (kA + kB)];
+  lds_u8* const a_ring = (lds_u8*)memory;
+  lds_u8* const b_ring = a_ring + 2 * kA;
+  // the tiles' biases, a word each, by turns: loads run up to three tiles ahead where tiles have but one step
+  __shared__ uint32_t biases[4][FORWARD ? BN : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / WJ, wj = wave % WJ;
-  int steps;
 
-  TileLoad<T, BM, A_STRIDED, WAVES> a;
-  std::conditional_t<B_KIND == B_CODES, CodeLoad<T, BN, WAVES>, TileLoad<T, BN, B_KIND == B_STRIDED, WAVES>> b;
-  auto fill = [&](lds_u8* tile) __attribute__((always_inline)) {
-    a.issue(tile);
-    if constexpr (B_KIND == B_CODES) {
-      b.put(tile + BM * 128);
-      b.fetch();
-    } else {
-      b.issue(tile + BM * 128);
-    }
-  };
-  // the tile's bias, asked for ahead of the tiles (a load waits for those before it) and put into LDS when the tile begins
-  __shared__ float biases[2][FORWARD ? BN : 1];
-  float own_bias = 0.0f;
-  auto begin = [&](const Tile& tile) __attribute__((always_inline)) {
-    if constexpr (FORWARD) {
-      const int j = tile.j * BN + (int)threadIdx.x;
-      own_bias = 0.0f;
-      if (p.bias && threadIdx.x < BN && j < p.cols) own_bias = (float)((const T*)p.bias)[j];
-    }
-    const int64_t r0 = tile.split * p.per_split, end = r0 + p.per_split < p.depth ? r0 + p.per_split : p.depth;
-    steps = (int)((end - r0 + Mma<T>::kStep - 1) / Mma<T>::kStep);
-    a.start(p.a, p.lda, tile.i * BM, p.rows, end, r0, wave, lane);
-    if constexpr (B_KIND == B_CODES) {
-      b.start(p, tile.j * BN, r0, end, threadIdx.x);
-      b.fetch();
-    } else {
-      b.start(p.b, p.ldb, tile.j * BN, p.cols, end, r0, wave, lane);
-    }
-    fill((lds_u8*)even);
-    if (steps > 1) fill((lds_u8*)odd);
-  };
-
-  f32x4 acc[MI][NJ];
-  // s_waitcnt's operands: for the loads, and for all but the newest stores of a tile
+  // s_waitcnt's operands: for all loads and stores, and for all but the newest stores, as many as every wave makes of a whole tile
   constexpr int kStores = MI * NJ / (sizeof(T) == 2 ? 2 : 1);
-  constexpr int kLoads = 15 << 8 | 7 << 4, kBehindStores = (kStores & 15) | (kStores >> 4) << 14 | kLoads;
   static_assert(kStores < 64, "s_waitcnt counts to 63");
+  constexpr int kWaitAll = 7 << 4 | 15 << 8, kWaitStored = (kStores & 15) | (kStores >> 4) << 14 | kWaitAll;
   auto meet = [&]() __attribute__((always_inline)) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   };
+
+  // What is loaded runs two steps ahead of what is multiplied (a checkpoint's codes, through their registers, three), from tile to tile;
+  // behind the last tile there is nothing left to load, and the loads give zeros.
+  LoadA a;
+  LoadB b;
+  a.set_up(p.lda, wave, lane);
+  if constexpr (CODED)
+    b.set_up(p);
+  else
+    b.set_up(p.ldb, wave, lane);
+  auto steps_of = [&](const Tile& tile, int64_t& r0, int64_t& end) __attribute__((always_inline)) {
+    r0 = tile.split * p.per_split;
+    end = r0 + p.per_split < p.depth ? r0 + p.per_split : p.depth;
+    return (int)((end - r0 + Mma<T>::kStep - 1) / Mma<T>::kStep);
+  };
+  struct Feed {
+    int turn = 0, left = 0;
+  } feed, code_feed;
+  auto feed_tile = [&]() __attribute__((always_inline)) {
+    if (feed.left == 0) {
+      Tile next;
+      feed.left = 0x7fffffff;
+      if (tile_of(p, feed.turn, next)) {
+        int64_t r0, end;
+        feed.left = steps_of(next, r0, end);
+        a.start(p.a, p.lda, next.i * BM, p.rows, end, r0);
+        if constexpr (!CODED) b.start(p.b, p.ldb, next.j * BN, p.cols, end, r0);
+        if constexpr (FORWARD) {
+          Window bias;
+          if (p.bias) {
+            bias.base = (const char*)p.bias + next.j * BN * (int)sizeof(T);
+            bias.left = (p.cols - next.j * BN) * (int64_t)sizeof(T);
+          }
+          const int part = wave % (BN / 64) * 64;
+          load_to_lds<sizeof(T)>(bias.rsrc(), (part + lane) * (uint32_t)sizeof(T), (lds_u8*)&biases[feed.turn & 3][part]);
+        }
+        feed.turn++;
+      } else {
+        a.stop();
+        if constexpr (!CODED) b.stop();
+      }
+    }
+    feed.left--;
+  };
+  auto fetch_codes = [&]() __attribute__((always_inline)) {
+    if constexpr (CODED) {
+      if (code_feed.left == 0) {
+        Tile next;
+        code_feed.left = 0x7fffffff;
+        if (tile_of(p, code_feed.turn, next)) {
+          int64_t r0, end;
+          code_feed.left = steps_of(next, r0, end);
+          b.start(p, next.j * BN, end, r0);
+          code_feed.turn++;
+        } else {
+          b.stop();
+        }
+      }
+      code_feed.left--;
+      b.fetch();
+    }
+  };
+  // The loads of a step, spread over the products: the card's address units take 64 bytes a clock, and a wave that waits for them to take
+  // one more issues no product (all at once after the barrier: 8192^3 in 877 us instead of %FIX%).
+  auto issue_a = [&](int n, int of, int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = n * LoadA::kLoads / of; q < (n + 1) * LoadA::kLoads / of; q++) a.issue(q, a_ring + slot * kA);
+    if (n + 1 == of) a.advance();
+  };
+  auto issue_b = [&](int n, int of, int slot) __attribute__((always_inline)) {
+    if constexpr (!CODED) {
+#pragma unroll
+      for (int q = n * LoadB::kLoads / of; q < (n + 1) * LoadB::kLoads / of; q++) b.issue(q, b_ring + slot * kB);
+      if (n + 1 == of) b.advance();
+    }
+  };
+  auto put_codes = [&](int slot) __attribute__((always_inline)) {
+    if constexpr (CODED) {
+#pragma unroll
+      for (int q = 0; q < LoadB::kPieces; q++) b.put(q, b_ring + slot * kB);
+    }
+  };
+
+  f32x4 acc[MI][NJ];
   // A step is four phases: (first, second half of the fragments along r) x (upper, lower half of the wave's rows).  Each phase
   // multiplies what was read from LDS in the phase before and reads for the next; B's fragments are replaced one by one as soon as their
   // last product is under way, which leaves the registers to the sums.  After the third phase nothing is left to read of
-  // the present tiles: once every wave is there and the next tiles have arrived, the present ones' memory takes those after the next.
+  // the step: once every wave is there and the next step has arrived, its memory takes the step after the next.
   Frag fa[2][MH], fb[NJ];
-  auto read_a = [&](const lds_u8* tile, int kk, int half, Frag (&f)[MH]) __attribute__((always_inline)) {
+  auto read_a = [&](int slot, int kk, int half, Frag (&f)[MH]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int m = 0; m < MH; m++) f[m] = TileRead<T, BM, A_STRIDED>::get(tile, wi * (BM / WI) + (half * MH + m) * 16, kk, lane);
+    for (int m = 0; m < MH; m++) f[m] = TileRead<T, BM, A_STRIDED>::get(a_ring + slot * kA, wi * (BM / WI) + (half * MH + m) * 16, kk, lane);
   };
-  auto read_b = [&](const lds_u8* tile, int kk, int n) __attribute__((always_inline)) {
-    fb[n] = TileRead<T, BN, B_KIND != B_ROWS>::get(tile + BM * 128, wj * (BN / WJ) + n * 16, kk, lane);
+  auto read_b = [&](int slot, int kk, int n) __attribute__((always_inline)) {
+    fb[n] = TileRead<T, BN, B_KIND != B_ROWS>::get(b_ring + slot * kB, wj * (BN / WJ) + n * 16, kk, lane);
   };
   auto multiply = [&](const Frag (&x)[MH], int half, int n) __attribute__((always_inline)) {
 #pragma unroll
     for (int m = 0; m < MH; m++) acc[half * MH + m][n] = Mma<T>::run(fb[n], x[m], acc[half * MH + m][n]);
   };
-  auto step = [&](lds_u8* now, lds_u8* next, int t) __attribute__((always_inline)) {
-    read_a(now, 0, 1, fa[1]);
-#pragma unroll
-    for (int n = 0; n < NJ; n++) multiply(fa[0], 0, n);
-    __builtin_amdgcn_sched_barrier(0);
-    read_a(now, 1, 0, fa[0]);
-#pragma unroll
-    for (int n = 0; n < NJ; n++) {
-      multiply(fa[1], 1, n);
-      read_b(now, 1, n);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    read_a(now, 1, 1, fa[1]);
-#pragma unroll
-    for (int n = 0; n < NJ; n++) multiply(fa[0], 0, n);
-    __builtin_amdgcn_sched_barrier(0);
-    if (t > 0) __builtin_amdgcn_s_waitcnt(kLoads);      // a tile's first two steps were waited for before it began
-    meet();
-    // behind a tile's last step these read what is there and nobody uses it
-    read_a(next, 0, 0, fa[0]);
-    if (t + 2 < steps) fill(now);
-#pragma unroll
-    for (int n = 0; n < NJ; n++) {
-      multiply(fa[1], 1, n);
-      read_b(next, 0, n);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  lds_u8* const first = (lds_u8*)even;
-  lds_u8* const second = (lds_u8*)odd;
 
-  // A workgroup takes tile after tile.  The next one's first two steps are asked for before the present one's results are stored, and
-  // the stores of a whole tile go on while the next one is multiplied.
+  // A workgroup takes tile after tile, and the stores of a whole tile go on while the next one is multiplied: they are newer than the
+  // loads of its first two steps.
   Tile tile;
   if (!tile_of(p, 0, tile)) return;
-  begin(tile);
-  __builtin_amdgcn_s_waitcnt(kLoads);
+  fetch_codes();
+#pragma unroll
+  for (int slot = 0; slot < 2; slot++) {
+    feed_tile();
+    issue_a(0, 1, slot);
+    issue_b(0, 1, slot);
+    put_codes(slot);
+    fetch_codes();
+  }
+  __builtin_amdgcn_s_waitcnt(kWaitAll);
+  meet();
+  bool stored = false;
+  int now = 0;      // the step's place
   for (int turn = 1;; turn++) {
-    if (FORWARD && threadIdx.x < BN) biases[turn & 1][threadIdx.x] = own_bias;
-    meet();
 #pragma unroll
     for (int m = 0; m < MI; m++)
 #pragma unroll
       for (int n = 0; n < NJ; n++) acc[m][n] = f32x4{0, 0, 0, 0};
-    read_a(first, 0, 0, fa[0]);
+    int64_t r0, end;
+    const int steps = steps_of(tile, r0, end);
+    read_a(now, 0, 0, fa[0]);
 #pragma unroll
-    for (int n = 0; n < NJ; n++) read_b(first, 0, n);
-    for (int t = 0; t < steps; t += 2) {
-      step(first, second, t);
-      if (t + 1 < steps) step(second, first, t + 1);
+    for (int n = 0; n < NJ; n++) read_b(now, 0, n);
+    for (int t = 0; t < steps; t++) {
+      const int next = now ^ 1;
+      read_a(now, 0, 1, fa[1]);
+#pragma unroll
+      for (int n = 0; n < NJ; n++) {
+        multiply(fa[0], 0, n);
+        if (t > 0) issue_b(n, NJ, next);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      read_a(now, 1, 0, fa[0]);
+#pragma unroll
+      for (int n = 0; n < NJ; n++) {
+        multiply(fa[1], 1, n);
+        read_b(now, 1, n);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      read_a(now, 1, 1, fa[1]);
+#pragma unroll
+      for (int n = 0; n < NJ; n++) multiply(fa[0], 0, n);
+      __builtin_amdgcn_sched_barrier(0);
+      if (stored && t == 0)
+        __builtin_amdgcn_s_waitcnt(kWaitStored);
+      else
+        __builtin_amdgcn_s_waitcnt(kWaitAll);
+      meet();
+      // behind a tile's last step these read the next tile's first one, which is read again when that begins
+      read_a(next, 0, 0, fa[0]);
+      feed_tile();
+      put_codes(now);
+      fetch_codes();
+#pragma unroll
+      for (int n = 0; n < NJ; n++) {
+        multiply(fa[1], 1, n);
+        read_b(next, 0, n);
+        issue_a(n, NJ, now);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      now = next;
     }
+    issue_b(0, 1, now ^ 1);      // of the step that the last one made room for: ahead of the stores
     const Tile done = tile;
     const bool more = tile_of(p, turn, tile);
-    if (more) begin(tile);
+    if (!more) __builtin_amdgcn_s_waitcnt(kWaitAll);      // no load is on its way to LDS when the workgroup ends
     __builtin_amdgcn_sched_barrier(0);
 
     const int i0 = done.i * BM, j0 = done.j * BN;
@@ -1084,7 +1176,10 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
     if constexpr (FORWARD) {
 #pragma unroll
       for (int n = 0; n < NJ; n++) {
-        const f32x4 v = *(const f32x4*)&biases[turn & 1][wj * (BN / WJ) + n * 16 + (l >> 4) * 4];
+        const u32x4 held = *(const u32x4*)&biases[(turn - 1) & 3][wj * (BN / WJ) + n * 16 + (l >> 4) * 4];
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = low_value<T>(held[e]);
 #pragma unroll
         for (int m = 0; m < MI; m++) acc[m][n] += v;
       }
@@ -1220,11 +1315,7 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
       }
     }
     if (!more) return;
-    // the next tile's first loads are older than this tile's stores, every one of which every wave has made of a whole tile
-    if (whole && (partial || p.wide))
-      __builtin_amdgcn_s_waitcnt(kBehindStores);
-    else
-      __builtin_amdgcn_s_waitcnt(kLoads);
+    stored = whole && (partial || p.wide);
   }
 }
 
@@ -1379,7 +1470,7 @@ int sum_rows(const float* partial, int64_t count, int64_t stride, int64_t cols, 
   return launch_status();
 }
 
-// workgroups of a tile whose LDS (two steps of both operands, and up to 12 KB beside them) a compute unit holds
+// workgroups of a tile whose LDS (two steps of both operands, and up to 14 KB beside them) a compute unit holds
 constexpr int slots_per_cu(int bm, int bn) { return bm + bn <= 128 ? 4 : bm + bn <= 256 ? 2 : 1; }
 struct Tiles {
   int bm, bn, splits;
@@ -1403,7 +1494,7 @@ int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s)
 
 template <typename T, int ACT>
 int forward_product(ProductArgs& p, hipStream_t s) {
-  const int64_t step = 128 / (int)sizeof(T), depth = (p.depth + step - 1) / step * step;
+  const int64_t step = Mma<T>::kStep, depth = (p.depth + step - 1) / step * step;
   auto tiles = [&](int bm, int bn) { return (int64_t)((p.rows + bm - 1) / bm) * ((p.cols + bn - 1) / bn); };
   const bool large = sizeof(T) == 2 && tiles(256, 256) >= kComputeUnits;
   // the pre-activation's codes need a whole group of columns in a tile; without an activation nobody asks for them
@@ -1412,7 +1503,7 @@ int forward_product(ProductArgs& p, hipStream_t s) {
       if constexpr (sizeof(T) == 2)
         if (large) return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
       if (tiles(128, 256) >= kComputeUnits / 2) return launch_product<T, 128, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
-      return launch_product<T, 64, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
+      return launch_product<T, 64, 256, 1, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
     }
   }
   if constexpr (sizeof(T) == 2)
