@@ -181,12 +181,21 @@ __device__ __forceinline__ void eight_values(u32x2 w, float inv, float lo, float
 // ---- activations: act(z) and act'(z) ----
 enum { ACT_NONE = GACT_ACT_NONE, ACT_GELU = GACT_ACT_GELU, ACT_GELU_TANH = GACT_ACT_GELU_TANH, ACT_SILU = GACT_ACT_SILU };
 // Exact to float's rounding for float; for 16-bit types, whose own rounding is at least 2^-12, the hardware's exponential and reciprocal and a
-// polynomial: 1 - Phi(|z|) = exp(-z^2/2) q(t), t = 1 / (1 + 0.425 |z| / sqrt 2), q of degree 6 fitted to erfc over [0, 9.5] (relative error 1e-5,
-// absolute error of Phi 4.3e-7).  In the epilogue of a product the library's erfc takes as long as the product of 1024 columns.
+// polynomial: log2(2 (1 - Phi(a))), a >= 0, is smooth, and a fit of degree 7 over [0, 6] gives 1 - Phi(a) to 3e-6 of itself (and falls beyond).
+// In the epilogue of a product of 1024 columns the library's erfc takes as long as the product, a quotient of polynomials a quarter of it.
 template <bool EXACT>
 __device__ __forceinline__ float sigmoid(float x) {
   if (EXACT) return 1.0f / (1.0f + expf(-x));
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
+}
+__device__ __forceinline__ float twice_upper_tail(float a) {
+  float p = __builtin_fmaf(a, -1.79147102e-06f, 6.08547037e-05f);
+  p = __builtin_fmaf(a, p, -0.000925627672f);
+  p = __builtin_fmaf(a, p, 0.00849229447f);
+  p = __builtin_fmaf(a, p, -0.0539352561f);
+  p = __builtin_fmaf(a, p, -0.458482679f);
+  p = __builtin_fmaf(a, p, -1.15124609f);
+  return __builtin_amdgcn_exp2f(a * p);
 }
 // the normal distribution's cumulative function and exp(-z^2/2)
 template <bool EXACT>
@@ -197,19 +206,17 @@ __device__ __forceinline__ void normal_cdf(float z, float& cdf, float& e) {
     return;
   }
   e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
-  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fabsf(z), 0.30052038200428270f, 1.0f));
-  float q = __builtin_fmaf(t, -0.079363826f, 0.2208909465f);
-  q = __builtin_fmaf(t, q, -0.02224172415f);
-  q = __builtin_fmaf(t, q, 0.1470668855f);
-  q = __builtin_fmaf(t, q, 0.113310361f);
-  q = __builtin_fmaf(t, q, 0.120337111f);
-  q = t * e * q;
+  const float q = 0.5f * twice_upper_tail(__builtin_fabsf(z));
   cdf = z < 0.0f ? q : 1.0f - q;
 }
 template <bool EXACT>
 __device__ __forceinline__ float activated(float z, int act) {
   switch (act) {
     case ACT_GELU: {
+      if (!EXACT) {      // max(z, 0) - |z| (1 - Phi(|z|)); the bound keeps an infinite z from meeting a tail of zero
+        const float a = __builtin_fabsf(z);
+        return 0.5f * __builtin_fmaf(-__builtin_amdgcn_fmed3f(a, 0.0f, 3e38f), twice_upper_tail(a), z + a);
+      }
       float cdf, e;
       normal_cdf<EXACT>(z, cdf, e);
       return z * cdf;
@@ -248,6 +255,8 @@ __device__ __forceinline__ float slope(float z, int act) {
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Checkpoints of rows.  32 lanes own a group: one 16-byte piece each (float: two), its minimum and maximum over the half wave.
 // ---------------------------------------------------------------------------------------------------------------------------------
+// One group at a time: four to a half wave, with their loads together and one division for all of their scales, take 84 us instead of 90 for
+// 134 M halves, but 14 instead of 11.5 for 10 M.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int groups,
                                                          uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale,
@@ -262,14 +271,12 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x
   float lo = __builtin_inff(), hi = -__builtin_inff();
 #pragma unroll
   for (int e = 0; e < kVec; e++)
-    if (e < n) lo = __builtin_fminf(lo, v[e]), hi = __builtin_fmaxf(hi, v[e]);
+    if ((WHOLE ? 0 : e) < n) lo = __builtin_fminf(lo, v[e]), hi = __builtin_fmaxf(hi, v[e]);
   lo = over_lanes<Least, 32>(lo);
   hi = over_lanes<Most, 32>(hi);
   const float s = scale_of(lo, hi);
-  if (n > 0) {
-    const u32x2 w = {four_codes(v[0], v[1], v[2], v[3], lo, s), four_codes(v[4], v[5], v[6], v[7], lo, s)};
-    *(u32x2*)(codes + row * ldc + col) = w;
-  }
+  if (n > 0)
+    *(u32x2*)(codes + row * ldc + col) = u32x2{four_codes(v[0], v[1], v[2], v[3], lo, s), four_codes(v[4], v[5], v[6], v[7], lo, s)};
   if (lane == 0) {
     scale[unit] = s;
     mn[unit] = lo;
@@ -1056,7 +1063,7 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
     }
   };
   // The loads of a step, spread over the products: the card's address units take 64 bytes a clock, and a wave that waits for them to take
-  // one more issues no product (all at once after the barrier: 8192^3 in 877 us instead of %FIX%).
+  // one more issues no product.
   auto issue_a = [&](int n, int of, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int q = n * LoadA::kLoads / of; q < (n + 1) * LoadA::kLoads / of; q++) a.issue(q, a_ring + slot * kA);
@@ -1370,16 +1377,19 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(ProductArgs p) {
     x[m] = (const T*)p.a + row * p.lda;
     acc[m] = f32x4{0, 0, 0, 0};
   }
-  constexpr int UNROLL = 4;
-  for (int64_t k0 = (int64_t)wave * SPAN * UNROLL; k0 < p.depth; k0 += (int64_t)WAVES * SPAN * UNROLL) {
+  // the waves take steps of 64 bytes in turn, UNROLL of them with all their loads on the way
+  constexpr int UNROLL = !WHOLE ? 2 : MT == 4 ? 4 : 8;
+  for (int64_t k0 = (int64_t)wave * SPAN; k0 < p.depth; k0 += (int64_t)WAVES * SPAN * UNROLL) {
     typename Mma<T>::Frag fw[UNROLL], fx[UNROLL][MT];
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
-      const int64_t k = k0 + u * SPAN + g * (16 / (int)sizeof(T));
+      const int64_t k = k0 + u * WAVES * SPAN + g * (16 / (int)sizeof(T));
       fw[u] = fragment_of<T, WHOLE>(w, k, p.depth);
-#pragma unroll
-      for (int m = 0; m < MT; m++) fx[u][m] = fragment_of<T, WHOLE>(x[m], k, p.depth);
     }
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+      for (int m = 0; m < MT; m++) fx[u][m] = fragment_of<T, WHOLE>(x[m], k0 + u * WAVES * SPAN + g * (16 / (int)sizeof(T)), p.depth);
 #pragma unroll
     for (int u = 0; u < UNROLL; u++)
 #pragma unroll
@@ -1719,9 +1729,12 @@ int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
         return launch_status();
       };
       using std::integral_constant;
-      if (rows <= 16) return run(integral_constant<int, 1>{}, integral_constant<int, 8>{});
-      if (rows <= 32) return run(integral_constant<int, 2>{}, integral_constant<int, 8>{});
-      return run(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+      // 16 waves where their depth is long: one turn of eight loads each up to 4096 halves (a workgroup has 16 columns, and few columns are few
+      // workgroups: 24 rows, 4096 to 1024 halves 13.4 us with 8 waves, 9.0 with 16)
+      auto by_depth = [&](auto mt) { return inner * (int)sizeof(T) >= 4096 ? run(mt, integral_constant<int, 16>{}) : run(mt, integral_constant<int, 8>{}); };
+      if (rows <= 16) return by_depth(integral_constant<int, 1>{});
+      if (rows <= 32) return by_depth(integral_constant<int, 2>{});
+      return by_depth(integral_constant<int, 4>{});
     }
     switch (activation) {
       case GACT_ACT_GELU: return forward_product<T, ACT_GELU>(p, s);

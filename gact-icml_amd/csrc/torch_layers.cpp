@@ -161,6 +161,8 @@ variable_list once(variable_list grads, const char* name) {
   if (!c10::GradMode::is_enabled()) return grads;
   const auto stop = std::make_shared<torch::autograd::DelayedError>(
       std::string("trying to differentiate twice a function that was marked with @once_differentiable: ") + name, (int64_t)grads.size());
+  for (at::Tensor& g : grads)      // the error's node hangs on tensors that need a gradient, which the result does through what was saved
+    if (g.defined()) g = g.detach().set_requires_grad(true);
   return (*stop)(std::move(grads));
 }
 void give_up(SavedVariable& v) { v.reset_data(); }

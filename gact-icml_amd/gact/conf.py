@@ -39,6 +39,12 @@ class QuantizationConfig:
         # reference's uint8 rule never sees.  They are packed to one bit per element, losslessly.
         self.compress_bool_masks = True
 
+        # ---- layers on 8-bit checkpoints (not in the reference) ----
+        # While the Controller's hooks are installed, the model's nn.Linear and nn.LayerNorm run on gact.ops.op_linear and
+        # op_layer_norm: they keep their input as 8-bit codes, rounded to nearest, which their backward kernels read where they
+        # lie.  What the other layers save goes through the hooks as before; `bit` and auto precision do not touch these.
+        self.checkpoint_layers = False
+
         # ---- seeds in device memory (not in the reference) ----
         # The iteration count that is added to every tensor's seed is read by the kernels from a word in device
         # memory instead of travelling as a launch argument.  Same noise; needed when the hooked pass is

@@ -7,6 +7,7 @@ import bisect
 
 import torch
 
+from . import layers
 from .autoprec import AutoPrecision
 from .conf import config
 from .quantizer import Quantizer
@@ -31,6 +32,7 @@ def _to_pinned_host(t):
 class Controller:
     def __init__(self, model):
         self._hooked = False
+        self._attached = []      # config.checkpoint_layers: the modules that run on checkpoints while the hooks are installed
         if not config.compress_activation:
             return      # hooks still work: they pass tensors through (or swap them when config.swap is set)
         self.model = model
@@ -49,6 +51,8 @@ class Controller:
 
     # ---- hooks (controller.py:53-60 of the reference: the default saved-tensor hooks of autograd) ----
     def install_hook(self):
+        if config.checkpoint_layers and config.compress_activation:
+            self._attached += layers.attach(self.model)
         _hooks._push_saved_tensors_default_hooks(self.quantize, self.dequantize)
         self._hooked = True
 
@@ -56,6 +60,8 @@ class Controller:
         if getattr(self, "_hooked", False):
             _hooks._pop_saved_tensors_default_hooks()
             self._hooked = False
+            layers.detach(self._attached)
+            self._attached = []
 
     def __enter__(self):
         self.install_hook()

@@ -16,6 +16,7 @@ The public names are in ``gact.ops``; nothing of this is in the reference, whose
 import collections
 
 import torch
+import torch.nn as nn
 
 from .cpp_extension import _abi
 
@@ -77,3 +78,50 @@ def op_linear(input, weight, bias=None, activation=None, residual=None):
     if torch.is_autocast_enabled("cuda"):
         input, weight, bias, residual = _cast(torch.get_autocast_dtype("cuda"), input, weight, bias, residual)
     return _abi.native().linear(input, weight, bias, act, residual)
+
+
+# ---- modules ----
+def _taken(module, input, most):
+    """Whether the operator takes this call of the module: anything else goes to torch's own."""
+    w = module.weight if module.weight is not None else input
+    return (input.is_cuda and w.is_cuda and input.device == w.device and input.layout is torch.strided and input.dim() >= 1
+            and input.dtype in (torch.float32, torch.float16, torch.bfloat16) and 0 < input.shape[-1] <= most
+            and (input.dtype is w.dtype or torch.is_autocast_enabled("cuda")) and not torch.overrides.has_torch_function((input, w))
+            and not torch._C._functorch.is_functorch_wrapped_tensor(input))
+
+
+class CheckpointedLinear(nn.Linear):
+    """nn.Linear on op_linear."""
+
+    def forward(self, input):
+        if _taken(self, input, 262144) and self.out_features <= 262144 and input.shape[-1] == self.in_features:
+            return op_linear(input, self.weight, self.bias)
+        return super().forward(input)
+
+
+class CheckpointedLayerNorm(nn.LayerNorm):
+    """nn.LayerNorm over the last dimension on op_layer_norm."""
+
+    def forward(self, input):
+        if len(self.normalized_shape) == 1 and _taken(self, input, 16384) and input.shape[-1] == self.normalized_shape[0]:
+            return op_layer_norm(input, self.weight, self.bias, self.eps)
+        return super().forward(input)
+
+
+_CHECKPOINTED = {nn.Linear: CheckpointedLinear, nn.LayerNorm: CheckpointedLayerNorm}
+
+
+def attach(model):
+    """The model's linear layers and layer norms (of exactly these classes) run on the operators from now on; returns them for detach."""
+    changed = [m for m in model.modules() if type(m) in _CHECKPOINTED]
+    for m in changed:
+        m.__class__ = _CHECKPOINTED[type(m)]      # parameters, hooks and copies of the module stay as they are
+    return changed
+
+
+def detach(changed):
+    """What attach returned, as torch's own again."""
+    for m in changed:
+        for own, checkpointed in _CHECKPOINTED.items():
+            if type(m) is checkpointed:
+                m.__class__ = own
