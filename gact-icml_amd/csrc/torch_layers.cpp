@@ -9,6 +9,7 @@
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
@@ -17,6 +18,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <cstdint>
@@ -156,6 +158,24 @@ void no_tangent(const std::optional<at::Tensor>& t, const char* operation) {
   TORCH_CHECK(!t.has_value() || !torch::autograd::isFwGradDefined(*t), operation, " has no forward-mode derivative");
 }
 
+// A leaf whose gradient's accumulator was made on the default stream - an eager graph of it is still alive - cannot be differentiated in a
+// pass that is being captured: autograd would make the default stream wait for the capture, which the runtime answers by ending it, and
+// torch by ending the process.
+void refuse_stale_leaves(std::initializer_list<const at::Tensor*> tensors, const at::Tensor& like) {
+  const c10::hip::HIPStream current = c10::hip::getCurrentHIPStream(like.device().index());
+  hipStreamCaptureStatus status;
+  if (current.stream() == nullptr || hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  for (const at::Tensor* t : tensors) {
+    if (!t || !t->requires_grad() || !t->is_leaf()) continue;
+    const std::shared_ptr<Node> accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!accumulator) continue;
+    const std::optional<c10::Stream> stream = accumulator->stream();
+    TORCH_CHECK(!stream || stream->id() != 0,
+                "a training pass is captured while an eager graph of one of its leaves, made on the default stream, is alive: drop it first");
+  }
+}
+const at::Tensor* held(const std::optional<at::Tensor>& t) { return t ? &*t : nullptr; }
+
 // results of a backward pass that is itself being differentiated: an error once somebody goes through them
 variable_list once(variable_list grads, const char* name) {
   if (!c10::GradMode::is_enabled()) return grads;
@@ -216,6 +236,7 @@ at::Tensor layer_norm(const at::Tensor& input, const std::optional<at::Tensor>& 
   for (const auto& t : {std::optional<at::Tensor>(input), weight, bias}) no_tangent(t, "op_layer_norm");
   const int64_t cols = input.size(-1);
   const bool keep = torch::autograd::compute_requires_grad(input, weight, bias);
+  if (keep) refuse_stale_leaves({&input, held(weight), held(bias)}, input);
   at::Tensor y;
   Kept k;
   at::Tensor stats;
@@ -328,6 +349,7 @@ at::Tensor linear(const at::Tensor& input, const at::Tensor& weight, const std::
   }
   for (const auto& t : {std::optional<at::Tensor>(input), std::optional<at::Tensor>(weight), bias, residual}) no_tangent(t, "op_linear");
   const bool needs = torch::autograd::compute_requires_grad(input, weight, bias, residual);
+  if (needs) refuse_stale_leaves({&input, &weight, held(bias), held(residual)}, input);
   const bool keep_x = needs && weight.requires_grad();
   const bool keep_z = needs && activation != GACT_ACT_NONE && torch::autograd::compute_requires_grad(input, weight, bias);
   at::Tensor y;

@@ -239,6 +239,31 @@ def test_captured_training_steps_replay_like_eager_ones(dtype):
         torch.cuda.synchronize()
 
 
+def test_a_capture_beside_an_eager_graph_of_its_leaves_is_refused():
+    """By the operator, before anything of autograd's is captured; without the eager graph the same capture goes through."""
+    x, w = normal(40, 32).requires_grad_(), normal(24, 32, seed=1).requires_grad_()
+    nw = torch.ones(32, device="cuda", requires_grad=True)
+    eager = ops.op_linear(ops.op_layer_norm(x, nw), w)
+    for call in (lambda: ops.op_linear(x, w), lambda: ops.op_layer_norm(x, nw)):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph of one of its leaves"):
+            with torch.cuda.graph(graph):
+                call()
+        with torch.no_grad():
+            call()
+    want = torch.autograd.grad(eager, [x, w, nw], torch.ones_like(eager))
+    del eager
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.op_linear(ops.op_layer_norm(x, nw), w)
+        got = torch.autograd.grad(y, [x, w, nw], torch.ones_like(y))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_two_streams_at_once():
     x, p = normal(2048, 256, dtype=torch.bfloat16), [t.detach() for t in block_parameters(256, 1024, torch.bfloat16)]
     dy = normal(2048, 256, dtype=torch.bfloat16, seed=9)
