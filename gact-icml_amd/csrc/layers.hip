@@ -859,30 +859,26 @@ struct CodeLoad {
     mn.advance(stat_step);
     left -= Mma<T>::kStep;
   }
-  // piece q's values
-  __device__ __forceinline__ void put(int q, lds_u8* tile) const {
-    const int t = threadIdx.x;
+  // Part k of the thread's values: 16 bytes of them.  One part behind each few products: all at once, after the barrier, they keep the matrix
+  // units waiting.
+  static constexpr int kParts = kPieces * (int)sizeof(T);
+  __device__ __forceinline__ void put(int k, lds_u8* tile) const {
+    const int t = threadIdx.x, q = k / (int)sizeof(T), h = k % (int)sizeof(T);
     if (kTotal < WAVES * 64 && t >= kTotal) return;      // floats of a small tile: fewer pieces than threads
     const uint32_t row = t / kAcross + q * kApart, block = t % kAcross;
     const float inv = (int)row < held_left ? inverse_of(s[q]) : 0.0f;      // rows behind the last one: zeros
-    lds_u8* to = tile + row * (COUNT * (int)sizeof(T)) + (block ^ Mma<T>::template block_turn<COUNT>(row)) * Mma<T>::kBlock;
+    lds_u8* to = tile + row * (COUNT * (int)sizeof(T)) + (block ^ Mma<T>::template block_turn<COUNT>(row)) * Mma<T>::kBlock + 16 * h;
     if constexpr (sizeof(T) == 2) {
       typedef T T8 __attribute__((ext_vector_type(8)));
+      T8 v;
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        T8 v;
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = (T)__builtin_fmaf(code_at(held[q][2 * h + (e >> 2)], e & 3), inv, lo[q]);
-        *(__attribute__((address_space(3))) T8*)(to + 16 * h) = v;
-      }
+      for (int e = 0; e < 8; e++) v[e] = (T)__builtin_fmaf(code_at(held[q][2 * h + (e >> 2)], e & 3), inv, lo[q]);
+      *(__attribute__((address_space(3))) T8*)to = v;
     } else {
+      f32x4 v;
 #pragma unroll
-      for (int h = 0; h < 4; h++) {
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(code_at(held[q][h], e), inv, lo[q]);
-        *(__attribute__((address_space(3))) f32x4*)(to + 16 * h) = v;
-      }
+      for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(code_at(held[q][h], e), inv, lo[q]);
+      *(__attribute__((address_space(3))) f32x4*)to = v;
     }
   }
 };
@@ -1076,10 +1072,10 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
       if (n + 1 == of) b.advance();
     }
   };
-  auto put_codes = [&](int slot) __attribute__((always_inline)) {
+  auto put_codes = [&](int n, int of, int slot) __attribute__((always_inline)) {
     if constexpr (CODED) {
 #pragma unroll
-      for (int q = 0; q < LoadB::kPieces; q++) b.put(q, b_ring + slot * kB);
+      for (int k = n * LoadB::kParts / of; k < (n + 1) * LoadB::kParts / of; k++) b.put(k, b_ring + slot * kB);
     }
   };
 
@@ -1111,7 +1107,7 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
     feed_tile();
     issue_a(0, 1, slot);
     issue_b(0, 1, slot);
-    put_codes(slot);
+    put_codes(0, 1, slot);
     fetch_codes();
   }
   __builtin_amdgcn_s_waitcnt(kWaitAll);
@@ -1156,15 +1152,23 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
       // behind a tile's last step these read the next tile's first one, which is read again when that begins
       read_a(next, 0, 0, fa[0]);
       feed_tile();
-      put_codes(now);
-      fetch_codes();
 #pragma unroll
       for (int n = 0; n < NJ; n++) {
         multiply(fa[1], 1, n);
         read_b(next, 0, n);
+        put_codes(n, NJ, now);
         issue_a(n, NJ, now);
+        if constexpr (CODED) {
+          // one product, then as much of the conversion as it leaves time for
+#pragma unroll
+          for (int m = 0; m < MH; m++) {
+            __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(2, 8, 0);
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
+      fetch_codes();
       now = next;
     }
     issue_b(0, 1, now ^ 1);      // of the step that the last one made room for: ahead of the stores
