@@ -179,7 +179,7 @@ __device__ __forceinline__ void eight_values(u32x2 w, float inv, float lo, float
 }
 
 // ---- activations: act(z) and act'(z) ----
-enum { ACT_NONE = GACT_ACT_NONE, ACT_GELU = GACT_ACT_GELU, ACT_GELU_TANH = GACT_ACT_GELU_TANH, ACT_SILU = GACT_ACT_SILU };
+enum { ACT_UNFINISHED = -1, ACT_NONE = GACT_ACT_NONE, ACT_GELU = GACT_ACT_GELU, ACT_GELU_TANH = GACT_ACT_GELU_TANH, ACT_SILU = GACT_ACT_SILU };
 // Exact to float's rounding for float; for 16-bit types, whose own rounding is at least 2^-12, the hardware's exponential and reciprocal and a
 // polynomial: log2(2 (1 - Phi(a))), a >= 0, is smooth, and a fit of degree 7 over [0, 6] gives 1 - Phi(a) to 3e-6 of itself (and falls beyond).
 // In the epilogue of a product of 1024 columns the library's erfc takes as long as the product, a quotient of polynomials a quarter of it.
@@ -974,7 +974,7 @@ enum { B_ROWS = 0, B_STRIDED = 1, B_CODES = 2 };
 template <typename T, int BM, int BN, int WI, int WJ, bool A_STRIDED, int B_KIND, int ACT, bool CODES>
 __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
   constexpr int WAVES = WI * WJ, MI = BM / WI / 16, MH = MI / 2, NJ = BN / WJ / 16;
-  constexpr bool FORWARD = B_KIND == B_ROWS, CODED = B_KIND == B_CODES;
+  constexpr bool FORWARD = B_KIND == B_ROWS && ACT != ACT_UNFINISHED, CODED = B_KIND == B_CODES;
   using Frag = typename Mma<T>::Frag;
   using LoadA = TileLoad<T, BM, A_STRIDED, WAVES>;
   using LoadB = std::conditional_t<CODED, CodeLoad<T, BN, WAVES>, TileLoad<T, BN, B_KIND == B_STRIDED, WAVES>>;
@@ -1259,7 +1259,7 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
         }
       }
     }
-    const bool partial = !FORWARD && p.splits > 1;
+    const bool partial = ACT == ACT_UNFINISHED || (!FORWARD && p.splits > 1);
     {
       if (partial || (p.wide && sizeof(T) == 4)) {      // 16 bytes are the four columns that a lane holds
 #pragma unroll
@@ -1365,8 +1365,9 @@ __device__ __forceinline__ typename Mma<T>::Frag fragment_of(const T* row, int64
   }
   return f;
 }
-template <typename T, int MT, int WAVES, bool WHOLE>
-__global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(ProductArgs p) {
+template <typename T, int MT, bool WHOLE>
+__global__ __launch_bounds__(512) void few_rows_kernel(ProductArgs p) {
+  constexpr int WAVES = 8;
   constexpr int SPAN = 4 * 16 / (int)sizeof(T);      // values along r of a fragment step of the wave
   __shared__ f32x4 shared[WAVES][MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
@@ -1383,17 +1384,19 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(ProductArgs p) {
   }
   // the waves take steps of 64 bytes in turn, UNROLL of them with all their loads on the way
   constexpr int UNROLL = !WHOLE ? 2 : MT == 4 ? 4 : 8;
-  for (int64_t k0 = (int64_t)wave * SPAN; k0 < p.depth; k0 += (int64_t)WAVES * SPAN * UNROLL) {
+  const int split = blockIdx.y;
+  const int64_t first = split * p.per_split, end = first + p.per_split < p.depth ? first + p.per_split : p.depth;
+  for (int64_t k0 = first + wave * SPAN; k0 < end; k0 += (int64_t)WAVES * SPAN * UNROLL) {
     typename Mma<T>::Frag fw[UNROLL], fx[UNROLL][MT];
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
       const int64_t k = k0 + u * WAVES * SPAN + g * (16 / (int)sizeof(T));
-      fw[u] = fragment_of<T, WHOLE>(w, k, p.depth);
+      fw[u] = fragment_of<T, WHOLE>(w, k, end);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; u++)
 #pragma unroll
-      for (int m = 0; m < MT; m++) fx[u][m] = fragment_of<T, WHOLE>(x[m], k0 + u * WAVES * SPAN + g * (16 / (int)sizeof(T)), p.depth);
+      for (int m = 0; m < MT; m++) fx[u][m] = fragment_of<T, WHOLE>(x[m], k0 + u * WAVES * SPAN + g * (16 / (int)sizeof(T)), end);
 #pragma unroll
     for (int u = 0; u < UNROLL; u++)
 #pragma unroll
@@ -1408,6 +1411,10 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(ProductArgs p) {
     for (int s = 1; s < WAVES; s++) v += shared[s][m][lane];
     const int row = m * 16 + i;
     if (row >= p.rows) continue;
+    if (p.splits) {      // to be finished
+      if (j0 + g * 4 < p.cols) *(f32x4*)((float*)p.out + ((int64_t)split * p.rows + row) * p.ldo + j0 + g * 4) = v;
+      continue;
+    }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const int c = j0 + g * 4 + e;
@@ -1418,6 +1425,57 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(ProductArgs p) {
       ((T*)p.out)[row * p.ldo + c] = (T)o;
     }
   }
+}
+
+// A forward product that was cut along its depth, or whose tiles are no whole groups of columns: the parts [splits][rows][ldp] added up, in order, then what
+// the products' epilogues do.  32 lanes own a group of 256 columns.
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ partial, int splits, int64_t ldp, const T* __restrict__ bias,
+                                                     const T* __restrict__ residual, int64_t ldr, int act, int64_t rows, int cols, int groups,
+                                                     T* __restrict__ y, uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale,
+                                                     float* __restrict__ mn) {
+  const int64_t unit = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int64_t row = unit / groups;
+  const int g = (int)(unit - row * groups), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int col = g * kGroup + lane * kVec, n = cols - col;
+  f32x4 part[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+    if (n > 4 * h) {
+      part[h] = *(const f32x4*)(partial + row * ldp + col + 4 * h);
+      for (int s = 1; s < splits; s++) part[h] += *(const f32x4*)(partial + (s * rows + row) * ldp + col + 4 * h);
+    }
+  float v[kVec], b[kVec];
+  if (bias)
+    load_cols<T, false>(bias + col, n, b);
+  else
+    for (int e = 0; e < kVec; e++) b[e] = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kVec; e++) v[e] = part[e >> 2][e & 3] + b[e];
+  if (codes) {
+    float lo = __builtin_inff(), hi = -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < kVec; e++)
+      if (e < n) lo = __builtin_fminf(lo, v[e]), hi = __builtin_fmaxf(hi, v[e]);
+    lo = over_lanes<Least, 32>(lo);
+    hi = over_lanes<Most, 32>(hi);
+    const float s = scale_of(lo, hi);
+    if (n > 0)
+      *(u32x2*)(codes + row * ldc + col) = u32x2{four_codes(v[0], v[1], v[2], v[3], lo, s), four_codes(v[4], v[5], v[6], v[7], lo, s)};
+    if (lane == 0) {
+      scale[unit] = s;
+      mn[unit] = lo;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kVec; e++) v[e] = activated<std::is_same<T, float>::value>(v[e], act);
+  if (residual) {
+    load_cols<T, WHOLE>(residual + row * ldr + col, n, b);
+#pragma unroll
+    for (int e = 0; e < kVec; e++) v[e] += b[e];
+  }
+  store_cols<T, WHOLE>(y + row * cols + col, n, v);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -1484,6 +1542,8 @@ int sum_rows(const float* partial, int64_t count, int64_t stride, int64_t cols, 
   return launch_status();
 }
 
+inline int64_t padded4(int64_t cols) { return (cols + 3) / 4 * 4; }
+
 // workgroups of a tile whose LDS (two steps of both operands, and up to 14 KB beside them) a compute unit holds
 constexpr int slots_per_cu(int bm, int bn) { return bm + bn <= 128 ? 4 : bm + bn <= 256 ? 2 : 1; }
 struct Tiles {
@@ -1506,6 +1566,47 @@ int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s)
   return launch_status();
 }
 
+// How a forward product is cut (times in us, halves / floats, rows x inner x outer).
+//  few       rows go to the kernel that reads the weights once and the activations once per 16 columns: up to 16 rows (16x1024x4096 5.2 / 8.1, as
+//            tiles 9.9 / 14.4; 16x8192x8192 41.8 / 79, as tiles 38.9 / 82), more where those reads, from the caches, come to no
+//            more than 64 MiB (64x1024x4096 7.9 / 16.7, as tiles 10.9 / 16.0; 64x4096x4096 23.3 / 52, as tiles 17.5 / 29.8), and
+//            operands of unaligned rows
+//  parts     of the depth, each a result of its own that finish_kernel adds up, where tiles or strips of columns alone would leave compute
+//            units idle: 24x4096x1024 11.8 / 27.1 whole, 8.6 / 12.8 in parts; 100x4096x4096 52 / 109 and 22 / 44, 256x4096x1024 35 / 106 and
+//            16 / 30.  A part has at least 1024 bytes of a row (few: 2048): 300x1024x1024 is 11.0 / 22.7 whole, 10.4 / 17.4 in parts
+//  finished  by that kernel; also where the pre-activation's codes are wanted and the tiles that hold whole groups of columns are fewer than half
+//            the compute units
+struct Forward {
+  bool few, finished;
+  int parts;
+  int64_t per_part;
+};
+inline Forward forward_of(int dtype, int64_t rows, int64_t inner, int64_t outer, bool codes, bool whole) {
+  const int64_t strips = (outer + 15) / 16;
+  const bool cached = (rows + 15) / 16 * 16 * strips * inner * size_of(dtype) <= ((int64_t)64 << 20);
+  Forward f = {rows <= 16 || (rows <= GACT_LINEAR_FEW_ROWS && (cached || !whole)), false, 1, inner};
+  const int64_t step = 128 / size_of(dtype), steps = (inner + step - 1) / step;
+  auto tiles = [&](int bm, int bn) { return ((rows + bm - 1) / bm) * ((outer + bn - 1) / bn); };
+  int64_t parts = 1;
+  if (f.few) {
+    if (strips <= kComputeUnits / 2) parts = kComputeUnits / strips;
+    if (parts > steps / 16) parts = steps / 16;
+    f.finished = codes;
+  } else {
+    if (codes ? tiles(128, 256) >= kComputeUnits / 2 : tiles(128, 128) >= kComputeUnits) return f;
+    if (tiles(64, 64) <= kComputeUnits) parts = 2 * kComputeUnits / tiles(64, 64);
+    if (parts > steps / 8) parts = steps / 8;
+    f.finished = codes;
+  }
+  if (parts > 16) parts = 16;
+  if (parts < 1) parts = 1;
+  const int64_t per = (steps + parts - 1) / parts;
+  f.parts = (int)((steps + per - 1) / per);
+  f.per_part = per * step;
+  f.finished |= f.parts > 1;
+  return f;
+}
+
 template <typename T, int ACT>
 int forward_product(ProductArgs& p, hipStream_t s) {
   const int64_t step = Mma<T>::kStep, depth = (p.depth + step - 1) / step * step;
@@ -1516,8 +1617,7 @@ int forward_product(ProductArgs& p, hipStream_t s) {
     if (p.codes) {
       if constexpr (sizeof(T) == 2)
         if (large) return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
-      if (tiles(128, 256) >= kComputeUnits / 2) return launch_product<T, 128, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
-      return launch_product<T, 64, 256, 1, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
+      return launch_product<T, 128, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
     }
   }
   if constexpr (sizeof(T) == 2)
@@ -1547,7 +1647,6 @@ inline Tiles tiles_of(int dtype, int64_t rows, int64_t cols, int64_t depth) {
   t.per_split = per * step;
   return t;
 }
-inline int64_t padded4(int64_t cols) { return (cols + 3) / 4 * 4; }
 
 template <typename T, bool AS, int BK>
 int backward_product(ProductArgs& p, int dtype, void* workspace, hipStream_t s) {
@@ -1692,16 +1791,29 @@ int gact_norm_backward(const void* dy, int64_t lddy, const void* weight, const v
   });
 }
 
+int64_t gact_linear_workspace_bytes(int dtype, int64_t rows, int64_t inner, int64_t outer, int codes) {
+  if (!known(dtype) || rows <= 0 || inner <= 0 || outer <= 0) return 0;
+  int64_t parts = 0;
+  for (bool whole : {false, true}) {
+    const Forward f = forward_of(dtype, rows, inner, outer, codes != 0, whole);
+    if (f.finished && f.parts > parts) parts = f.parts;
+  }
+  return parts * rows * padded4(outer) * (int64_t)sizeof(float);
+}
+
 int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
                 int activation, int dtype, int64_t rows, int64_t inner, int64_t outer, void* y, void* codes, int64_t ldc, float* scale,
-                float* mn, void* stream) {
+                float* mn, void* workspace, void* stream) {
   if (!known(dtype) || !layer_sizes(rows, inner, outer) || activation < GACT_ACT_NONE || activation > GACT_ACT_SILU) return GACT_EINVAL;
   if (rows == 0) return GACT_OK;
   if (!x || !weight || !y || (codes && (!scale || !mn || activation == GACT_ACT_NONE)) || (residual && ldr < outer && rows > 1)) return GACT_EINVAL;
   if (codes && !codes_fit(codes, outer, ldc)) return GACT_EALIGN;
-  const bool few = !codes && rows <= GACT_LINEAR_FEW_ROWS;
   const bool whole = operand_fits(x, ldx, dtype, inner) && operand_fits(weight, ldw, dtype, inner);
-  if (!whole && !few) return GACT_EALIGN;
+  const Forward f = forward_of(dtype, rows, inner, outer, codes != nullptr, whole);
+  if (!whole && !f.few) return GACT_EALIGN;
+  if (f.finished && (!workspace || !aligned16(workspace))) return GACT_EALIGN;
+  const int64_t groups = (outer + kGroup - 1) / kGroup, units = (rows * groups + 7) / 8;
+  if (!blocks_fit(units)) return GACT_ELIMIT;
   ProductArgs p = {};
   p.a = x;
   p.b = weight;
@@ -1710,8 +1822,8 @@ int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
   p.rows = (int)rows;
   p.cols = (int)outer;
   p.depth = inner;
-  p.out = y;
-  p.ldo = outer;
+  p.out = f.finished ? workspace : y;
+  p.ldo = f.finished ? padded4(outer) : outer;
   p.bias = bias;
   p.residual = residual;
   p.ldr = ldr;
@@ -1720,32 +1832,38 @@ int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
   p.ldc = ldc;
   p.scale = scale;
   p.mn = mn;
-  p.wide = whole_rows(y, dtype, outer, outer) && (!residual || whole_rows(residual, dtype, outer, ldr));
+  p.per_split = f.per_part;
+  p.splits = f.finished ? f.parts : 0;
+  const bool wide = whole_rows(y, dtype, outer, outer) && (!residual || whole_rows(residual, dtype, outer, ldr));
+  p.wide = wide;
   fresh_launch();
   hipStream_t s = (hipStream_t)stream;
   return with_type(dtype, [&](auto zero) -> int {
     using T = decltype(zero);
-    if (few) {
-      auto run = [&](auto mt, auto waves) {
-        constexpr int MT = decltype(mt)::value, W = decltype(waves)::value;
-        auto kernel = whole ? few_rows_kernel<T, MT, W, true> : few_rows_kernel<T, MT, W, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((outer + 15) / 16)), dim3(W * 64), 0, s, p);
+    int rc;
+    if (f.few) {
+      auto run = [&](auto mt) {
+        constexpr int MT = decltype(mt)::value;
+        auto kernel = whole ? few_rows_kernel<T, MT, true> : few_rows_kernel<T, MT, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((outer + 15) / 16), (unsigned)f.parts), dim3(512), 0, s, p);
         return launch_status();
       };
-      using std::integral_constant;
-      // 16 waves where their depth is long: one turn of eight loads each up to 4096 halves (a workgroup has 16 columns, and few columns are few
-      // workgroups: 24 rows, 4096 to 1024 halves 13.4 us with 8 waves, 9.0 with 16)
-      auto by_depth = [&](auto mt) { return inner * (int)sizeof(T) >= 4096 ? run(mt, integral_constant<int, 16>{}) : run(mt, integral_constant<int, 8>{}); };
-      if (rows <= 16) return by_depth(integral_constant<int, 1>{});
-      if (rows <= 32) return by_depth(integral_constant<int, 2>{});
-      return by_depth(integral_constant<int, 4>{});
+      rc = rows <= 16 ? run(std::integral_constant<int, 1>{}) : rows <= 32 ? run(std::integral_constant<int, 2>{}) : run(std::integral_constant<int, 4>{});
+    } else if (f.finished) {
+      rc = launch_product<T, 64, 64, 2, 2, false, B_ROWS, ACT_UNFINISHED>(p, f.parts, f.per_part, s);
+    } else {
+      switch (activation) {
+        case GACT_ACT_GELU: return forward_product<T, ACT_GELU>(p, s);
+        case GACT_ACT_GELU_TANH: return forward_product<T, ACT_GELU_TANH>(p, s);
+        case GACT_ACT_SILU: return forward_product<T, ACT_SILU>(p, s);
+        default: return forward_product<T, ACT_NONE>(p, s);
+      }
     }
-    switch (activation) {
-      case GACT_ACT_GELU: return forward_product<T, ACT_GELU>(p, s);
-      case GACT_ACT_GELU_TANH: return forward_product<T, ACT_GELU_TANH>(p, s);
-      case GACT_ACT_SILU: return forward_product<T, ACT_SILU>(p, s);
-      default: return forward_product<T, ACT_NONE>(p, s);
-    }
+    if (rc != GACT_OK || !f.finished) return rc;
+    auto kernel = wide ? finish_kernel<T, true> : finish_kernel<T, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3(256), 0, s, (const float*)workspace, f.parts, padded4(outer), (const T*)bias,
+                       (const T*)residual, ldr, activation, rows, (int)outer, (int)groups, (T*)y, (uint8_t*)codes, ldc, scale, mn);
+    return launch_status();
   });
 }
 

@@ -366,15 +366,16 @@ at::Tensor linear(const at::Tensor& input, const at::Tensor& weight, const std::
     if (x.rows) {
       Rows a = x, w = rows_of(weight, "weight"), r;
       int64_t depth = inner;
-      if (keep_z || x.rows > GACT_LINEAR_FEW_ROWS) {
+      if (x.rows > GACT_LINEAR_FEW_ROWS) {
         a = product_rows(a, at);
         w = product_rows(w, at);
         depth = round_up(inner, 16 / (int64_t)a.held.element_size());      // behind the last column both are padded copies with zeros
       }
       if (residual) r = rows_of(*residual, "residual");
+      const at::Tensor ws = at.bytes(gact_linear_workspace_bytes(dtype_code(dtype), x.rows, depth, outer, keep_z));
       check_status(gact_linear(a.data(), a.ld, w.data(), w.ld, in(b), residual ? r.data() : nullptr, r.ld, activation, dtype_code(dtype),
                                x.rows, depth, outer, out(y), out(z.codes), keep_z ? z.codes.size(1) : 0, (float*)out(z.scale),
-                               (float*)out(z.mn), at.stream));
+                               (float*)out(z.mn), out(ws), at.stream));
     }
   }
   if (needs) {

@@ -76,7 +76,8 @@ SIGNATURES = {
     "gact_norm_forward": (_i32, [_vp, _i64, _vp, _vp, _i32, _i64, _i64, _f32, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "gact_norm_workspace_bytes": (_i64, [_i64, _i64]),
     "gact_norm_backward": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
-    "gact_linear": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp]),
+    "gact_linear_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i32]),
+    "gact_linear": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "gact_activation_workspace_bytes": (_i64, [_i64, _i64]),
     "gact_activation_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i32, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
     "gact_product_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64]),

@@ -261,10 +261,12 @@ int gact_norm_backward(const void* dy, int64_t lddy, const void* weight, const v
 
 /* y [rows, outer] = act(x [rows, inner] weight [outer, inner]^T + bias) + residual, y contiguous; bias and residual may be null.  With
  * `codes` (and an activation): also the checkpoint of z = x weight^T + bias.  x and weight: 16-byte aligned rows of whole 16-byte pieces (else
- * GACT_EALIGN), except for up to GACT_LINEAR_FEW_ROWS rows without codes. */
+ * GACT_EALIGN), except for up to GACT_LINEAR_FEW_ROWS rows.  workspace: gact_linear_workspace_bytes() of the same sizes (codes: whether they
+ * are asked for), 16-byte aligned; may be null where that is 0. */
+int64_t gact_linear_workspace_bytes(int dtype, int64_t rows, int64_t inner, int64_t outer, int codes);
 int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
                 int activation, int dtype, int64_t rows, int64_t inner, int64_t outer, void* y, void* codes, int64_t ldc, float* scale,
-                float* mn, void* stream);
+                float* mn, void* workspace, void* stream);
 
 /* dz [rows, cols] = dy act'(z) with z from its checkpoint (codes null and activation GACT_ACT_NONE: dz = dy), rows lddz apart (cols rounded up to a
  * multiple of 8, the columns behind the last one zero); dbias [cols] = the column sums of dz before rounding, through `workspace`

@@ -40,13 +40,13 @@ def test_library_refuses_before_it_touches_the_gpu():
     assert norm(16385, None, 0, None) == EINVAL and norm(8, 16, 16, None) == EINVAL and norm(8, 16, 24, 16) == EALIGN
     assert L.gact_norm_backward(16, 8, None, 16, 16, 16, 16, 16, 0, 0, 8, 16, None, None, None, None) == EINVAL    # no rows
     assert L.gact_norm_backward(16, 8, None, 16, 16, 16, 16, 16, 0, 4, 8, 16, 16, None, None, None) == EINVAL      # sums without workspace
-    linear = lambda ldx=8, x=16, act=0, codes=None, rows=100, inner=8: L.gact_linear(  # noqa: E731
-        x, ldx, 16, 8, None, None, 0, act, 0, rows, inner, 8, 16, codes, 16, 16, 16, None)
+    linear = lambda ldx=8, x=16, act=0, codes=None, rows=100, inner=8, ws=None: L.gact_linear(  # noqa: E731
+        x, ldx, 16, 8, None, None, 0, act, 0, rows, inner, 8, 16, codes, 16, 16, 16, ws, None)
     assert linear(act=4) == EINVAL and linear(rows=-1) == EINVAL and linear(inner=0) == EINVAL
     assert linear(codes=16) == EINVAL                                                            # codes without an activation
     assert linear(x=8) == EALIGN and linear(ldx=9) == EALIGN and linear(ldx=4, inner=8) == EALIGN
-    assert linear(act=1, codes=8) == EALIGN
-    assert L.gact_linear(16, 1 << 21, 16, 8, None, None, 0, 0, 0, 100, 8, 8, 16, None, 0, None, None, None) == EALIGN   # beyond a tile's window
+    assert linear(act=1, codes=8) == EALIGN and linear(act=1, codes=16) == EALIGN and linear(act=1, codes=16, ws=8) == EALIGN   # workspace
+    assert L.gact_linear(16, 1 << 21, 16, 8, None, None, 0, 0, 0, 100, 8, 8, 16, None, 0, None, None, None, None) == EALIGN   # beyond a tile's window
     act = lambda codes, which, dz, lddz, db, ws: L.gact_activation_backward(16, 9, codes, 16, 16, 16, which, 0, 4, 9, dz, lddz, db, ws, None)  # noqa: E731
     assert act(None, 1, 16, 16, None, None) == EINVAL and act(16, 1, None, 16, None, None) == EINVAL
     assert act(16, 1, 16, 16, 16, None) == EINVAL and act(16, 1, 16, 12, None, None) == EALIGN and act(16, 1, 16, 24, None, None) == EALIGN

@@ -171,9 +171,10 @@ def kept_activation(x, w, b, act):
     codes = torch.zeros(rows, (outer + 15) // 16 * 16, dtype=torch.int8, device="cuda")
     scale, mn = (torch.zeros(rows, (outer + 255) // 256, device="cuda") for _ in range(2))
     y = torch.empty(rows, outer, dtype=x.dtype, device="cuda")
+    ws = torch.empty(_abi.lib().gact_linear_workspace_bytes(_abi.dtype_code(x.dtype), rows, whole, outer, 1) + 16, dtype=torch.uint8, device="cuda")
     _abi.check(_abi.lib().gact_linear(x.data_ptr(), whole, w.data_ptr(), whole, _abi.ptr(b), None, 0, {"gelu": 1, "gelu_tanh": 2, "silu": 3}[act],
                                       _abi.dtype_code(x.dtype), rows, whole, outer, y.data_ptr(), codes.data_ptr(), codes.stride(0),
-                                      scale.data_ptr(), mn.data_ptr(), _abi.stream_of(x)))
+                                      scale.data_ptr(), mn.data_ptr(), _abi.ptr(ws), _abi.stream_of(x)))
     return codes, scale, mn
 
 
@@ -237,6 +238,14 @@ def test_linear_of_many_tiles(dtype):
     """Enough of them for the largest tiles, none of whose edges the sizes meet."""
     check_linear(4200, 136, 4104, dtype, "gelu", True, True)
     check_linear(4099, 200, 4099, dtype, "silu", True, False)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows,inner,outer", [(1, 4096, 264), (24, 2056, 264), (64, 4100, 72), (65, 1030, 48), (100, 2104, 520), (300, 4000, 130),
+                                              (50, 4096, 4096)])
+def test_linear_cut_along_its_depth(rows, inner, outer, dtype):
+    for act, with_bias, with_residual in ((None, True, True), ("gelu", True, False), ("silu", False, True)):
+        check_linear(rows, inner, outer, dtype, act, with_bias, with_residual)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)

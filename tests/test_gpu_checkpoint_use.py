@@ -292,7 +292,7 @@ def test_nothing_is_written_beside_the_results():
     stream = torch.cuda.current_stream().cuda_stream
     for dtype in (torch.float32, torch.bfloat16):
         code, esz = _abi.dtype_code(dtype), torch.empty((), dtype=dtype).element_size()
-        for rows, inner, outer in ((3, 16, 9), (70, 24, 33), (130, 264, 257), (300, 72, 520)):
+        for rows, inner, outer in ((3, 16, 9), (70, 24, 33), (130, 264, 257), (300, 72, 520), (24, 2056, 33), (100, 2104, 133)):
             guard = 4096
             held = []
 
@@ -310,7 +310,8 @@ def test_nothing_is_written_beside_the_results():
             c = [room(rows * ldc), room(rows * gx * 4), room(rows * gx * 4)]
             for act, codes in ((0, None), (1, z[0])):
                 assert L.gact_linear(x.data_ptr(), inner, w.data_ptr(), inner, None, None, 0, act, code, rows, inner, outer, room(rows * outer * esz),
-                                     codes, ldz, z[1], z[2], stream) == 0
+                                     codes, ldz, z[1], z[2], room(L.gact_linear_workspace_bytes(code, rows, inner, outer, codes is not None)),
+                                     stream) == 0
             assert L.gact_checkpoint(x.data_ptr(), code, rows, inner, inner, c[0], ldc, c[1], c[2], stream) == 0
             assert L.gact_restore(c[0], ldc, c[1], c[2], code, rows, inner, room(rows * inner * esz), stream) == 0
             assert L.gact_activation_backward(g.data_ptr(), ldg, z[0], ldz, z[1], z[2], 1, code, rows, outer, room(rows * ldg * esz), ldg,
