@@ -173,9 +173,16 @@ __device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float 
   return __builtin_amdgcn_cvt_pk_u8_f32(__builtin_fmaf(d - lo, scale, 0.5f) - 0.5f, 3, w);
 }
 __device__ __forceinline__ float code_at(uint32_t w, int e) { return (float)(uint8_t)(w >> (8 * e)); }
+// A value is a float before it is rounded to T, in every kernel: the empty statement keeps the compiler from making one instruction of the
+// sum and its rounding to a half, which rounds once and differs in one of 2^13 values.
+__device__ __forceinline__ float value_of(uint32_t w, int e, float inv, float lo) {
+  float v = __builtin_fmaf(code_at(w, e), inv, lo);
+  asm("" : "+v"(v));
+  return v;
+}
 __device__ __forceinline__ void eight_values(u32x2 w, float inv, float lo, float (&v)[kVec]) {
 #pragma unroll
-  for (int e = 0; e < kVec; e++) v[e] = __builtin_fmaf(code_at(w[e >> 2], e & 3), inv, lo);
+  for (int e = 0; e < kVec; e++) v[e] = value_of(w[e >> 2], e & 3, inv, lo);
 }
 
 // ---- activations: act(z) and act'(z) ----
@@ -872,12 +879,12 @@ struct CodeLoad {
       typedef T T8 __attribute__((ext_vector_type(8)));
       T8 v;
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = (T)__builtin_fmaf(code_at(held[q][2 * h + (e >> 2)], e & 3), inv, lo[q]);
+      for (int e = 0; e < 8; e++) v[e] = (T)value_of(held[q][2 * h + (e >> 2)], e & 3, inv, lo[q]);
       *(__attribute__((address_space(3))) T8*)to = v;
     } else {
       f32x4 v;
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(code_at(held[q][h], e), inv, lo[q]);
+      for (int e = 0; e < 4; e++) v[e] = value_of(held[q][h], e, inv, lo[q]);
       *(__attribute__((address_space(3))) f32x4*)to = v;
     }
   }
@@ -1546,10 +1553,6 @@ inline int64_t padded4(int64_t cols) { return (cols + 3) / 4 * 4; }
 
 // workgroups of a tile whose LDS (two steps of both operands, and up to 14 KB beside them) a compute unit holds
 constexpr int slots_per_cu(int bm, int bn) { return bm + bn <= 128 ? 4 : bm + bn <= 256 ? 2 : 1; }
-struct Tiles {
-  int bm, bn, splits;
-  int64_t per_split;
-};
 
 template <typename T, int BM, int BN, int WI, int WJ, bool AS, int BK, int ACT = ACT_NONE, bool CODES = false>
 int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s) {
@@ -1566,106 +1569,127 @@ int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s)
   return launch_status();
 }
 
-// How a forward product is cut (times in us, halves / floats, rows x inner x outer).
+// How a product is cut: the side of its tiles, and parts of its depth whose sums are added up afterwards.  Of the cuts there are the one with the
+// least estimated time is taken.  A step of a tile takes as long as one workgroup alone on a compute unit needs for it, or as the unit's share of
+// all workgroups needs; parts cost a launch and the traffic of their sums.  us per step of 128 bytes, alone / shared, from timings of
+// 19 products of 76 million to 17 billion multiplications, each in all of its cuts, both types, forward and with codes (whole, rows x inner x outer):
+//   halves  1024x1024x1024   in tiles of 64  8.5   of 128 10.8   of 256 23.7, in two parts of 64 14.6
+//           1024x1024x4096                  16.5          12.7          24.6
+//           4096x1024x4096                  61.3          37.1          33.3
+//           512x4096x1024                   34.5          42.9          72.1, in 2 / 4 / 8 parts of 64 18.1 / 17.7 / 22.8
+//           8192x512x512, dW                88            118           196, in 8 parts of 64 23.8
+//   floats  1024x1024x1024                  22.7          67.5
+//           4096x1024x4096                 264           249
+//           512x4096x1024                   78           253, in 4 parts of 64 42.8
+// Over the 113 of them that leave a choice the estimate's cut takes 1.2 % longer than the best one.
+struct Rate {
+  float alone, shared;
+};
+constexpr Rate kRates[2][2][3] = {      // [codes][halves, floats][64, 128, 256]
+    {{{0.33f, 0.23f}, {0.5f, 0.53f}, {1.3f, 1.75f}}, {{0.6f, 0.52f}, {2.0f, 1.95f}}},
+    {{{0.6f, 0.33f}, {0.95f, 0.65f}, {1.85f, 2.15f}}, {{0.9f, 0.62f}, {2.3f, 2.1f}}}};
+struct Cut {
+  int side, parts;
+  int64_t per_part;
+};
+inline Cut cut_of(int dtype, bool coded, int64_t rows, int64_t cols, int64_t depth, int largest, int largest_in_parts) {
+  const int64_t step = 128 / size_of(dtype), steps = (depth + step - 1) / step;
+  Cut cut = {64, 1, steps * step};
+  float least = __builtin_inff();
+  for (int n = 0; n < (dtype == GACT_F32 ? 2 : 3); n++) {
+    const int side = 64 << n;
+    if (side > largest) break;
+    const int64_t tiles = ((rows + side - 1) / side) * ((cols + side - 1) / side), slots = kComputeUnits * slots_per_cu(side, side);
+    const Rate rate = kRates[coded][dtype == GACT_F32][n];
+    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      if (parts > 1 && (parts * 4 > steps || side > largest_in_parts)) break;
+      const int64_t per = (steps + parts - 1) / parts, made = (steps + per - 1) / per, work = tiles * made;
+      const float alone = rate.alone * (float)((work + slots - 1) / slots);
+      const float shared = rate.shared * (float)((work + kComputeUnits - 1) / kComputeUnits);
+      const float sums = made == 1 ? 0.0f : 3.0f + (float)(rows * cols) * (float)(8 * made + size_of(dtype)) * 0.25e-6f;
+      const float us = (float)per * (alone > shared ? alone : shared) + sums;
+      if (us < least) {
+        least = us;
+        cut = {side, (int)made, per * step};
+      }
+      if (work >= slots) break;      // more parts only add to the sums
+    }
+  }
+  return cut;
+}
+
+// How a forward product is run (times in us, halves / floats, rows x inner x outer).
 //  few       rows go to the kernel that reads the weights once and the activations once per 16 columns: up to 16 rows (16x1024x4096 5.2 / 8.1, as
 //            tiles 9.9 / 14.4; 16x8192x8192 41.8 / 79, as tiles 38.9 / 82), more where those reads, from the caches, come to no
 //            more than 64 MiB (64x1024x4096 7.9 / 16.7, as tiles 10.9 / 16.0; 64x4096x4096 23.3 / 52, as tiles 17.5 / 29.8), and
-//            operands of unaligned rows
-//  parts     of the depth, each a result of its own that finish_kernel adds up, where tiles or strips of columns alone would leave compute
-//            units idle: 24x4096x1024 11.8 / 27.1 whole, 8.6 / 12.8 in parts; 100x4096x4096 52 / 109 and 22 / 44, 256x4096x1024 35 / 106 and
-//            16 / 30.  A part has at least 1024 bytes of a row (few: 2048): 300x1024x1024 is 11.0 / 22.7 whole, 10.4 / 17.4 in parts
-//  finished  by that kernel; also where the pre-activation's codes are wanted and the tiles that hold whole groups of columns are fewer than half
-//            the compute units
+//            operands of unaligned rows.  In parts of at least 2048 bytes of a row where the strips of columns leave half the compute units
+//            idle: 24x4096x1024 11.8 / 27.1 whole, 8.6 / 12.8 in parts
+//  finished  by finish_kernel: parts; and the pre-activation's codes, where the tiles that hold whole groups of columns are too few.  Halves: fewer
+//            than half the compute units (1024x1024x4096, at half, 25.0 in such tiles, 27.6 finished; 512x1024x4096 23.9 and 21.6; 2048x1024x4096
+//            27.3 and 44.6).  Floats, whose tiles are bound by the matrix pipe alone: fewer than the compute units (1024x1024x4096 138 and 80;
+//            2048x1024x4096, at all of them, 139 and 150)
 struct Forward {
   bool few, finished;
-  int parts;
-  int64_t per_part;
+  Cut cut;      // few: parts alone.  Of codes that are not finished: nothing
 };
 inline Forward forward_of(int dtype, int64_t rows, int64_t inner, int64_t outer, bool codes, bool whole) {
   const int64_t strips = (outer + 15) / 16;
   const bool cached = (rows + 15) / 16 * 16 * strips * inner * size_of(dtype) <= ((int64_t)64 << 20);
-  Forward f = {rows <= 16 || (rows <= GACT_LINEAR_FEW_ROWS && (cached || !whole)), false, 1, inner};
-  const int64_t step = 128 / size_of(dtype), steps = (inner + step - 1) / step;
-  auto tiles = [&](int bm, int bn) { return ((rows + bm - 1) / bm) * ((outer + bn - 1) / bn); };
-  int64_t parts = 1;
+  Forward f = {rows <= 16 || (rows <= GACT_LINEAR_FEW_ROWS && (cached || !whole)), codes, {0, 1, inner}};
   if (f.few) {
-    if (strips <= kComputeUnits / 2) parts = kComputeUnits / strips;
+    const int64_t step = 128 / size_of(dtype), steps = (inner + step - 1) / step;
+    int64_t parts = strips <= kComputeUnits / 2 ? kComputeUnits / strips : 1;
     if (parts > steps / 16) parts = steps / 16;
-    f.finished = codes;
+    if (parts > 1) {
+      const int64_t per = (steps + parts - 1) / parts;
+      f.cut = {0, (int)((steps + per - 1) / per), per * step};
+    }
   } else {
-    if (codes ? tiles(128, 256) >= kComputeUnits / 2 : tiles(128, 128) >= kComputeUnits) return f;
-    if (tiles(64, 64) <= kComputeUnits) parts = 2 * kComputeUnits / tiles(64, 64);
-    if (parts > steps / 8) parts = steps / 8;
-    f.finished = codes;
+    const int64_t tiles = ((rows + 127) / 128) * ((outer + 255) / 256);
+    if (codes && tiles >= (dtype == GACT_F32 ? kComputeUnits : kComputeUnits / 2)) f.finished = false;
+    f.cut = cut_of(dtype, false, rows, outer, inner, codes ? 64 : 256, 64);
   }
-  if (parts > 16) parts = 16;
-  if (parts < 1) parts = 1;
-  const int64_t per = (steps + parts - 1) / parts;
-  f.parts = (int)((steps + per - 1) / per);
-  f.per_part = per * step;
-  f.finished |= f.parts > 1;
+  if (!codes) f.finished = f.cut.parts > 1;
   return f;
 }
 
 template <typename T, int ACT>
-int forward_product(ProductArgs& p, hipStream_t s) {
+int forward_product(ProductArgs& p, int side, hipStream_t s) {
   const int64_t step = Mma<T>::kStep, depth = (p.depth + step - 1) / step * step;
-  auto tiles = [&](int bm, int bn) { return (int64_t)((p.rows + bm - 1) / bm) * ((p.cols + bn - 1) / bn); };
-  const bool large = sizeof(T) == 2 && tiles(256, 256) >= kComputeUnits;
-  // the pre-activation's codes need a whole group of columns in a tile; without an activation nobody asks for them
+  // the pre-activation's codes need a whole group of columns in a tile; without an activation nobody asks for them.  The larger ones where they fill
+  // the card (16384x1024x4096 halves 165, the others 205)
   if constexpr (ACT != ACT_NONE) {
     if (p.codes) {
       if constexpr (sizeof(T) == 2)
-        if (large) return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
+        if ((int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256) >= kComputeUnits)
+          return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
       return launch_product<T, 128, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
     }
   }
   if constexpr (sizeof(T) == 2)
-    if (large) return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT>(p, 1, depth, s);
-  if (tiles(128, 128) >= kComputeUnits) return launch_product<T, 128, 128, 2, 2, false, B_ROWS, ACT>(p, 1, depth, s);
+    if (side == 256) return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT>(p, 1, depth, s);
+  if (side == 128) return launch_product<T, 128, 128, 2, 2, false, B_ROWS, ACT>(p, 1, depth, s);
   return launch_product<T, 64, 64, 2, 2, false, B_ROWS, ACT>(p, 1, depth, s);
-}
-
-// how a backward product is cut: the tile, and the parts of its depth where the tiles alone leave compute units idle
-inline Tiles tiles_of(int dtype, int64_t rows, int64_t cols, int64_t depth) {
-  Tiles t = {64, 64, 1, 0};
-  const int64_t step = 128 / size_of(dtype), steps = (depth + step - 1) / step;
-  auto tiles = [&](int side) { return ((rows + side - 1) / side) * ((cols + side - 1) / side); };
-  // as many workgroups as the card holds, in the largest tiles that leave each at least 8 steps
-  if (dtype != GACT_F32 && tiles(256) * (steps / 8) >= kComputeUnits)
-    t.bm = t.bn = 256;
-  else if (tiles(128) * (steps / 8) >= kComputeUnits)
-    t.bm = t.bn = 128;
-  const int64_t slots = kComputeUnits * slots_per_cu(t.bm, t.bn);
-  int64_t splits = tiles(t.bm) >= slots ? 1 : slots / tiles(t.bm);
-  const int64_t most = steps / (t.bm == 64 ? 4 : 8);
-  if (splits > most) splits = most;
-  if (splits > 64) splits = 64;
-  if (splits < 1) splits = 1;
-  const int64_t per = (steps + splits - 1) / splits;
-  t.splits = (int)((steps + per - 1) / per);
-  t.per_split = per * step;
-  return t;
 }
 
 template <typename T, bool AS, int BK>
 int backward_product(ProductArgs& p, int dtype, void* workspace, hipStream_t s) {
-  const Tiles t = tiles_of(dtype, p.rows, p.cols, p.depth);
+  const Cut t = cut_of(dtype, BK == B_CODES, p.rows, p.cols, p.depth, 256, 256);
   void* out = p.out;
-  if (t.splits > 1) {
+  if (t.parts > 1) {
     if (!workspace || !aligned16(workspace)) return GACT_EALIGN;
     p.out = workspace;
     p.ldo = padded4(p.cols);
   }
   int rc = GACT_ESHAPE;
   if constexpr (sizeof(T) == 2)
-    if (t.bm == 256) rc = launch_product<T, 256, 256, 2, 4, AS, BK>(p, t.splits, t.per_split, s);
-  if (t.bm == 128) rc = launch_product<T, 128, 128, 2, 2, AS, BK>(p, t.splits, t.per_split, s);
-  if (t.bm == 64) rc = launch_product<T, 64, 64, 2, 2, AS, BK>(p, t.splits, t.per_split, s);
-  if (rc != GACT_OK || t.splits == 1) return rc;
+    if (t.side == 256) rc = launch_product<T, 256, 256, 2, 4, AS, BK>(p, t.parts, t.per_part, s);
+  if (t.side == 128) rc = launch_product<T, 128, 128, 2, 2, AS, BK>(p, t.parts, t.per_part, s);
+  if (t.side == 64) rc = launch_product<T, 64, 64, 2, 2, AS, BK>(p, t.parts, t.per_part, s);
+  if (rc != GACT_OK || t.parts == 1) return rc;
   const int64_t blocks = ((int64_t)p.rows * (p.ldo / 4) + 255) / 256;
   if (!blocks_fit(blocks)) return GACT_ELIMIT;
-  hipLaunchKernelGGL((join_splits_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, (const float*)workspace, t.splits, (int64_t)p.rows,
+  hipLaunchKernelGGL((join_splits_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, (const float*)workspace, t.parts, (int64_t)p.rows,
                      p.cols, (int)p.ldo, (T*)out);
   return launch_status();
 }
@@ -1796,7 +1820,7 @@ int64_t gact_linear_workspace_bytes(int dtype, int64_t rows, int64_t inner, int6
   int64_t parts = 0;
   for (bool whole : {false, true}) {
     const Forward f = forward_of(dtype, rows, inner, outer, codes != 0, whole);
-    if (f.finished && f.parts > parts) parts = f.parts;
+    if (f.finished && f.cut.parts > parts) parts = f.cut.parts;
   }
   return parts * rows * padded4(outer) * (int64_t)sizeof(float);
 }
@@ -1832,8 +1856,8 @@ int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
   p.ldc = ldc;
   p.scale = scale;
   p.mn = mn;
-  p.per_split = f.per_part;
-  p.splits = f.finished ? f.parts : 0;
+  p.per_split = f.cut.per_part;
+  p.splits = f.finished ? f.cut.parts : 0;
   const bool wide = whole_rows(y, dtype, outer, outer) && (!residual || whole_rows(residual, dtype, outer, ldr));
   p.wide = wide;
   fresh_launch();
@@ -1845,23 +1869,23 @@ int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
       auto run = [&](auto mt) {
         constexpr int MT = decltype(mt)::value;
         auto kernel = whole ? few_rows_kernel<T, MT, true> : few_rows_kernel<T, MT, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((outer + 15) / 16), (unsigned)f.parts), dim3(512), 0, s, p);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((outer + 15) / 16), (unsigned)f.cut.parts), dim3(512), 0, s, p);
         return launch_status();
       };
       rc = rows <= 16 ? run(std::integral_constant<int, 1>{}) : rows <= 32 ? run(std::integral_constant<int, 2>{}) : run(std::integral_constant<int, 4>{});
     } else if (f.finished) {
-      rc = launch_product<T, 64, 64, 2, 2, false, B_ROWS, ACT_UNFINISHED>(p, f.parts, f.per_part, s);
+      rc = launch_product<T, 64, 64, 2, 2, false, B_ROWS, ACT_UNFINISHED>(p, f.cut.parts, f.cut.per_part, s);
     } else {
       switch (activation) {
-        case GACT_ACT_GELU: return forward_product<T, ACT_GELU>(p, s);
-        case GACT_ACT_GELU_TANH: return forward_product<T, ACT_GELU_TANH>(p, s);
-        case GACT_ACT_SILU: return forward_product<T, ACT_SILU>(p, s);
-        default: return forward_product<T, ACT_NONE>(p, s);
+        case GACT_ACT_GELU: return forward_product<T, ACT_GELU>(p, f.cut.side, s);
+        case GACT_ACT_GELU_TANH: return forward_product<T, ACT_GELU_TANH>(p, f.cut.side, s);
+        case GACT_ACT_SILU: return forward_product<T, ACT_SILU>(p, f.cut.side, s);
+        default: return forward_product<T, ACT_NONE>(p, f.cut.side, s);
       }
     }
     if (rc != GACT_OK || !f.finished) return rc;
     auto kernel = wide ? finish_kernel<T, true> : finish_kernel<T, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3(256), 0, s, (const float*)workspace, f.parts, padded4(outer), (const T*)bias,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3(256), 0, s, (const float*)workspace, f.cut.parts, padded4(outer), (const T*)bias,
                        (const T*)residual, ldr, activation, rows, (int)outer, (int)groups, (T*)y, (uint8_t*)codes, ldc, scale, mn);
     return launch_status();
   });
@@ -1896,8 +1920,9 @@ int gact_activation_backward(const void* dy, int64_t lddy, const void* codes, in
 
 int64_t gact_product_workspace_bytes(int dtype, int64_t rows, int64_t cols, int64_t depth) {
   if (!known(dtype) || rows <= 0 || cols <= 0 || depth <= 0) return 0;
-  const Tiles t = tiles_of(dtype, rows, cols, depth);
-  return t.splits == 1 ? 0 : t.splits * rows * padded4(cols) * (int64_t)sizeof(float);
+  const int parts = cut_of(dtype, false, rows, cols, depth, 256, 256).parts, of_codes = cut_of(dtype, true, rows, cols, depth, 256, 256).parts;
+  const int64_t most = parts > of_codes ? parts : of_codes;
+  return most == 1 ? 0 : most * rows * padded4(cols) * (int64_t)sizeof(float);
 }
 
 int gact_product(const void* a, int64_t lda, const void* b, int64_t ldb, int dtype, int64_t rows, int64_t depth, int64_t cols, void* out,

@@ -162,6 +162,15 @@ def test_layer_norm_of_many_rows_adds_up_every_one():
         assert torch.equal(db, torch.full_like(db, float(rows // 2)))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows,outer,cols", [(64, 64, 640), (300, 300, 1032), (200, 1300, 2056), (50, 4096, 4096)])
+def test_checkpoint_product_has_the_values_that_restore_gives(rows, outer, cols, dtype):
+    """Rows of the unit matrix pick values one by one: a value rounded in another way than op_restore rounds it is seen."""
+    c = ops.op_checkpoint(normal(rows, cols, dtype=dtype))
+    got = ops.op_checkpoint_product(torch.eye(rows, outer, dtype=dtype, device="cuda"), c)
+    assert torch.equal(got[:rows], ops.op_restore(c)) and not got[rows:].any()
+
+
 # ---- linear layers ----
 def kept_activation(x, w, b, act):
     """Codes, scale and min of x w^T + b as the forward pass keeps them: the same call of the library, on rows of whole 16-byte pieces."""
