@@ -262,8 +262,10 @@ __device__ __forceinline__ float slope(float z, int act) {
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Checkpoints of rows.  32 lanes own a group: one 16-byte piece each (float: two), its minimum and maximum over the half wave.
 // ---------------------------------------------------------------------------------------------------------------------------------
-// One group at a time: four to a half wave, with their loads together and one division for all of their scales, take 84 us instead of 90 for
-// 134 M halves, but 14 instead of 11.5 for 10 M.
+// Bound by memory: 32768x4096 halves 84 us (4.8 TB/s), 16384x1024 floats 16.6 (5.1), 25088x384 halves 11.7, of which the launch and the one
+// load that nothing overlaps are half.  One group at a time: four to a half wave, with their loads together and one division for all of their
+// scales, take 84 us instead of 90 for 134 M halves, but 14 instead of 11.5 for 10 M.  A group shorter than 256 leaves lanes idle (771
+// columns of halves, 22.7 us for 25088 rows, 2.6 TB/s).
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int groups,
                                                          uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale,
@@ -290,6 +292,8 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x
   }
 }
 
+// The values again, the same lanes: 32768x4096 halves 72 us (5.7 TB/s), 16384x1024 12.0 (4.3), 25088x384 8.3.  1 / scale is made by every
+// lane: the division is hidden behind the loads.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scale,
                                                       const float* __restrict__ mn, int64_t rows, int cols, int groups,
@@ -305,7 +309,8 @@ __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* __restrict_
   store_cols<T, WHOLE>(out + row * cols + col, n, v);
 }
 
-// rows copied to a stride that the products can load 16 bytes at a time from, the columns behind the last one zero
+// rows copied to a stride that the products can load 16 bytes at a time from, the columns behind the last one zero.  25088x771 halves 18.6 us
+// (4.2 TB/s); a product that reads such rows value by value takes several times as long as on whole pieces.
 template <typename T>
 __global__ __launch_bounds__(256) void pad_rows_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, T* __restrict__ out,
                                                        int ldo) {
@@ -347,7 +352,9 @@ __device__ __forceinline__ float row_sum(float v, float* shared, int turn) {
   return v;
 }
 
-// U consecutive rows at a time: their loads are on the way together, and their scales are one division (see scales_of).
+// mean = sum / cols, var = sum (x - mean)^2 / cols from the row in registers, in floats: one read, one write of x, and the codes.  Bound by memory:
+// 401408x96 floats 68 us (5.2 TB/s), 65536x1024 halves 72 (4.7), 16384x4096 halves 67 (5.1), 16384x1024 halves 25 (3.4: half of it launch,
+// ramp and the tail).  U consecutive rows at a time: their loads are on the way together, and their scales are one division (see scales_of).
 template <typename T, int LPR, int NC, int U, bool WHOLE>
 __global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_forward_kernel(
     const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias, int64_t rows, int cols, float per_col,
@@ -456,6 +463,8 @@ __global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_forward_kernel(
 
 // xh = (value - mean) rstd, g = dy w: dx = rstd (g - mean(g) - xh mean(g xh)); a thread adds up dy xh and dy of its columns over the
 // rows it sees, a workgroup writes one row of partial sums.  While a row is worked on, the next one's loads are on the way.
+// Reads dy and the codes, writes dx: 401408x96 floats 72 us (4.9 TB/s), 65536x1024 halves 78 (4.3), 16384x4096 halves 83 (4.0), 16384x1024
+// halves 25 (3.3), the column sums included (they take 3 us, 15 of 85 at 4096 columns).
 constexpr int kNormThreads = 512;   // waves that share a row of partial sums (with 4 of them and twice the workgroups there is twice as much to add up)
 template <int LPR>
 using SharedRows = RowShape<LPR, kNormThreads>;
@@ -594,7 +603,8 @@ __global__ __launch_bounds__(SharedRows<LPR>::kThreads) void norm_backward_kerne
   }
 }
 
-// out[c] = sum of partial[p][c]; `stride` values from one partial row to the next.  16 waves per 64 columns.
+// out[c] = sum of partial[p][c], in the same order whatever runs beside it; `stride` values from one partial row to the next.  16 waves per 64
+// columns: 512 rows of 4096 columns 4.6 us, bound by the latency of a few loads in turn.
 template <typename T>
 __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict__ partial, int count, int64_t stride, int cols,
                                                         T* __restrict__ out0, T* __restrict__ out1) {
@@ -628,6 +638,8 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
 // ---------------------------------------------------------------------------------------------------------------------------------
 // dz = dy act'(z) from the checkpoint of z, and the column sums of dz before they are rounded.  A thread owns 8 columns and walks
 // down `per` rows; without codes (no activation) dz is dy, copied to the products' stride where `dz` is given.
+// Bound by memory, 32768x4096 halves GELU 134 us (5.0 TB/s), SiLU 128, sums alone 47 (5.7); 16384x1024 23, 22 and 11.  32 lanes and 256
+// columns to a row, as the codes' groups are: narrower outputs leave lanes idle (401408x96 floats 195 us, 1.8 TB/s).
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __restrict__ dy, int64_t lddy, const uint8_t* __restrict__ codes,
@@ -687,6 +699,14 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __res
 // 16-byte pieces by the row's number, the others their blocks of 16 columns.
 //
 // B supplies the matrix instruction's rows and A its columns, so that a lane holds four consecutive j of one i.
+//
+// 8192x8192x8192 halves: forward 785 to 890 us (1233 to 1400 TFLOP/s), dx 786, dW from codes 1045 (1055), forward with GELU and its codes 837;
+// 16384x1024x4096: 109, 103, 140 to 150, 165; floats 4096x4096x4096 976 (141 of the 152 that the library's product reaches).  Zeros in place of
+// numbers take 695: the clock drops under the matrix units' load, and the numbers' share of the time is power's.  Without its loads the forward
+// product takes 582, so what else there is to gain lies in the loads' path to LDS.
+// Measured and not taken, forward 8192x8192x8192: four steps of 64 bytes in LDS with a barrier to each 877 to 912 us; two groups of waves that take
+// turns between loading and multiplying 897; four waves of 128x128 873, with a slower epilogue.  16384x1024x4096: stores that bypass the caches
+// 174 to 182 us where plain ones take 170.
 // ---------------------------------------------------------------------------------------------------------------------------------
 [[maybe_unused]] constexpr uint32_t kNowhere = 0x80000000u;   // beyond every window: such a load gives zero
 
@@ -1337,7 +1357,7 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
   }
 }
 
-// the splits' partial sums [splits][rows][ldp] added up, in order
+// the parts' sums [splits][rows][ldp] added up, in order: 4 parts of 4096x1024 floats 12.6 us (5.8 TB/s, from the caches in part)
 template <typename T>
 __global__ __launch_bounds__(256) void join_splits_kernel(const float* __restrict__ partial, int splits, int64_t rows, int cols, int ldp,
                                                           T* __restrict__ out) {
@@ -1355,7 +1375,9 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const float* __restric
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // The forward product of a few rows (up to 64): the weights are read once, straight into the matrix instruction's fragments, by
-// workgroups of 16 output columns whose waves share the depth; their sums meet in LDS.
+// workgroups of 16 output columns whose waves share the depth; their sums meet in LDS.  Bound by the weights' bytes: 1x4096x4096 halves 10 us
+// (3.4 TB/s), 16x4096x16384 36.5 (3.7), 16x8192x8192 floats 79 (3.4); 1x1024x4096 4.6, launch and latency.  16 waves to a workgroup are no
+// faster (9.7 and 9.1 for 1x4096x4096, 11.6 and 9.6 the other way for 24x1024x4096 floats).
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, bool WHOLE>
 __device__ __forceinline__ typename Mma<T>::Frag fragment_of(const T* row, int64_t k, int64_t depth) {
@@ -1435,7 +1457,7 @@ __global__ __launch_bounds__(512) void few_rows_kernel(ProductArgs p) {
 }
 
 // A forward product that was cut along its depth, or whose tiles are no whole groups of columns: the parts [splits][rows][ldp] added up, in order, then what
-// the products' epilogues do.  32 lanes own a group of 256 columns.
+// the products' epilogues do.  32 lanes own a group of 256 columns.  1024x4096 halves with GELU and codes, one part: 28 us with its product.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ partial, int splits, int64_t ldp, const T* __restrict__ bias,
                                                      const T* __restrict__ residual, int64_t ldr, int act, int64_t rows, int cols, int groups,
@@ -1512,7 +1534,8 @@ int with_type(int dtype, F&& f) {
   }
 }
 
-// threads of a row, its pieces per thread, and the rows that a thread of the forward pass takes at a time
+// threads of a row, its pieces per thread, and the rows that a thread of the forward pass takes at a time: the fewest threads whose registers
+// hold the row without spilling beside the next row's loads
 template <typename F>
 int with_row_shape(int64_t cols, F&& f) {
   using std::integral_constant;
@@ -1525,7 +1548,9 @@ int with_row_shape(int64_t cols, F&& f) {
   if (cols <= 8192) return f(integral_constant<int, 512>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
   return f(integral_constant<int, 512>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
 }
-// workgroups of a layer norm's backward pass: each leaves one row of partial sums
+// workgroups of a layer norm's backward pass: each leaves one row of partial sums.  At most 512, 256 of them / 1024 of them instead: 401408x96
+// floats 71 us, 101 / 75; 65536x1024 halves 78, 75 / 84; 16384x4096 83, 125 / 99.  Rows beyond 4096 columns fill a compute unit by
+// themselves, at most 256: 8192x8192 87, with 512 99
 inline int64_t norm_blocks(int64_t rows, int64_t cols) {
   const int64_t at_a_time = cols <= 128 ? kNormThreads / 16 : cols <= 256 ? kNormThreads / 32 : cols <= 1024 ? kNormThreads / 64 : 1;
   const int64_t needed = (rows + at_a_time - 1) / at_a_time, most = cols <= 4096 ? 512 : 256;
@@ -1533,7 +1558,9 @@ inline int64_t norm_blocks(int64_t rows, int64_t cols) {
   const int64_t shared = needed / 8 > kComputeUnits ? needed / 8 : kComputeUnits;     // enough turns to pay for a row of partial sums
   return shared < most ? shared : most;
 }
-inline int64_t strip_rows(int64_t rows, int64_t cols) {   // rows of a workgroup of the activation's backward pass
+// rows of a workgroup of the activation's backward pass: about 2048 workgroups; 65536x1024 halves 73 us, with 1024 of them 82, with 4096 73;
+// 16384x4096 72, 83 and 74; 16384x1024 23, 25 and 25
+inline int64_t strip_rows(int64_t rows, int64_t cols) {
   const int64_t across = (cols + kGroup - 1) / kGroup;
   int64_t per = (rows * across + 2047) / 2048;
   per = (per + 7) / 8 * 8;
