@@ -47,14 +47,16 @@ int dtype_code(at::ScalarType t) {
 
 void check_status(int rc) { TORCH_CHECK(rc == GACT_OK, "gact: ", gact_strerror(rc)); }
 
+c10::DispatchKeySet wrapped_keys() {
+  return c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::ZeroTensor,
+                              c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper});
+}
 // a tensor (or parameter) itself, no subclass and no wrapper, dense on the GPU
 const at::Tensor& tensor_of(PyObject* o, const char* name) {
   TORCH_CHECK_TYPE(THPVariable_Check(o), name, " must be a tensor");
   const at::Tensor& t = THPVariable_Unpack(o);
   TORCH_CHECK(t.defined() && t.is_cuda(), name, " must be a CUDA tensor!");
-  static const c10::DispatchKeySet wrapped({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::ZeroTensor,
-                                            c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper});
-  TORCH_CHECK(t.layout() == at::kStrided && t.has_storage() && !t.key_set().has_any(wrapped), name, " must be a plain dense tensor");
+  TORCH_CHECK(t.layout() == at::kStrided && t.has_storage() && !t.key_set().has_any(wrapped_keys()), name, " must be a plain dense tensor");
   TORCH_CHECK(dtype_code(t.scalar_type()) >= 0, "The type of ", name, " is not correct!");
   return t;
 }
@@ -186,6 +188,24 @@ variable_list once(variable_list grads, const char* name) {
   return (*stop)(std::move(grads));
 }
 void give_up(SavedVariable& v) { v.reset_data(); }
+// What was saved, as it was saved: hooks for saved tensors may give back anything, and the kernels would read it as if it were the same
+at::Tensor again(SavedVariable& v, at::ScalarType dtype, c10::IntArrayRef shape, const at::Tensor& grad, bool dense = true) {
+  const at::Tensor t = v.unpack();
+  TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.scalar_type() == dtype && t.device() == grad.device() && t.sizes() == shape &&
+                  (!dense || (t.is_contiguous() && !t.is_neg())),
+              "the hooks for saved tensors gave back another tensor than they were given");
+  return t;
+}
+Kept again(SavedVariable& codes, SavedVariable& scale, SavedVariable& mn, int64_t rows, int64_t cols, const at::Tensor& grad) {
+  const int64_t groups = (cols + kGroup - 1) / kGroup;
+  return {again(codes, at::kChar, {rows, round_up(cols, 16)}, grad), again(scale, at::kFloat, {rows, groups}, grad),
+          again(mn, at::kFloat, {rows, groups}, grad)};
+}
+// a gradient that the kernels can read: no batch of them, no subclass
+void check_grad(const at::Tensor& t) {
+  TORCH_CHECK(t.layout() == at::kStrided && t.has_storage() && t.is_cuda() && !t.key_set().has_any(wrapped_keys()),
+              "the gradient must be a plain dense tensor");
+}
 
 // ---- layer norm ----
 struct LayerNormBackward : public Node {
@@ -201,7 +221,11 @@ struct LayerNormBackward : public Node {
     variable_list result(3);
     if (!grads[0].defined()) return result;
     TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
-    const at::Tensor w = has_weight ? weight.unpack() : at::Tensor(), st = stats.unpack(), c = codes.unpack(), s = scale.unpack(), m = mn.unpack();
+    check_grad(grads[0]);
+    const int64_t cols = grads[0].size(-1), rows = grads[0].numel() / cols;
+    const at::Tensor w = has_weight ? again(weight, grads[0].scalar_type(), {cols}, grads[0], false) : at::Tensor();
+    const at::Tensor st = again(stats, at::kFloat, {rows, 2}, grads[0]);
+    const Kept k = again(codes, scale, mn, rows, cols, grads[0]);
     {
       const at::AutoDispatchBelowADInplaceOrView below;
       const Place at(grads[0]);
@@ -218,7 +242,7 @@ struct LayerNormBackward : public Node {
         if (need_b) db = at.empty({dy.cols}, dtype);
         const at::Tensor ws = need_w || need_b ? at.bytes(gact_norm_workspace_bytes(dy.rows, dy.cols)) : at::Tensor();
         const at::Tensor dense = w.defined() ? (w.is_neg() ? w.resolve_neg() : w).contiguous() : w;
-        check_status(gact_norm_backward(dy.data(), dy.ld, in(dense), in(c), c.size(1), (const float*)in(s), (const float*)in(m),
+        check_status(gact_norm_backward(dy.data(), dy.ld, in(dense), in(k.codes), k.codes.size(1), (const float*)in(k.scale), (const float*)in(k.mn),
                                         (const float*)in(st), dtype_code(dtype), dy.rows, dy.cols, out(dx), out(dw), out(db),
                                         (float*)out(ws), at.stream));
       }
@@ -286,11 +310,13 @@ struct LinearBackward : public Node {
     TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
     const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1), need_b = task_should_compute_output(2);
     if (task_should_compute_output(3)) result[3] = dy;
+    check_grad(dy);
+    const int64_t rows = dy.numel() / outer;
     at::Tensor w;
     Kept k, z;
-    if (need_x) w = weight.unpack();
-    if (need_w) k = {codes.unpack(), scale.unpack(), mn.unpack()};
-    if (activation != GACT_ACT_NONE && (need_x || need_w || need_b)) z = {z_codes.unpack(), z_scale.unpack(), z_mn.unpack()};
+    if (need_x) w = again(weight, dy.scalar_type(), {outer, inner}, dy, false);
+    if (need_w) k = again(codes, scale, mn, rows, inner, dy);
+    if (activation != GACT_ACT_NONE && (need_x || need_w || need_b)) z = again(z_codes, z_scale, z_mn, rows, outer, dy);
     {
       const at::AutoDispatchBelowADInplaceOrView below;
       const Place at(dy);

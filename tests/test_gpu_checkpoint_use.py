@@ -264,6 +264,31 @@ def test_a_capture_beside_an_eager_graph_of_its_leaves_is_refused():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_saved_tensors_go_through_hooks_and_come_back_as_they_were():
+    x, w, b = normal(70, 48).requires_grad_(), normal(40, 48, seed=1).requires_grad_(), normal(40, seed=2).requires_grad_()
+    nw = normal(48, seed=3).requires_grad_()
+    dy, dn = normal(70, 40, seed=4), normal(70, 48, seed=5)
+    calls = (lambda: (ops.op_linear(x, w, b, "gelu"), [x, w, b], dy), lambda: (ops.op_layer_norm(x, nw), [x, nw], dn))
+    for call in calls:
+        y, leaves, g = call()
+        want = torch.autograd.grad(y, leaves, g)
+        with torch.autograd.graph.save_on_cpu():
+            y, leaves, g = call()
+        assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(y, leaves, g), want))
+        for change in (lambda t: t.double(), lambda t: t[:1], lambda t: t.cpu(), lambda t: t.reshape(1, -1)):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+                y, leaves, g = call()
+            with pytest.raises(RuntimeError, match="gave back another tensor"):
+                torch.autograd.grad(y, leaves, g)
+
+
+def test_a_batch_of_gradients_is_refused():
+    x, w, nw = normal(6, 16).requires_grad_(), normal(8, 16, seed=1).requires_grad_(), normal(16, seed=2).requires_grad_()
+    for y, leaf in ((ops.op_linear(x, w), w), (ops.op_linear(x, w, None, "silu"), x), (ops.op_layer_norm(x, nw), nw)):
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaf, torch.ones(3, *y.shape, device="cuda"), is_grads_batched=True)
+
+
 def test_two_streams_at_once():
     x, p = normal(2048, 256, dtype=torch.bfloat16), [t.detach() for t in block_parameters(256, 1024, torch.bfloat16)]
     dy = normal(2048, 256, dtype=torch.bfloat16, seed=9)
