@@ -260,19 +260,20 @@ __device__ __forceinline__ float slope(float z, int act) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// Checkpoints of rows.  32 lanes own a group: one 16-byte piece each (float: two), its minimum and maximum over the half wave.
+// Checkpoints of rows.  32 lanes (16 of rows of up to 128 columns) own a group: one 16-byte piece each (float: two), its minimum and maximum over
+// those lanes.
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Bound by memory: 32768x4096 halves 84 us (4.8 TB/s), 16384x1024 floats 16.6 (5.1), 25088x384 halves 11.7, of which the launch and the one
 // load that nothing overlaps are half.  One group at a time: four to a half wave, with their loads together and one division for all of their
 // scales, take 84 us instead of 90 for 134 M halves, but 14 instead of 11.5 for 10 M.  A group shorter than 256 leaves lanes idle (771
 // columns of halves, 22.7 us for 25088 rows, 2.6 TB/s).
-template <typename T, bool WHOLE>
+template <typename T, int LANES, bool WHOLE>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int groups,
                                                          uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale,
                                                          float* __restrict__ mn) {
-  const int64_t unit = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int64_t unit = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const int64_t row = unit / groups;
-  const int g = (int)(unit - row * groups), lane = threadIdx.x & 31;
+  const int g = (int)(unit - row * groups), lane = threadIdx.x % LANES;
   if (row >= rows) return;
   const int col = g * kGroup + lane * kVec, n = cols - col;
   float v[kVec];
@@ -281,8 +282,8 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x
 #pragma unroll
   for (int e = 0; e < kVec; e++)
     if ((WHOLE ? 0 : e) < n) lo = __builtin_fminf(lo, v[e]), hi = __builtin_fmaxf(hi, v[e]);
-  lo = over_lanes<Least, 32>(lo);
-  hi = over_lanes<Most, 32>(hi);
+  lo = over_lanes<Least, LANES>(lo);
+  hi = over_lanes<Most, LANES>(hi);
   const float s = scale_of(lo, hi);
   if (n > 0)
     *(u32x2*)(codes + row * ldc + col) = u32x2{four_codes(v[0], v[1], v[2], v[3], lo, s), four_codes(v[4], v[5], v[6], v[7], lo, s)};
@@ -294,13 +295,13 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x
 
 // The values again, the same lanes: 32768x4096 halves 72 us (5.7 TB/s), 16384x1024 12.0 (4.3), 25088x384 8.3.  1 / scale is made by every
 // lane: the division is hidden behind the loads.
-template <typename T, bool WHOLE>
+template <typename T, int LANES, bool WHOLE>
 __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scale,
                                                       const float* __restrict__ mn, int64_t rows, int cols, int groups,
                                                       T* __restrict__ out) {
-  const int64_t unit = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+  const int64_t unit = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
   const int64_t row = unit / groups;
-  const int g = (int)(unit - row * groups), lane = threadIdx.x & 31;
+  const int g = (int)(unit - row * groups), lane = threadIdx.x % LANES;
   if (row >= rows) return;
   const int col = g * kGroup + lane * kVec, n = cols - col;
   if (n <= 0) return;
@@ -639,15 +640,17 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
 // dz = dy act'(z) from the checkpoint of z, and the column sums of dz before they are rounded.  A thread owns 8 columns and walks
 // down `per` rows; without codes (no activation) dz is dy, copied to the products' stride where `dz` is given.
 // Bound by memory, 32768x4096 halves GELU 134 us (5.0 TB/s), SiLU 128, sums alone 47 (5.7); 16384x1024 23, 22 and 11.  32 lanes and 256
-// columns to a row, as the codes' groups are: narrower outputs leave lanes idle (401408x96 floats 195 us, 1.8 TB/s).
+// columns to a row, as the codes' groups are, 16 lanes where 128 columns are enough: 401408x96 halves 56 (3.4).  In floats GELU's exact error
+// function counts: 401408x96 120 us (2.9 TB/s), SiLU 89.
 // ---------------------------------------------------------------------------------------------------------------------------------
-template <typename T, bool WHOLE>
+template <typename T, int LANES, bool WHOLE>
 __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __restrict__ dy, int64_t lddy, const uint8_t* __restrict__ codes,
                                                                   int64_t ldc, const float* __restrict__ scale,
                                                                   const float* __restrict__ mn, int act, int64_t rows, int cols, int per,
                                                                   T* __restrict__ dz, int64_t lddz, float* __restrict__ partial) {
-  __shared__ float shared[4][32][kVec + 1];
-  const int lane = threadIdx.x & 31, strip = threadIdx.x >> 5;     // 8 rows at a time
+  constexpr int kRows = 256 / LANES;      // at a time
+  __shared__ float shared[4][LANES][kVec + 1];
+  const int lane = threadIdx.x % LANES, strip = threadIdx.x / LANES;
   const int col = (int)blockIdx.x * kGroup + lane * kVec;
   const int groups = (cols + kGroup - 1) / kGroup;
   const int64_t first = (int64_t)blockIdx.y * per, last = first + per < rows ? first + per : rows;
@@ -656,7 +659,7 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __res
 #pragma unroll
   for (int e = 0; e < kVec; e++) sum[e] = 0.0f;
   if (left > 0 || (dz && col < lddz)) {
-    for (int64_t row = first + strip; row < last; row += 8) {
+    for (int64_t row = first + strip; row < last; row += kRows) {
       float g[kVec], z[kVec];
       load_cols<T, WHOLE>(dy + row * lddy + col, left, g);
       if (codes && left > 0) {
@@ -671,15 +674,17 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __res
     }
   }
   if (!partial) return;
-  // strips 2i and 2i + 1 share a wave
+  // over the rows of a wave, then over the waves
 #pragma unroll
-  for (int e = 0; e < kVec; e++) sum[e] += __shfl_xor(sum[e], 32);
-  if ((strip & 1) == 0)
+  for (int o = LANES; o < 64; o *= 2)
 #pragma unroll
-    for (int e = 0; e < kVec; e++) shared[strip >> 1][lane][e] = sum[e];
+    for (int e = 0; e < kVec; e++) sum[e] += __shfl_xor(sum[e], o);
+  if ((threadIdx.x & 63) < LANES)
+#pragma unroll
+    for (int e = 0; e < kVec; e++) shared[threadIdx.x >> 6][lane][e] = sum[e];
   __syncthreads();
-  const int c = (int)threadIdx.x;   // 256 columns
-  if ((int)blockIdx.x * kGroup + c < cols) {
+  const int c = (int)threadIdx.x;
+  if (c < LANES * kVec && (int)blockIdx.x * kGroup + c < cols) {
     float s = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; w++) s += shared[w][c / kVec][c % kVec];
@@ -1383,12 +1388,14 @@ template <typename T, bool WHOLE>
 __device__ __forceinline__ typename Mma<T>::Frag fragment_of(const T* row, int64_t k, int64_t depth) {
   using Frag = typename Mma<T>::Frag;
   constexpr int N = 16 / (int)sizeof(T);
+  typedef T Unaligned __attribute__((ext_vector_type(N), aligned(sizeof(T))));
   Frag f;
   if (WHOLE) {
     if (k < depth) return *(const Frag*)(row + k);
 #pragma unroll
     for (int e = 0; e < N; e++) f[e] = (T)0.0f;
   } else {
+    if (k + N <= depth) return *(const Unaligned*)(row + k);
 #pragma unroll
     for (int e = 0; e < N; e++) f[e] = k + e < depth ? row[k + e] : (T)0.0f;
   }
@@ -1412,7 +1419,7 @@ __global__ __launch_bounds__(512) void few_rows_kernel(ProductArgs p) {
     acc[m] = f32x4{0, 0, 0, 0};
   }
   // the waves take steps of 64 bytes in turn, UNROLL of them with all their loads on the way
-  constexpr int UNROLL = !WHOLE ? 2 : MT == 4 ? 4 : 8;
+  constexpr int UNROLL = !WHOLE || MT == 4 ? 4 : 8;
   const int split = blockIdx.y;
   const int64_t first = split * p.per_split, end = first + p.per_split < p.depth ? first + p.per_split : p.depth;
   for (int64_t k0 = first + wave * SPAN; k0 < end; k0 += (int64_t)WAVES * SPAN * UNROLL) {
@@ -1558,13 +1565,17 @@ inline int64_t norm_blocks(int64_t rows, int64_t cols) {
   const int64_t shared = needed / 8 > kComputeUnits ? needed / 8 : kComputeUnits;     // enough turns to pay for a row of partial sums
   return shared < most ? shared : most;
 }
+// lanes of a group where groups are walked one by one: a row of at most 128 columns needs 16 of them (401408x96 floats,
+// checkpoint 36 us, with 32 lanes 65, GELU's backward pass 120 and 198; halves 35 and 65, 56 and 91)
+inline int lanes_of(int64_t cols) { return cols <= 128 ? 16 : 32; }
 // rows of a workgroup of the activation's backward pass: about 2048 workgroups; 65536x1024 halves 73 us, with 1024 of them 82, with 4096 73;
 // 16384x4096 72, 83 and 74; 16384x1024 23, 25 and 25
 inline int64_t strip_rows(int64_t rows, int64_t cols) {
   const int64_t across = (cols + kGroup - 1) / kGroup;
   int64_t per = (rows * across + 2047) / 2048;
-  per = (per + 7) / 8 * 8;
-  if (per < 8) per = 8;
+  const int64_t at_a_time = 256 / lanes_of(cols);
+  per = (per + at_a_time - 1) / at_a_time * at_a_time;
+  if (per < at_a_time) per = at_a_time;
   while ((rows + per - 1) / per > 65535) per *= 2;
   return per;
 }
@@ -1738,12 +1749,14 @@ int gact_checkpoint(const void* x, int dtype, int64_t rows, int64_t cols, int64_
   if (rows == 0) return GACT_OK;
   if (!x || !codes || !scale || !mn) return GACT_EINVAL;
   if (!codes_fit(codes, cols, ldc)) return GACT_EALIGN;
-  const int64_t groups = (cols + kGroup - 1) / kGroup, blocks = (rows * groups + 7) / 8;
+  const int64_t groups = (cols + kGroup - 1) / kGroup, units = 256 / lanes_of(cols), blocks = (rows * groups + units - 1) / units;
   if (!blocks_fit(blocks)) return GACT_ELIMIT;
   fresh_launch();
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    auto kernel = whole_rows(x, dtype, cols, ldx) ? checkpoint_kernel<T, true> : checkpoint_kernel<T, false>;
+    const bool whole = whole_rows(x, dtype, cols, ldx);
+    auto kernel = lanes_of(cols) == 16 ? (whole ? checkpoint_kernel<T, 16, true> : checkpoint_kernel<T, 16, false>)
+                                       : (whole ? checkpoint_kernel<T, 32, true> : checkpoint_kernel<T, 32, false>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, (int)cols, ldx, (int)groups,
                        (uint8_t*)codes, ldc, scale, mn);
     return launch_status();
@@ -1756,12 +1769,14 @@ int gact_restore(const void* codes, int64_t ldc, const float* scale, const float
   if (rows == 0) return GACT_OK;
   if (!codes || !scale || !mn || !out) return GACT_EINVAL;
   if (!codes_fit(codes, cols, ldc) || !aligned16(out)) return GACT_EALIGN;
-  const int64_t groups = (cols + kGroup - 1) / kGroup, blocks = (rows * groups + 7) / 8;
+  const int64_t groups = (cols + kGroup - 1) / kGroup, units = 256 / lanes_of(cols), blocks = (rows * groups + units - 1) / units;
   if (!blocks_fit(blocks)) return GACT_ELIMIT;
   fresh_launch();
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    auto kernel = whole_rows(out, dtype, cols, cols) ? restore_kernel<T, true> : restore_kernel<T, false>;
+    const bool whole = whole_rows(out, dtype, cols, cols);
+    auto kernel = lanes_of(cols) == 16 ? (whole ? restore_kernel<T, 16, true> : restore_kernel<T, 16, false>)
+                                       : (whole ? restore_kernel<T, 32, true> : restore_kernel<T, 32, false>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)codes, ldc, scale, mn, rows,
                        (int)cols, (int)groups, (T*)out);
     return launch_status();
@@ -1935,7 +1950,9 @@ int gact_activation_backward(const void* dy, int64_t lddy, const void* codes, in
   fresh_launch();
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    auto kernel = whole_rows(dy, dtype, cols, lddy) ? activation_backward_kernel<T, true> : activation_backward_kernel<T, false>;
+    const bool whole = whole_rows(dy, dtype, cols, lddy);
+    auto kernel = lanes_of(cols) == 16 ? (whole ? activation_backward_kernel<T, 16, true> : activation_backward_kernel<T, 16, false>)
+                                       : (whole ? activation_backward_kernel<T, 32, true> : activation_backward_kernel<T, 32, false>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)((cols + kGroup - 1) / kGroup), (unsigned)strips), dim3(256), 0, (hipStream_t)stream,
                        (const T*)dy, lddy, (const uint8_t*)codes, ldc, scale, mn, activation, rows, (int)cols, (int)per, (T*)dz, lddz,
                        dbias ? workspace : nullptr);

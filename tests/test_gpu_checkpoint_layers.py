@@ -22,7 +22,7 @@ def normal(*shape, dtype=torch.float32, seed=0, scale=1.0):
 
 # ---- checkpoints ----
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 8), (3, 7), (2, 255), (5, 256), (4, 257), (33, 264), (17, 512), (9, 771), (70, 1000), (3, 4096)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 8), (3, 7), (2, 255), (5, 256), (4, 257), (33, 264), (17, 512), (9, 771), (70, 1000), (3, 4096), (37, 121), (300, 128), (41, 129)])
 def test_checkpoint_codes_and_values(rows, cols, dtype):
     x = normal(rows, cols, dtype=dtype)
     kept = ops.op_checkpoint(x)
@@ -230,7 +230,7 @@ def check_linear(rows, inner, outer, dtype, act, with_bias, with_residual, view=
 
 
 LINEAR_SHAPES = [(1, 1, 1), (1, 64, 16), (3, 9, 5), (16, 256, 48), (17, 100, 33), (33, 264, 40), (64, 520, 257), (65, 128, 128), (100, 771, 130),
-                 (129, 64, 384), (200, 1000, 263), (260, 320, 520), (1030, 136, 516)]
+                 (129, 64, 384), (200, 1000, 263), (260, 320, 520), (1030, 136, 516), (5000, 24, 96), (700, 16, 125)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
@@ -251,7 +251,7 @@ def test_linear_of_many_tiles(dtype):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("rows,inner,outer", [(1, 4096, 264), (24, 2056, 264), (64, 4100, 72), (65, 1030, 48), (100, 2104, 520), (300, 4000, 130),
-                                              (50, 4096, 4096)])
+                                              (50, 4096, 4096), (20, 2047, 4100)])
 def test_linear_cut_along_its_depth(rows, inner, outer, dtype):
     for act, with_bias, with_residual in ((None, True, True), ("gelu", True, False), ("silu", False, True)):
         check_linear(rows, inner, outer, dtype, act, with_bias, with_residual)
