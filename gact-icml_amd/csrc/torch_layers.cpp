@@ -394,8 +394,8 @@ at::Tensor linear(const at::Tensor& input, const at::Tensor& weight, const std::
       Rows a = x, w = rows_of(weight, "weight"), r;
       int64_t depth = inner;
       // unaligned rows: few of them go to the kernel as they are where that costs less than copies of both operands (64 rows, 8191 to 8192: halves
-      // 246 us as they are, 94 copied, floats 205 and 190; 37 rows, 4095 to 4096: 46 and 30, 44 and 51; 17 rows, 771 to 1285: 6, three launches more
-      // copied; up to 16 rows never: 8191 to 8192 98 and 94, floats 74 and 190)
+      // 246 us as they are, 94 copied, floats 205 and 190; 37 rows, 4095 to 4096: 46 and 30, 44 and 51; 17 rows, 771 to 1285: 6 as they are, and a
+      // copy is a launch of 4).  Up to 16 rows never: 8191 to 8192 98 and 74 us, no more than the copies for 64 rows
       if (x.rows > GACT_LINEAR_FEW_ROWS || (x.rows > 16 && inner * outer * (int64_t)input.element_size() >= kLargeWeights)) {
         a = product_rows(a, at);
         w = product_rows(w, at);
