@@ -1541,16 +1541,24 @@ int with_type(int dtype, F&& f) {
   }
 }
 
-// threads of a row, its pieces per thread, and the rows that a thread of the forward pass takes at a time: the fewest threads whose registers
-// hold the row without spilling beside the next row's loads
-template <typename F>
+// Threads of a row, its pieces per thread, and the rows that a thread of the forward pass takes at a time: few threads, whose sums need no
+// exchange through LDS, as far as the registers hold the row.  us forward / backward, and with other numbers of threads:
+//   401408x96 floats 71 / 73, 32 threads 91 / 124           100352x192 halves 32 / 32, 64 threads 50 / 51
+//   65536x512 halves 40 / 43, 32 threads 41 / 46            65536x1024 halves 72 / 81, 256 threads 110 / 194
+//   16384x2048 halves 37 / 40, 64 and 256 threads the other way round 46 / 66: the forward pass has no sums to keep between rows
+//   16384x4096 halves 67 / 88, 512 threads 72 / 93          8192x8192 halves 71 / 93, 256 threads 84 / 96
+template <bool BACKWARD, typename F>
 int with_row_shape(int64_t cols, F&& f) {
   using std::integral_constant;
   if (cols <= 128) return f(integral_constant<int, 16>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
   if (cols <= 256) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
   if (cols <= 512) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
   if (cols <= 1024) return f(integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
-  if (cols <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  if constexpr (BACKWARD) {
+    if (cols <= 2048) return f(integral_constant<int, 64>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  } else {
+    if (cols <= 2048) return f(integral_constant<int, 256>{}, integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  }
   if (cols <= 4096) return f(integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
   if (cols <= 8192) return f(integral_constant<int, 512>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
   return f(integral_constant<int, 512>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
@@ -1559,7 +1567,7 @@ int with_row_shape(int64_t cols, F&& f) {
 // floats 71 us, 101 / 75; 65536x1024 halves 78, 75 / 84; 16384x4096 83, 125 / 99.  Rows beyond 4096 columns fill a compute unit by
 // themselves, at most 256: 8192x8192 87, with 512 99
 inline int64_t norm_blocks(int64_t rows, int64_t cols) {
-  const int64_t at_a_time = cols <= 128 ? kNormThreads / 16 : cols <= 256 ? kNormThreads / 32 : cols <= 1024 ? kNormThreads / 64 : 1;
+  const int64_t at_a_time = cols <= 128 ? kNormThreads / 16 : cols <= 256 ? kNormThreads / 32 : cols <= 2048 ? kNormThreads / 64 : 1;
   const int64_t needed = (rows + at_a_time - 1) / at_a_time, most = cols <= 4096 ? 512 : 256;
   if (needed <= kComputeUnits) return needed;
   const int64_t shared = needed / 8 > kComputeUnits ? needed / 8 : kComputeUnits;     // enough turns to pay for a row of partial sums
@@ -1809,7 +1817,7 @@ int gact_norm_forward(const void* x, int64_t ldx, const void* weight, const void
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     const bool whole = whole_rows(x, dtype, cols, ldx) && whole_rows(y, dtype, cols, cols) && aligned16(weight) && aligned16(bias);
-    return with_row_shape(cols, [&](auto lpr, auto nc, auto at_a_time) {
+    return with_row_shape<false>(cols, [&](auto lpr, auto nc, auto at_a_time) {
       constexpr int LPR = decltype(lpr)::value, NC = decltype(nc)::value, U = decltype(at_a_time)::value;
       auto run = [&](auto kernel, int u) {
         const int64_t blocks = (rows + RowShape<LPR>::kRows * u - 1) / (RowShape<LPR>::kRows * u);
@@ -1819,7 +1827,8 @@ int gact_norm_forward(const void* x, int64_t ldx, const void* weight, const void
                            stats);
         return launch_status();
       };
-      // few rows: one at a time, on as many compute units as there are
+      // few rows: one at a time, on as many compute units as there are (2000x1024 halves 5.7 us, two at a time 6.6; 8000x512 7.0, four 8.5;
+      // 25088x384, above the bound, four 19.8)
       if (U > 1 && rows < (int64_t)kComputeUnits * 4 * RowShape<LPR>::kRows * U)
         return whole ? run(norm_forward_kernel<T, LPR, NC, 1, true>, 1) : run(norm_forward_kernel<T, LPR, NC, 1, false>, 1);
       return whole ? run(norm_forward_kernel<T, LPR, NC, U, true>, U) : run(norm_forward_kernel<T, LPR, NC, U, false>, U);
@@ -1844,7 +1853,7 @@ int gact_norm_backward(const void* dy, int64_t lddy, const void* weight, const v
     using T = decltype(zero);
     const bool whole = whole_rows(dy, dtype, cols, lddy) && whole_rows(dx, dtype, cols, cols) && aligned16(weight);
     const int64_t blocks = norm_blocks(rows, cols);
-    const int rc = with_row_shape(cols, [&](auto lpr, auto nc, auto) {
+    const int rc = with_row_shape<true>(cols, [&](auto lpr, auto nc, auto) {
       constexpr int LPR = decltype(lpr)::value, NC = decltype(nc)::value;
       auto kernel = whole ? norm_backward_kernel<T, LPR, NC, true> : norm_backward_kernel<T, LPR, NC, false>;
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(SharedRows<LPR>::kThreads), 0, (hipStream_t)stream, (const T*)dy, lddy,
@@ -1873,6 +1882,7 @@ int gact_linear(const void* x, int64_t ldx, const void* weight, int64_t ldw, con
   if (!known(dtype) || !layer_sizes(rows, inner, outer) || activation < GACT_ACT_NONE || activation > GACT_ACT_SILU) return GACT_EINVAL;
   if (rows == 0) return GACT_OK;
   if (!x || !weight || !y || (codes && (!scale || !mn || activation == GACT_ACT_NONE)) || (residual && ldr < outer && rows > 1)) return GACT_EINVAL;
+  if ((rows > 1 && ldx < inner) || (outer > 1 && ldw < inner)) return GACT_EINVAL;
   if (codes && !codes_fit(codes, outer, ldc)) return GACT_EALIGN;
   const bool whole = operand_fits(x, ldx, dtype, inner) && operand_fits(weight, ldw, dtype, inner);
   const Forward f = forward_of(dtype, rows, inner, outer, codes != nullptr, whole);

@@ -44,7 +44,8 @@ def test_library_refuses_before_it_touches_the_gpu():
         x, ldx, 16, 8, None, None, 0, act, 0, rows, inner, 8, 16, codes, 16, 16, 16, ws, None)
     assert linear(act=4) == EINVAL and linear(rows=-1) == EINVAL and linear(inner=0) == EINVAL
     assert linear(codes=16) == EINVAL                                                            # codes without an activation
-    assert linear(x=8) == EALIGN and linear(ldx=9) == EALIGN and linear(ldx=4, inner=8) == EALIGN
+    assert linear(x=8) == EALIGN and linear(ldx=9) == EALIGN and linear(ldx=4, inner=8) == EINVAL
+    assert linear(ldx=4, rows=9) == EINVAL and linear(ldx=-8, rows=9) == EINVAL                  # rows over one another
     assert linear(act=1, codes=8) == EALIGN and linear(act=1, codes=16) == EALIGN and linear(act=1, codes=16, ws=8) == EALIGN   # workspace
     assert L.gact_linear(16, 1 << 21, 16, 8, None, None, 0, 0, 0, 100, 8, 8, 16, None, 0, None, None, None, None) == EALIGN   # beyond a tile's window
     act = lambda codes, which, dz, lddz, db, ws: L.gact_activation_backward(16, 9, codes, 16, 16, 16, which, 0, 4, 9, dz, lddz, db, ws, None)  # noqa: E731
