@@ -282,6 +282,23 @@ def test_saved_tensors_go_through_hooks_and_come_back_as_they_were():
                 torch.autograd.grad(y, leaves, g)
 
 
+def test_inference_mode_gives_the_same_results():
+    x, w, b, nw = normal(70, 48), normal(40, 48, seed=1).requires_grad_(), normal(40, seed=2).requires_grad_(), normal(48, seed=3).requires_grad_()
+
+    def step():
+        h = ops.op_layer_norm(x, nw)
+        c = ops.op_checkpoint(h.detach())
+        return [h, ops.op_linear(h, w, b, "gelu"), ops.op_linear(h[:1], w, b), ops.op_restore(c), ops.op_checkpoint_product(normal(70, 24, seed=4), c)]
+
+    want = step()
+    with torch.inference_mode():
+        got = step()
+    assert all(t.is_inference() and not t.requires_grad for t in got)
+    with torch.no_grad():
+        plain = step()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(got, want, plain))
+
+
 def test_a_batch_of_gradients_is_refused():
     x, w, nw = normal(6, 16).requires_grad_(), normal(8, 16, seed=1).requires_grad_(), normal(16, seed=2).requires_grad_()
     for y, leaf in ((ops.op_linear(x, w), w), (ops.op_linear(x, w, None, "silu"), x), (ops.op_layer_norm(x, nw), nw)):
