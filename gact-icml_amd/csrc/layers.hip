@@ -34,6 +34,9 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 constexpr int kGroup = 256;
 constexpr int kVec = 8;   // columns of a lane's piece
 
+// The workgroup's number in a launch of grid_of(): beyond 2^32 threads a launch goes on along y
+__device__ __forceinline__ int64_t block_of() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // ---- eight consecutive columns ----
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[kVec]) {
@@ -271,7 +274,7 @@ template <typename T, int LANES, bool WHOLE>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int groups,
                                                          uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale,
                                                          float* __restrict__ mn) {
-  const int64_t unit = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int64_t unit = block_of() * (256 / LANES) + threadIdx.x / LANES;
   const int64_t row = unit / groups;
   const int g = (int)(unit - row * groups), lane = threadIdx.x % LANES;
   if (row >= rows) return;
@@ -299,7 +302,7 @@ template <typename T, int LANES, bool WHOLE>
 __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scale,
                                                       const float* __restrict__ mn, int64_t rows, int cols, int groups,
                                                       T* __restrict__ out) {
-  const int64_t unit = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int64_t unit = block_of() * (256 / LANES) + threadIdx.x / LANES;
   const int64_t row = unit / groups;
   const int g = (int)(unit - row * groups), lane = threadIdx.x % LANES;
   if (row >= rows) return;
@@ -316,7 +319,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void pad_rows_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, T* __restrict__ out,
                                                        int ldo) {
   const int per = ldo / kVec;
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t unit = block_of() * 256 + threadIdx.x;
   const int64_t row = unit / per;
   if (row >= rows) return;
   const int col = (int)(unit - row * per) * kVec;
@@ -364,8 +367,8 @@ __global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_forward_kernel(
   using Shape = RowShape<LPR>;
   __shared__ float shared[2 * Shape::kWaves];
   const int lane = threadIdx.x % LPR;
-  const int64_t row0 = ((int64_t)blockIdx.x * Shape::kRows + threadIdx.x / LPR) * U;
-  if (Shape::kRows > 1 && row0 >= rows) return;
+  const int64_t row0 = (block_of() * Shape::kRows + threadIdx.x / LPR) * U;
+  if (row0 >= rows) return;      // all of the row's threads, so none waits for another
   const int there = U == 1 || rows - row0 >= U ? U : (int)(rows - row0);      // of the U rows
   float v[U][NC][kVec];
 #pragma unroll
@@ -1525,6 +1528,12 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 inline int size_of(int dtype) { return dtype == GACT_F32 ? 4 : 2; }
 inline bool known(int dtype) { return dtype == GACT_F32 || dtype == GACT_F16 || dtype == GACT_BF16; }
 inline bool blocks_fit(int64_t blocks) { return blocks > 0 && blocks <= 0x7fffffff; }
+// A launch takes fewer than 2^32 threads along x: `blocks` workgroups along x where they fit, else in as many equal rows along y as it takes
+// (block_of() counts them; up to a row's worth behind the last one find nothing to do)
+inline dim3 grid_of(int64_t blocks, int threads) {
+  const int64_t most = 0xffffffff / threads, down = (blocks + most - 1) / most;
+  return dim3((unsigned)((blocks + down - 1) / down), (unsigned)down);
+}
 constexpr int64_t kMostCols = GACT_LAYER_MAX_COLS;
 constexpr int kComputeUnits = 256;
 
@@ -1767,7 +1776,7 @@ int gact_checkpoint(const void* x, int dtype, int64_t rows, int64_t cols, int64_
     const bool whole = whole_rows(x, dtype, cols, ldx);
     auto kernel = lanes_of(cols) == 16 ? (whole ? checkpoint_kernel<T, 16, true> : checkpoint_kernel<T, 16, false>)
                                        : (whole ? checkpoint_kernel<T, 32, true> : checkpoint_kernel<T, 32, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, (int)cols, ldx, (int)groups,
+    hipLaunchKernelGGL(kernel, grid_of(blocks, 256), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, (int)cols, ldx, (int)groups,
                        (uint8_t*)codes, ldc, scale, mn);
     return launch_status();
   });
@@ -1787,7 +1796,7 @@ int gact_restore(const void* codes, int64_t ldc, const float* scale, const float
     const bool whole = whole_rows(out, dtype, cols, cols);
     auto kernel = lanes_of(cols) == 16 ? (whole ? restore_kernel<T, 16, true> : restore_kernel<T, 16, false>)
                                        : (whole ? restore_kernel<T, 32, true> : restore_kernel<T, 32, false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)codes, ldc, scale, mn, rows,
+    hipLaunchKernelGGL(kernel, grid_of(blocks, 256), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)codes, ldc, scale, mn, rows,
                        (int)cols, (int)groups, (T*)out);
     return launch_status();
   });
@@ -1803,7 +1812,7 @@ int gact_pad_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t 
   fresh_launch();
   return with_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, (int)cols, ldx,
+    hipLaunchKernelGGL((pad_rows_kernel<T>), grid_of(blocks, 256), dim3(256), 0, (hipStream_t)stream, (const T*)x, rows, (int)cols, ldx,
                        (T*)out, (int)ldo);
     return launch_status();
   });
@@ -1824,7 +1833,7 @@ int gact_norm_forward(const void* x, int64_t ldx, const void* weight, const void
       auto run = [&](auto kernel, int u) {
         const int64_t blocks = (rows + RowShape<LPR>::kRows * u - 1) / (RowShape<LPR>::kRows * u);
         if (!blocks_fit(blocks)) return GACT_ELIMIT;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(RowShape<LPR>::kThreads), 0, (hipStream_t)stream, (const T*)x, ldx,
+        hipLaunchKernelGGL(kernel, grid_of(blocks, RowShape<LPR>::kThreads), dim3(RowShape<LPR>::kThreads), 0, (hipStream_t)stream, (const T*)x, ldx,
                            (const T*)weight, (const T*)bias, rows, (int)cols, 1.0f / (float)cols, eps, (T*)y, (uint8_t*)codes, ldc, scale, mn,
                            stats);
         return launch_status();

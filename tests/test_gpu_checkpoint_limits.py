@@ -1,0 +1,58 @@
+"""The layers on 8-bit checkpoints at their limits: launches of 2^32 threads and more."""
+import pytest
+import torch
+
+from gact import ops
+from gact.cpp_extension import _abi
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _give_memory_back():
+    torch.cuda.empty_cache()
+    yield
+    torch.cuda.empty_cache()
+
+
+def repeated(rows, cols, dtype, period):
+    """[rows, cols] of which every `period` rows are the same, and those rows."""
+    g = torch.Generator(device="cuda").manual_seed(rows % 1000 + cols)
+    small = torch.randn(period, cols, generator=g, device="cuda").to(dtype)
+    x = torch.empty(rows, cols, dtype=dtype, device="cuda")
+    x.view(-1, period, cols).copy_(small)
+    return x, small
+
+
+def all_like(big, small):
+    """Whether every part of `big` is `small`."""
+    return all(bool((part == small).all()) for part in big.view(-1, *small.shape).split(1 << 14))
+
+
+# threads of the launch over 2^32: (groups / groups of a workgroup) of 256 threads.  Sixteen lanes to a group, then 32 with a short last group
+@pytest.mark.parametrize("rows,cols,a_workgroup", [((1 << 28) + 64, 1, 16), ((1 << 26) + 64, 257, 8)])
+def test_checkpoint_of_more_groups_than_a_launch_is_wide(rows, cols, a_workgroup):
+    assert rows * -(-cols // 256) // a_workgroup * 256 > 1 << 32
+    x, small = repeated(rows, cols, torch.float16, 64)
+    kept, want = ops.op_checkpoint(x), ops.op_checkpoint(small)
+    del x
+    assert all_like(kept.codes[:, :cols].contiguous(), want.codes[:, :cols])
+    assert all_like(kept.scale, want.scale) and all_like(kept.min, want.min)
+    back = ops.op_restore(kept)
+    assert all_like(back, ops.op_restore(want))
+
+
+def test_layer_norm_of_more_rows_than_a_launch_is_wide():
+    rows, cols = (1 << 24) + 64, 1025        # 256 threads to a row
+    x, small = repeated(rows, cols, torch.bfloat16, 64)
+    w, b = torch.linspace(0.5, 2, cols, device="cuda").bfloat16(), torch.linspace(-1, 1, cols, device="cuda").bfloat16()
+    with torch.no_grad():
+        assert all_like(ops.op_layer_norm(x, w, b), ops.op_layer_norm(small, w, b))
+
+
+def test_rows_padded_to_more_pieces_than_a_launch_is_wide():
+    rows, cols, to = (1 << 23) + 64, 3, 4096
+    x, small = repeated(rows, cols, torch.float16, 64)
+    out = torch.empty(rows, to, dtype=torch.float16, device="cuda")
+    _abi.check(_abi.lib().gact_pad_rows(x.data_ptr(), _abi.dtype_code(x.dtype), rows, cols, cols, out.data_ptr(), to, _abi.stream_of(x)))
+    assert all_like(out, torch.nn.functional.pad(small, (0, to - cols)))
