@@ -298,7 +298,8 @@ struct LinearBackward : public Node {
   SavedVariable weight, codes, scale, mn, z_codes, z_scale, z_mn;
   int activation = GACT_ACT_NONE;
   int64_t inner = 0, outer = 0;
-  bool has_weight = false, has_codes = false, released = false;
+  at::ScalarType weight_dtype = at::kFloat;      // under autocast not the layer's type
+  bool released = false;
   std::string name() const override { return "OpLinearBackward"; }
   void release_variables() override {
     for (SavedVariable* v : {&weight, &codes, &scale, &mn, &z_codes, &z_scale, &z_mn}) give_up(*v);
@@ -315,7 +316,7 @@ struct LinearBackward : public Node {
     const int64_t rows = dy.numel() / outer;
     at::Tensor w;
     Kept k, z;
-    if (need_x) w = again(weight, dy.scalar_type(), {outer, inner}, dy, false);
+    if (need_x) w = again(weight, weight_dtype, {outer, inner}, dy, false);
     if (need_w) k = again(codes, scale, mn, rows, inner, dy);
     if (activation != GACT_ACT_NONE && (need_x || need_w || need_b)) z = again(z_codes, z_scale, z_mn, rows, outer, dy);
     {
@@ -328,7 +329,7 @@ struct LinearBackward : public Node {
       shape.back() = inner;
       if (g.rows == 0) {
         if (need_x) result[0] = at.zeros(shape, dtype);
-        if (need_w) result[1] = at.zeros({outer, inner}, dtype);
+        if (need_w) result[1] = at.zeros({outer, inner}, weight_dtype);
         if (need_b) result[2] = at.zeros({outer}, dtype);
         return result;
       }
@@ -349,20 +350,24 @@ struct LinearBackward : public Node {
                                               out(result[2]), (float*)out(ws), at.stream));
       }
       if (need_x) {
-        const Rows held = product_rows(rows_of(w, "weight"), at);
+        const Rows held = product_rows(rows_of(w.to(dtype), "weight"), at);
         result[0] = at.empty(shape, dtype);
         const at::Tensor ws = at.bytes(gact_product_workspace_bytes(code, g.rows, inner, outer));
         check_status(gact_product(dz.data(), dz.ld, held.data(), held.ld, code, g.rows, outer, inner, out(result[0]), out(ws), at.stream));
       }
-      if (need_w) result[1] = weight_product(dz, k, inner, dtype, at);
+      if (need_w) result[1] = weight_product(dz, k, inner, dtype, at).to(weight_dtype);
     }
     return once(std::move(result), "op_linear");
   }
 };
 
+// `autocast`: the weight may be of another type and is rounded to the layer's in the call.  The node saves the weight itself and rounds it again: a
+// rounded copy would be memory of its own until the backward pass, and hooks for saved tensors that leave a model's parameters as they are
+// would not know it
 at::Tensor linear(const at::Tensor& input, const at::Tensor& weight, const std::optional<at::Tensor>& bias, int activation,
-                  const std::optional<at::Tensor>& residual) {
-  check_like(weight, input, "weight");
+                  const std::optional<at::Tensor>& residual, bool autocast) {
+  TORCH_CHECK(autocast || weight.scalar_type() == input.scalar_type(), "The type of weight is not correct!");
+  TORCH_CHECK(weight.device() == input.device(), "weight is on another device");
   TORCH_CHECK(input.dim() >= 1 && weight.dim() == 2 && weight.size(1) == input.size(-1), "weight must be [outer, ",
               input.dim() ? std::to_string(input.size(-1)) : std::string("-"), "], got ", weight.sizes());
   const int64_t outer = weight.size(0), inner = weight.size(1);
@@ -391,7 +396,7 @@ at::Tensor linear(const at::Tensor& input, const at::Tensor& weight, const std::
     if (keep_z) z = room_for(x.rows, outer, at);
     if (keep_x) k = x.rows ? compress(x, at) : room_for(0, inner, at);
     if (x.rows) {
-      Rows a = x, w = rows_of(weight, "weight"), r;
+      Rows a = x, w = rows_of(weight.to(dtype), "weight"), r;
       int64_t depth = inner;
       // unaligned rows: few of them go to the kernel as they are where that costs less than copies of both operands (64 rows, 8191 to 8192: halves
       // 246 us as they are, 94 copied, floats 205 and 190; 37 rows, 4095 to 4096: 46 and 30, 44 and 51; 17 rows, 771 to 1285: 6 as they are, and a
@@ -414,6 +419,7 @@ at::Tensor linear(const at::Tensor& input, const at::Tensor& weight, const std::
     node->activation = activation;
     node->inner = inner;
     node->outer = outer;
+    node->weight_dtype = weight.scalar_type();
     if (input.requires_grad()) node->weight = SavedVariable(weight, false);
     if (keep_x) {
       node->codes = SavedVariable(k.codes, false);
@@ -454,16 +460,16 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// linear(x, weight, bias or None, activation's number, residual or None) -> y
+// linear(x, weight, bias or None, activation's number, residual or None, whether autocast is on) -> y
 PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 5);
+  arguments(n, 6);
   const int64_t act = integer_of(args[3]);
   TORCH_CHECK(act >= GACT_ACT_NONE && act <= GACT_ACT_SILU, "unknown activation");
   const at::Tensor& x = tensor_of(args[0], "data");
   const at::Tensor& weight = tensor_of(args[1], "weight");
   const std::optional<at::Tensor> bias = tensor_or_none(args[2], "bias"), residual = tensor_or_none(args[4], "residual");
-  return THPVariable_Wrap(linear(x, weight, bias, (int)act, residual));
+  return THPVariable_Wrap(linear(x, weight, bias, (int)act, residual, args[5] == Py_True));
   END_HANDLE_TH_ERRORS
 }
 

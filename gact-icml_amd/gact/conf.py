@@ -42,7 +42,9 @@ class QuantizationConfig:
         # ---- layers on 8-bit checkpoints (not in the reference) ----
         # While the Controller's hooks are installed, the model's nn.Linear and nn.LayerNorm run on gact.ops.op_linear and
         # op_layer_norm: they keep their input as 8-bit codes, rounded to nearest, which their backward kernels read where they
-        # lie.  What the other layers save goes through the hooks as before; `bit` and auto precision do not touch these.
+        # lie.  What the other layers save goes through the hooks as before; `bit` and auto precision do not touch these codes, nor
+        # weights that are the model's parameters, under autocast either.  (A weight that is computed in the pass - a weight norm's - is a
+        # saved tensor like any other to the hooks.)
         self.checkpoint_layers = False
 
         # ---- seeds in device memory (not in the reference) ----

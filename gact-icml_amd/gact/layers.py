@@ -71,13 +71,15 @@ def op_linear(input, weight, bias=None, activation=None, residual=None):
 
     For the backward pass it keeps the 8-bit checkpoint of the input and, under an activation, of the value it is applied to; the
     gradients are those of the checkpoints' values.  (relu is not among them: its derivative jumps at zero, where 8 bits do not hold
-    the sign.)  Under autocast it runs in autocast's type."""
+    the sign.)  Under autocast it runs in autocast's type; the weight that it saves is the one it was given, which the backward pass rounds
+    again."""
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise RuntimeError("unknown activation %r (expected one of %s)" % (activation, sorted(k for k in _ACTIVATIONS if k)))
-    if torch.is_autocast_enabled("cuda"):
-        input, weight, bias, residual = _cast(torch.get_autocast_dtype("cuda"), input, weight, bias, residual)
-    return _abi.native().linear(input, weight, bias, act, residual)
+    autocast = torch.is_autocast_enabled("cuda")
+    if autocast:      # the weight is rounded in the call
+        input, bias, residual = _cast(torch.get_autocast_dtype("cuda"), input, bias, residual)
+    return _abi.native().linear(input, weight, bias, act, residual, autocast)
 
 
 # ---- modules ----
