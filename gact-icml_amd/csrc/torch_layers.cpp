@@ -65,9 +65,21 @@ std::optional<at::Tensor> tensor_or_none(PyObject* o, const char* name) {
   if (o == Py_None) return std::nullopt;
   return tensor_of(o, name);
 }
-void check_like(const at::Tensor& t, const at::Tensor& like, const char* name) {
-  TORCH_CHECK(t.scalar_type() == like.scalar_type(), "The type of ", name, " is not correct!");
+// The type that autocast runs an operator in; its arguments may then be of others
+using Autocast = std::optional<at::ScalarType>;
+void check_like(const at::Tensor& t, const at::Tensor& like, const char* name, const Autocast& autocast) {
+  TORCH_CHECK(autocast || t.scalar_type() == like.scalar_type(), "The type of ", name, " is not correct!");
   TORCH_CHECK(t.device() == like.device(), name, " is on another device");
+}
+void check_vector(const std::optional<at::Tensor>& t, const char* name, int64_t size, const at::Tensor& like, const Autocast& autocast) {
+  if (!t) return;
+  check_like(*t, like, name, autocast);
+  TORCH_CHECK(t->dim() == 1 && t->size(0) == size, "The dimension of ", name, " is not correct!");
+}
+// the argument as autocast's operators take it, differentiably
+at::Tensor cast(const at::Tensor& t, const Autocast& autocast) { return autocast ? t.to(*autocast) : t; }
+std::optional<at::Tensor> cast(const std::optional<at::Tensor>& t, const Autocast& autocast) {
+  return t && autocast ? std::optional<at::Tensor>(t->to(*autocast)) : t;
 }
 
 // Everything a call needs to know about where it runs
@@ -152,10 +164,9 @@ at::Tensor weight_product(const Rows& grad, const Kept& k, int64_t cols, at::Sca
   return result;
 }
 
-at::Tensor vector_of(const at::Tensor& t, const char* name, int64_t size, const at::Tensor& like) {
-  check_like(t, like, name);
-  TORCH_CHECK(t.dim() == 1 && t.size(0) == size, "The dimension of ", name, " is not correct!");
-  return t.is_contiguous() && !t.is_neg() ? t : t.resolve_neg().contiguous();
+at::Tensor dense(const std::optional<at::Tensor>& t) {
+  if (!t) return at::Tensor();
+  return t->is_contiguous() && !t->is_neg() ? *t : t->resolve_neg().contiguous();
 }
 void no_tangent(const std::optional<at::Tensor>& t, const char* operation) {
   TORCH_CHECK(!t.has_value() || !torch::autograd::isFwGradDefined(*t), operation, " has no forward-mode derivative");
@@ -255,21 +266,25 @@ struct LayerNormBackward : public Node {
   }
 };
 
-at::Tensor layer_norm(const at::Tensor& input, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias, double eps) {
-  TORCH_CHECK(input.dim() >= 1 && input.size(-1) > 0 && input.size(-1) <= GACT_NORM_MAX_COLS, "layer norm takes 1 to ", GACT_NORM_MAX_COLS,
+at::Tensor layer_norm(const at::Tensor& x_given, const std::optional<at::Tensor>& w_given, const std::optional<at::Tensor>& b_given, double eps,
+                      const Autocast& autocast) {
+  TORCH_CHECK(x_given.dim() >= 1 && x_given.size(-1) > 0 && x_given.size(-1) <= GACT_NORM_MAX_COLS, "layer norm takes 1 to ", GACT_NORM_MAX_COLS,
               " columns");
-  for (const auto& t : {std::optional<at::Tensor>(input), weight, bias}) no_tangent(t, "op_layer_norm");
-  const int64_t cols = input.size(-1);
-  const bool keep = torch::autograd::compute_requires_grad(input, weight, bias);
-  if (keep) refuse_stale_leaves({&input, held(weight), held(bias)}, input);
+  const int64_t cols = x_given.size(-1);
+  check_vector(w_given, "weight", cols, x_given, autocast);
+  check_vector(b_given, "bias", cols, x_given, autocast);
+  for (const auto& t : {std::optional<at::Tensor>(x_given), w_given, b_given}) no_tangent(t, "op_layer_norm");
+  const bool keep = torch::autograd::compute_requires_grad(x_given, w_given, b_given);
+  if (keep) refuse_stale_leaves({&x_given, held(w_given), held(b_given)}, x_given);
+  const at::Tensor input = cast(x_given, autocast);
+  const std::optional<at::Tensor> weight = cast(w_given, autocast), bias = cast(b_given, autocast);
   at::Tensor y;
   Kept k;
   at::Tensor stats;
   {
     const at::AutoDispatchBelowADInplaceOrView below;
     const Place at(input);
-    const at::Tensor w = weight ? vector_of(*weight, "weight", cols, input) : at::Tensor();
-    const at::Tensor b = bias ? vector_of(*bias, "bias", cols, input) : at::Tensor();
+    const at::Tensor w = dense(weight), b = dense(bias);
     const Rows x = rows_of(input, "data", GACT_NORM_MAX_COLS);
     y = at.empty(input.sizes(), input.scalar_type());
     if (keep) {
@@ -361,27 +376,28 @@ struct LinearBackward : public Node {
   }
 };
 
-// `autocast`: the weight may be of another type and is rounded to the layer's in the call.  The node saves the weight itself and rounds it again: a
-// rounded copy would be memory of its own until the backward pass, and hooks for saved tensors that leave a model's parameters as they are
-// would not know it
-at::Tensor linear(const at::Tensor& input, const at::Tensor& weight, const std::optional<at::Tensor>& bias, int activation,
-                  const std::optional<at::Tensor>& residual, bool autocast) {
-  TORCH_CHECK(autocast || weight.scalar_type() == input.scalar_type(), "The type of weight is not correct!");
-  TORCH_CHECK(weight.device() == input.device(), "weight is on another device");
-  TORCH_CHECK(input.dim() >= 1 && weight.dim() == 2 && weight.size(1) == input.size(-1), "weight must be [outer, ",
-              input.dim() ? std::to_string(input.size(-1)) : std::string("-"), "], got ", weight.sizes());
+// Under autocast the node saves the weight as it was given and rounds it again: a rounded copy would be memory of its own until the backward
+// pass, and hooks for saved tensors that leave a model's parameters as they are would not know it
+at::Tensor linear(const at::Tensor& x_given, const at::Tensor& weight, const std::optional<at::Tensor>& b_given, int activation,
+                  const std::optional<at::Tensor>& r_given, const Autocast& autocast) {
+  check_like(weight, x_given, "weight", autocast);
+  TORCH_CHECK(x_given.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x_given.size(-1), "weight must be [outer, ",
+              x_given.dim() ? std::to_string(x_given.size(-1)) : std::string("-"), "], got ", weight.sizes());
   const int64_t outer = weight.size(0), inner = weight.size(1);
   TORCH_CHECK(inner > 0 && inner <= GACT_LAYER_MAX_COLS && outer > 0 && outer <= GACT_LAYER_MAX_COLS, "a linear layer takes 1 to ",
               GACT_LAYER_MAX_COLS, " columns on either side");
-  c10::SmallVector<int64_t, 5> shape(input.sizes().begin(), input.sizes().end());
+  check_vector(b_given, "bias", outer, x_given, autocast);
+  c10::SmallVector<int64_t, 5> shape(x_given.sizes().begin(), x_given.sizes().end());
   shape.back() = outer;
-  if (residual) {
-    check_like(*residual, input, "residual");
-    TORCH_CHECK(residual->sizes() == c10::IntArrayRef(shape), "residual must have the result's shape ", c10::IntArrayRef(shape));
+  if (r_given) {
+    check_like(*r_given, x_given, "residual", autocast);
+    TORCH_CHECK(r_given->sizes() == c10::IntArrayRef(shape), "residual must have the result's shape ", c10::IntArrayRef(shape));
   }
-  for (const auto& t : {std::optional<at::Tensor>(input), std::optional<at::Tensor>(weight), bias, residual}) no_tangent(t, "op_linear");
-  const bool needs = torch::autograd::compute_requires_grad(input, weight, bias, residual);
-  if (needs) refuse_stale_leaves({&input, &weight, held(bias), held(residual)}, input);
+  for (const auto& t : {std::optional<at::Tensor>(x_given), std::optional<at::Tensor>(weight), b_given, r_given}) no_tangent(t, "op_linear");
+  const bool needs = torch::autograd::compute_requires_grad(x_given, weight, b_given, r_given);
+  if (needs) refuse_stale_leaves({&x_given, &weight, held(b_given), held(r_given)}, x_given);
+  const at::Tensor input = cast(x_given, autocast);
+  const std::optional<at::Tensor> bias = cast(b_given, autocast), residual = cast(r_given, autocast);
   const bool keep_x = needs && weight.requires_grad();
   const bool keep_z = needs && activation != GACT_ACT_NONE && torch::autograd::compute_requires_grad(input, weight, bias);
   at::Tensor y;
@@ -390,7 +406,7 @@ at::Tensor linear(const at::Tensor& input, const at::Tensor& weight, const std::
     const at::AutoDispatchBelowADInplaceOrView below;
     const Place at(input);
     const at::ScalarType dtype = input.scalar_type();
-    const at::Tensor b = bias ? vector_of(*bias, "bias", outer, input) : at::Tensor();
+    const at::Tensor b = dense(bias);
     const Rows x = rows_of(input, "data");
     y = at.empty(shape, dtype);
     if (keep_z) z = room_for(x.rows, outer, at);
@@ -449,18 +465,26 @@ int64_t integer_of(PyObject* o) {
 }
 void arguments(Py_ssize_t n, Py_ssize_t wanted) { TORCH_CHECK_TYPE(n == wanted, "expected ", wanted, " arguments, got ", n); }
 
-// layer_norm(x, weight or None, bias or None, eps) -> y
+Autocast autocast_of(PyObject* o) {
+  if (o == Py_None) return std::nullopt;
+  TORCH_CHECK_TYPE(THPDtype_Check(o), "a type is expected");
+  const at::ScalarType t = ((THPDtype*)o)->scalar_type;
+  TORCH_CHECK(dtype_code(t) >= 0, "autocast's type is not correct");
+  return t;
+}
+
+// layer_norm(x, weight or None, bias or None, eps, autocast's type or None) -> y
 PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 4);
+  arguments(n, 5);
   const double eps = number_of(args[3]);
   const at::Tensor& x = tensor_of(args[0], "data");
   const std::optional<at::Tensor> weight = tensor_or_none(args[1], "weight"), bias = tensor_or_none(args[2], "bias");
-  return THPVariable_Wrap(layer_norm(x, weight, bias, eps));
+  return THPVariable_Wrap(layer_norm(x, weight, bias, eps, autocast_of(args[4])));
   END_HANDLE_TH_ERRORS
 }
 
-// linear(x, weight, bias or None, activation's number, residual or None, whether autocast is on) -> y
+// linear(x, weight, bias or None, activation's number, residual or None, autocast's type or None) -> y
 PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments(n, 6);
@@ -469,7 +493,7 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor& x = tensor_of(args[0], "data");
   const at::Tensor& weight = tensor_of(args[1], "weight");
   const std::optional<at::Tensor> bias = tensor_or_none(args[2], "bias"), residual = tensor_or_none(args[4], "residual");
-  return THPVariable_Wrap(linear(x, weight, bias, (int)act, residual, args[5] == Py_True));
+  return THPVariable_Wrap(linear(x, weight, bias, (int)act, residual, autocast_of(args[5])));
   END_HANDLE_TH_ERRORS
 }
 

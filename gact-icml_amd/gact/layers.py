@@ -51,19 +51,11 @@ def op_checkpoint_product(grad, checkpoint):
     return _abi.native().checkpoint_product(*_parts(checkpoint), grad)
 
 
-def _cast(dtype, *tensors):
-    """As a torch operator's arguments under autocast: differentiably, floating tensors of the GPU only."""
-    return tuple(t.to(dtype) if isinstance(t, torch.Tensor) and t.is_cuda and t.is_floating_point() and t.dtype is not torch.float64 else t
-                 for t in tensors)
-
-
 def op_layer_norm(input, weight=None, bias=None, eps=1e-5):
     """Layer norm over the last dimension.  For the backward pass it keeps the 8-bit checkpoint of the input and each row's mean and
     1 / sqrt(var + eps); gradients are those of the checkpoint's values under that mean and deviation.  Under autocast it runs in
     float32, as torch's does."""
-    if torch.is_autocast_enabled("cuda"):
-        input, weight, bias = _cast(torch.float32, input, weight, bias)
-    return _abi.native().layer_norm(input, weight, bias, eps)
+    return _abi.native().layer_norm(input, weight, bias, eps, torch.float32 if torch.is_autocast_enabled("cuda") else None)
 
 
 def op_linear(input, weight, bias=None, activation=None, residual=None):
@@ -76,9 +68,7 @@ def op_linear(input, weight, bias=None, activation=None, residual=None):
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise RuntimeError("unknown activation %r (expected one of %s)" % (activation, sorted(k for k in _ACTIVATIONS if k)))
-    autocast = torch.is_autocast_enabled("cuda")
-    if autocast:      # the weight is rounded in the call
-        input, bias, residual = _cast(torch.get_autocast_dtype("cuda"), input, bias, residual)
+    autocast = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None
     return _abi.native().linear(input, weight, bias, act, residual, autocast)
 
 

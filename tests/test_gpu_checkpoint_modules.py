@@ -75,3 +75,40 @@ def test_autocast_keeps_no_copy_of_the_weight():
         y = layers.op_linear(empty, w)
     dw, = torch.autograd.grad(y, [w], torch.empty_like(y))
     assert dw.dtype is torch.float32 and not dw.any()
+
+
+def test_a_capture_beside_an_eager_graph_is_refused_under_autocast():
+    """Whichever argument is the leaf: what the operator runs on is a copy of it, and its backward pass ends in the leaf."""
+    x, w, b, r = normal(40, 32), normal(24, 32, seed=1), normal(24, seed=2), normal(40, 24, seed=3)
+    half = normal(40, 32, dtype=torch.bfloat16)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for n in range(4):
+            args = [t.clone().requires_grad_(k == n) for k, t in enumerate((x, w, b, r))]
+            eager = layers.op_linear(args[0], args[1], args[2], None, args[3])
+            with pytest.raises(RuntimeError, match="eager graph of one of its leaves"):
+                with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                    layers.op_linear(args[0], args[1], args[2], None, args[3])
+            torch.autograd.grad(eager, [args[n]], torch.ones_like(eager))
+            del eager
+        leaf = half.clone().requires_grad_()
+        eager = layers.op_layer_norm(leaf)
+        with pytest.raises(RuntimeError, match="eager graph of one of its leaves"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                layers.op_layer_norm(leaf)
+
+
+def test_refusals_under_autocast():
+    x, w = normal(8, 16), normal(4, 16, seed=1)
+    with torch.autocast("cuda", dtype=torch.float16):
+        for bad in (lambda: layers.op_linear(x, w.double()), lambda: layers.op_linear(x.double(), w), lambda: layers.op_linear(x, w, normal(4).int()),
+                    lambda: layers.op_layer_norm(x.double())):
+            with pytest.raises(RuntimeError, match="type of"):
+                bad()
+        with pytest.raises(RuntimeError, match="dimension of bias"):
+            layers.op_linear(x, w, normal(5))
+        with pytest.raises(RuntimeError, match="dimension of weight"):
+            layers.op_layer_norm(x, normal(8))
+        with pytest.raises(RuntimeError, match="residual"):
+            layers.op_linear(x, w, None, None, normal(8, 5))
+        with pytest.raises(RuntimeError, match="CUDA"):
+            layers.op_linear(x, w.cpu())
