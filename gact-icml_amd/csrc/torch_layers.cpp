@@ -52,12 +52,13 @@ c10::DispatchKeySet wrapped_keys() {
   return c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::ZeroTensor,
                               c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper});
 }
+bool plain(const at::Tensor& t) { return t.layout() == at::kStrided && t.has_storage() && !t.key_set().has_any(wrapped_keys()); }
 // a tensor (or parameter) itself, no subclass and no wrapper, dense on the GPU
 const at::Tensor& tensor_of(PyObject* o, const char* name) {
   TORCH_CHECK_TYPE(THPVariable_Check(o), name, " must be a tensor");
   const at::Tensor& t = THPVariable_Unpack(o);
   TORCH_CHECK(t.defined() && t.is_cuda(), name, " must be a CUDA tensor!");
-  TORCH_CHECK(t.layout() == at::kStrided && t.has_storage() && !t.key_set().has_any(wrapped_keys()), name, " must be a plain dense tensor");
+  TORCH_CHECK(plain(t), name, " must be a plain dense tensor");
   TORCH_CHECK(dtype_code(t.scalar_type()) >= 0, "The type of ", name, " is not correct!");
   return t;
 }
@@ -215,8 +216,7 @@ Kept again(SavedVariable& codes, SavedVariable& scale, SavedVariable& mn, int64_
 }
 // a gradient that the kernels can read: no batch of them, no subclass
 void check_grad(const at::Tensor& t) {
-  TORCH_CHECK(t.layout() == at::kStrided && t.has_storage() && t.is_cuda() && !t.key_set().has_any(wrapped_keys()),
-              "the gradient must be a plain dense tensor");
+  TORCH_CHECK(t.is_cuda() && plain(t), "the gradient must be a plain dense tensor");
 }
 
 // ---- layer norm ----
@@ -497,6 +497,37 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// takes(x, weight or None, bias or None, whether it is a linear layer and no layer norm, whether autocast is on) -> whether the operator runs
+// these arguments: what it would refuse, and what a trace or a mode of torch's would not see, is for torch's own
+PyObject* py_takes(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 5);
+  const bool linear = args[3] == Py_True, autocast = args[4] == Py_True;
+  if (gact_torch_dispatched()) Py_RETURN_FALSE;
+  const at::Tensor* given[3] = {};
+  for (int i = 0; i < 3; i++) {
+    if (i && args[i] == Py_None) continue;
+    if (!THPVariable_Check(args[i])) Py_RETURN_FALSE;
+    const at::Tensor& t = THPVariable_Unpack(args[i]);
+    if (!t.defined() || !t.is_cuda() || !plain(t) || dtype_code(t.scalar_type()) < 0 || torch::autograd::isFwGradDefined(t)) Py_RETURN_FALSE;
+    given[i] = &t;
+    if (t.device() != given[0]->device() || (t.scalar_type() != given[0]->scalar_type() && !autocast)) Py_RETURN_FALSE;
+  }
+  const at::Tensor &x = *given[0], *const weight = given[1], *const bias = given[2];
+  const int64_t most = linear ? GACT_LAYER_MAX_COLS : GACT_NORM_MAX_COLS;
+  if (x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > most || x.numel() / x.size(-1) > GACT_LAYER_MAX_ROWS) Py_RETURN_FALSE;
+  int64_t across = x.size(-1);
+  if (linear) {
+    if (!weight || weight->dim() != 2 || weight->size(1) != across || weight->size(0) < 1 || weight->size(0) > most) Py_RETURN_FALSE;
+    across = weight->size(0);
+  } else if (weight && (weight->dim() != 1 || weight->size(0) != across)) {
+    Py_RETURN_FALSE;
+  }
+  if (bias && (bias->dim() != 1 || bias->size(0) != across)) Py_RETURN_FALSE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* tuple_of(const Kept& k) {
   PyObject* const t = PyTuple_New(3);
   if (!t) return nullptr;
@@ -592,6 +623,6 @@ PyObject* py_checkpoint_product(PyObject*, PyObject* const* args, Py_ssize_t n) 
 
 }  // namespace
 
-PyMethodDef gact_layer_methods[] = {FASTCALL("layer_norm", py_layer_norm), FASTCALL("linear", py_linear), FASTCALL("checkpoint", py_checkpoint),
+PyMethodDef gact_layer_methods[] = {FASTCALL("layer_norm", py_layer_norm), FASTCALL("linear", py_linear), FASTCALL("takes", py_takes), FASTCALL("checkpoint", py_checkpoint),
                                     FASTCALL("restore", py_restore), FASTCALL("checkpoint_product", py_checkpoint_product),
                                     {nullptr, nullptr, 0, nullptr}};

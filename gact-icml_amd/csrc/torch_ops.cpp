@@ -38,12 +38,12 @@ namespace {
 constexpr int64_t kGroup = 256;
 
 // torch.empty, called below, would mean something else: a mode that looks at every call, a transform, a trace
-bool ordinary_call() {
+bool dispatched_call() {
   static const c10::DispatchKeySet special({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::Tracer,
                                             c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchVmapMode});
-  return !c10::impl::tls_local_dispatch_key_set().included_.has_any(special) && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
-         !at::impl::torch_function_mode_enabled();
+  return c10::impl::tls_local_dispatch_key_set().included_.has_any(special) || c10::impl::TorchDispatchModeTLS::any_modes_set();
 }
+bool ordinary_call() { return !dispatched_call() && !at::impl::torch_function_mode_enabled(); }
 
 // a tensor (or parameter) itself, no subclass and no wrapper, no lazily negated view, dense on the GPU
 const at::Tensor* plain(PyObject* o) {
@@ -552,6 +552,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "gact_torch", "The operators' host 
 
 }  // namespace
 
+bool gact_torch_dispatched() { return dispatched_call(); }
 bool gact_torch_ordinary() { return ordinary_call(); }
 at::Tensor gact_torch_empty(c10::IntArrayRef shape, at::ScalarType dtype, c10::Device device) { return make(shape, dtype, device); }
 

@@ -73,20 +73,20 @@ def op_linear(input, weight, bias=None, activation=None, residual=None):
 
 
 # ---- modules ----
-def _taken(module, input, most):
+def _taken(module, input, linear):
     """Whether the operator takes this call of the module: anything else goes to torch's own."""
-    w = module.weight if module.weight is not None else input
-    return (input.is_cuda and w.is_cuda and input.device == w.device and input.layout is torch.strided and input.dim() >= 1
-            and input.dtype in (torch.float32, torch.float16, torch.bfloat16) and 0 < input.shape[-1] <= most
-            and (input.dtype is w.dtype or torch.is_autocast_enabled("cuda")) and not torch.overrides.has_torch_function((input, w))
-            and not torch._C._functorch.is_functorch_wrapped_tensor(input))
+    if not (isinstance(input, torch.Tensor) and input.is_cuda):
+        return False
+    weight, bias = module.weight, module.bias
+    return (not torch.overrides.has_torch_function(tuple(t for t in (input, weight, bias) if t is not None))
+            and _abi.native().takes(input, weight, bias, linear, torch.is_autocast_enabled("cuda")))
 
 
 class CheckpointedLinear(nn.Linear):
     """nn.Linear on op_linear."""
 
     def forward(self, input):
-        if _taken(self, input, 262144) and self.out_features <= 262144 and input.shape[-1] == self.in_features:
+        if _taken(self, input, True):
             return op_linear(input, self.weight, self.bias)
         return super().forward(input)
 
@@ -95,7 +95,7 @@ class CheckpointedLayerNorm(nn.LayerNorm):
     """nn.LayerNorm over the last dimension on op_layer_norm."""
 
     def forward(self, input):
-        if len(self.normalized_shape) == 1 and _taken(self, input, 16384) and input.shape[-1] == self.normalized_shape[0]:
+        if len(self.normalized_shape) == 1 and _taken(self, input, False) and input.shape[-1] == self.normalized_shape[0]:
             return op_layer_norm(input, self.weight, self.bias, self.eps)
         return super().forward(input)
 

@@ -112,3 +112,107 @@ def test_refusals_under_autocast():
             layers.op_linear(x, w, None, None, normal(8, 5))
         with pytest.raises(RuntimeError, match="CUDA"):
             layers.op_linear(x, w.cpu())
+
+
+class Wrapped(torch.Tensor):
+    """A tensor around another, as a distributed tensor is: torch's functions go past it, the dispatcher's operators come to it."""
+    __torch_function__ = torch._C._disabled_torch_function_impl
+
+    @staticmethod
+    def __new__(cls, inner):
+        t = torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+        t.inner = inner
+        return t
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        bare = lambda v: v.inner if isinstance(v, cls) else v  # noqa: E731
+        return torch.utils._pytree.tree_map_only(torch.Tensor, cls, func(*[bare(a) for a in args], **(kwargs or {})))
+
+
+def pair(kind, *args, **kwargs):
+    """The layer on checkpoints and torch's own, of the same parameters."""
+    torch.manual_seed(0)
+    own = kind(*args, **kwargs).cuda()
+    layer = copy.deepcopy(own)
+    for p in own.parameters():
+        torch.nn.init.normal_(p, 0, 0.3)
+    layer.load_state_dict(own.state_dict())
+    assert len(layers.attach(layer)) == 1
+    return layer, own
+
+
+PAIRS = [(nn.Linear, 16, 8), (nn.LayerNorm, 16)]
+
+
+@pytest.mark.parametrize("kind", PAIRS, ids=lambda k: k[0].__name__)
+def test_transforms_of_the_layers_are_torchs(kind):
+    from torch.func import functional_call, grad, jvp, vmap
+    layer, own = pair(*kind)
+    x, p = normal(5, 16), {n: t.detach() for n, t in own.named_parameters()}
+    got, want = (grad(lambda q: functional_call(m, q, (x,)).square().sum())(p) for m in (layer, own))
+    assert all(torch.equal(got[n], want[n]) for n in p)
+    many = {n: torch.stack([t, 2 * t, -t]) for n, t in p.items()}
+    got, want = (vmap(lambda q: functional_call(m, q, (x,)))(many) for m in (layer, own))
+    assert got.shape[0] == 3 and torch.equal(got, want)
+    got, want = (vmap(m)(normal(4, 5, 16, seed=1)) for m in (layer, own))
+    assert torch.equal(got, want)
+    got, want = (jvp(m, (x,), (normal(5, 16, seed=2),)) for m in (layer, own))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got, want = (jvp(lambda q: functional_call(m, q, (x,)), (p,), (p,)) for m in (layer, own))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("kind", PAIRS, ids=lambda k: k[0].__name__)
+def test_forward_mode_traces_and_modes_see_torchs_layers(kind):
+    import torch.autograd.forward_ad as forward
+    from torch._subclasses import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    layer, own = pair(*kind)
+    x, t = normal(5, 16), normal(5, 16, seed=1)
+    with forward.dual_level():
+        got, want = (forward.unpack_dual(m(forward.make_dual(x, t))) for m in (layer, own))
+        assert torch.equal(got.primal, want.primal) and torch.equal(got.tangent, want.tangent)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        assert layer(mode.from_tensor(x)).shape == own(mode.from_tensor(x)).shape
+    traced = torch.jit.trace(layer, x)
+    assert torch.equal(traced(t), own(t))
+    graph = make_fx(layer)(x)
+    assert torch.equal(graph(t), own(t))
+    assert torch.equal(layer(Wrapped(x)).inner, own(x).detach())
+    w = layer.weight
+    del layer.weight
+    layer.weight = Wrapped(w.detach())
+    assert torch.equal(layer(x).inner, own(x).detach())
+
+
+def test_sizes_that_the_operators_do_not_have_are_torchs():
+    layer, own = pair(nn.Linear, 16, 8)
+    x = normal(5, 16)
+    for m in (layer, own):
+        m.weight, m.bias = nn.Parameter(m.weight[:0]), None
+    assert layer(x).shape == own(x).shape == (5, 0)
+    layer, own = pair(nn.Linear, 16, 8)
+    for m in (layer, own):
+        m.bias = nn.Parameter(m.bias[:1])         # for all columns
+    assert torch.equal(layer(x), own(x))
+    layer, own = pair(nn.LayerNorm, 16)
+    with pytest.raises(RuntimeError) as got:
+        layer(normal(5, 8))
+    with pytest.raises(RuntimeError) as want:
+        own(normal(5, 8))
+    assert str(got.value) == str(want.value)
+
+
+def test_plain_calls_are_the_operators(monkeypatch):
+    calls = []
+    linear, norm = layers.op_linear, layers.op_layer_norm
+    monkeypatch.setattr(layers, "op_linear", lambda *a: calls.append("linear") or linear(*a))
+    monkeypatch.setattr(layers, "op_layer_norm", lambda *a: calls.append("norm") or norm(*a))
+    model = nn.Sequential(*(pair(*kind)[0] for kind in ((nn.LayerNorm, 16), (nn.Linear, 16, 8), (nn.Linear, 8, 8, False)))).cuda()
+    x = normal(5, 16)
+    for around in (torch.enable_grad(), torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16)):
+        calls.clear()
+        with around:
+            model(x), model(x[0]), model(x.view(1, 5, 16))
+        assert calls == ["norm", "linear", "linear"] * 3
