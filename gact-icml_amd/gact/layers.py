@@ -17,6 +17,7 @@ import collections
 
 import torch
 import torch.nn as nn
+from torch.utils._device import DeviceContext
 
 from .cpp_extension import _abi
 
@@ -73,12 +74,20 @@ def op_linear(input, weight, bias=None, activation=None, residual=None):
 
 
 # ---- modules ----
+def _overridden(tensors):
+    """Whether a tensor's __torch_function__ or a mode's wants to see torch's call.  A default device is such a mode, too, and looks at
+    calls that make tensors only."""
+    return torch.overrides.has_torch_function(tensors) and not (
+        all(type(t) in (torch.Tensor, nn.Parameter) for t in tensors)
+        and all(isinstance(m, DeviceContext) for m in torch.overrides._get_current_function_mode_stack()))
+
+
 def _taken(module, input, linear):
     """Whether the operator takes this call of the module: anything else goes to torch's own."""
     if not (isinstance(input, torch.Tensor) and input.is_cuda):
         return False
     weight, bias = module.weight, module.bias
-    return (not torch.overrides.has_torch_function(tuple(t for t in (input, weight, bias) if t is not None))
+    return (not _overridden(tuple(t for t in (input, weight, bias) if t is not None))
             and _abi.native().takes(input, weight, bias, linear, torch.is_autocast_enabled("cuda")))
 
 

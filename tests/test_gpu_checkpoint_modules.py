@@ -205,14 +205,26 @@ def test_sizes_that_the_operators_do_not_have_are_torchs():
 
 
 def test_plain_calls_are_the_operators(monkeypatch):
+    """With a default device set, too, which is a mode of torch's functions; any other such mode sees torch's."""
     calls = []
     linear, norm = layers.op_linear, layers.op_layer_norm
     monkeypatch.setattr(layers, "op_linear", lambda *a: calls.append("linear") or linear(*a))
     monkeypatch.setattr(layers, "op_layer_norm", lambda *a: calls.append("norm") or norm(*a))
     model = nn.Sequential(*(pair(*kind)[0] for kind in ((nn.LayerNorm, 16), (nn.Linear, 16, 8), (nn.Linear, 8, 8, False)))).cuda()
     x = normal(5, 16)
-    for around in (torch.enable_grad(), torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16)):
+    for around in (torch.enable_grad(), torch.no_grad(), torch.device("cuda"), torch.autocast("cuda", dtype=torch.bfloat16)):
         calls.clear()
         with around:
             model(x), model(x[0]), model(x.view(1, 5, 16))
         assert calls == ["norm", "linear", "linear"] * 3
+
+    class Seen(torch.overrides.TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(func)
+            return func(*args, **(kwargs or {}))
+
+    calls.clear()
+    seen = []
+    with torch.device("cuda"), Seen():
+        model(x)
+    assert not calls and nn.functional.linear in seen and nn.functional.layer_norm in seen
