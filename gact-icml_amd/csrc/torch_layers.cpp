@@ -463,7 +463,11 @@ int64_t integer_of(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) throw python_error();
   return v;
 }
-void arguments(Py_ssize_t n, Py_ssize_t wanted) { TORCH_CHECK_TYPE(n == wanted, "expected ", wanted, " arguments, got ", n); }
+// How many there are, and that no trace is being recorded: of these operators it would hold the results' allocations and nothing that fills them
+void arguments(Py_ssize_t n, Py_ssize_t wanted) {
+  TORCH_CHECK_TYPE(n == wanted, "expected ", wanted, " arguments, got ", n);
+  TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer), "the layers on 8-bit checkpoints cannot be traced");
+}
 
 Autocast autocast_of(PyObject* o) {
   if (o == Py_None) return std::nullopt;
@@ -501,7 +505,7 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // these arguments: what it would refuse, and what a trace or a mode of torch's would not see, is for torch's own
 PyObject* py_takes(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arguments(n, 5);
+  TORCH_CHECK_TYPE(n == 5, "expected 5 arguments, got ", n);
   const bool linear = args[3] == Py_True, autocast = args[4] == Py_True;
   if (gact_torch_dispatched()) Py_RETURN_FALSE;
   const at::Tensor* given[3] = {};

@@ -228,3 +228,13 @@ def test_plain_calls_are_the_operators(monkeypatch):
     with torch.device("cuda"), Seen():
         model(x)
     assert not calls and nn.functional.linear in seen and nn.functional.layer_norm in seen
+
+
+def test_the_operators_themselves_are_not_traced():
+    x, w = normal(5, 16), normal(8, 16, seed=1)
+    kept = layers.op_checkpoint(x)
+    for call in (lambda t: layers.op_linear(t, w), lambda t: layers.op_layer_norm(t), lambda t: layers.op_checkpoint(t).scale,
+                 lambda t: layers.op_restore(kept), lambda t: layers.op_checkpoint_product(t, kept)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, x)
+    assert torch.equal(layers.op_linear(x, w), layers.op_linear(x, w))          # and are none the worse for it
