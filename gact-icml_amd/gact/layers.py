@@ -91,8 +91,17 @@ def _taken(module, input, linear):
             and _abi.native().takes(input, weight, bias, linear, torch.is_autocast_enabled("cuda")))
 
 
-class CheckpointedLinear(nn.Linear):
+class _Swapped:
+    """A module that runs on an operator while it is attached.  Its copies and pickles are torch's own modules: nothing would ever detach them
+    (a running average of the model, say), and they load where this package is not there."""
+
+    def __reduce_ex__(self, protocol):
+        return (object.__new__, (self._own,)) + super().__reduce_ex__(protocol)[2:]
+
+
+class CheckpointedLinear(_Swapped, nn.Linear):
     """nn.Linear on op_linear."""
+    _own = nn.Linear
 
     def forward(self, input):
         if _taken(self, input, True):
@@ -100,8 +109,9 @@ class CheckpointedLinear(nn.Linear):
         return super().forward(input)
 
 
-class CheckpointedLayerNorm(nn.LayerNorm):
+class CheckpointedLayerNorm(_Swapped, nn.LayerNorm):
     """nn.LayerNorm over the last dimension on op_layer_norm."""
+    _own = nn.LayerNorm
 
     def forward(self, input):
         if len(self.normalized_shape) == 1 and _taken(self, input, False) and input.shape[-1] == self.normalized_shape[0]:
@@ -116,7 +126,7 @@ def attach(model):
     """The model's linear layers and layer norms (of exactly these classes) run on the operators from now on; returns them for detach."""
     changed = [m for m in model.modules() if type(m) in _CHECKPOINTED]
     for m in changed:
-        m.__class__ = _CHECKPOINTED[type(m)]      # parameters, hooks and copies of the module stay as they are
+        m.__class__ = _CHECKPOINTED[type(m)]      # the module's parameters and hooks stay as they are
     return changed
 
 

@@ -1,0 +1,48 @@
+"""How a model's layers come to run on 8-bit checkpoints and stop to, as far as it goes without a GPU."""
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+import torch.nn as nn
+
+from gact import layers
+from gact.conf import config
+from gact.controller import Controller
+
+
+@pytest.fixture(autouse=True)
+def _restore_config():
+    saved = copy.copy(config.__dict__)
+    yield
+    config.__dict__.update(saved)
+
+
+def a_model():
+    torch.manual_seed(0)
+    return nn.Sequential(nn.Linear(6, 8), nn.GELU(), nn.LayerNorm(8), nn.Linear(8, 3, bias=False))
+
+
+def test_copies_of_attached_layers_are_torchs_own():
+    """An average of the model's weights, say, whose layers nobody would take back."""
+    model, x = a_model(), torch.randn(5, 6)
+    kinds, want = [type(m) for m in model], model(x)
+    model[0].extra = [1, 2]
+    hooked = model[2].register_forward_hook(lambda m, a, y: y + 1)
+    changed = layers.attach(model)
+    held = io.BytesIO()
+    torch.save(model[0], held)
+    held.seek(0)
+    average = torch.optim.swa_utils.AveragedModel(model)
+    copies = [copy.deepcopy(model[0]), copy.copy(model[0]), pickle.loads(pickle.dumps(model[0])), torch.load(held, weights_only=False),
+              average.module[0]]
+    assert all(type(m) is nn.Linear and m.extra == [1, 2] for m in copies)
+    assert [type(m) for m in average.module] == kinds and [type(m) for m in copy.deepcopy(model)] == kinds
+    assert all(torch.equal(m(x), model[0](x)) for m in copies)
+    twin = copy.deepcopy(model[2])
+    assert torch.equal(twin(want.new_ones(2, 8)), model[2](want.new_ones(2, 8)))       # its hooks too
+    assert type(model[0]) is layers.CheckpointedLinear and type(model[2]) is layers.CheckpointedLayerNorm
+    layers.detach(changed)
+    hooked.remove()
+    assert [type(m) for m in model] == kinds and torch.equal(model(x), want)
