@@ -52,7 +52,7 @@ class Controller:
     # ---- hooks (controller.py:53-60 of the reference: the default saved-tensor hooks of autograd) ----
     def install_hook(self):
         if config.checkpoint_layers and config.compress_activation:
-            self._attached += layers.attach(self.model)
+            self._attached += layers.hold(self.model)
         _hooks._push_saved_tensors_default_hooks(self.quantize, self.dequantize)
         self._hooked = True
 
@@ -60,8 +60,8 @@ class Controller:
         if getattr(self, "_hooked", False):
             _hooks._pop_saved_tensors_default_hooks()
             self._hooked = False
-            layers.detach(self._attached)
-            self._attached = []
+            attached, self._attached = self._attached, []
+            layers.release(attached)
 
     def __enter__(self):
         self.install_hook()

@@ -14,6 +14,7 @@ was given), before anything is launched.
 The public names are in ``gact.ops``; nothing of this is in the reference, whose layers save through the hooks only.
 """
 import collections
+import weakref
 
 import torch
 import torch.nn as nn
@@ -136,3 +137,25 @@ def detach(changed):
         for own, checkpointed in _CHECKPOINTED.items():
             if type(m) is checkpointed:
                 m.__class__ = own
+
+
+# attached module -> how many hold it
+_held = weakref.WeakKeyDictionary()
+
+
+def hold(model):
+    """attach for one of several that may want the same layers; returns what is to be given to release.  Layers that were attached by `attach`
+    itself, and modules that were made as Checkpointed ones, are not theirs."""
+    modules = attach(model) + [m for m in model.modules() if m in _held]
+    for m in modules:
+        _held[m] = _held.get(m, 0) + 1
+    return modules
+
+
+def release(modules):
+    """The layers are torch's own again once the last one that held them lets go."""
+    for m in modules:
+        _held[m] -= 1
+        if _held[m] == 0:
+            del _held[m]
+            detach([m])

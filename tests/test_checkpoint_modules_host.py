@@ -46,3 +46,27 @@ def test_copies_of_attached_layers_are_torchs_own():
     layers.detach(changed)
     hooked.remove()
     assert [type(m) for m in model] == kinds and torch.equal(model(x), want)
+
+
+def test_layers_stay_attached_until_the_last_controller_leaves():
+    config.checkpoint_layers, config.auto_prec = True, False
+    model = a_model()
+    kinds, swapped = [type(m) for m in model], [layers.CheckpointedLinear, nn.GELU, layers.CheckpointedLayerNorm, layers.CheckpointedLinear]
+    whole, part = Controller(model), Controller(model[0])
+    for order in ((whole, part), (part, whole)):
+        for c in (whole, part):
+            c.install_hook()
+        assert [type(m) for m in model] == swapped
+        order[0].uninstall_hook()
+        assert [type(m) for m in model] == (swapped if order[0] is part else swapped[:1] + kinds[1:])
+        order[1].uninstall_hook()
+        assert [type(m) for m in model] == kinds
+    whole.install_hook()
+    own = layers.CheckpointedLinear(8, 8)
+    model.append(own)                       # was made so, and stays so
+    part.install_hook()
+    whole.uninstall_hook()
+    whole.uninstall_hook()                  # gone already
+    assert [type(m) for m in model] == swapped[:1] + kinds[1:] + [layers.CheckpointedLinear]
+    part.uninstall_hook()
+    assert [type(m) for m in model] == kinds + [layers.CheckpointedLinear] and not len(layers._held)
