@@ -23,6 +23,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <memory>
+#include <mutex>
 #include <string>
 
 #include "gact_hip.h"
@@ -226,10 +227,12 @@ struct LayerNormBackward : public Node {
   bool released = false;
   std::string name() const override { return "OpLayerNormBackward"; }
   void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
     for (SavedVariable* v : {&weight, &stats, &codes, &scale, &mn}) give_up(*v);
     released = true;
   }
   variable_list apply(variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);      // what is saved is not released beside a pass that reads it
     variable_list result(3);
     if (!grads[0].defined()) return result;
     TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
@@ -317,10 +320,12 @@ struct LinearBackward : public Node {
   bool released = false;
   std::string name() const override { return "OpLinearBackward"; }
   void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
     for (SavedVariable* v : {&weight, &codes, &scale, &mn, &z_codes, &z_scale, &z_mn}) give_up(*v);
     released = true;
   }
   variable_list apply(variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
     variable_list result(4);
     const at::Tensor& dy = grads[0];
     if (!dy.defined()) return result;

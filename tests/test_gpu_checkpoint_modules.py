@@ -1,6 +1,7 @@
 """A model's layers on 8-bit checkpoints where torch's own would be called in other ways than a plain training step: autocast under the
 Controller's hooks."""
 import copy
+import threading
 
 import pytest
 import torch
@@ -238,3 +239,29 @@ def test_the_operators_themselves_are_not_traced():
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(call, x)
     assert torch.equal(layers.op_linear(x, w), layers.op_linear(x, w))          # and are none the worse for it
+
+
+def test_one_graph_differentiated_by_several_threads():
+    """Each of them gets the gradients; of those that let go of what was saved the first one does."""
+    x, w, nw = normal(600, 264).requires_grad_(), normal(136, 264, seed=1).requires_grad_(), normal(264, seed=2).requires_grad_()
+    dy = normal(600, 136, seed=3)
+    for retain in (True, False):
+        y = layers.op_linear(layers.op_layer_norm(x, nw), w, None, "silu")
+        want = torch.autograd.grad(y, [x, w, nw], dy, retain_graph=True)
+        got, errors = [], []
+
+        def run():
+            try:
+                got.append(torch.autograd.grad(y, [x, w, nw], dy, retain_graph=retain))
+            except RuntimeError as e:
+                errors.append(str(e))
+
+        threads = [threading.Thread(target=run) for _ in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert len(got) + len(errors) == 4 and (len(got) == 4 if retain else got)
+        assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+        assert all("second time" in e for e in errors), errors
