@@ -351,31 +351,31 @@ struct LinearBackward : public Node {
         if (need_x) result[0] = at.zeros(shape, dtype);
         if (need_w) result[1] = at.zeros({outer, inner}, weight_dtype);
         if (need_b) result[2] = at.zeros({outer}, dtype);
-        return result;
+      } else {
+        // dz: the gradient itself where there is no activation and the products can load it
+        Rows dz = g;
+        const int64_t piece = 16 / (int64_t)g.held.element_size();
+        const bool fits = outer % piece == 0 && g.ld % piece == 0 && aligned(g.data());
+        const bool own = (need_x || need_w) && (activation != GACT_ACT_NONE || !fits);
+        if (own) {
+          dz.ld = round_up(outer, 8);
+          dz.held = at.empty({g.rows, dz.ld}, dtype);
+        }
+        if (need_b) result[2] = at.empty({outer}, dtype);
+        if (own || need_b) {
+          const at::Tensor ws = need_b ? at.bytes(gact_activation_workspace_bytes(g.rows, outer)) : at::Tensor();
+          check_status(gact_activation_backward(g.data(), g.ld, in(z.codes), z.codes.defined() ? z.codes.size(1) : 0,
+                                                (const float*)in(z.scale), (const float*)in(z.mn), activation, code, g.rows, outer,
+                                                own ? out(dz.held) : nullptr, dz.ld, out(result[2]), (float*)out(ws), at.stream));
+        }
+        if (need_x) {
+          const Rows held = product_rows(rows_of(w.to(dtype), "weight"), at);
+          result[0] = at.empty(shape, dtype);
+          const at::Tensor ws = at.bytes(gact_product_workspace_bytes(code, g.rows, inner, outer));
+          check_status(gact_product(dz.data(), dz.ld, held.data(), held.ld, code, g.rows, outer, inner, out(result[0]), out(ws), at.stream));
+        }
+        if (need_w) result[1] = weight_product(dz, k, inner, dtype, at).to(weight_dtype);
       }
-      // dz: the gradient itself where there is no activation and the products can load it
-      Rows dz = g;
-      const int64_t piece = 16 / (int64_t)g.held.element_size();
-      const bool fits = outer % piece == 0 && g.ld % piece == 0 && aligned(g.data());
-      const bool own = (need_x || need_w) && (activation != GACT_ACT_NONE || !fits);
-      if (own) {
-        dz.ld = round_up(outer, 8);
-        dz.held = at.empty({g.rows, dz.ld}, dtype);
-      }
-      if (need_b) result[2] = at.empty({outer}, dtype);
-      if (own || need_b) {
-        const at::Tensor ws = need_b ? at.bytes(gact_activation_workspace_bytes(g.rows, outer)) : at::Tensor();
-        check_status(gact_activation_backward(g.data(), g.ld, in(z.codes), z.codes.defined() ? z.codes.size(1) : 0, (const float*)in(z.scale),
-                                              (const float*)in(z.mn), activation, code, g.rows, outer, own ? out(dz.held) : nullptr, dz.ld,
-                                              out(result[2]), (float*)out(ws), at.stream));
-      }
-      if (need_x) {
-        const Rows held = product_rows(rows_of(w.to(dtype), "weight"), at);
-        result[0] = at.empty(shape, dtype);
-        const at::Tensor ws = at.bytes(gact_product_workspace_bytes(code, g.rows, inner, outer));
-        check_status(gact_product(dz.data(), dz.ld, held.data(), held.ld, code, g.rows, outer, inner, out(result[0]), out(ws), at.stream));
-      }
-      if (need_w) result[1] = weight_product(dz, k, inner, dtype, at).to(weight_dtype);
     }
     return once(std::move(result), "op_linear");
   }

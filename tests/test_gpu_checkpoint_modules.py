@@ -265,3 +265,12 @@ def test_one_graph_differentiated_by_several_threads():
         assert len(got) + len(errors) == 4 and (len(got) == 4 if retain else got)
         assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
         assert all("second time" in e for e in errors), errors
+
+
+def test_gradients_of_empty_batches_are_not_differentiated_either():
+    x, w, nw = torch.empty(0, 16, device="cuda", requires_grad=True), normal(8, 16).requires_grad_(), normal(16, seed=1).requires_grad_()
+    for y, leaf in ((layers.op_linear(x, w, None, "gelu"), w), (layers.op_linear(x, w), x), (layers.op_layer_norm(x, nw), nw)):
+        g, = torch.autograd.grad(y, [leaf], torch.empty_like(y).requires_grad_(), create_graph=True)
+        assert not g.any()
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
