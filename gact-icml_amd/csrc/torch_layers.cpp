@@ -619,12 +619,19 @@ PyObject* py_checkpoint_product(PyObject*, PyObject* const* args, Py_ssize_t n) 
   const at::Tensor& grad = tensor_of(args[5], "grad");
   TORCH_CHECK(grad.scalar_type() == g.dtype, "The type of grad is not correct!");
   TORCH_CHECK(grad.device() == g.kept.codes.device(), "grad is on another device");
-  const at::AutoDispatchBelowADInplaceOrView below;
-  const Place at(grad);
-  Rows r = rows_of(grad, "grad");
-  TORCH_CHECK(r.rows == g.rows, "grad has ", r.rows, " rows, the checkpoint ", g.rows);
-  if (r.rows) r = product_rows(r, at);
-  return THPVariable_Wrap(weight_product(r, g.kept, g.cols, g.dtype, at));
+  no_tangent(grad, "op_checkpoint_product");
+  at::Tensor result;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Place at(grad);
+    Rows r = rows_of(grad, "grad");
+    TORCH_CHECK(r.rows == g.rows, "grad has ", r.rows, " rows, the checkpoint ", g.rows);
+    if (r.rows) r = product_rows(r, at);
+    result = weight_product(r, g.kept, g.cols, g.dtype, at);
+  }
+  // no backward pass: the result of a gradient that has a history says so to who goes through it
+  if (torch::autograd::compute_requires_grad(grad)) result = once({result}, "op_checkpoint_product")[0];
+  return THPVariable_Wrap(result);
   END_HANDLE_TH_ERRORS
 }
 

@@ -30,7 +30,8 @@ Checkpoint = collections.namedtuple("Checkpoint", "codes scale min shape dtype")
 
 
 def op_checkpoint(input):
-    """The 8-bit checkpoint of a float32, float16 or bfloat16 tensor [..., cols]."""
+    """The 8-bit checkpoint of a float32, float16 or bfloat16 tensor [..., cols].  Codes are whole numbers: neither this nor op_restore has a
+    derivative, and their results have no history."""
     codes, scale, mn = _abi.native().checkpoint(input)
     return Checkpoint(codes, scale, mn, input.shape, input.dtype)
 
@@ -49,7 +50,8 @@ def op_restore(checkpoint):
 
 def op_checkpoint_product(grad, checkpoint):
     """[outer, cols] = grad [..., outer] transposed times the checkpoint's values [..., cols], both as rows: the weight's gradient of a
-    linear layer whose input the checkpoint holds.  The values enter the product in the checkpoint's type, as op_restore gives them."""
+    linear layer whose input the checkpoint holds.  The values enter the product in the checkpoint's type, as op_restore gives them.  It has no
+    backward pass: going through the result of a gradient that has a history is an error."""
     return _abi.native().checkpoint_product(*_parts(checkpoint), grad)
 
 

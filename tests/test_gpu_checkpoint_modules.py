@@ -274,3 +274,22 @@ def test_gradients_of_empty_batches_are_not_differentiated_either():
         assert not g.any()
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.sum().backward()
+
+
+def test_a_product_of_a_gradient_with_a_history_is_not_differentiated():
+    """Where a custom function's backward pass uses it under create_graph, say."""
+    import torch.autograd.forward_ad as forward
+    kept, g = layers.op_checkpoint(normal(70, 24)), normal(70, 16, seed=1)
+    want = layers.op_checkpoint_product(g, kept)
+    assert not want.requires_grad
+    g.requires_grad_()
+    with torch.no_grad():
+        assert not layers.op_checkpoint_product(g, kept).requires_grad
+    for grad, rows in ((g, kept), (torch.empty(0, 16, device="cuda", requires_grad=True), layers.op_checkpoint(normal(0, 24)))):
+        got = layers.op_checkpoint_product(grad, rows)
+        assert torch.equal(got.detach(), want if rows is kept else torch.zeros_like(want))
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            got.sum().backward()
+    with forward.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            layers.op_checkpoint_product(forward.make_dual(g.detach(), g.detach()), kept)
