@@ -223,9 +223,11 @@ template <bool EXACT>
 __device__ __forceinline__ float activated(float z, int act) {
   switch (act) {
     case ACT_GELU: {
-      if (!EXACT) {      // max(z, 0) - |z| (1 - Phi(|z|)); the bound keeps an infinite z from meeting a tail of zero
-        const float a = __builtin_fabsf(z);
-        return 0.5f * __builtin_fmaf(-__builtin_amdgcn_fmed3f(a, 0.0f, 3e38f), twice_upper_tail(a), z + a);
+      if (!EXACT) {
+        // max(z, 0) - |z| (1 - Phi(|z|)), the maximum as z / 2 + |z| / 2, which the largest z do not overflow; the bound keeps an infinite z
+        // from meeting a tail of zero
+        const float a = __builtin_fabsf(z), h = 0.5f * a;
+        return __builtin_fmaf(-__builtin_amdgcn_fmed3f(h, 0.0f, 1.5e38f), twice_upper_tail(a), __builtin_fmaf(0.5f, z, h));
       }
       float cdf, e;
       normal_cdf<EXACT>(z, cdf, e);

@@ -1,4 +1,4 @@
-"""The layers on 8-bit checkpoints at their limits: launches of 2^32 threads and more."""
+"""The layers on 8-bit checkpoints at their limits: launches of 2^32 threads and more, the largest values."""
 import pytest
 import torch
 
@@ -56,3 +56,19 @@ def test_rows_padded_to_more_pieces_than_a_launch_is_wide():
     out = torch.empty(rows, to, dtype=torch.float16, device="cuda")
     _abi.check(_abi.lib().gact_pad_rows(x.data_ptr(), _abi.dtype_code(x.dtype), rows, cols, cols, out.data_ptr(), to, _abi.stream_of(x)))
     assert all_like(out, torch.nn.functional.pad(small, (0, to - cols)))
+
+
+@pytest.mark.parametrize("rows,outer", [(3, 264), (40, 264), (200, 264), (700, 2056), (4100, 4104)])
+def test_activations_of_the_largest_values(rows, outer):
+    """z up to bfloat16's largest value, of either sign: all three activations leave z as it is there, or nothing of it.  Through the kernel of few
+    rows, parts, the finishing kernel and the products' own epilogues, with codes and without."""
+    x, w = torch.zeros(rows, 8, dtype=torch.bfloat16, device="cuda"), torch.zeros(outer, 8, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = 2.0 ** 60
+    w[:, 0] = torch.tensor([1.75 * 2.0 ** 67, 1.0 * 2.0 ** 67, -1.5 * 2.0 ** 67, 2.0 ** -50, -2.0 ** -50], device="cuda").repeat(-(-outer // 5))[:outer]
+    z = (x[0, 0].double() * w[:, 0].double()).expand(rows, outer)
+    for act in ("gelu", "gelu_tanh", "silu"):
+        with torch.no_grad():
+            assert torch.equal(ops.op_linear(x, w, None, act).double(), z.clamp(min=0))
+        leaf = w.clone().requires_grad_()
+        y = ops.op_linear(x, leaf, None, act)
+        assert torch.equal(y.detach().double(), z.clamp(min=0))
