@@ -1219,8 +1219,11 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
     __builtin_amdgcn_sched_barrier(0);
 
     const int i0 = done.i * BM, j0 = done.j * BN;
-    int l = lane;       // the addresses below are made here, not before the loop, where they would take registers from it
-    asm volatile("" : "+v"(l));
+    // the lane's number, counted again: it and the addresses below are made here, not before the loop, where they would take registers from it
+    // (with the codes of 256 x 256 there is not one left)
+    uint32_t all = ~0u;
+    asm volatile("" : "+s"(all));
+    const int l = (int)__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0));
     const int i_lane = i0 + wi * (BM / WI) + (l & 15);
     const int j_wave = j0 + wj * (BN / WJ);
     const int j_lane = j_wave + (l >> 4) * 4;
