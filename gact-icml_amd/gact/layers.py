@@ -5,7 +5,9 @@ The saved-tensor hooks of the Controller hand the backward pass a whole dequanti
 at any time.  Rounding is to nearest, so a pass is repeatable and needs no seeds.
 
 A checkpoint holds every row in groups of 256 columns, the last of them shorter, with a float scale and minimum each; its codes are those
-of ``op_quantize(x.float(), 8, ..., rng_stream="deterministic")`` and, where 256 divides the columns, ``op_dequantize`` takes them.
+of ``op_quantize(x.float(), 8, ..., rng_stream="deterministic")`` and, where 256 divides the columns, ``op_dequantize`` takes them.  As
+there, a NaN among numbers becomes its group's minimum, and a group of NaN alone, or of a range beyond float's (an infinity's), becomes NaN: the
+results of a row that is not finite are not finite, but a weight's gradient from a finite gradient of the result need not show a NaN of the input.
 
 Arguments are float32, float16 or bfloat16 tensors on one GPU, of one type, with any strides; a layout that the kernels do not load is copied
 first.  The work goes to the current stream.  Whatever cannot be taken raises a RuntimeError (a TypeError where no tensor

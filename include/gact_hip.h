@@ -227,7 +227,8 @@ int gact_quantize_batched_static(gact_batch_entry* table, const int32_t* bits, i
  * A checkpoint of a matrix [rows, cols] of any element type: codes (one byte each, rows `ldc` bytes apart, ldc a multiple of 16
  * and at least cols, 16-byte aligned), and a float scale and minimum per row and group of 256 columns, [rows, ceil(cols/256)], the last
  * group of a row being shorter.  Codes, scale and minimum are those of gact_quantize of the values widened to float at 8 bit with
- * GACT_NOISE_CONST (equal to it where 256 divides cols); a code stands for code / scale + min.
+ * GACT_NOISE_CONST (equal to it where 256 divides cols); a code stands for code / scale + min.  As there, a NaN is passed over by minimum and
+ * maximum and gets code 0, which stands for the minimum; a group of NaN alone, or of a range that no float holds (an infinity's), stands for NaN.
  * `ld...` are elements from one row to the next.  Rows up to GACT_LAYER_MAX_ROWS, columns up to GACT_LAYER_MAX_COLS. */
 #define GACT_LAYER_MAX_ROWS 0x40000000
 #define GACT_LAYER_MAX_COLS 262144

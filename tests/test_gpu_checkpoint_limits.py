@@ -1,6 +1,7 @@
 """The layers on 8-bit checkpoints at their limits: launches of 2^32 threads and more, the largest values."""
 import pytest
 import torch
+import torch.nn.functional as F
 
 from gact import ops
 from gact.cpp_extension import _abi
@@ -72,3 +73,71 @@ def test_activations_of_the_largest_values(rows, outer):
         leaf = w.clone().requires_grad_()
         y = ops.op_linear(x, leaf, None, act)
         assert torch.equal(y.detach().double(), z.clamp(min=0))
+
+
+def normal(*shape, dtype=torch.float32, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed + 31 * len(shape))
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def test_a_nan_among_numbers_is_kept_as_its_groups_minimum():
+    """As op_quantize keeps it; an infinity's group stands for nothing, and so does one of nothing but NaN."""
+    nan, inf = float("nan"), float("inf")
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        x = normal(6, 600, dtype=dtype)
+        x[1, 3], x[2, 300], x[3, 599], x[4, 256:512], x[5, :2] = nan, inf, -inf, nan, torch.tensor([inf, -inf], dtype=dtype)
+        back, clean = ops.op_restore(ops.op_checkpoint(x)), x.clone()
+        clean[1, 3] = torch.cat([x[1, :3], x[1, 4:256]]).min()
+        want = ops.op_restore(ops.op_checkpoint(clean))
+        lost = torch.zeros(6, 600, dtype=torch.bool, device="cuda")
+        lost[2, 256:512] = lost[3, 512:] = lost[4, 256:512] = lost[5, :256] = True
+        assert torch.equal(back.isnan(), lost) and torch.equal(back[~lost], want[~lost])
+        assert back[1, 3] == clean[1, 3]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,outer", [(10, 40), (50, 520), (200, 264), (700, 2056)])
+def test_gradients_of_unfinite_inputs(rows, outer, dtype):
+    """dx of the other rows does not see them.  dW from a finite dy sees an infinity in its group's columns, a NaN as that group's minimum;
+    behind an activation the row's slopes are not known, and every column of dW is lost."""
+    w, dy = normal(outer, 300, dtype=dtype, seed=1, scale=0.05), normal(rows, outer, dtype=dtype, seed=2)
+
+    def grads(x, act):
+        leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+        return torch.autograd.grad(ops.op_linear(leaves[0], leaves[1], None, act), leaves, dy)
+
+    for bad in (float("inf"), float("nan")):
+        x = normal(rows, 300, dtype=dtype)
+        x[7, 3] = bad
+        clean = x.clone()
+        clean[7, 3] = torch.cat([x[7, :3], x[7, 4:256]]).min()
+        (dx, dw), (want_dx, want_dw) = grads(x, None), grads(clean, None)
+        assert torch.equal(dx, want_dx)
+        if bad != bad:
+            assert torch.equal(dw, want_dw)
+        else:
+            assert dw[:, :256].isnan().all() and torch.equal(dw[:, 256:], want_dw[:, 256:])
+        others = torch.arange(rows, device="cuda") != 7
+        for act in ("gelu", "gelu_tanh", "silu"):
+            (dx, dw), (want_dx, _) = grads(x, act), grads(clean, act)
+            assert torch.equal(dx[others], want_dx[others]) and dx[7].isnan().all() and dw.isnan().all()
+        leaves = [t.requires_grad_() for t in (x.clone(), torch.ones(300, dtype=dtype, device="cuda"), torch.zeros(300, dtype=dtype, device="cuda"))]
+        dn = normal(rows, 300, dtype=dtype, seed=3)
+        dx, dnw, dnb = torch.autograd.grad(ops.op_layer_norm(*leaves), leaves, dn)
+        assert dx[7].isnan().all() and dx[others].isfinite().all() and dnw.isnan().all() and dnb.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,outer", [(10, 40), (50, 520), (200, 264), (700, 2056), (4100, 4104)])
+def test_infinities_through_an_activation_are_torchs(rows, outer, dtype):
+    x, w = normal(rows, 24, dtype=dtype), normal(outer, 24, dtype=dtype, seed=1)
+    plain = x.clone()
+    x[7, 3] = float("inf")
+    z = torch.where(w[:, 3] > 0, float("inf"), -float("inf")).double()
+    others = torch.arange(rows, device="cuda") != 7
+    for act, of in (("gelu", F.gelu), ("gelu_tanh", lambda v: F.gelu(v, approximate="tanh")), ("silu", F.silu)):
+        want = of(z)
+        for leaf in (w, w.clone().requires_grad_()):        # codes of z kept, and not
+            y = ops.op_linear(x, leaf, None, act).detach()
+            assert torch.equal(y[others], ops.op_linear(plain, leaf, None, act).detach()[others])
+            assert torch.equal(y[7].isnan(), want.isnan()) and torch.equal(y[7].isposinf(), want.isposinf())
