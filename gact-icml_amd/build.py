@@ -18,6 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc", "gact_hip.hip")
 LAYERS_SRC = os.path.join(HERE, "csrc", "layers.hip")         # linked into the same library
+LAYERS_HDR = os.path.join(HERE, "csrc", "layer_cuts.h")
 PROBE_SRC = os.path.join(HERE, "csrc", "stream_probe.hip")   # compute-free traffic probes for bench.py
 HDR = os.path.join(ROOT, "include", "gact_hip.h")
 OUT_DIR = os.path.join(HERE, "gact", "lib")
@@ -62,7 +63,7 @@ def up_to_date():
         if torch_mark() not in f.read():     # built for another torch
             return False
     t = min(os.path.getmtime(p) for p in built)
-    return all(os.path.getmtime(p) <= t for p in (SRC, LAYERS_SRC, PROBE_SRC, TORCH_SRC, TORCH_LAYERS_SRC, TORCH_HDR, HDR, os.path.abspath(__file__)))
+    return all(os.path.getmtime(p) <= t for p in (SRC, LAYERS_SRC, LAYERS_HDR, PROBE_SRC, TORCH_SRC, TORCH_LAYERS_SRC, TORCH_HDR, HDR, os.path.abspath(__file__)))
 
 
 def torch_mark():

@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "gact_hip.h"
+#include "layer_cuts.h"
 
 namespace {
 
@@ -1532,7 +1533,6 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* __restrict__ p
 inline void fresh_launch() { (void)hipGetLastError(); }
 inline int launch_status() { return hipGetLastError() == hipSuccess ? GACT_OK : GACT_ELAUNCH; }
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-inline int size_of(int dtype) { return dtype == GACT_F32 ? 4 : 2; }
 inline bool known(int dtype) { return dtype == GACT_F32 || dtype == GACT_F16 || dtype == GACT_BF16; }
 inline bool blocks_fit(int64_t blocks) { return blocks > 0 && blocks <= 0x7fffffff; }
 // A launch takes fewer than 2^32 threads along x: `blocks` workgroups along x where they fit, else in as many equal rows along y as it takes
@@ -1542,7 +1542,6 @@ inline dim3 grid_of(int64_t blocks, int threads) {
   return dim3((unsigned)((blocks + down - 1) / down), (unsigned)down);
 }
 constexpr int64_t kMostCols = GACT_LAYER_MAX_COLS;
-constexpr int kComputeUnits = 256;
 
 // rows that every lane's piece lies whole and aligned in
 inline bool whole_rows(const void* p, int dtype, int64_t cols, int64_t ld) {
@@ -1615,9 +1614,6 @@ int sum_rows(const float* partial, int64_t count, int64_t stride, int64_t cols, 
 
 inline int64_t padded4(int64_t cols) { return (cols + 3) / 4 * 4; }
 
-// workgroups of a tile whose LDS (two steps of both operands, and up to 14 KB beside them) a compute unit holds
-constexpr int slots_per_cu(int bm, int bn) { return bm + bn <= 128 ? 4 : bm + bn <= 256 ? 2 : 1; }
-
 template <typename T, int BM, int BN, int WI, int WJ, bool AS, int BK, int ACT = ACT_NONE, bool CODES = false>
 int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s) {
   p.tiles_i = (p.rows + BM - 1) / BM;
@@ -1633,99 +1629,14 @@ int launch_product(ProductArgs& p, int splits, int64_t per_split, hipStream_t s)
   return launch_status();
 }
 
-// How a product is cut: the side of its tiles, and parts of its depth whose sums are added up afterwards.  Of the cuts there are the one with the
-// least estimated time is taken.  A step of a tile takes as long as one workgroup alone on a compute unit needs for it, or as the unit's share of
-// all workgroups needs; parts cost a launch and the traffic of their sums.  us per step of 128 bytes, alone / shared, from timings of
-// 19 products of 76 million to 17 billion multiplications, each in all of its cuts, both types, forward and with codes (whole, rows x inner x outer):
-//   halves  1024x1024x1024   in tiles of 64  8.5   of 128 10.8   of 256 23.7, in two parts of 64 14.6
-//           1024x1024x4096                  16.5          12.7          24.6
-//           4096x1024x4096                  61.3          37.1          33.3
-//           512x4096x1024                   34.5          42.9          72.1, in 2 / 4 / 8 parts of 64 18.1 / 17.7 / 22.8
-//           8192x512x512, dW                88            118           196, in 8 parts of 64 23.8
-//   floats  1024x1024x1024                  22.7          67.5
-//           4096x1024x4096                 264           249
-//           512x4096x1024                   78           253, in 4 parts of 64 42.8
-// Over the 113 of them that leave a choice the estimate's cut takes 1.2 % longer than the best one.
-struct Rate {
-  float alone, shared;
-};
-constexpr Rate kRates[2][2][3] = {      // [codes][halves, floats][64, 128, 256]
-    {{{0.33f, 0.23f}, {0.5f, 0.53f}, {1.3f, 1.75f}}, {{0.6f, 0.52f}, {2.0f, 1.95f}}},
-    {{{0.6f, 0.33f}, {0.95f, 0.65f}, {1.85f, 2.15f}}, {{0.9f, 0.62f}, {2.3f, 2.1f}}}};
-struct Cut {
-  int side, parts;
-  int64_t per_part;
-};
-inline Cut cut_of(int dtype, bool coded, int64_t rows, int64_t cols, int64_t depth, int largest, int largest_in_parts) {
-  const int64_t step = 128 / size_of(dtype), steps = (depth + step - 1) / step;
-  Cut cut = {64, 1, steps * step};
-  float least = __builtin_inff();
-  for (int n = 0; n < (dtype == GACT_F32 ? 2 : 3); n++) {
-    const int side = 64 << n;
-    if (side > largest) break;
-    const int64_t tiles = ((rows + side - 1) / side) * ((cols + side - 1) / side), slots = kComputeUnits * slots_per_cu(side, side);
-    const Rate rate = kRates[coded][dtype == GACT_F32][n];
-    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-      if (parts > 1 && (parts * 4 > steps || side > largest_in_parts)) break;
-      const int64_t per = (steps + parts - 1) / parts, made = (steps + per - 1) / per, work = tiles * made;
-      const float alone = rate.alone * (float)((work + slots - 1) / slots);
-      const float shared = rate.shared * (float)((work + kComputeUnits - 1) / kComputeUnits);
-      const float sums = made == 1 ? 0.0f : 3.0f + (float)(rows * cols) * (float)(8 * made + size_of(dtype)) * 0.25e-6f;
-      const float us = (float)per * (alone > shared ? alone : shared) + sums;
-      if (us < least) {
-        least = us;
-        cut = {side, (int)made, per * step};
-      }
-      if (work >= slots) break;      // more parts only add to the sums
-    }
-  }
-  return cut;
-}
-
-// How a forward product is run (times in us, halves / floats, rows x inner x outer).
-//  few       rows go to the kernel that reads the weights once and the activations once per 16 columns: up to 16 rows (16x1024x4096 5.2 / 8.1, as
-//            tiles 9.9 / 14.4; 16x8192x8192 41.8 / 79, as tiles 38.9 / 82), more where those reads, from the caches, come to no
-//            more than 64 MiB (64x1024x4096 7.9 / 16.7, as tiles 10.9 / 16.0; 64x4096x4096 23.3 / 52, as tiles 17.5 / 29.8), and
-//            operands of unaligned rows.  In parts of at least 2048 bytes of a row where the strips of columns leave half the compute units
-//            idle: 24x4096x1024 11.8 / 27.1 whole, 8.6 / 12.8 in parts
-//  finished  by finish_kernel: parts; and the pre-activation's codes, where the tiles that hold whole groups of columns are too few.  Halves: fewer
-//            than half the compute units (1024x1024x4096, at half, 25.0 in such tiles, 27.6 finished; 512x1024x4096 23.9 and 21.6; 2048x1024x4096
-//            27.3 and 44.6).  Floats, whose tiles are bound by the matrix pipe alone: fewer than the compute units (1024x1024x4096 138 and 80;
-//            2048x1024x4096, at all of them, 139 and 150)
-struct Forward {
-  bool few, finished;
-  Cut cut;      // few: parts alone.  Of codes that are not finished: nothing
-};
-inline Forward forward_of(int dtype, int64_t rows, int64_t inner, int64_t outer, bool codes, bool whole) {
-  const int64_t strips = (outer + 15) / 16;
-  const bool cached = (rows + 15) / 16 * 16 * strips * inner * size_of(dtype) <= ((int64_t)64 << 20);
-  Forward f = {rows <= 16 || (rows <= GACT_LINEAR_FEW_ROWS && (cached || !whole)), codes, {0, 1, inner}};
-  if (f.few) {
-    const int64_t step = 128 / size_of(dtype), steps = (inner + step - 1) / step;
-    int64_t parts = strips <= kComputeUnits / 2 ? kComputeUnits / strips : 1;
-    if (parts > steps / 16) parts = steps / 16;
-    if (parts > 1) {
-      const int64_t per = (steps + parts - 1) / parts;
-      f.cut = {0, (int)((steps + per - 1) / per), per * step};
-    }
-  } else {
-    const int64_t tiles = ((rows + 127) / 128) * ((outer + 255) / 256);
-    if (codes && tiles >= (dtype == GACT_F32 ? kComputeUnits : kComputeUnits / 2)) f.finished = false;
-    f.cut = cut_of(dtype, false, rows, outer, inner, codes ? 64 : 256, 64);
-  }
-  if (!codes) f.finished = f.cut.parts > 1;
-  return f;
-}
-
 template <typename T, int ACT>
 int forward_product(ProductArgs& p, int side, hipStream_t s) {
   const int64_t step = Mma<T>::kStep, depth = (p.depth + step - 1) / step * step;
-  // the pre-activation's codes need a whole group of columns in a tile; without an activation nobody asks for them.  The larger ones where they fill
-  // the card (16384x1024x4096 halves 165, the others 205)
+  // the pre-activation's codes need a whole group of columns in a tile; without an activation nobody asks for them
   if constexpr (ACT != ACT_NONE) {
     if (p.codes) {
       if constexpr (sizeof(T) == 2)
-        if ((int64_t)((p.rows + 255) / 256) * ((p.cols + 255) / 256) >= kComputeUnits)
+        if (coded_rows_of(sizeof(T) == 4, p.rows, p.cols) == 256)
           return launch_product<T, 256, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
       return launch_product<T, 128, 256, 2, 4, false, B_ROWS, ACT, true>(p, 1, depth, s);
     }
