@@ -335,7 +335,7 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const T* __restrict__ x, 
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Layer norm.  LPR threads own a row and hold it in registers: NC pieces of 8 columns each, LPR * 8 columns apart, so that a group
-// of 256 columns is one piece of 32 neighbouring threads (LPR 16: two pieces of 16).  LPR up to 64: 256 / LPR rows per workgroup;
+// of 256 columns is one piece of 32 neighbouring threads (LPR 16: rows of up to 128 columns, one piece).  LPR up to 64: 256 / LPR rows per workgroup;
 // above: a workgroup of LPR threads per row.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int LPR, int THREADS = 256>
@@ -409,40 +409,30 @@ __global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_forward_kernel(
     for (int u = 0; u < U; u++)
       if (u < there) *(f32x2*)(stats + 2 * (row0 + u)) = f32x2{mean[u], rstd[u]};
   if (codes) {
-    constexpr int PAIR = LPR == 16 && NC > 1 ? 2 : 1;   // pieces of a group
-    constexpr int GLANES = LPR < 32 ? 16 : 32, K = U * (NC / PAIR);
+    static_assert(LPR >= 32 || NC == 1, "a group is one piece");
+    constexpr int GLANES = LPR < 32 ? 16 : 32, K = U * NC;
     const int groups = (cols + kGroup - 1) / kGroup;
     float lo[K], hi[K], s[K];
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      const int u = k / (NC / PAIR), c0 = k % (NC / PAIR) * PAIR;
+      const int u = k / NC, c = k % NC, left = cols - (c * Shape::kSpan + lane * kVec);
       lo[k] = __builtin_inff();
       hi[k] = -__builtin_inff();
 #pragma unroll
-      for (int c = c0; c < c0 + PAIR; c++) {
-        const int left = cols - (c * Shape::kSpan + lane * kVec);
-#pragma unroll
-        for (int e = 0; e < kVec; e++)
-          if ((WHOLE ? 0 : e) < left) lo[k] = __builtin_fminf(lo[k], v[u][c][e]), hi[k] = __builtin_fmaxf(hi[k], v[u][c][e]);
-      }
+      for (int e = 0; e < kVec; e++)
+        if ((WHOLE ? 0 : e) < left) lo[k] = __builtin_fminf(lo[k], v[u][c][e]), hi[k] = __builtin_fmaxf(hi[k], v[u][c][e]);
       lo[k] = over_lanes<Least, GLANES>(lo[k]);
       hi[k] = over_lanes<Most, GLANES>(hi[k]);
     }
     scales_of<K>(lo, hi, s);
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      const int u = k / (NC / PAIR), c0 = k % (NC / PAIR) * PAIR;
-      if (u >= there) continue;
-#pragma unroll
-      for (int c = c0; c < c0 + PAIR; c++) {
-        const int col = c * Shape::kSpan + lane * kVec;
-        const float (&w)[kVec] = v[u][c];
-        if (col < cols)
-          *(u32x2*)(codes + (row0 + u) * ldc + col) =
-              u32x2{four_codes(w[0], w[1], w[2], w[3], lo[k], s[k]), four_codes(w[4], w[5], w[6], w[7], lo[k], s[k])};
-      }
-      const int col = c0 * Shape::kSpan + lane * kVec;
-      if (lane % GLANES == 0 && col < cols) {
+      const int u = k / NC, c = k % NC, col = c * Shape::kSpan + lane * kVec;
+      if (u >= there || col >= cols) continue;
+      const float (&w)[kVec] = v[u][c];
+      *(u32x2*)(codes + (row0 + u) * ldc + col) =
+          u32x2{four_codes(w[0], w[1], w[2], w[3], lo[k], s[k]), four_codes(w[4], w[5], w[6], w[7], lo[k], s[k])};
+      if (lane % GLANES == 0) {
         scale[(row0 + u) * groups + col / kGroup] = s[k];
         mn[(row0 + u) * groups + col / kGroup] = lo[k];
       }
@@ -668,11 +658,11 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __res
   float sum[kVec];
 #pragma unroll
   for (int e = 0; e < kVec; e++) sum[e] = 0.0f;
-  if (left > 0 || (dz && col < lddz)) {
+  if (left > 0) {
     for (int64_t row = first + strip; row < last; row += kRows) {
       float g[kVec], z[kVec];
       load_cols<T, WHOLE>(dy + row * lddy + col, left, g);
-      if (codes && left > 0) {
+      if (codes) {
         const int64_t group = row * groups + blockIdx.x;
         eight_values(*(const u32x2*)(codes + row * ldc + col), inverse_of(scale[group]), mn[group], z);
 #pragma unroll
