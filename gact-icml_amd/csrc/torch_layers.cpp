@@ -458,6 +458,12 @@ at::Tensor linear(const at::Tensor& x_given, const at::Tensor& weight, const std
 }
 
 // ---- what Python calls ----
+// the operator itself: its allocations and launches may wait for the GPU, and other threads of Python's go on meanwhile
+template <typename F>
+auto without_gil(const F& call) {
+  const WithoutGil released;
+  return call();
+}
 double number_of(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw python_error();
@@ -489,7 +495,8 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const double eps = number_of(args[3]);
   const at::Tensor& x = tensor_of(args[0], "data");
   const std::optional<at::Tensor> weight = tensor_or_none(args[1], "weight"), bias = tensor_or_none(args[2], "bias");
-  return THPVariable_Wrap(layer_norm(x, weight, bias, eps, autocast_of(args[4])));
+  const Autocast autocast = autocast_of(args[4]);
+  return THPVariable_Wrap(without_gil([&] { return layer_norm(x, weight, bias, eps, autocast); }));
   END_HANDLE_TH_ERRORS
 }
 
@@ -502,7 +509,8 @@ PyObject* py_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor& x = tensor_of(args[0], "data");
   const at::Tensor& weight = tensor_of(args[1], "weight");
   const std::optional<at::Tensor> bias = tensor_or_none(args[2], "bias"), residual = tensor_or_none(args[4], "residual");
-  return THPVariable_Wrap(linear(x, weight, bias, (int)act, residual, autocast_of(args[5])));
+  const Autocast autocast = autocast_of(args[5]);
+  return THPVariable_Wrap(without_gil([&] { return linear(x, weight, bias, (int)act, residual, autocast); }));
   END_HANDLE_TH_ERRORS
 }
 
@@ -557,10 +565,12 @@ PyObject* py_checkpoint(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments(n, 1);
   const at::Tensor& input = tensor_of(args[0], "data");
-  const at::AutoDispatchBelowADInplaceOrView below;
-  const Place at(input);
-  const Rows x = rows_of(input, "data");
-  return tuple_of(x.rows ? compress(x, at) : room_for(0, x.cols, at));
+  return tuple_of(without_gil([&] {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Place at(input);
+    const Rows x = rows_of(input, "data");
+    return x.rows ? compress(x, at) : room_for(0, x.cols, at);
+  }));
   END_HANDLE_TH_ERRORS
 }
 
@@ -601,13 +611,15 @@ PyObject* py_restore(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments(n, 5);
   const Given g = given(args);
-  const at::AutoDispatchBelowADInplaceOrView below;
-  const Place at(g.kept.codes);
-  const at::Tensor result = at.empty(g.shape, g.dtype);
-  if (g.rows)
-    check_status(gact_restore(in(g.kept.codes), g.kept.codes.size(1), (const float*)in(g.kept.scale), (const float*)in(g.kept.mn),
-                              dtype_code(g.dtype), g.rows, g.cols, out(result), at.stream));
-  return THPVariable_Wrap(result);
+  return THPVariable_Wrap(without_gil([&] {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    const Place at(g.kept.codes);
+    const at::Tensor result = at.empty(g.shape, g.dtype);
+    if (g.rows)
+      check_status(gact_restore(in(g.kept.codes), g.kept.codes.size(1), (const float*)in(g.kept.scale), (const float*)in(g.kept.mn),
+                                dtype_code(g.dtype), g.rows, g.cols, out(result), at.stream));
+    return result;
+  }));
   END_HANDLE_TH_ERRORS
 }
 
@@ -620,18 +632,19 @@ PyObject* py_checkpoint_product(PyObject*, PyObject* const* args, Py_ssize_t n) 
   TORCH_CHECK(grad.scalar_type() == g.dtype, "The type of grad is not correct!");
   TORCH_CHECK(grad.device() == g.kept.codes.device(), "grad is on another device");
   no_tangent(grad, "op_checkpoint_product");
-  at::Tensor result;
-  {
-    const at::AutoDispatchBelowADInplaceOrView below;
-    const Place at(grad);
-    Rows r = rows_of(grad, "grad");
-    TORCH_CHECK(r.rows == g.rows, "grad has ", r.rows, " rows, the checkpoint ", g.rows);
-    if (r.rows) r = product_rows(r, at);
-    result = weight_product(r, g.kept, g.cols, g.dtype, at);
-  }
-  // no backward pass: the result of a gradient that has a history says so to who goes through it
-  if (torch::autograd::compute_requires_grad(grad)) result = once({result}, "op_checkpoint_product")[0];
-  return THPVariable_Wrap(result);
+  return THPVariable_Wrap(without_gil([&] {
+    at::Tensor result;
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const Place at(grad);
+      Rows r = rows_of(grad, "grad");
+      TORCH_CHECK(r.rows == g.rows, "grad has ", r.rows, " rows, the checkpoint ", g.rows);
+      if (r.rows) r = product_rows(r, at);
+      result = weight_product(r, g.kept, g.cols, g.dtype, at);
+    }
+    // no backward pass: the result of a gradient that has a history says so to who goes through it
+    return torch::autograd::compute_requires_grad(grad) ? once({result}, "op_checkpoint_product")[0] : result;
+  }));
   END_HANDLE_TH_ERRORS
 }
 

@@ -108,13 +108,6 @@ void* stream_on(c10::Device device) { return c10::hip::getCurrentHIPStream(devic
 const void* in(const at::Tensor& t) { return t.const_data_ptr(); }
 void* out(const at::Tensor& t) { return t.mutable_data_ptr(); }
 
-// The GIL is released as long as this lives, and is back before an exception that leaves its scope becomes one of Python's
-struct WithoutGil {
-  PyThreadState* const state = PyEval_SaveThread();
-  WithoutGil() = default;
-  WithoutGil(const WithoutGil&) = delete;
-  ~WithoutGil() { PyEval_RestoreThread(state); }
-};
 // The library's call with the GIL released and the data's device current
 template <typename F>
 int on(c10::Device device, const F& call) {

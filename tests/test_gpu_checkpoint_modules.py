@@ -2,6 +2,7 @@
 Controller's hooks."""
 import copy
 import threading
+import time
 
 import pytest
 import torch
@@ -293,3 +294,54 @@ def test_a_product_of_a_gradient_with_a_history_is_not_differentiated():
     with forward.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             layers.op_checkpoint_product(forward.make_dual(g.detach(), g.detach()), kept)
+
+
+def test_other_threads_go_on_while_a_call_waits_for_room_to_launch():
+    """Behind a kernel that takes long, enough calls to fill the queue to the GPU: the one that finds it full waits without the GIL."""
+    x, w = normal(8, 64), normal(16, 64, seed=1)
+    kept, g = layers.op_checkpoint(x), normal(8, 16, seed=2)
+    for call in (lambda: layers.op_layer_norm(x), lambda: layers.op_linear(x, w), lambda: layers.op_checkpoint(x), lambda: layers.op_restore(kept),
+                 lambda: layers.op_checkpoint_product(g, kept)):
+        call()
+        torch.cuda.synchronize()
+        gaps, done = [], threading.Event()
+
+        def tick():
+            last = time.perf_counter()
+            while not done.is_set():
+                time.sleep(0.0005)
+                now = time.perf_counter()
+                gaps.append(now - last)
+                last = now
+
+        ticking = threading.Thread(target=tick)
+        ticking.start()
+        longest, start = 0, time.perf_counter()
+        torch.cuda._sleep(2000000000)
+        for _ in range(40000):
+            before = time.perf_counter()
+            call()
+            longest = max(longest, time.perf_counter() - before)
+            if longest > 0.1 or before - start > 5:
+                break
+        done.set()
+        ticking.join()
+        torch.cuda.synchronize()
+        if longest <= 0.1:
+            pytest.skip("the queue was not full before the GPU was done")
+        assert max(gaps) < longest / 2
+
+
+def test_an_error_of_a_hook_for_saved_tensors_is_raised():
+    x, w = normal(8, 64), normal(16, 64, seed=1).requires_grad_()
+
+    def refuse(t):
+        raise KeyError("not here")
+
+    for call in (lambda: layers.op_linear(x, w, None, "gelu"), lambda: layers.op_layer_norm(x, w[0])):
+        with torch.autograd.graph.saved_tensors_hooks(refuse, lambda t: t), pytest.raises(KeyError, match="not here"):
+            call()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, refuse):
+            y = call()
+        with pytest.raises(KeyError, match="not here"):
+            y.sum().backward()
