@@ -1925,7 +1925,8 @@ int gact_checkpoint_product(const void* grad, int64_t ldg, const void* codes, in
   if (!known(dtype) || !layer_sizes(rows, outer, inner) || rows == 0) return GACT_EINVAL;
   if (!grad || !codes || !scale || !mn || !out) return GACT_EINVAL;
   const int64_t padded = (outer * size_of(dtype) + 15) / 16 * 16 / size_of(dtype);
-  if (!operand_fits(grad, ldg, dtype, padded) || !codes_fit(codes, inner, ldc)) return GACT_EALIGN;
+  // offsets within a step's rows are 32 bits wide, of the codes as of the other operand
+  if (!operand_fits(grad, ldg, dtype, padded) || !codes_fit(codes, inner, ldc) || ldc > 4 * kMostCols) return GACT_EALIGN;
   ProductArgs p = {};
   p.a = grad;
   p.b = codes;

@@ -279,8 +279,8 @@ int gact_activation_backward(const void* dy, int64_t lddy, const void* codes, in
 
 /* out [rows, cols] = a [rows, depth] b [depth, cols], and out [outer, inner] = grad [rows, outer]^T times the values, rounded to `dtype`, of a
  * checkpoint [rows, inner] (rows > 0); out contiguous.  Operands: 16-byte aligned rows of whole 16-byte pieces, `ld` leaving room for the
- * last one; what lies behind the last column of `a` up to its piece's end must be zero.  workspace: gact_product_workspace_bytes()
- * of (rows, cols, depth), or (outer, inner, rows); 16-byte aligned. */
+ * last one, and rows (of codes, too) at most 4 GACT_LAYER_MAX_COLS apart; what lies behind the last column of `a` up to its piece's end must be
+ * zero.  workspace: gact_product_workspace_bytes() of (rows, cols, depth), or (outer, inner, rows); 16-byte aligned. */
 int64_t gact_product_workspace_bytes(int dtype, int64_t rows, int64_t cols, int64_t depth);
 int gact_product(const void* a, int64_t lda, const void* b, int64_t ldb, int dtype, int64_t rows, int64_t depth, int64_t cols, void* out,
                  void* workspace, void* stream);

@@ -10,6 +10,7 @@ import torch.nn as nn
 from gact import layers
 from gact.conf import config
 from gact.controller import Controller
+from gact.cpp_extension import _abi
 
 
 @pytest.fixture(autouse=True)
@@ -70,3 +71,10 @@ def test_layers_stay_attached_until_the_last_controller_leaves():
     assert [type(m) for m in model] == swapped[:1] + kinds[1:] + [layers.CheckpointedLinear]
     part.uninstall_hook()
     assert [type(m) for m in model] == kinds + [layers.CheckpointedLinear] and not len(layers._held)
+
+
+def test_library_refuses_products_of_codes_whose_rows_are_too_far_apart():
+    """Past 32 bits of offset within a step: codes would be read from other rows."""
+    L = _abi.lib()
+    for ldc in ((1 << 20) + 16, 1 << 26, 1 << 34):
+        assert L.gact_checkpoint_product(16, 8, 16, ldc, 16, 16, 2, 64, 8, 8, 16, None, None) == -2
