@@ -208,7 +208,7 @@ at::Tensor again(SavedVariable& v, at::ScalarType dtype, c10::IntArrayRef shape,
   TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.scalar_type() == dtype && t.device() == grad.device() && t.sizes() == shape &&
                   (!dense || (t.is_contiguous() && !t.is_neg())),
               "the hooks for saved tensors gave back another tensor than they were given");
-  return t;
+  return dense && !aligned(in(t)) ? t.clone() : t;      // a place in a larger buffer, say
 }
 Kept again(SavedVariable& codes, SavedVariable& scale, SavedVariable& mn, int64_t rows, int64_t cols, const at::Tensor& grad) {
   const int64_t groups = (cols + kGroup - 1) / kGroup;

@@ -332,6 +332,29 @@ def test_other_threads_go_on_while_a_call_waits_for_room_to_launch():
         assert max(gaps) < longest / 2
 
 
+def test_hooks_for_saved_tensors_may_give_back_other_addresses():
+    """Everything that a pass saves in one buffer, one behind the other."""
+    x, w, b = normal(70, 48).requires_grad_(), normal(40, 48, seed=1).requires_grad_(), normal(40, seed=2).requires_grad_()
+    nw = normal(48, seed=3).requires_grad_()
+    buffer, used = torch.empty(1 << 20, dtype=torch.uint8, device="cuda"), []
+
+    def pack(t):
+        size, start = t.element_size(), sum(used)
+        start += -start % size + size        # as the type's alignment allows
+        used.append(start + t.numel() * size - sum(used))
+        place = buffer[start:start + t.numel() * size].view(t.dtype).view(t.shape)
+        with torch.no_grad():
+            place.copy_(t)
+        return place
+
+    for call, dy in ((lambda: layers.op_linear(x, w, b, "gelu"), normal(70, 40, seed=4)), (lambda: layers.op_layer_norm(x, nw), normal(70, 48, seed=5))):
+        want = torch.autograd.grad(call(), [x, w, b, nw], dy, allow_unused=True)
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            y = call()
+        got = torch.autograd.grad(y, [x, w, b, nw], dy, allow_unused=True)
+        assert all((g is None and v is None) or torch.equal(g, v) for g, v in zip(got, want))
+
+
 def test_an_error_of_a_hook_for_saved_tensors_is_raised():
     x, w = normal(8, 64), normal(16, 64, seed=1).requires_grad_()
 
