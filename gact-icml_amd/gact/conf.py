@@ -43,7 +43,7 @@ class QuantizationConfig:
         # While the Controller's hooks are installed, the model's nn.Linear and nn.LayerNorm run on gact.ops.op_linear and
         # op_layer_norm: they keep their input as 8-bit codes, rounded to nearest, which their backward kernels read where they
         # lie.  What the other layers save goes through the hooks as before; `bit` and auto precision do not touch these codes, nor
-        # weights that are the model's parameters, under autocast either.  (A weight that is computed in the pass - a weight norm's - is a
+        # weights that are the model's parameters, under autocast either, and `swap` leaves the codes on the GPU.  (A weight that is computed in the pass - a weight norm's - is a
         # saved tensor like any other to the hooks.)
         self.checkpoint_layers = False
 

@@ -20,6 +20,7 @@ import weakref
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 from torch.utils._device import DeviceContext
 
 from .cpp_extension import _abi
@@ -87,11 +88,10 @@ def _overridden(tensors):
         and all(isinstance(m, DeviceContext) for m in torch.overrides._get_current_function_mode_stack()))
 
 
-def _taken(module, input, linear):
-    """Whether the operator takes this call of the module: anything else goes to torch's own."""
+def _taken(input, weight, bias, linear):
+    """Whether the operator takes this call of a module: anything else goes to torch's own."""
     if not (isinstance(input, torch.Tensor) and input.is_cuda):
         return False
-    weight, bias = module.weight, module.bias
     return (not _overridden(tuple(t for t in (input, weight, bias) if t is not None))
             and _abi.native().takes(input, weight, bias, linear, torch.is_autocast_enabled("cuda")))
 
@@ -109,9 +109,10 @@ class CheckpointedLinear(_Swapped, nn.Linear):
     _own = nn.Linear
 
     def forward(self, input):
-        if _taken(self, input, True):
-            return op_linear(input, self.weight, self.bias)
-        return super().forward(input)
+        weight, bias = self.weight, self.bias       # once: either may be computed each time it is asked for
+        if _taken(input, weight, bias, True):
+            return op_linear(input, weight, bias)
+        return F.linear(input, weight, bias)
 
 
 class CheckpointedLayerNorm(_Swapped, nn.LayerNorm):
@@ -119,9 +120,10 @@ class CheckpointedLayerNorm(_Swapped, nn.LayerNorm):
     _own = nn.LayerNorm
 
     def forward(self, input):
-        if len(self.normalized_shape) == 1 and _taken(self, input, False) and input.shape[-1] == self.normalized_shape[0]:
-            return op_layer_norm(input, self.weight, self.bias, self.eps)
-        return super().forward(input)
+        weight, bias = self.weight, self.bias
+        if len(self.normalized_shape) == 1 and _taken(input, weight, bias, False) and input.shape[-1] == self.normalized_shape[0]:
+            return op_layer_norm(input, weight, bias, self.eps)
+        return F.layer_norm(input, self.normalized_shape, weight, bias, self.eps)
 
 
 _CHECKPOINTED = {nn.Linear: CheckpointedLinear, nn.LayerNorm: CheckpointedLayerNorm}

@@ -368,3 +368,21 @@ def test_an_error_of_a_hook_for_saved_tensors_is_raised():
             y = call()
         with pytest.raises(KeyError, match="not here"):
             y.sum().backward()
+
+
+@pytest.mark.parametrize("kind", PAIRS, ids=lambda k: k[0].__name__)
+def test_a_weight_that_is_computed_is_computed_once_a_call(kind):
+    calls = []
+
+    class Doubled(nn.Module):
+        def forward(self, weight):
+            calls.append(weight)
+            return 2 * weight
+
+    layer, own = pair(*kind)
+    x = normal(5, 16)
+    torch.nn.utils.parametrize.register_parametrization(layer, "weight", Doubled())
+    calls.clear()
+    y = layer(x)
+    assert len(calls) == 1
+    assert torch.equal(y, (layers.op_linear if kind[0] is nn.Linear else layers.op_layer_norm)(x, 2 * own.weight, own.bias))
