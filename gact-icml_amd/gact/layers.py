@@ -143,6 +143,8 @@ def detach(changed):
         for own, checkpointed in _CHECKPOINTED.items():
             if type(m) is checkpointed:
                 m.__class__ = own
+            elif type(m).__bases__ == (checkpointed,) and torch.nn.utils.parametrize.is_parametrized(m):
+                type(m).__bases__ = (own,)      # parametrized meanwhile: the class is the module's and its copies' own
 
 
 # attached module -> how many hold it

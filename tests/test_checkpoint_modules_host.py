@@ -78,3 +78,17 @@ def test_library_refuses_products_of_codes_whose_rows_are_too_far_apart():
     L = _abi.lib()
     for ldc in ((1 << 20) + 16, 1 << 26, 1 << 34):
         assert L.gact_checkpoint_product(16, 8, 16, ldc, 16, 16, 2, 64, 8, 8, 16, None, None) == -2
+
+
+def test_layers_that_were_parametrized_while_attached_are_detached():
+    model, x = a_model(), torch.randn(5, 6)
+    changed = layers.attach(model)
+    for n in (0, 2):
+        torch.nn.utils.parametrize.register_parametrization(model[n], "weight", nn.Softplus())
+    twin, want = copy.deepcopy(model), model(x)
+    layers.detach(changed)
+    for m in (model, twin):
+        assert not any(isinstance(layer, (layers.CheckpointedLinear, layers.CheckpointedLayerNorm)) for layer in m)
+        assert torch.equal(m(x), want)
+    torch.nn.utils.parametrize.remove_parametrizations(model[0], "weight")
+    assert type(model[0]) is nn.Linear
