@@ -96,12 +96,16 @@ def _taken(input, weight, bias, linear):
             and _abi.native().takes(input, weight, bias, linear, torch.is_autocast_enabled("cuda")))
 
 
+_attached = weakref.WeakSet()
+
+
 class _Swapped:
-    """A module that runs on an operator while it is attached.  Its copies and pickles are torch's own modules: nothing would ever detach them
-    (a running average of the model, say), and they load where this package is not there."""
+    """Copies and pickles of a module that runs on an operator because it is attached are torch's own modules: nothing would ever detach them
+    (a running average of the model, say), and they load where this package is not there.  A module that was made so stays so."""
 
     def __reduce_ex__(self, protocol):
-        return (object.__new__, (self._own,)) + super().__reduce_ex__(protocol)[2:]
+        made = super().__reduce_ex__(protocol)
+        return (object.__new__, (self._own,)) + made[2:] if self in _attached else made
 
 
 class CheckpointedLinear(_Swapped, nn.Linear):
@@ -134,12 +138,14 @@ def attach(model):
     changed = [m for m in model.modules() if type(m) in _CHECKPOINTED]
     for m in changed:
         m.__class__ = _CHECKPOINTED[type(m)]      # the module's parameters and hooks stay as they are
+    _attached.update(changed)
     return changed
 
 
 def detach(changed):
     """What attach returned, as torch's own again."""
     for m in changed:
+        _attached.discard(m)
         for own, checkpointed in _CHECKPOINTED.items():
             if type(m) is checkpointed:
                 m.__class__ = own

@@ -49,6 +49,13 @@ def test_copies_of_attached_layers_are_torchs_own():
     assert [type(m) for m in model] == kinds and torch.equal(model(x), want)
 
 
+def test_copies_of_layers_that_were_made_so_stay_so():
+    own = layers.CheckpointedLinear(6, 8)
+    assert layers.attach(own) == []
+    for m in (copy.deepcopy(own), copy.copy(own), pickle.loads(pickle.dumps(own))):
+        assert type(m) is layers.CheckpointedLinear and torch.equal(m.weight, own.weight)
+
+
 def test_layers_stay_attached_until_the_last_controller_leaves():
     config.checkpoint_layers, config.auto_prec = True, False
     model = a_model()
