@@ -271,10 +271,12 @@ __device__ __forceinline__ float slope(float z, int act) {
 // Checkpoints of rows.  32 lanes (16 of rows of up to 128 columns) own a group: one 16-byte piece each (float: two), its minimum and maximum over
 // those lanes.
 // ---------------------------------------------------------------------------------------------------------------------------------
-// Bound by memory: 32768x4096 halves 84 us (4.8 TB/s), 16384x1024 floats 16.6 (5.1), 25088x384 halves 11.7, of which the launch and the one
-// load that nothing overlaps are half.  One group at a time: four to a half wave, with their loads together and one division for all of their
+// Times, here and of the kernels below up to the products, are of launches one behind the other whose inputs are in no cache; a small tensor that
+// the caches hold takes less (the restore of 25088x384 right behind its checkpoint 6 to 7 us, layer norm of 16384x1024 21 each way).
+// Bound by memory: 32768x4096 halves 83 us (4.9 TB/s), floats 115 (5.9), 16384x1024 floats 16.9 (5.0), 25088x384 halves 12.1, of which the launch
+// and the one load that nothing overlaps are half.  One group at a time: four to a half wave, with their loads together and one division for all of their
 // scales, take 84 us instead of 90 for 134 M halves, but 14 instead of 11.5 for 10 M.  A group shorter than 256 leaves lanes idle (771
-// columns of halves, 22.7 us for 25088 rows, 2.6 TB/s).
+// columns of halves, 23 us for 25088 rows, 2.6 TB/s).
 template <typename T, int LANES, bool WHOLE>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int groups,
                                                          uint8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale,
@@ -301,8 +303,8 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(const T* __restrict__ x
   }
 }
 
-// The values again, the same lanes: 32768x4096 halves 72 us (5.7 TB/s), 16384x1024 12.0 (4.3), 25088x384 8.3.  1 / scale is made by every
-// lane: the division is hidden behind the loads.
+// The values again, the same lanes: 32768x4096 halves 73 us (5.5 TB/s), floats 118 (5.7), 16384x1024 halves 12.0 (4.2), 25088x384 8.7.  1 / scale
+// is made by every lane: the division is hidden behind the loads.
 template <typename T, int LANES, bool WHOLE>
 __global__ __launch_bounds__(256) void restore_kernel(const uint8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scale,
                                                       const float* __restrict__ mn, int64_t rows, int cols, int groups,
@@ -362,7 +364,7 @@ __device__ __forceinline__ float row_sum(float v, float* shared, int turn) {
 }
 
 // mean = sum / cols, var = sum (x - mean)^2 / cols from the row in registers, in floats: one read, one write of x, and the codes.  Bound by memory:
-// 401408x96 floats 68 us (5.2 TB/s), 65536x1024 halves 72 (4.7), 16384x4096 halves 67 (5.1), 16384x1024 halves 25 (3.4: half of it launch,
+// 401408x96 floats 71 us (5.0 TB/s), 65536x1024 halves 73 (4.6), 16384x4096 halves 67 (5.0), 16384x1024 halves 26 (3.3: half of it launch,
 // ramp and the tail).  U consecutive rows at a time: their loads are on the way together, and their scales are one division (see scales_of).
 template <typename T, int LPR, int NC, int U, bool WHOLE>
 __global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_forward_kernel(
@@ -462,8 +464,8 @@ __global__ __launch_bounds__(RowShape<LPR>::kThreads) void norm_forward_kernel(
 
 // xh = (value - mean) rstd, g = dy w: dx = rstd (g - mean(g) - xh mean(g xh)); a thread adds up dy xh and dy of its columns over the
 // rows it sees, a workgroup writes one row of partial sums.  While a row is worked on, the next one's loads are on the way.
-// Reads dy and the codes, writes dx: 401408x96 floats 72 us (4.9 TB/s), 65536x1024 halves 78 (4.3), 16384x4096 halves 83 (4.0), 16384x1024
-// halves 25 (3.3), the column sums included (they take 3 us, 15 of 85 at 4096 columns).
+// Reads dy and the codes, writes dx: 401408x96 floats 74 us (4.8 TB/s), 65536x1024 halves 80 (4.2), 16384x4096 halves 86 (3.9), 16384x1024
+// halves 26 (3.3), the column sums included (they take 4 us, 14 of 86 at 4096 columns).
 constexpr int kNormThreads = 512;   // waves that share a row of partial sums (with 4 of them and twice the workgroups there is twice as much to add up)
 template <int LPR>
 using SharedRows = RowShape<LPR, kNormThreads>;
@@ -639,9 +641,9 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
 // down `per` rows; without codes (no activation) dz is dy, copied to the products' stride where `dz` is given.  dz is rounded to T, as dy and
 // a checkpoint's values are where they enter a product: the matrix instructions of 16-bit types take nothing wider, and those of floats run
 // at a tenth of their rate.  (bfloat16, 16384 rows: an error of 0.0024 of the outputs' norm where products of unrounded dz have 0.0017.)
-// Bound by memory, 32768x4096 halves GELU 134 us (5.0 TB/s), SiLU 128, sums alone 47 (5.7); 16384x1024 23, 22 and 11.  32 lanes and 256
+// Bound by memory, 32768x4096 halves GELU 132 us (5.1 TB/s), SiLU 130, sums alone 47 (5.7); 16384x1024 24, 22 and 11.  32 lanes and 256
 // columns to a row, as the codes' groups are, 16 lanes where 128 columns are enough: 401408x96 halves 56 (3.4).  In floats GELU's exact error
-// function counts: 401408x96 120 us (2.9 TB/s), SiLU 89.
+// function counts where a quarter of the lanes has no columns: 401408x96 112 us (3.1 TB/s), SiLU 87 (4.0); 32768x4096 272 (4.5) and 253 (4.8).
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int LANES, bool WHOLE>
 __global__ __launch_bounds__(256) void activation_backward_kernel(const T* __restrict__ dy, int64_t lddy, const uint8_t* __restrict__ codes,

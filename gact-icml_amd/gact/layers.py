@@ -69,8 +69,9 @@ def op_linear(input, weight, bias=None, activation=None, residual=None):
     """activation(input weight^T + bias) + residual in one kernel; activation None, "gelu", "gelu_tanh" or "silu".
 
     For the backward pass it keeps the 8-bit checkpoint of the input and, under an activation, of the value it is applied to; the
-    gradients are those of the checkpoints' values.  (relu is not among them: its derivative jumps at zero, where 8 bits do not hold
-    the sign.)  Under autocast it runs in autocast's type; the weight that it saves is the one it was given, which the backward pass rounds
+    gradients are those of the checkpoints' values; under an activation its gradient dz is rounded to the layer's type before dx and dW,
+    as the matrix instructions take it (bias gradients add it up unrounded).  (relu is not among them: its derivative jumps at zero, where
+    8 bits do not hold the sign.)  Under autocast it runs in autocast's type; the weight that it saves is the one it was given, which the backward pass rounds
     again."""
     act = _ACTIVATIONS.get(activation)
     if act is None:
