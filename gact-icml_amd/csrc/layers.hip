@@ -52,6 +52,14 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[kVec]) {
     for (int e = 0; e < kVec; e++) v[e] = (float)a[e];
   }
 }
+// A result is a float before it is rounded to T, in every kernel and whichever way it is stored: the empty statement keeps the compiler from making
+// one instruction of the last operation and its rounding to a half, which rounds once and differs in one of 2^13 values - of rows at one address and
+// not of the same rows at another.
+template <typename T>
+__device__ __forceinline__ T rounded(float v) {
+  if constexpr (std::is_same<T, f16>::value) asm("" : "+v"(v));
+  return (T)v;
+}
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[kVec]) {
   if constexpr (std::is_same<T, float>::value) {
@@ -61,7 +69,7 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[kVec]) {
     typedef T T8 __attribute__((ext_vector_type(8)));
     T8 a;
 #pragma unroll
-    for (int e = 0; e < kVec; e++) a[e] = (T)v[e];
+    for (int e = 0; e < kVec; e++) a[e] = rounded<T>(v[e]);
     *(T8*)p = a;
   }
 }
@@ -96,12 +104,12 @@ __device__ __forceinline__ void store_cols(T* p, int64_t n, const float (&v)[kVe
   } else if (n >= kVec) {
     typename Loose<T>::Eight a;
 #pragma unroll
-    for (int e = 0; e < kVec; e++) a[e] = (T)v[e];
+    for (int e = 0; e < kVec; e++) a[e] = rounded<T>(v[e]);
     *(typename Loose<T>::Eight*)p = a;
   } else {
 #pragma unroll
     for (int e = 0; e < kVec; e++)
-      if (e < n) p[e] = (T)v[e];
+      if (e < n) p[e] = rounded<T>(v[e]);
   }
 }
 
@@ -632,7 +640,7 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
 #pragma unroll
     for (int w = 0; w < 16; w++) s += shared[w][threadIdx.x];
     T* out = blockIdx.y ? out1 : out0;
-    if (out) out[col] = (T)s;
+    if (out) out[col] = rounded<T>(s);
   }
 }
 
@@ -986,7 +994,7 @@ __device__ __forceinline__ u32x2 rounded4(f32x4 v) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   T4 o;
 #pragma unroll
-  for (int e = 0; e < 4; e++) o[e] = (T)v[e];
+  for (int e = 0; e < 4; e++) o[e] = rounded<T>(v[e]);
   return __builtin_bit_cast(u32x2, o);
 }
 template <typename T>
@@ -1355,7 +1363,7 @@ __global__ __launch_bounds__(WI* WJ * 64) void product_kernel(ProductArgs p) {
             for (int e = 0; e < 4; e++) {
               const int j = j_lane + n * 16 + e;
               if (j >= p.cols) continue;
-              ((T*)p.out)[i * p.ldo + j] = (T)(FORWARD && p.residual ? v[e] + (float)((const T*)p.residual)[i * p.ldr + j] : v[e]);
+              ((T*)p.out)[i * p.ldo + j] = rounded<T>(FORWARD && p.residual ? v[e] + (float)((const T*)p.residual)[i * p.ldr + j] : v[e]);
             }
           }
           __builtin_amdgcn_sched_barrier(0);
@@ -1380,7 +1388,7 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const float* __restric
   for (int s = 1; s < splits; s++) v += *(const f32x4*)(partial + (s * rows + row) * ldp + col);
 #pragma unroll
   for (int e = 0; e < 4; e++)
-    if (col + e < cols) out[row * cols + col + e] = (T)v[e];
+    if (col + e < cols) out[row * cols + col + e] = rounded<T>(v[e]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -1463,7 +1471,7 @@ __global__ __launch_bounds__(512) void few_rows_kernel(ProductArgs p) {
       float o = v[e] + (p.bias ? (float)((const T*)p.bias)[c] : 0.0f);
       o = activated<std::is_same<T, float>::value>(o, p.act);
       if (p.residual) o += (float)((const T*)p.residual)[row * p.ldr + c];
-      ((T*)p.out)[row * p.ldo + c] = (T)o;
+      ((T*)p.out)[row * p.ldo + c] = rounded<T>(o);
     }
   }
 }

@@ -141,3 +141,33 @@ def test_infinities_through_an_activation_are_torchs(rows, outer, dtype):
             y = ops.op_linear(x, leaf, None, act).detach()
             assert torch.equal(y[others], ops.op_linear(plain, leaf, None, act).detach()[others])
             assert torch.equal(y[7].isnan(), want.isnan()) and torch.equal(y[7].isposinf(), want.isposinf())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,inner,outer", [(3, 40, 33), (40, 264, 520), (200, 72, 264), (700, 72, 2057), (4100, 72, 4104)])
+def test_results_do_not_depend_on_addresses(rows, inner, outer, dtype):
+    """Biases, a norm's weights, residuals and gradients that begin at any element of a larger tensor, or take every second one."""
+    x, w = normal(rows, inner, dtype=dtype), normal(outer, inner, dtype=dtype, seed=1, scale=0.1)
+    room = normal(2 * outer + 2 * inner + 16, dtype=dtype, seed=4)
+    wide = normal(rows, max(inner, outer) + 16, dtype=dtype, seed=2)
+    copy = lambda t: t.clone(memory_format=torch.contiguous_format)  # noqa: E731
+    for first, step in ((1, 1), (3, 1), (6, 1), (2, 2)):
+        b, nw = room[first:first + step * outer:step], room[first + 1:first + 1 + step * inner:step]
+        r = dy = wide[:, first:first + outer]
+        for act in (None, "gelu"):
+            pair = []
+            for args in ((b, r, dy), map(copy, (b, r, dy))):
+                bias, residual, g = args
+                leaves = [x.clone().requires_grad_(), w.clone().requires_grad_(), bias.detach().requires_grad_()]
+                y = ops.op_linear(*leaves, act, residual)
+                with torch.no_grad():
+                    pair.append([y.detach(), ops.op_linear(x, w, bias, act), ops.op_linear(x, w, bias, act, residual)])
+                pair[-1] += torch.autograd.grad(y, leaves, g)
+            assert all(torch.equal(a, c) for a, c in zip(*pair)), (first, step, act)
+        pair = []
+        n = wide[:, first:first + inner]
+        for args in ((n, nw, b[:1].expand(inner), n), map(copy, (n, nw, b[:1].expand(inner), n))):
+            leaves = [t.detach().requires_grad_() for t in args]
+            y = ops.op_layer_norm(*leaves[:3])
+            pair.append([y.detach()] + list(torch.autograd.grad(y, leaves[:3], leaves[3].detach())))
+        assert all(torch.equal(a, c) for a, c in zip(*pair)), (first, step)
