@@ -386,3 +386,32 @@ def test_a_weight_that_is_computed_is_computed_once_a_call(kind):
     y = layer(x)
     assert len(calls) == 1
     assert torch.equal(y, (layers.op_linear if kind[0] is nn.Linear else layers.op_layer_norm)(x, 2 * own.weight, own.bias))
+
+
+def test_a_step_captured_under_autocast_sees_the_weights_as_they_are_at_replay():
+    x, dy = normal(300, 72), normal(300, 72, dtype=torch.bfloat16, seed=1)
+    state = [1 + normal(72, scale=0.1), normal(72, seed=2), normal(200, 72, scale=0.1), normal(200, seed=3), normal(72, 200, seed=4, scale=0.1), normal(72, seed=5)]
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in [x] + state]
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            h = layers.op_layer_norm(*leaves[:3])
+            y = layers.op_linear(layers.op_linear(h, *leaves[3:5], "gelu"), *leaves[5:])
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for rep in range(4):
+        for n, p in enumerate(state):
+            p.add_(normal(*p.shape, seed=100 * rep + n, scale=0.05))
+        x.copy_(normal(300, 72, seed=7 + rep))
+        graph.replay()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), rep
+        torch.cuda.synchronize()
