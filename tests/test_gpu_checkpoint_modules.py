@@ -1,5 +1,5 @@
-"""A model's layers on 8-bit checkpoints where torch's own would be called in other ways than a plain training step: autocast under the
-Controller's hooks."""
+"""The layers on 8-bit checkpoints where they are called in other ways than a plain training step: autocast, the Controller's and other hooks for
+saved tensors, transforms, traces and modes, recomputation, several threads."""
 import copy
 import threading
 import time
@@ -415,3 +415,37 @@ def test_a_step_captured_under_autocast_sees_the_weights_as_they_are_at_replay()
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), rep
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_layers_give_the_same_gradients(reentrant):
+    """torch's recomputation in the backward pass, which saves through hooks of its own and stops the forward pass halfway, by an exception."""
+    from torch.utils.checkpoint import checkpoint
+    model = nn.Sequential(*(nn.Sequential(nn.LayerNorm(64), nn.Linear(64, 200), nn.Linear(200, 64)) for _ in range(3))).cuda()
+    x, dy = normal(70, 64).requires_grad_(), normal(70, 64, seed=1)
+    config.checkpoint_layers, config.auto_prec = True, False
+    leaves, seen = [x] + list(model.parameters()), []
+
+    def grads(run, hooked=False):
+        for t in leaves:
+            t.grad = None
+        if hooked:
+            with Controller(model) as controller:
+                run(x).backward(dy)
+            seen.append(controller.quantizer.tid)
+        else:
+            changed = layers.attach(model)
+            run(x).backward(dy)
+            layers.detach(changed)
+        return [t.grad for t in leaves]
+
+    def recomputed(h):
+        for part in model:
+            h = checkpoint(part, h, use_reentrant=reentrant)
+        return h
+
+    want = grads(model)
+    assert all(torch.equal(a, b) for a, b in zip(grads(recomputed), want))
+    # of what is saved only the parts' inputs, which recomputation keeps, are for the Controller's hooks to compress
+    grads(recomputed, True)
+    assert seen == [3]
