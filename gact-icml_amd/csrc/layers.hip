@@ -4,10 +4,11 @@
 // A checkpoint of a matrix of T holds every row in groups of 256 columns, the last one shorter.  Per group: the minimum and a scale,
 // both float, scale = float(255 / (double(max - min) + 2e-6)); per value: code = rint(max(fma(x - min, scale, 0.5) - 0.5, 0)).
 // That is the 8-bit code of gact_quantize on the values widened to float, rounded to nearest (GACT_NOISE_CONST).
-// (A NaN: code 0, and left out of minimum and maximum, as there.)  A code stands for code / scale + min, computed as fma(code, 1 / scale, min): one division per group and not one per value, which
+// (A NaN: code 0, and left out of minimum and maximum, as there.)
+// A code stands for code / scale + min, computed as fma(code, 1 / scale, min): one division per group and not one per value, which
 // differs from the quotient by a rounding of float.
 //
-// Compiled with -ffp-contract=off: every operation is the one it spells.
+// Compiled with -ffp-contract=off: every operation is the one it spells (but for roundings to a half, see rounded()).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
