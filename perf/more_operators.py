@@ -1,0 +1,485 @@
+"""Operators that a training step of a transformer needs beside the layers on 8-bit checkpoints: attention whose backward pass recomputes
+the probabilities, its relative position bias by buckets, and an AdamW step over many tensors with states in 8 or 32 bits.
+
+Each case is one pass through the public entry points of gact.ops.  `run` computes it either with elementary torch operations
+in 32 bits (`own` false) or with the framework's operators (`own` true); `exact` has the same values from the definitions in
+64 bits.  Run from the root of the repository.
+
+Attention: query [batch, heads, queries, width], key and value [batch, key heads, keys, width], heads a multiple of the key heads, each of
+which is shared by as many neighbouring heads.  A mask [batch, keys] says which keys are there; causal hides the keys behind
+i + keys - queries from query i; a query that nothing is left for gets zeros.  The bias has a value for each head and distance, at
+j - i + queries - 1, of which distance zero (a query and its own key) is number keys - 1.
+
+Buckets of distances (key - query): half of the buckets for keys behind the query, half for those at it and before; of each half the first
+half holds one distance each, the others reach up to max_distance in equal steps of the logarithm, and whatever lies further is in the last
+one.  One-directional: all buckets for keys before the query, those behind it are in the first one.
+
+States in 8 bits hold a tensor's elements in groups of 256, the last of them shorter, each group with the largest magnitude of either state.
+A code c of the first moment stands for c |c| / 127^2 of the largest, one of the second for c^4 / 255^4 of it; a value gets the code it is
+nearest to on the scale of the root, and no value above zero the code 0.  The roundings of the codes are part of the format.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+_DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+_BYTES = {"f32": 4, "f16": 2, "bf16": 2}
+_GROUP = 256
+_BETAS, _EPS, _DECAY, _LR = (0.9, 0.999), 1e-8, 0.01, 1e-3
+_MOST_PAIRS = 2 * 32 * 4096 * 4096 // 2         # heads x queries x keys of the largest listed case (half of them hidden)
+_MOST_ELEMENTS = 1 << 26
+
+
+def _attention(name, batch, heads, kv_heads, queries, keys, width, dtype, train=False, causal=False, mask=False, buckets=0):
+    return {"name": name, "kind": "attention", "batch": batch, "heads": heads, "kv_heads": kv_heads, "queries": queries, "keys": keys,
+            "width": width, "dtype": dtype, "train": train, "causal": causal, "mask": mask, "buckets": buckets}
+
+
+def _bias(name, heads, queries, keys, buckets, both, dtype):
+    return {"name": name, "kind": "bias", "heads": heads, "queries": queries, "keys": keys, "buckets": buckets, "both": both, "dtype": dtype}
+
+
+def _adamw(name, model, layers, width, bits, dtype, step):
+    return {"name": name, "kind": "adamw", "model": model, "layers": layers, "width": width, "bits": bits, "dtype": dtype, "step": step}
+
+
+def listed():
+    return [
+        # the next token of each of 24 sequences of different lengths: latency
+        _attention("token_bf16", 24, 16, 16, 1, 517, 64, "bf16", mask=True),
+        # one token behind a long context, four heads to a key head: the keys and values have to be read, and little else
+        _attention("token_long_f16", 1, 32, 8, 1, 65537, 128, "f16"),
+        # two long prompts
+        _attention("prompt_bf16", 2, 32, 8, 4096, 4096, 128, "bf16", causal=True),
+        # a training step of a BERT-large layer, batch 32 x 512 tokens, padded
+        _attention("train_bf16", 32, 16, 16, 512, 512, 64, "bf16", train=True, mask=True),
+        # the first stage of a Swin-Tiny-like model at batch 128: windows of 49 tokens, in single precision
+        _attention("train_windows_f32", 8192, 3, 3, 49, 49, 32, "f32", train=True),
+        # a training step with a learned position bias, at a length that no tile divides
+        _attention("train_bias_f16", 8, 16, 16, 1000, 1000, 64, "f16", train=True, buckets=32),
+        # a few images' tokens that look back over a longer context, shared key heads, a width that is no power of two
+        _attention("train_odd_f16", 3, 6, 2, 197, 771, 72, "f16", train=True, causal=True),
+        # the bias alone and its gradient: a small model's, and a long context's
+        _bias("bias_few_f32", 12, 197, 197, 32, True, "f32"),
+        _bias("bias_long_bf16", 64, 16384, 16384, 32, False, "bf16"),
+        # an optimizer's step of a BERT-large model's 24 layers, states in 8 bits; of six of them in 16-bit weights with float states; and of the
+        # biases and norms that a fine-tuning step of a few layers trains
+        _adamw("adamw8_large_f32", "layers", 24, 1024, 8, "f32", 1000),
+        _adamw("adamw32_bf16", "layers", 6, 1024, 32, "bf16", 7),
+        _adamw("adamw8_few_f16", "vectors", 3, 771, 8, "f16", 1),
+    ]
+
+
+def _spread(rng, low, high):
+    """A size whose logarithm is uniform; one in three as it comes, the others whole eighths or whole groups of 64."""
+    n = int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+    step = rng.choice((1, 8, 64))
+    return max(low, n // step * step)
+
+
+def draw(rng):
+    kind = rng.choice(("token", "prompt", "train", "train", "train", "bias", "adamw", "adamw"))
+    dtype = rng.choice(("bf16", "bf16", "f16", "f16", "f32"))
+    if kind == "bias":
+        case = _bias("", _spread(rng, 1, 64), _spread(rng, 1, 16384), _spread(rng, 1, 16384), 2 * _spread(rng, 4, 64), rng.random() < 0.5, dtype)
+    elif kind == "adamw":
+        model = rng.choice(("layers", "vectors", "mixed"))
+        width = _spread(rng, 16, 1024)
+        elements = 12 * width * width if model == "layers" else 13 * width
+        layers = _spread(rng, 1, max(1, min(40, _MOST_ELEMENTS // elements)))
+        case = _adamw("", model, layers, width, rng.choice((8, 8, 32)), dtype, rng.choice((1, 2, 100, 100000)))
+    else:
+        kv_heads = _spread(rng, 1, 16)
+        heads = kv_heads * rng.choice((1, 1, 1, 2, 4))
+        # whole 16-byte pieces mostly, and a few widths that are none
+        width = rng.choice((32, 64, 64, 64, 80, 96, 128, 128, 8 * rng.randint(1, 16), rng.randint(1, 128)))
+        # single precision runs at a sixteenth of the rate: smaller ones; a training step does three and a half times the work
+        most = _MOST_PAIRS // (16 if dtype == "f32" else 1) // (4 if kind == "train" else 1)
+        if kind == "token":
+            queries = rng.choice((1, 1, 1, 2, 5))
+            keys = _spread(rng, 16, 65536)
+            most = min(most, 1 << 22)
+        else:
+            queries = _spread(rng, 4, 4096)
+            keys = rng.choice((queries, queries, _spread(rng, 4, 4096)))
+        batch = _spread(rng, 1, max(1, min(512, most // (heads * queries * keys))))
+        case = _attention("", batch, heads, kv_heads, queries, keys, width, dtype, kind == "train", rng.random() < 0.4, rng.random() < 0.4,
+                          rng.choice((0, 0, 32, 64)))
+    del case["name"]
+    return case
+
+
+def _shapes(case):
+    """The parameters of the case's model."""
+    w, shapes = case["width"], []
+    for n in range(case["layers"]):
+        vectors = [(w,)] * 4 + [(w,), (4 * w,), (w,), (w,), (w,)]
+        if case["model"] == "layers" or (case["model"] == "mixed" and n % 2):
+            shapes += [(w, w)] * 4 + [(4 * w, w), (w, 4 * w)]
+        shapes += vectors
+        if case["model"] == "mixed":
+            shapes += [(n + 1,), (w, 3, n % 3 + 1)]
+    return shapes
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dtype = _DTYPES[case["dtype"]]
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=gen, device="cuda")
+
+    state = {"case": case}
+    if case["kind"] == "adamw":
+        _prepare_adamw(case, state, randn, dtype)
+        return state
+    if case["kind"] == "bias":
+        state["table"] = randn(case["buckets"], case["heads"]).to(dtype).requires_grad_()
+        state["dy"] = 0.02 * randn(case["heads"], case["queries"] + case["keys"] - 1)
+        return state
+    b, h, g, m, n, w = (case[k] for k in ("batch", "heads", "kv_heads", "queries", "keys", "width"))
+    # as a model has them: the heads of a token side by side, in the results of three projections; a few channels larger than the others
+    size = 1 + 2 * (torch.rand(w, generator=gen, device="cuda") < 0.05)
+    state["q"] = (randn(b, m, h, w) * size).to(dtype).transpose(1, 2)
+    state["k"] = (randn(b, n, g, w) * size).to(dtype).transpose(1, 2)
+    state["v"] = randn(b, n, g, w).to(dtype).transpose(1, 2)
+    if case["mask"]:
+        length = torch.randint(max(1, n // 4), n + 1, (b,), generator=gen, device="cuda")
+        state["mask"] = torch.arange(n, device="cuda")[None, :] < length[:, None]
+    if case["buckets"]:
+        state["table"] = randn(case["buckets"], h).to(dtype)
+    if case["train"]:
+        state["dy"] = (0.02 * randn(b, m, h, w)).to(dtype).transpose(1, 2)
+        for name in ("q", "k", "v", "table"):
+            if name in state:
+                state[name] = state[name].requires_grad_()
+    return state
+
+
+def _prepare_adamw(case, state, randn, dtype):
+    shapes, step = _shapes(case), case["step"]
+    # every tensor has a place of whole groups in one buffer, as gradients that are reduced together have
+    sizes = [math.prod(s) for s in shapes]
+    places = [0]
+    for n in sizes:
+        places.append(places[-1] + -(-n // _GROUP) * _GROUP)
+    total = places[-1]
+    # layers and channels differ in size by orders of magnitude
+    size = torch.tensor([10.0 ** (-3 - i % 4) for i in range(len(shapes))], device="cuda")
+    groups = torch.tensor([-(-n // _GROUP) for n in sizes], device="cuda")
+    there = torch.arange(total, device="cuda") - torch.tensor(places[:-1], device="cuda").repeat_interleave(groups * _GROUP)
+    there = there < torch.tensor(sizes, device="cuda").repeat_interleave(groups * _GROUP)
+    size = size.repeat_interleave(groups).mul_(randn(total // _GROUP).abs()).repeat_interleave(_GROUP).mul_(there)
+    flat = {"p": (0.05 * randn(total) * there).to(dtype), "g": (randn(total) * size).to(dtype)}
+    flat["m"] = randn(total) * size * (0.0 if step == 1 else 0.3)
+    flat["v"] = (0.2 + randn(total).square()) * size.square() * (0.0 if step == 1 else min(1.0, step * 1e-3))
+    if case["bits"] == 8:
+        flat["m"], flat["v"], flat["most"] = _encode(flat["m"], flat["v"])
+    state["flat"] = flat
+
+    def views(t):
+        return [t[o:o + n].view(s) for o, n, s in zip(places, sizes, shapes)]
+
+    state["params"], state["grads"], moments = views(flat["p"]), views(flat["g"]), (views(flat["m"]), views(flat["v"]))
+    scales = [None] * len(shapes)
+    if case["bits"] == 8:
+        scales = [flat["most"][o // _GROUP:-(-(o + n) // _GROUP)] for o, n in zip(places, sizes)]
+    state["states"] = list(zip(*moments, scales))
+
+
+# ---- states in 8 bits ----
+def _encode(m, v):
+    """float32 values of whole groups -> codes of either, and the largest magnitudes [groups, 2]."""
+    gm, gv = m.view(-1, _GROUP), v.view(-1, _GROUP)
+    most = torch.stack([gm.abs().amax(1), gv.amax(1)], 1)
+    # a group that has next to nothing is one of zeros
+    most = torch.where(most < torch.tensor([1e-30, 1e-28], device=m.device), torch.zeros_like(most), most)
+    inverse = (torch.tensor([127.0 ** 2, 255.0 ** 4], dtype=torch.float64, device=m.device) / most.double()).float()
+    inverse = torch.where(most > 0, inverse, torch.zeros_like(most))
+    # next to a border the root is taken in 64 bits
+    c = torch.floor(torch.sqrt((gm.abs() * inverse[:, :1]).double()) + 0.5) * torch.sign(gm)
+    d = torch.floor(torch.sqrt(torch.sqrt((gv * inverse[:, 1:]).double())) + 0.5)
+    d = torch.where((gv > 0) & (most[:, 1:] > 0), d.clamp(min=1), d)
+    return c.view(-1).to(torch.int8), d.view(-1).to(torch.uint8), most
+
+
+def _decode(c, d, most):
+    """Codes -> float32 values."""
+    unit = (most.double() / torch.tensor([127.0 ** 2, 255.0 ** 4], dtype=torch.float64, device=most.device)).float()
+    c, square = c.float().view(-1, _GROUP), d.float().view(-1, _GROUP).square()
+    return (c * c.abs() * unit[:, :1]).view(-1), (square * square * unit[:, 1:]).view(-1)
+
+
+# ---- the plain form: elementary operations in 32 bits ----
+def _plain_buckets(case, device):
+    """The bucket of every distance, in the bias's order."""
+    m, n, buckets = case["queries"], case["keys"], case["buckets"]
+    d = torch.arange(m + n - 1, device=device) - (n - 1)
+    both = case.get("both", not case.get("causal"))
+    per = buckets // 2 if both else buckets
+    away = d.abs() if both else (-d).clamp(min=0)
+    near = per // 2
+    # whole powers of the ratio fall on a border: 64 bits, and a little more than the quotient
+    far = near + (torch.log(away.clamp(min=1).double() / near) / math.log(128 / near) * (per - near) + 1e-9).floor().long()
+    at = torch.where(away < near, away, far.clamp(max=per - 1))
+    return at + per * (d > 0) if both else at
+
+
+def _by_bucket(along, at, buckets):
+    """[heads, distances] -> sums [buckets, heads]."""
+    return (at[None, :] == torch.arange(buckets, device=at.device)[:, None]).to(along.dtype) @ along.t().contiguous()
+
+
+def _plain_bias(state):
+    case, table = state["case"], state["table"].detach()
+    at = _plain_buckets(case, table.device)
+    return {"y": table.float()[at].t().contiguous(), "dtable": _by_bucket(state["dy"].double(), at, case["buckets"]).to(table.dtype)}
+
+
+def _seen(state, device):
+    """Which keys a query sees: [batch or 1, 1, queries or 1, keys], or None."""
+    case, seen = state["case"], None
+    if case["mask"]:
+        seen = state["mask"][:, None, None, :]
+    if case["causal"]:
+        m, n = case["queries"], case["keys"]
+        before = torch.arange(n, device=device)[None, :] <= torch.arange(m, device=device)[:, None] + (n - m)
+        seen = before if seen is None else seen & before
+    return seen
+
+
+def _plain_attention(state):
+    case = state["case"]
+    b, h, g, m, n, w = (case[k] for k in ("batch", "heads", "kv_heads", "queries", "keys", "width"))
+    dtype, r, scale = state["q"].dtype, h // g, 1 / math.sqrt(w)
+    # the heads that share a key head as rows of one product
+    q = state["q"].detach().float().reshape(b, g, r * m, w)
+    k, v = (state[name].detach().float().contiguous() for name in ("k", "v"))
+    s = (q @ k.transpose(2, 3).contiguous()).mul_(scale).view(b, h, m, n)
+    if case["buckets"]:
+        at = _plain_buckets(case, s.device)
+        place = torch.arange(n, device=s.device)[None, :] - torch.arange(m, device=s.device)[:, None] + (m - 1)
+        s += state["table"].detach().float()[at].t()[:, place]
+    seen = _seen(state, s.device)
+    if seen is not None:
+        s.masked_fill_(~seen, -math.inf)
+    most = s.amax(3, keepdim=True)
+    p = torch.exp(s.sub_(torch.where(most == -math.inf, torch.zeros_like(most), most)))
+    total = p.sum(3, keepdim=True)
+    p /= torch.where(total == 0, torch.ones_like(total), total)
+    rows = p.view(b, g, r * m, n)
+    y = (rows @ v).view(b, h, m, w)
+    out = {"y": y.to(dtype)}
+    if not case["train"]:
+        return out
+    dy = state["dy"].float().reshape(b, g, r * m, w)
+    out["dv"] = (rows.transpose(2, 3).contiguous() @ dy).to(dtype)
+    ds = (dy @ v.transpose(2, 3).contiguous()).view(b, h, m, n)
+    ds -= (dy.view(b, h, m, w) * y).sum(3, keepdim=True)
+    ds *= p
+    if case["buckets"]:
+        # the diagonals one below the other: query i, from the last one on, begins i places further right
+        turned = torch.nn.functional.pad(ds.sum(0, dtype=torch.float64).flip(1), (0, m)).view(h, -1)
+        along = turned[:, :m * (m + n - 1)].reshape(h, m, m + n - 1).sum(1)
+        out["dtable"] = _by_bucket(along, at, case["buckets"]).to(dtype)
+    ds = ds.view(b, g, r * m, n)
+    out["dq"] = ((ds @ k) * scale).view(b, h, m, w).to(dtype)
+    out["dk"] = ((ds.transpose(2, 3).contiguous() @ q) * scale).to(dtype)
+    return out
+
+
+def _rounded(flat):
+    """The float moments after the step: products and sums are rounded together, which 64 bits hold but for the last bits."""
+    g = flat["g"].float()
+    m, v = _decode(flat["m"], flat["v"], flat["most"]) if "most" in flat else (flat["m"], flat["v"])
+    beta, rest = (torch.tensor([f(b) for b in _BETAS], dtype=torch.float32).tolist() for f in (float, lambda b: 1 - b))
+    return (m.double() * beta[0] + (g * rest[0]).double()).float(), (v.double() * beta[1] + (g * g * rest[1]).double()).float()
+
+
+def _plain_adamw(state):
+    flat, step = state["flat"], state["case"]["step"]
+    first, second = (1 - beta ** step for beta in _BETAS)
+    m, v = _rounded(flat)
+    p = flat["p"].float() * (1 - _LR * _DECAY) - (_LR / first) * (m / (torch.sqrt(v) / math.sqrt(second) + _EPS))
+    # in place, as an optimizer's step is
+    flat["p"].copy_(p)
+    kept = (m, v)
+    if "most" in flat:
+        kept = _encode(m, v)
+        flat["most"].copy_(kept[2])
+    flat["m"].copy_(kept[0])
+    flat["v"].copy_(kept[1])
+    m, v = _decode(*kept) if "most" in flat else (flat["m"], flat["v"])
+    return {"params": flat["p"], "exp_avg": m, "exp_avg_sq": v}
+
+
+# ---- the framework's operators ----
+def _ops():
+    package = os.path.abspath("gact-icml_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from gact import ops
+
+    return ops
+
+
+def _own(state):
+    ops, case = _ops(), state["case"]
+    if case["kind"] == "adamw":
+        flat = state["flat"]
+        ops.op_adamw(state["params"], state["grads"], state["states"], case["step"], _LR, _BETAS, _EPS, _DECAY)
+        m, v = flat["m"], flat["v"]
+        if case["bits"] == 8:       # what the codes stand for, as a program that saves or inspects them asks for it
+            m, v = ops.op_adamw_values([(m, v, flat["most"])])
+        return {"params": flat["p"], "exp_avg": m, "exp_avg_sq": v}
+    if case["kind"] == "bias":
+        y = ops.op_position_bias(state["table"], case["queries"], case["keys"], bidirectional=case["both"])
+        return {"y": y.detach(), "dtable": torch.autograd.grad(y, state["table"], state["dy"])[0]}
+
+    def attend():
+        bias = None
+        if case["buckets"]:
+            bias = ops.op_position_bias(state["table"], case["queries"], case["keys"], bidirectional=not case["causal"])
+        return ops.op_attention(state["q"], state["k"], state["v"], bias, state.get("mask"), case["causal"])
+
+    if not case["train"]:
+        with torch.no_grad():
+            return {"y": attend()}
+    y = attend()
+    names = [n for n in ("v", "table", "q", "k") if n in state]
+    grads = torch.autograd.grad(y, [state[n] for n in names], state["dy"])
+    return {"y": y.detach(), **{"d" + n: g for n, g in zip(names, grads)}}
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return {"attention": _plain_attention, "bias": _plain_bias, "adamw": _plain_adamw}[state["case"]["kind"]](state)
+
+
+def _elements(case):
+    return sum(math.prod(s) for s in _shapes(case))
+
+
+def work(case):
+    """What a pass cannot do without: every input read and every output written once (the expanded 8-bit states are outputs of their own), the
+    products of the pairs that are not hidden by causal: two forward, five backward."""
+    if case["kind"] == "adamw":
+        n, t = _elements(case), _BYTES[case["dtype"]]
+        return {"bytes": n * (3 * t + (4 + 2 + 8 if case["bits"] == 8 else 16)), "flops": 20 * n}
+    if case["kind"] == "bias":
+        size = case["heads"] * (case["queries"] + case["keys"] - 1)
+        return {"bytes": 8 * size + 2 * _BYTES[case["dtype"]] * case["buckets"] * case["heads"], "flops": size}
+    b, h, g, m, n, w = (case[k] for k in ("batch", "heads", "kv_heads", "queries", "keys", "width"))
+    pairs = m * n
+    if case["causal"]:
+        pairs = sum(min(n, max(0, i + n - m + 1)) for i in range(m))
+    size = 2 * h * m * w + 2 * g * n * w
+    if case["train"]:
+        size += 3 * h * m * w + 4 * g * n * w
+    return {"bytes": _BYTES[case["dtype"]] * b * size, "flops": (14 if case["train"] else 4) * b * h * pairs * w}
+
+
+# ---- the definitions in 64 bits ----
+def _exact_bucket(distance, buckets, both):
+    if both and distance > 0:
+        return buckets // 2 + _exact_bucket(-distance, buckets // 2, False)
+    per, away = (buckets // 2, abs(distance)) if both else (buckets, max(0, -distance))
+    near = per // 2
+    if away < near:
+        return away
+    # the largest k with (away / near)^steps >= (128 / near)^k, in whole numbers
+    steps, k = per - near, 0
+    while k + 1 < steps and away ** steps * near ** (k + 1) >= 128 ** (k + 1) * near ** steps:
+        k += 1
+    return near + k
+
+
+def _exact_index(case):
+    both = case.get("both", not case.get("causal"))
+    # every distance beyond the furthest border is in its side's last bucket
+    known = {}
+    at = []
+    for t in range(case["queries"] + case["keys"] - 1):
+        d = max(-129, min(129, t - (case["keys"] - 1)))
+        if d not in known:
+            known[d] = _exact_bucket(d, case["buckets"], both)
+        at.append(known[d])
+    return torch.tensor(at, device="cuda")
+
+
+def _exact_attention(case, state):
+    b, h, g, m, n, w = (case[k] for k in ("batch", "heads", "kv_heads", "queries", "keys", "width"))
+    if b * h * m * n * w * (14 if case["train"] else 4) > 4e13:
+        return None
+    names = ("y",) + (("dv", "dq", "dk") if case["train"] else ())
+    r, parts = h // g, {name: [] for name in names}
+    index = _exact_index(case) if case["buckets"] else None
+    along = torch.zeros(h, m + n - 1, dtype=torch.float64, device="cuda")
+    i, j = torch.arange(m, device="cuda")[:, None], torch.arange(n, device="cuda")[None, :]
+    most = max(1, (1 << 28) // (h * m * n))
+    for first in range(0, b, most):       # a few batch entries at a time
+        last = min(b, first + most)
+        q = state["q"][first:last].double()
+        k, v = (state[name][first:last].double().repeat_interleave(r, 1) for name in ("k", "v"))
+        s = torch.matmul(q, k.mT.contiguous()) / math.sqrt(w)
+        if index is not None:
+            s = s + state["table"].double()[index].t()[:, j - i + m - 1]
+        hidden = torch.zeros(last - first, 1, m, n, dtype=torch.bool, device="cuda")
+        if case["mask"]:
+            hidden |= ~state["mask"][first:last, None, None, :]
+        if case["causal"]:
+            hidden |= j - i > n - m
+        s = s.masked_fill(hidden, -math.inf)
+        p = torch.softmax(s, 3).nan_to_num(0.0)
+        del s
+        y = torch.matmul(p, v)
+        parts["y"].append(y)
+        if case["train"]:
+            dy = state["dy"][first:last].double()
+            dp = torch.matmul(dy, v.mT.contiguous())
+            ds = p * (dp - (p * dp).sum(3, keepdim=True))
+            del dp
+            if index is not None:
+                along.index_add_(1, (j - i + m - 1).reshape(-1), ds.sum(0).reshape(h, -1))
+            parts["dq"].append(torch.matmul(ds, k) / math.sqrt(w))
+            dk, dv = torch.matmul(ds.mT.contiguous(), q) / math.sqrt(w), torch.matmul(p.mT.contiguous(), dy)
+            parts["dk"].append(dk.view(-1, g, r, n, w).sum(2))
+            parts["dv"].append(dv.view(-1, g, r, n, w).sum(2))
+    out = {name: torch.cat(parts[name]) for name in names}
+    if case["train"] and index is not None:
+        out["dtable"] = torch.zeros(case["buckets"], h, dtype=torch.float64, device="cuda").index_add_(0, index, along.t())
+    return out if not case["train"] else {name: out[name] for name in ("y", "dv", "dtable", "dq", "dk") if name in out}
+
+
+def _exact_adamw(case, flat):
+    (one, two), step = _BETAS, case["step"]
+    p, g, m, v = (flat[name].double() for name in ("p", "g", "m", "v"))
+
+    def values(c, d, most):
+        c, d, most = c.double().view(-1, _GROUP), d.double().view(-1, _GROUP), most.double()
+        return (c * c.abs() * most[:, :1] / 127.0 ** 2).view(-1), (d ** 4 * most[:, 1:] / 255.0 ** 4).view(-1)
+
+    if case["bits"] == 8:
+        m, v = values(m, v, flat["most"])
+    m, v = one * m + (1 - one) * g, two * v + (1 - two) * g * g
+    p = p * (1 - _LR * _DECAY) - _LR * (m / (1 - one ** step)) / ((v / (1 - two ** step)).sqrt() + _EPS)
+    if case["bits"] == 8:
+        # which code a value gets is the format's own, with its roundings
+        m, v = values(*_encode(*_rounded(flat)))
+    return {"params": p, "exp_avg": m, "exp_avg_sq": v}
+
+
+def exact(case, seed):
+    state = {n: v.detach() if isinstance(v, torch.Tensor) else v for n, v in prepare(case, seed).items()}
+    if case["kind"] == "adamw":
+        return _exact_adamw(case, state["flat"])
+    if case["kind"] == "bias":
+        at = _exact_index(case)
+        sums = torch.zeros(case["buckets"], case["heads"], dtype=torch.float64, device="cuda")
+        return {"y": state["table"].double()[at].t(), "dtable": sums.index_add_(0, at, state["dy"].double().t())}
+    return _exact_attention(case, state)
