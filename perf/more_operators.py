@@ -29,6 +29,7 @@ own = False
 _DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 _BYTES = {"f32": 4, "f16": 2, "bf16": 2}
 _GROUP = 256
+_UNITS = (127.0 ** 2, 4228250624.0)      # of the codes' powers; 255^4 is no float, and this the nearest one
 _BETAS, _EPS, _DECAY, _LR = (0.9, 0.999), 1e-8, 0.01, 1e-3
 _MOST_PAIRS = 2 * 32 * 4096 * 4096 // 2         # heads x queries x keys of the largest listed case (half of them hidden)
 _MOST_ELEMENTS = 1 << 26
@@ -198,7 +199,7 @@ def _encode(m, v):
     most = torch.stack([gm.abs().amax(1), gv.amax(1)], 1)
     # a group that has next to nothing is one of zeros
     most = torch.where(most < torch.tensor([1e-30, 1e-28], device=m.device), torch.zeros_like(most), most)
-    inverse = (torch.tensor([127.0 ** 2, 255.0 ** 4], dtype=torch.float64, device=m.device) / most.double()).float()
+    inverse = (torch.tensor(_UNITS, dtype=torch.float64, device=m.device) / most.double()).float()
     inverse = torch.where(most > 0, inverse, torch.zeros_like(most))
     # next to a border the root is taken in 64 bits
     c = torch.floor(torch.sqrt((gm.abs() * inverse[:, :1]).double()) + 0.5) * torch.sign(gm)
@@ -209,7 +210,7 @@ def _encode(m, v):
 
 def _decode(c, d, most):
     """Codes -> float32 values."""
-    unit = (most.double() / torch.tensor([127.0 ** 2, 255.0 ** 4], dtype=torch.float64, device=most.device)).float()
+    unit = (most.double() / torch.tensor(_UNITS, dtype=torch.float64, device=most.device)).float()
     c, square = c.float().view(-1, _GROUP), d.float().view(-1, _GROUP).square()
     return (c * c.abs() * unit[:, :1]).view(-1), (square * square * unit[:, 1:]).view(-1)
 
