@@ -19,15 +19,24 @@ ROOT = os.path.dirname(HERE)
 SRC = os.path.join(HERE, "csrc", "gact_hip.hip")
 LAYERS_SRC = os.path.join(HERE, "csrc", "layers.hip")         # linked into the same library
 LAYERS_HDR = os.path.join(HERE, "csrc", "layer_cuts.h")
+DEVICE_HDR = os.path.join(HERE, "csrc", "device.h")
+ATTENTION_SRCS = [os.path.join(HERE, "csrc", n) for n in ("attention.hip", "attention_f32.hip", "attention_f16.hip", "attention_bf16.hip")]
+ATTENTION_HDR = os.path.join(HERE, "csrc", "attention.h")
+ADAMW_SRC = os.path.join(HERE, "csrc", "adamw.hip")
 PROBE_SRC = os.path.join(HERE, "csrc", "stream_probe.hip")   # compute-free traffic probes for bench.py
 HDR = os.path.join(ROOT, "include", "gact_hip.h")
 OUT_DIR = os.path.join(HERE, "gact", "lib")
 OUT = os.path.join(OUT_DIR, "libgact_hip.so")
 TORCH_SRC = os.path.join(HERE, "csrc", "torch_ops.cpp")
 TORCH_LAYERS_SRC = os.path.join(HERE, "csrc", "torch_layers.cpp")
-TORCH_HDR = os.path.join(HERE, "csrc", "torch_layers.h")
+TORCH_ATTENTION_SRC = os.path.join(HERE, "csrc", "torch_attention.cpp")
+TORCH_ADAMW_SRC = os.path.join(HERE, "csrc", "torch_adamw.cpp")
+TORCH_HDRS = [os.path.join(HERE, "csrc", n) for n in ("torch_layers.h", "torch_common.h")]
 TORCH_OUT = os.path.join(OUT_DIR, "gact_torch.so")
 PROBE_OUT = os.path.join(OUT_DIR, "libgact_probe.so")
+# of libgact_hip.so and of gact_torch.so
+SOURCES = [SRC, LAYERS_SRC] + ATTENTION_SRCS + [ADAMW_SRC]
+TORCH_SRCS = [TORCH_SRC, TORCH_LAYERS_SRC, TORCH_ATTENTION_SRC, TORCH_ADAMW_SRC]
 
 HIPCC_FLAGS = [
     "-O3",
@@ -63,7 +72,7 @@ def up_to_date():
         if torch_mark() not in f.read():     # built for another torch
             return False
     t = min(os.path.getmtime(p) for p in built)
-    return all(os.path.getmtime(p) <= t for p in (SRC, LAYERS_SRC, LAYERS_HDR, PROBE_SRC, TORCH_SRC, TORCH_LAYERS_SRC, TORCH_HDR, HDR, os.path.abspath(__file__)))
+    return all(os.path.getmtime(p) <= t for p in SOURCES + TORCH_SRCS + TORCH_HDRS + [LAYERS_HDR, DEVICE_HDR, ATTENTION_HDR, PROBE_SRC, HDR, os.path.abspath(__file__)])
 
 
 def torch_mark():
@@ -87,7 +96,7 @@ def torch_command():
     for path in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", path]
     # libtorch.so itself stays out: it would pull in every library torch was built with
-    return cmd + ["-o", TORCH_OUT, TORCH_SRC, TORCH_LAYERS_SRC, "-L", OUT_DIR, "-l:libgact_hip.so", "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10",
+    return cmd + ["-o", TORCH_OUT] + TORCH_SRCS + ["-L", OUT_DIR, "-l:libgact_hip.so", "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10",
                   "-lc10_hip", "-Wl,-rpath,$ORIGIN"]
 
 
@@ -97,8 +106,8 @@ def build(force=False, extra=()):
     os.makedirs(OUT_DIR, exist_ok=True)
     include = ["-I", os.path.join(ROOT, "include")]
     with tempfile.TemporaryDirectory() as tmp:
-        objects = [os.path.join(tmp, "gact_hip.o"), os.path.join(tmp, "layers.o")]
-        jobs = [[hipcc()] + HIPCC_FLAGS + list(extra) + include + ["-c", "-o", o, src] for o, src in zip(objects, (SRC, LAYERS_SRC))]
+        objects = [os.path.join(tmp, os.path.basename(src) + ".o") for src in SOURCES]
+        jobs = [[hipcc()] + HIPCC_FLAGS + list(extra) + include + ["-c", "-o", o, src] for o, src in zip(objects, SOURCES)]
         jobs.append([hipcc()] + HIPCC_FLAGS + ["-shared", "-o", PROBE_OUT, PROBE_SRC])
         running = [(job, subprocess.Popen(job)) for job in jobs]       # side by side: each is one compiler on one core
         for job, process in running:

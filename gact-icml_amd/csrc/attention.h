@@ -1,0 +1,858 @@
+// Attention's kernels, for one element type: the three sources that compile them differ in it alone, and are built side by side.
+//
+//   s_ij = scale q_i.k_j + bias[j - i + queries - 1]      hidden: absent keys, and with `causal` keys behind i + keys - queries
+//   p_ij = exp(s_ij - L_i), L_i = log sum_j exp(s_ij)      o_i = sum_j p_ij v_j
+//   ds_ij = p_ij (do_i.v_j - do_i.o_i)                     dq_i = scale sum_j ds_ij k_j, dk_j = scale sum_i ds_ij q_i, dv_j = sum_i p_ij do_i
+//
+// Exponentials are of base 2: scores, biases and L are held multiplied by log2(e).  Probabilities and ds enter their products rounded to T, which is
+// what the matrix instructions of 16-bit types take; sums, maxima and L are floats.
+//
+// All kernels are built alike.  A wave owns 32 rows of one side (queries; keys in the kernel of dk and dv) and keeps them in registers as the matrix
+// instruction's columns; the other side passes by in tiles of rows that are in LDS, its rows being the instruction's rows.  A lane so has 16 of the 32
+// scores of one of its own rows, the lane 32 further on the others: a maximum or sum over the other side stays in the lane but for one exchange, and the
+// scores are in place as the second product's operand, whose depth is the tile's rows in whatever order - its other operand is read from the
+// tile through the transposing LDS read in the same order.  Neither scores nor probabilities leave the registers.
+#pragma once
+#include "device.h"
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// rows of [batch, head, row, width], strides in bytes
+struct Side {
+  const char* p;
+  int64_t batch, head, row;
+  __device__ __forceinline__ const char* at(int64_t b, int64_t h, int64_t r) const { return p + b * batch + h * head + r * row; }
+};
+
+struct AttentionArgs {
+  Side q, k, v, out, d_out, dq, dk, dv;
+  float* lse;                // [batch, heads, queries]; infinite for a query that sees nothing
+  float* delta;              // the same: do_i.o_i
+  int8_t* rest;              // [batch, queries, heads, width]: what rounding o to T has left out, see Rest; may be null
+  const float* bias;         // [heads, queries + keys - 1], times log2(e)
+  const uint8_t* mask;       // [batch, keys]
+  int64_t mask_stride;
+  float* along;              // sums of ds along the diagonals, of every 32 queries
+  int64_t along_stride;
+  int heads, kv_heads, group, queries, keys, width;
+  bool causal;
+  float scale, scale2;       // and times log2(e)
+  uint32_t tiles, blocks;    // of a head, and in all
+  int splits, per_split;     // keys of a split, whole blocks of 32
+  float* part;               // [tile, split][32, width rounded up]
+  float* part_stats;         // [tile, split][32, 2]
+  // keys that query i sees
+  __device__ __forceinline__ int seen(int i) const {
+    const int n = i + keys - queries + 1;
+    return !causal || n > keys ? keys : n;
+  }
+  __device__ __forceinline__ int8_t* rest_at(int b, int head, int query) const {
+    return rest ? rest + (((int64_t)b * queries + query) * heads + head) * width : nullptr;
+  }
+  __device__ __forceinline__ int distances() const { return queries + keys - 1; }
+};
+
+namespace {
+
+template <typename T>
+struct Matrix {
+  using Frag = std::conditional_t<std::is_same<T, bf16>::value, bf16x8, std::conditional_t<std::is_same<T, f16>::value, f16x8, f32x4>>;
+  // 16 bytes a lane and operand: 16 values of depth of 16-bit types, 8 floats
+  static __device__ __forceinline__ f32x16 run(Frag a, Frag b, f32x16 c) {
+    if constexpr (std::is_same<T, bf16>::value) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    if constexpr (std::is_same<T, f16>::value) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int t = 0; t < 4; t++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], b[t], c, 0, 0, 0);
+    }
+    return c;
+  }
+};
+// the row, within 32, of element e of a result: lanes 32 and up have the rows 4 further down
+constexpr int row_of(int e) { return 8 * (e >> 2) + (e & 3); }
+
+// Rows of DP values (the width rounded up to 32) in LDS, W bytes each.  A row's pieces of 16 bytes are permuted by turn() of its number: the 16 rows of
+// which the product's first operand takes a piece each, and the four rows of which the transposing read takes 64 bytes (of floats: the rows r and r + 4
+// whose 128 bytes go together), lie in different banks.
+template <typename T, int DP>
+struct Tile {
+  using Frag = typename Matrix<T>::Frag;
+  static constexpr int kEsz = (int)sizeof(T), kWide = DP * kEsz;
+  static constexpr int W = kWide <= 64 ? 64 : kWide <= 128 ? 128 : kWide <= 256 ? 256 : 512;
+  static constexpr int kRows = W <= 256 ? 64 : 32;
+  static constexpr int NC = kWide / 32, ND = DP / 32;
+  static constexpr __device__ __forceinline__ uint32_t turn(uint32_t r) {
+    const uint32_t a = r & 1, b = (r >> 1) & 1, c = (r >> 2) & 1, d = (r >> 3) & 1;
+    if (W == 64) return c | d << 1;
+    if (W == 128) return b << 2 | c << 1 | d;
+    return sizeof(T) == 2 ? a << 2 | b << 3 | c | d << 1 : a << 2 | b << 1 | c << 3 | d;
+  }
+  // pieces 2c and 2c + 1 of rows first .. first + 31: lane l has row l % 32
+  static __device__ __forceinline__ Frag direct(const lds_u8* tile, int first, int c, int lane) {
+    const uint32_t r = lane & 31, g = lane >> 5;
+    return *(const __attribute__((address_space(3))) Frag*)(tile + first * W + r * W + (((2 * c) ^ g ^ turn(r)) * 16));
+  }
+  // acc[32 values of the width, 32 columns] += the tile's rows transposed [., 32 rows] times p [32 rows, 32 columns]
+  static __device__ __forceinline__ void add(f32x16 (&acc)[ND], const lds_u8* tile, int first, const f32x16& p, int lane) {
+    const uint32_t i = lane & 15, half = (lane >> 4) & 1, g = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        Frag b;
+#pragma unroll
+        for (int e = 0; e < 8; e++) b[e] = rounded<T>(p[8 * s + e]);
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          const uint32_t r = 4 * g + (i >> 2), piece = 4 * d + 2 * half + ((i & 3) >> 1);
+          const lds_u8* lo = tile + (first + 16 * s) * W + r * W + ((piece ^ turn(r)) * 16) + (i & 1) * 8;
+          const lds_u8* hi = tile + (first + 16 * s) * W + (r + 8) * W + ((piece ^ turn(r + 8)) * 16) + (i & 1) * 8;
+          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo);
+          const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
+          const Frag a = __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+          acc[d] = Matrix<T>::run(a, b, acc[d]);
+        }
+      }
+    } else {
+      // the addresses anew each time, beside products of 64 cycles: kept from one block to the next they would take more registers than there are
+      uint32_t l = lane & 31;
+      asm volatile("" : "+v"(l));
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const uint32_t r = row_of(e) + 4 * g;
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+          const float a = *(const __attribute__((address_space(3))) float*)(tile + (first + r) * W + (((8 * d + (l >> 2)) ^ turn(r)) * 16) + (l & 3) * 4);
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[e], acc[d], 0, 0, 0);
+        }
+      }
+    }
+  }
+};
+
+// Loads rows into a tile, straight to LDS: an instruction of a wave fills 1 KB.  What lies behind the width or the last row becomes zero.
+template <typename T, int DP, int ROWS, int WAVES>
+struct RowsLoad {
+  using Shape = Tile<T, DP>;
+  static constexpr int W = Shape::W, kLoads = ROWS * W / 1024 / WAVES;
+  static_assert(kLoads >= 1, "a wave takes at least one load");
+  uint32_t at[kLoads];
+  int wave;
+  static __device__ __forceinline__ uint32_t row(int wave, int q, int lane) { return ((wave * kLoads + q) * 1024 + lane * 16) / W; }
+  __device__ __forceinline__ void set_up(int64_t stride, int width, int w, int lane) {
+    wave = w;
+#pragma unroll
+    for (int q = 0; q < kLoads; q++) {
+      const uint32_t r = row(w, q, lane), piece = ((lane * 16 % W) / 16) ^ Shape::turn(r);
+      at[q] = (int)piece * 16 < width * Shape::kEsz ? r * (uint32_t)stride + piece * 16 : kNowhere;
+    }
+  }
+  // from `base` on, of which `left` rows are there; absent[r]: row r is left out
+  __device__ __forceinline__ void issue(const char* base, int left, int64_t stride, int width, bool some_absent, uint64_t there, lds_u8* to, int lane) const {
+    Window window;
+    window.base = base;
+    window.left = left <= 0 ? 0 : (left - 1) * stride + width * Shape::kEsz;
+    const __amdgpu_buffer_rsrc_t rsrc = window.rsrc();
+#pragma unroll
+    for (int q = 0; q < kLoads; q++) {
+      uint32_t from = at[q];
+      if (some_absent && !((there >> row(wave, q, lane)) & 1)) from = kNowhere;
+      load_to_lds<16>(rsrc, from, to + (wave * kLoads + q) * 1024);
+    }
+  }
+};
+
+// `count` floats from `at` on of an array of `size`, 64 to a wave's instruction; zeros where the array ends on either side
+__device__ __forceinline__ void load_floats(const float* base, int64_t size, int64_t at, int count, int turn, int waves, lds_u8* to, int lane) {
+  Window window;
+  window.base = (const char*)base;
+  window.left = size * 4;
+  const __amdgpu_buffer_rsrc_t rsrc = window.rsrc();
+  for (int l = turn; l * 64 < count; l += waves) {
+    const int64_t from = at + l * 64 + lane;
+    load_to_lds<4>(rsrc, from < 0 || from >= size ? kNowhere : (uint32_t)from * 4, to + l * 256);
+  }
+}
+
+// all loads and stores are done, and all LDS reads
+__device__ __forceinline__ void wait_all() { __builtin_amdgcn_s_waitcnt(7 << 4); }
+__device__ __forceinline__ void meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// a wave's LDS accesses are executed in its order, and the compiler keeps it
+__device__ __forceinline__ void in_turn() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// a and b: a value of the lane's and the one of the lane 32 further on, in whichever order
+__device__ __forceinline__ float most_of_both(float v) {
+  uint32_t a = __builtin_bit_cast(uint32_t, v), b = a;
+  swap_rows32(a, b);
+  return __builtin_fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float sum_of_both(float v) {
+  uint32_t a = __builtin_bit_cast(uint32_t, v), b = a;
+  swap_rows32(a, b);
+  return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+// Workgroups go to the 8 XCDs in turn: each XCD has a run of consecutive pieces of work, so that the tiles of a head, which read the same rows, share its L2
+__device__ __forceinline__ bool work_of(uint32_t blocks, uint32_t& w) {
+  const uint32_t id = (uint32_t)block_of(), xcd = id % 8, most = blocks / 8, rest = blocks % 8;
+  w = xcd * most + (xcd < rest ? xcd : rest) + id / 8;
+  return id < blocks;
+}
+
+// pieces 2c and 2c + 1 of one row, from memory
+template <typename T, int NC>
+__device__ __forceinline__ void own_row(const char* row, bool there, int width, int lane, typename Matrix<T>::Frag (&f)[NC]) {
+#pragma unroll
+  for (int c = 0; c < NC; c++) {
+    const int piece = 2 * c + (lane >> 5);
+    f[c] = typename Matrix<T>::Frag{};
+    if (there && piece * 16 < width * (int)sizeof(T)) f[c] = *(const typename Matrix<T>::Frag*)(row + piece * 16);
+  }
+}
+// What a result of 16 bits leaves out of a float, in eight bits: at most half a step, 2^-8 (bfloat16) or 2^-11 of the value's power of two, in 127ths.
+// ds_ij = p_ij (do_i.v_j - do_i.o_i) is a difference of nearly equal numbers where one key has most of the probability: with o as it was rounded
+// dq and dk were off by 0.0040 of their norm (bfloat16, scores of deviation 2) where the other roundings leave 0.0024; a byte of each o is what that takes.
+template <typename T>
+struct Rest {
+  static constexpr bool kept = sizeof(T) == 2;
+  static constexpr float kSteps = 127.0f * (std::is_same<T, bf16>::value ? 256.0f : 2048.0f);
+  static constexpr uint32_t kLeast = std::is_same<T, bf16>::value ? 1u << 23 : 113u << 23;      // the power of two below which steps stay the same
+  static __device__ __forceinline__ uint32_t power(T v) {
+    const uint32_t e = __builtin_bit_cast(uint32_t, (float)v) & 0x7f800000u;
+    return e > kLeast ? e : kLeast;
+  }
+  static __device__ __forceinline__ uint32_t of(float exact, T v) {
+    const float x = (exact - (float)v) * __builtin_bit_cast(float, 0x7f000000u - power(v)) * kSteps;
+    return (uint32_t)(int)__builtin_rintf(__builtin_fminf(__builtin_fmaxf(x, -127.0f), 127.0f)) & 0xff;
+  }
+  static __device__ __forceinline__ float add(T v, uint32_t code) {
+    return __builtin_fmaf((float)(int8_t)code, __builtin_bit_cast(float, power(v)) * (1.0f / kSteps), (float)v);
+  }
+};
+// four neighbouring values of a row, and what they leave out
+template <typename T>
+__device__ __forceinline__ void store4(char* row, int8_t* rest, int col, f32x4 v) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 o;
+#pragma unroll
+  for (int t = 0; t < 4; t++) o[t] = rounded<T>(v[t]);
+  *(T4*)(row + col * sizeof(T)) = o;
+  if constexpr (Rest<T>::kept) {
+    if (!rest) return;
+    uint32_t w = 0;
+#pragma unroll
+    for (int t = 0; t < 4; t++) w |= Rest<T>::of(v[t], o[t]) << (8 * t);
+    *(uint32_t*)(rest + col) = w;
+  }
+}
+// acc, whose columns are a wave's rows, to memory: a lane has four neighbouring values of its row at a time
+template <typename T, int ND>
+__device__ __forceinline__ void store_row(char* row, int8_t* rest, int width, int lane, const f32x16 (&acc)[ND], float factor) {
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int col = 32 * d + row_of(e) + 4 * (lane >> 5);
+      if (col < width) store4<T>(row, rest, col, f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]} * factor);
+    }
+}
+
+// hidden scores of a block of 32 rows of the tile: the lane sees rows below `seen`, and of those the ones whose bit is set
+__device__ __forceinline__ void hide(f32x16& s, int seen, uint32_t there, int lane) {
+  const int g4 = 4 * (lane >> 5);
+#pragma unroll
+  for (int e = 0; e < 16; e++) {
+    const bool sees = row_of(e) + g4 < seen && (there >> (row_of(e) + g4) & 1);
+    s[e] = sees ? s[e] : -__builtin_inff();
+  }
+}
+
+// what the kernels over keys share: which keys of a tile there are.  The bytes of the next tile but one are on their way while a tile is worked on.
+struct Present {
+  const uint8_t* mask;
+  int keys;
+  uint32_t byte = 0;
+  __device__ __forceinline__ void ask(int key) { byte = mask && key < keys ? mask[key] : 0; }
+  __device__ __forceinline__ uint64_t answer() const { return mask ? __ballot(byte != 0) : ~0ull; }
+};
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// The forward pass.  APART: for few queries the waves of a workgroup have the same 32 rows (the queries of all heads that share a key head), take the
+// keys in turn, each in tiles of its own, and add up at the end; splits of the keys go to workgroups of their own, which join_kernel adds up.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP, int WAVES, bool APART, bool BIAS>
+__global__ __launch_bounds__(WAVES * 64) void attention_forward_kernel(AttentionArgs p) {
+  using Shape = Tile<T, DP>;
+  using Frag = typename Shape::Frag;
+  constexpr int R = APART ? 32 : Shape::kRows, NB = R / 32, W = Shape::W, NC = Shape::NC, ND = Shape::ND;
+  constexpr int kTile = R * W, kRing = 4 * kTile, BM = APART ? 32 : WAVES * 32;
+  constexpr int kBias = BIAS && !APART ? (BM + R + 63) / 64 * 256 : 0;
+  using Load = RowsLoad<T, DP, R, APART ? 1 : WAVES>;
+  __shared__ __attribute__((aligned(1024))) uint8_t memory[(APART ? WAVES : 1) * kRing + 2 * kBias];
+  uint32_t w;
+  if (!work_of(p.blocks, w)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  lds_u8* const ring = (lds_u8*)memory + (APART ? wave * kRing : 0);
+  lds_u8* const biases = (lds_u8*)memory + (APART ? WAVES : 1) * kRing;
+
+  const int split = APART ? (int)(w % p.splits) : 0;
+  const uint32_t unit = APART ? w / p.splits : w;
+  const int tile = (int)(p.causal ? p.tiles - 1 - unit % p.tiles : unit % p.tiles);      // the longest first
+  const uint32_t bh = unit / p.tiles;
+  const int heads = APART ? p.kv_heads : p.heads, b = bh / heads, h = bh % heads;
+  const int kv = APART ? h : h / p.group;
+  // the lane's query; behind the last one: that one, of which nothing is stored
+  int head = h, query = tile * BM + (APART ? 0 : wave * 32) + (lane & 31);
+  bool own;
+  if constexpr (APART) {
+    own = query < p.group * p.queries;
+    query = own ? query : p.group * p.queries - 1;
+    head = h * p.group + query / p.queries;
+    query %= p.queries;
+  } else {
+    own = query < p.queries;
+    query = own ? query : p.queries - 1;
+  }
+  Frag q[NC];
+  own_row<T, NC>(p.q.at(b, head, query), true, p.width, lane, q);
+  const int seen = p.seen(query);
+  // of the wave's queries: what all of them see, and what any does
+  const int first = APART ? 0 : tile * BM + wave * 32, last = APART ? p.queries - 1 : tile * BM + BM - 1;
+  const int all_see = p.seen(first < p.queries ? first : p.queries - 1), some_see = p.seen(APART ? last : first + 31 < p.queries ? first + 31 : p.queries - 1);
+  const int from = split * (APART ? p.per_split : 0);
+  int to = p.seen(last < p.queries ? last : p.queries - 1);
+  if (APART && from + p.per_split < to) to = from + p.per_split;
+  // tiles of the wave: every WAVES-th block of keys where they are apart
+  const int step = APART ? WAVES * R : R, begin = from + (APART ? wave * R : 0);
+  const int steps = to > begin ? (to - begin + step - 1) / step : 0;
+
+  Load load_k, load_v;
+  load_k.set_up(p.k.row, p.width, APART ? 0 : wave, lane);
+  load_v.set_up(p.v.row, p.width, APART ? 0 : wave, lane);
+  Present present{p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.keys};
+  auto issue = [&](int t, uint64_t there) __attribute__((always_inline)) {
+    const int key = begin + t * step;
+    lds_u8* const at = ring + (t & 1) * 2 * kTile;
+    load_k.issue(p.k.at(b, kv, key), p.keys - key, p.k.row, p.width, false, there, at, lane);
+    load_v.issue(p.v.at(b, kv, key), p.keys - key, p.v.row, p.width, p.mask != nullptr, there, at + kTile, lane);      // what is absent may be a NaN
+    if constexpr (kBias > 0)
+      load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), (int64_t)key - (tile * BM + BM - 1) + p.queries - 1, BM + R - 1, wave, WAVES,
+                  biases + (t & 1) * kBias, lane);
+  };
+  const float unit2 = BIAS ? 1.0f : p.scale2;      // with a bias the scores are multiplied before it is added
+  const float* const far = BIAS && APART ? p.bias + (int64_t)head * p.distances() + p.queries - 1 - query : nullptr;
+  float most = -__builtin_inff(), total = 0.0f;
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) acc[d] = f32x16{};
+
+  uint64_t there = 0, next = 0;
+  present.ask(begin + lane);
+  next = present.answer();
+  if (steps > 0) issue(0, next);
+  present.ask(begin + step + lane);
+  for (int t = 0; t < steps; t++) {
+    wait_all();
+    if (!APART) meet();
+    __builtin_amdgcn_sched_barrier(0);
+    there = next;
+    next = present.answer();
+    if (t + 1 < steps) issue(t + 1, next);
+    present.ask(begin + (t + 2) * step + lane);
+    const int key = begin + t * step;
+    if (key >= some_see) continue;
+    const lds_u8* const keys = ring + (t & 1) * 2 * kTile;
+    f32x16 s[NB];
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      s[n] = f32x16{};
+#pragma unroll
+      for (int c = 0; c < NC; c++) s[n] = Matrix<T>::run(Shape::direct(keys, 32 * n, c, lane), q[c], s[n]);
+    }
+    if constexpr (BIAS) {
+      const int g4 = 4 * (lane >> 5);
+#pragma unroll
+      for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const int r = 32 * n + row_of(e) + g4;
+          float add;
+          if constexpr (APART)
+            add = far[key + r < p.keys ? key + r : p.keys - 1];
+          else
+            add = ((const __attribute__((address_space(3))) float*)(biases + (t & 1) * kBias))[r - (wave * 32 + (lane & 31)) + BM - 1];
+          s[n][e] = __builtin_fmaf(s[n][e], p.scale2, add);
+        }
+    }
+    const bool edge = key + R > all_see || (p.mask && (R == 64 ? ~there : ~there & 0xffffffffu) != 0);
+    if (edge) {
+#pragma unroll
+      for (int n = 0; n < NB; n++) hide(s[n], seen - key - 32 * n, (uint32_t)(there >> (32 * n)), lane);
+    }
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) m = __builtin_fmaxf(m, s[n][e]);
+    m = most_of_both(m);
+    // the maximum follows when it is left behind by 2^8, which probabilities of every type hold: mostly in the first tile alone
+    if (__ballot(m > most + 8.0f / unit2)) {
+      m = __builtin_fmaxf(m, most);
+      const float factor = m > most ? __builtin_amdgcn_exp2f((most - m) * unit2) : 1.0f;
+      most = m;
+      total *= factor;
+#pragma unroll
+      for (int d = 0; d < ND; d++) acc[d] *= factor;
+    }
+    const float off = most == -__builtin_inff() ? 0.0f : most * unit2;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        s[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], unit2, -off));
+        total += s[n][e];
+      }
+      Shape::add(acc, keys + kTile, 32 * n, s[n], lane);
+    }
+  }
+  wait_all();
+
+  total = sum_of_both(total);
+  most = most == -__builtin_inff() ? most : most * unit2;
+  if constexpr (!APART) {
+    if (!own) return;
+    store_row<T, ND>((char*)p.out.at(b, head, query), p.rest_at(b, head, query), p.width, lane, acc, total > 0.0f ? 1.0f / total : total);
+    if (p.lse && lane < 32)
+      p.lse[((int64_t)b * p.heads + head) * p.queries + query] = total == 0.0f ? __builtin_inff() : most + __builtin_amdgcn_logf(total);
+  } else {
+    // the waves' maxima and sums, then each wave adds up its share of the values
+    constexpr int kAll = ND * 16, kShare = kAll / WAVES;
+    static_assert((WAVES * kAll + 2 * WAVES) * 256 <= (int)sizeof(memory) || WAVES == 1, "the rings hold the waves' results");
+    __attribute__((address_space(3))) float* const all = (__attribute__((address_space(3))) float*)(lds_u8*)memory;
+    __attribute__((address_space(3))) float* const stats = all + WAVES * kAll * 64;
+    meet();
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) all[(wave * kAll + 16 * d + e) * 64 + lane] = acc[d][e];
+    stats[(2 * wave) * 64 + lane] = most;
+    stats[(2 * wave + 1) * 64 + lane] = total;
+    __syncthreads();
+    float factor[WAVES];
+    most = -__builtin_inff();
+#pragma unroll
+    for (int o = 0; o < WAVES; o++) most = __builtin_fmaxf(most, stats[(2 * o) * 64 + lane]);
+    total = 0.0f;
+#pragma unroll
+    for (int o = 0; o < WAVES; o++) {
+      const float m = stats[(2 * o) * 64 + lane];
+      factor[o] = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - most);
+      total = __builtin_fmaf(stats[(2 * o + 1) * 64 + lane], factor[o], total);
+    }
+    const bool whole = p.splits == 1;
+    const float scale = !whole ? 1.0f : total > 0.0f ? 1.0f / total : total;
+    const int64_t place = ((int64_t)unit * p.splits + split) * 32 + (lane & 31);
+    char* const row = (char*)p.out.at(b, head, query);
+#pragma unroll
+    for (int n = 0; n < kShare; n += 4) {
+      const int k = wave * kShare + n, col = 32 * (k / 16) + row_of(k % 16) + 4 * (lane >> 5);
+      f32x4 v;
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        v[t] = 0.0f;
+#pragma unroll
+        for (int o = 0; o < WAVES; o++) v[t] = __builtin_fmaf(all[(o * kAll + k + t) * 64 + lane], factor[o], v[t]);
+        v[t] *= scale;
+      }
+      if (!own || col >= p.width) continue;
+      if (whole) {
+        store4<T>(row, p.rest_at(b, head, query), col, v);
+      } else {
+        *(f32x4*)(p.part + place * DP + col) = v;
+      }
+    }
+    if (own && wave == 0 && lane < 32) {
+      if (!whole)
+        *(f32x2*)(p.part_stats + place * 2) = f32x2{most, total};
+      else if (p.lse)
+        p.lse[((int64_t)b * p.heads + head) * p.queries + query] = total == 0.0f ? __builtin_inff() : most + __builtin_amdgcn_logf(total);
+    }
+  }
+}
+
+// The splits' results as one: a workgroup has a row, its lanes the width, its waves the splits.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p) {
+  constexpr int kLanes = DP / 4, kDown = 256 / kLanes;
+  __shared__ f32x4 sums[kDown][kLanes];
+  __shared__ float totals[kDown];
+  const int64_t at = block_of();
+  const int rows = p.group * p.queries, row = (int)(at % rows), lane = threadIdx.x % kLanes, down = threadIdx.x / kLanes;
+  const int64_t bh = at / rows;
+  if (bh >= (int64_t)(p.blocks / p.splits / p.tiles)) return;
+  const int tile = row / 32;
+  const uint32_t unit = (uint32_t)(bh * p.tiles + (p.causal ? p.tiles - 1 - tile : tile));
+  const int64_t first = (int64_t)unit * p.splits * 32 + row % 32;
+  float most = -__builtin_inff();
+  for (int s = 0; s < p.splits; s++) most = __builtin_fmaxf(most, p.part_stats[(first + 32 * (int64_t)s) * 2]);
+  f32x4 sum = {};
+  float total = 0.0f;
+  if (down < kDown) {
+    for (int s = down; s < p.splits; s += kDown) {
+      const int64_t place = first + 32 * (int64_t)s;
+      const f32x2 stat = *(const f32x2*)(p.part_stats + place * 2);
+      const float factor = stat[0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(stat[0] - most);
+      total = __builtin_fmaf(stat[1], factor, total);
+      if (lane * 4 < p.width) sum += *(const f32x4*)(p.part + place * DP + lane * 4) * factor;
+    }
+    sums[down][lane] = sum;
+    if (lane == 0) totals[down] = total;
+  }
+  __syncthreads();
+  if (down != 0) return;
+  sum = f32x4{};
+  total = 0.0f;
+  for (int d = 0; d < kDown; d++) {
+    sum += sums[d][lane];
+    total += totals[d];
+  }
+  const int b = (int)(bh / p.kv_heads), head = (int)(bh % p.kv_heads) * p.group + row / p.queries, query = row % p.queries;
+  sum *= total > 0.0f ? 1.0f / total : total;
+  if (lane * 4 < p.width) store4<T>((char*)p.out.at(b, head, query), p.rest_at(b, head, query), lane * 4, sum);
+  if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + head) * p.queries + query] = total == 0.0f ? __builtin_inff() : most + __builtin_amdgcn_logf(total);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// dq, and do_i.o_i for the other kernel.  With a bias: the sums of ds along the diagonals, of the wave's 32 queries.  A block of 32 keys adds to 63
+// neighbouring diagonals, to which the wave's lanes add in LDS - lanes 0 to 31 and 32 to 63 each in a copy of their own, so that no two lanes add to one
+// sum at a time and the order of additions is always the same.  After a block the first 32 of the diagonals are complete and leave.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP, int WAVES, bool BIAS>
+__global__ __launch_bounds__(WAVES * 64) void attention_dq_kernel(AttentionArgs p) {
+  using Shape = Tile<T, DP>;
+  using Frag = typename Shape::Frag;
+  constexpr int R = Shape::kRows, NB = R / 32, W = Shape::W, NC = Shape::NC, ND = Shape::ND, BM = WAVES * 32;
+  constexpr int kTile = R * W, kBias = BIAS ? (BM + R + 63) / 64 * 256 : 0;
+  using Load = RowsLoad<T, DP, R, WAVES>;
+  __shared__ __attribute__((aligned(1024))) uint8_t memory[4 * kTile + 2 * kBias];
+  __shared__ float diagonals[BIAS ? WAVES : 1][2][64];
+  uint32_t w;
+  if (!work_of(p.blocks, w)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  lds_u8* const ring = (lds_u8*)memory;
+  lds_u8* const biases = ring + 4 * kTile;
+  const int tile = (int)(p.causal ? p.tiles - 1 - w % p.tiles : w % p.tiles);
+  const uint32_t bh = w / p.tiles;
+  const int b = bh / p.heads, h = bh % p.heads, kv = h / p.group;
+  const int first = tile * BM + wave * 32, mine = first + (lane & 31), last = tile * BM + BM - 1;
+  const bool own = mine < p.queries;
+  const int query = own ? mine : p.queries - 1;
+  Frag q[NC], dy[NC];
+  own_row<T, NC>(p.q.at(b, h, query), own, p.width, lane, q);
+  own_row<T, NC>(p.d_out.at(b, h, query), own, p.width, lane, dy);
+  const int64_t at = ((int64_t)b * p.heads + h) * p.queries + query;
+  const float lse = own ? p.lse[at] : __builtin_inff();
+  float delta = 0.0f;
+  {
+    Frag o[NC];
+    own_row<T, NC>(p.out.at(b, h, query), own, p.width, lane, o);
+    const int8_t* const rest = p.rest_at(b, h, query);
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      u32x2 code = {};
+      const int piece = 2 * c + (lane >> 5);
+      if constexpr (Rest<T>::kept)
+        if (rest && piece * 8 < p.width) code = *(const u32x2*)(rest + piece * 8);
+#pragma unroll
+      for (int e = 0; e < 16 / (int)sizeof(T); e++) {
+        float exact = (float)o[c][e];
+        if constexpr (Rest<T>::kept)
+          if (rest) exact = Rest<T>::add(o[c][e], code[e >> 2] >> (8 * (e & 3)));
+        delta = __builtin_fmaf(exact, (float)dy[c][e], delta);
+      }
+    }
+    delta = sum_of_both(delta);
+    if (own && lane < 32) p.delta[at] = delta;
+  }
+  const int seen = p.seen(query);
+  const int all_see = p.seen(first < p.queries ? first : p.queries - 1), some_see = p.seen(first + 31 < p.queries ? first + 31 : p.queries - 1);
+  const int to = p.seen(last < p.queries ? last : p.queries - 1);
+  const int steps = to > 0 ? (to + R - 1) / R : 0;
+
+  Load load_k, load_v;
+  load_k.set_up(p.k.row, p.width, wave, lane);
+  load_v.set_up(p.v.row, p.width, wave, lane);
+  Present present{p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.keys};
+  auto issue = [&](int t, uint64_t there) __attribute__((always_inline)) {
+    const int key = t * R;
+    lds_u8* const to = ring + (t & 1) * 2 * kTile;
+    load_k.issue(p.k.at(b, kv, key), p.keys - key, p.k.row, p.width, p.mask != nullptr, there, to, lane);
+    load_v.issue(p.v.at(b, kv, key), p.keys - key, p.v.row, p.width, p.mask != nullptr, there, to + kTile, lane);
+    if constexpr (BIAS)
+      load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), (int64_t)key - last + p.queries - 1, BM + R - 1, wave, WAVES,
+                  biases + (t & 1) * kBias, lane);
+  };
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) acc[d] = f32x16{};
+  typedef __attribute__((address_space(3))) float lds_float;
+  lds_float* const sums = (lds_float*)diagonals[BIAS ? wave : 0][0];
+  if constexpr (BIAS) {
+    sums[lane] = 0.0f;
+    sums[64 + lane] = 0.0f;
+  }
+  // of the diagonals of the wave's queries, which begin at key 0 and query first + 31
+  float* const along = BIAS && p.along ? p.along + ((bh * (int64_t)p.tiles + tile) * WAVES + wave) * p.along_stride : nullptr;
+
+  uint64_t there = 0, next = 0;
+  present.ask(lane);
+  next = present.answer();
+  if (steps > 0) issue(0, next);
+  present.ask(R + lane);
+  for (int t = 0; t < steps; t++) {
+    wait_all();
+    meet();
+    __builtin_amdgcn_sched_barrier(0);
+    there = next;
+    next = present.answer();
+    if (t + 1 < steps) issue(t + 1, next);
+    present.ask((t + 2) * R + lane);
+    const int key = t * R;
+    const lds_u8* const keys = ring + (t & 1) * 2 * kTile;
+    const bool edge = key + R > all_see || (p.mask && (R == 64 ? ~there : ~there & 0xffffffffu) != 0);
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      if (key + 32 * n < some_see) {
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(keys, 32 * n, c, lane), q[c], s);
+#pragma unroll
+        for (int c = 0; c < NC; c++) dp = Matrix<T>::run(Shape::direct(keys + kTile, 32 * n, c, lane), dy[c], dp);
+        const int g4 = 4 * (lane >> 5);
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          float off = -lse;
+          if constexpr (BIAS)
+            off += ((const lds_float*)(biases + (t & 1) * kBias))[32 * n + row_of(e) + g4 - (wave * 32 + (lane & 31)) + BM - 1];
+          s[e] = __builtin_fmaf(s[e], p.scale2, off);
+        }
+        if (edge) hide(s, seen - key - 32 * n, (uint32_t)(there >> (32 * n)), lane);
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(s[e]) * (dp[e] - delta);
+        if constexpr (BIAS) {
+          if (along) {
+            in_turn();
+            lds_float* const mine_at = sums + (lane >> 5) * 64 + 31 - (lane & 31) + g4;
+#pragma unroll
+            for (int e = 0; e < 16; e++) __hip_atomic_fetch_add(mine_at + row_of(e), s[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+          }
+        }
+        Shape::add(acc, keys, 32 * n, s, lane);
+      }
+      if constexpr (BIAS) {
+        if (along) {
+          in_turn();
+          const float a = sums[lane], c = sums[64 + lane];
+          if (lane < 32) along[key + 32 * n + lane] = a + c;
+          sums[(lane + 32) & 63] = lane < 32 ? 0.0f : a;
+          sums[64 + ((lane + 32) & 63)] = lane < 32 ? 0.0f : c;
+        }
+      }
+    }
+  }
+  wait_all();
+  if constexpr (BIAS)
+    if (along && lane < 32) along[steps * R + lane] = sums[lane] + sums[64 + lane];
+  if (own && p.dq.p) store_row<T, ND>((char*)p.dq.at(b, h, query), nullptr, p.width, lane, acc, p.scale);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// dk and dv: a wave has 32 keys, and the queries of all heads that share the key head pass by.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP, int WAVES, bool BIAS>
+__global__ __launch_bounds__(WAVES * 64) void attention_dkv_kernel(AttentionArgs p) {
+  using Shape = Tile<T, DP>;
+  using Frag = typename Shape::Frag;
+  constexpr int R = Shape::kRows, NB = R / 32, W = Shape::W, NC = Shape::NC, ND = Shape::ND, BM = WAVES * 32;
+  constexpr int kTile = R * W, kBias = BIAS ? (BM + R + 63) / 64 * 256 : 0, kStats = 256;
+  using Load = RowsLoad<T, DP, R, WAVES>;
+  typedef __attribute__((address_space(3))) float lds_float;
+  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+  __shared__ __attribute__((aligned(1024))) uint8_t memory[4 * kTile + 4 * kStats + 2 * kBias];
+  uint32_t w;
+  if (!work_of(p.blocks, w)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  lds_u8* const ring = (lds_u8*)memory;
+  lds_u8* const stats = ring + 4 * kTile;
+  lds_u8* const biases = stats + 4 * kStats;
+  const int tile = (int)(w % p.tiles);
+  const uint32_t bh = w / p.tiles;
+  const int b = bh / p.kv_heads, kv = bh % p.kv_heads;
+  const int first = tile * BM + wave * 32, key = first + (lane & 31);
+  const bool own = key < p.keys && (!p.mask || p.mask[(int64_t)b * p.mask_stride + key]);
+  Frag k[NC], v[NC];
+  own_row<T, NC>(p.k.at(b, kv, key), own, p.width, lane, k);
+  own_row<T, NC>(p.v.at(b, kv, key), own, p.width, lane, v);
+  // queries from `seen_from` on see the lane's key
+  const int behind = p.keys - p.queries;
+  const int seen_from = p.causal && key > behind ? key - behind : 0;
+  const int all_from = p.causal && first + 31 > behind ? first + 31 - behind : 0, some_from = p.causal && first > behind ? first - behind : 0;
+  const int begin = (p.causal && tile * BM > behind ? tile * BM - behind : 0) / R * R;
+  const int per_head = begin < p.queries ? (p.queries - begin + R - 1) / R : 0, steps = per_head * p.group;
+
+  Load load_q, load_dy;
+  load_q.set_up(p.q.row, p.width, wave, lane);
+  load_dy.set_up(p.d_out.row, p.width, wave, lane);
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    const int head = kv * p.group + t / per_head, query = begin + t % per_head * R;
+    lds_u8* const to = ring + (t & 1) * 2 * kTile;
+    load_q.issue(p.q.at(b, head, query), p.queries - query, p.q.row, p.width, false, 0, to, lane);
+    load_dy.issue(p.d_out.at(b, head, query), p.queries - query, p.d_out.row, p.width, false, 0, to + kTile, lane);
+    const int64_t at = ((int64_t)b * p.heads + head) * p.queries;
+    if (wave < 2) load_floats((wave ? p.delta : p.lse) + at, p.queries, query, R, 0, 1, stats + (2 * (t & 1) + wave) * kStats, lane);
+    if constexpr (BIAS)
+      load_floats(p.bias + (int64_t)head * p.distances(), p.distances(), (int64_t)tile * BM - (query + R - 1) + p.queries - 1, BM + R - 1, wave, WAVES,
+                  biases + (t & 1) * kBias, lane);
+  };
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
+
+  if (steps > 0) issue(0);
+  for (int t = 0; t < steps; t++) {
+    wait_all();
+    meet();
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 1 < steps) issue(t + 1);
+    const int query = begin + t % per_head * R;
+    const lds_u8* const rows = ring + (t & 1) * 2 * kTile;
+    const lds_float* const lse = (const lds_float*)(stats + 2 * (t & 1) * kStats);
+    const lds_float* const delta = (const lds_float*)(stats + (2 * (t & 1) + 1) * kStats);
+    const bool edge = query < all_from || query + R > p.queries;
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      if (query + 32 * n + 31 < some_from || query + 32 * n >= p.queries) continue;
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(rows, 32 * n, c, lane), k[c], s);
+#pragma unroll
+      for (int c = 0; c < NC; c++) dp = Matrix<T>::run(Shape::direct(rows + kTile, 32 * n, c, lane), v[c], dp);
+      const int g4 = 4 * (lane >> 5);
+#pragma unroll
+      for (int e4 = 0; e4 < 16; e4 += 4) {
+        const f32x4 l = *(const lds_f32x4*)(lse + 32 * n + row_of(e4) + g4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float off = -l[e];
+          if constexpr (BIAS)
+            off += ((const lds_float*)(biases + (t & 1) * kBias))[wave * 32 + (lane & 31) - (32 * n + row_of(e4) + e + g4) + R - 1];
+          s[e4 + e] = __builtin_fmaf(s[e4 + e], p.scale2, off);
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const int i = query + 32 * n + row_of(e) + g4;
+          s[e] = i >= seen_from && i < p.queries ? s[e] : -__builtin_inff();
+        }
+      }
+#pragma unroll
+      for (int e4 = 0; e4 < 16; e4 += 4) {
+        const f32x4 x = *(const lds_f32x4*)(delta + 32 * n + row_of(e4) + g4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          s[e4 + e] = __builtin_amdgcn_exp2f(s[e4 + e]);
+          dp[e4 + e] = s[e4 + e] * (dp[e4 + e] - x[e]);
+        }
+      }
+      Shape::add(dv, rows + kTile, 32 * n, s, lane);
+      Shape::add(dk, rows, 32 * n, dp, lane);
+    }
+  }
+  wait_all();
+  if (key >= p.keys) return;
+  // an absent key's lane has seen zeros for it
+  const float there = own ? 1.0f : 0.0f;
+  if (!own) {
+#pragma unroll
+    for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
+  }
+  if (p.dk.p) store_row<T, ND>((char*)p.dk.at(b, kv, key), nullptr, p.width, lane, dk, p.scale * there);
+  if (p.dv.p) store_row<T, ND>((char*)p.dv.at(b, kv, key), nullptr, p.width, lane, dv, there);
+}
+
+// ---- launches ----
+// the width rounded up to whole blocks of the products
+template <typename F>
+int with_width(int width, F&& f) {
+  using std::integral_constant;
+  if (width <= 32) return f(integral_constant<int, 32>{});
+  if (width <= 64) return f(integral_constant<int, 64>{});
+  if (width <= 96) return f(integral_constant<int, 96>{});
+  return f(integral_constant<int, 128>{});
+}
+template <typename K>
+int launch(K kernel, int64_t blocks, int threads, const AttentionArgs& p, hipStream_t s) {
+  if (blocks == 0) return GACT_OK;
+  if (!blocks_fit(blocks)) return GACT_ELIMIT;
+  hipLaunchKernelGGL(kernel, grid_of(blocks, threads), dim3((unsigned)threads), 0, s, p);
+  return launch_status();
+}
+
+// few queries: waves of a workgroup that take the keys in turn, as many as LDS holds tiles for
+template <typename T, int DP>
+constexpr int apart_waves() { return Tile<T, DP>::W == 512 ? 2 : 4; }
+
+}  // namespace
+
+// what attention.hip asks of the three sources; `waves` of a workgroup: 2 or 4; `apart` as above
+template <typename T>
+int attention_forward(AttentionArgs p, int64_t batch, int waves, bool apart, hipStream_t s) {
+  return with_width(p.width, [&](auto width) {
+    constexpr int DP = decltype(width)::value, A = apart_waves<T, DP>();
+    const int64_t heads = batch * (apart ? p.kv_heads : p.heads), rows = apart ? (int64_t)p.group * p.queries : p.queries;
+    const int64_t tall = apart ? 32 : waves * 32, tiles = (rows + tall - 1) / tall, blocks = heads * tiles * (apart ? p.splits : 1);
+    p.tiles = (uint32_t)tiles;
+    p.blocks = (uint32_t)blocks;
+    if (apart) {
+      const int rc = p.bias ? launch(attention_forward_kernel<T, DP, A, true, true>, blocks, A * 64, p, s)
+                            : launch(attention_forward_kernel<T, DP, A, true, false>, blocks, A * 64, p, s);
+      return rc != GACT_OK || p.splits == 1 ? rc : launch(attention_join_kernel<T, DP>, heads * rows, 256, p, s);
+    }
+    if (waves == 2)
+      return p.bias ? launch(attention_forward_kernel<T, DP, 2, false, true>, blocks, 128, p, s)
+                    : launch(attention_forward_kernel<T, DP, 2, false, false>, blocks, 128, p, s);
+    return p.bias ? launch(attention_forward_kernel<T, DP, 4, false, true>, blocks, 256, p, s)
+                  : launch(attention_forward_kernel<T, DP, 4, false, false>, blocks, 256, p, s);
+  });
+}
+template <typename T>
+int attention_backward(AttentionArgs p, int64_t batch, int waves_dq, int waves_dkv, hipStream_t s) {
+  return with_width(p.width, [&](auto width) {
+    constexpr int DP = decltype(width)::value;
+    auto shape = [&](int64_t heads, int64_t rows, int waves) {
+      const int64_t tiles = (rows + waves * 32 - 1) / (waves * 32);
+      p.tiles = (uint32_t)tiles;
+      p.blocks = (uint32_t)(heads * tiles);
+      return heads * tiles;
+    };
+    const int64_t blocks = shape(batch * p.heads, p.queries, waves_dq);
+    int rc;
+    if (waves_dq == 2)
+      rc = p.bias ? launch(attention_dq_kernel<T, DP, 2, true>, blocks, 128, p, s) : launch(attention_dq_kernel<T, DP, 2, false>, blocks, 128, p, s);
+    else
+      rc = p.bias ? launch(attention_dq_kernel<T, DP, 4, true>, blocks, 256, p, s) : launch(attention_dq_kernel<T, DP, 4, false>, blocks, 256, p, s);
+    if (rc != GACT_OK || !(p.dk.p || p.dv.p)) return rc;
+    const int64_t others = shape(batch * p.kv_heads, p.keys, waves_dkv);
+    if (waves_dkv == 2)
+      return p.bias ? launch(attention_dkv_kernel<T, DP, 2, true>, others, 128, p, s) : launch(attention_dkv_kernel<T, DP, 2, false>, others, 128, p, s);
+    return p.bias ? launch(attention_dkv_kernel<T, DP, 4, true>, others, 256, p, s) : launch(attention_dkv_kernel<T, DP, 4, false>, others, 256, p, s);
+  });
+}

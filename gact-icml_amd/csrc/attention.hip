@@ -1,0 +1,354 @@
+// Attention's host side, its small kernels, and the relative position bias.
+#include "attention.h"
+
+#include <math.h>
+
+extern template int attention_forward<float>(AttentionArgs, int64_t, int, bool, hipStream_t);
+extern template int attention_forward<f16>(AttentionArgs, int64_t, int, bool, hipStream_t);
+extern template int attention_forward<bf16>(AttentionArgs, int64_t, int, bool, hipStream_t);
+extern template int attention_backward<float>(AttentionArgs, int64_t, int, int, hipStream_t);
+extern template int attention_backward<f16>(AttentionArgs, int64_t, int, int, hipStream_t);
+extern template int attention_backward<bf16>(AttentionArgs, int64_t, int, int, hipStream_t);
+
+namespace {
+
+constexpr float kLog2e = 1.44269504f;
+// A bias of this or less hides the key, as -inf does: with the lowest value of a type for a whole row the scores would be lost in it
+constexpr float kHidden = -1e30f;
+
+// The bias as the kernels add it.  A launch of its own (2 us): in the kernels the product and the comparison would be made for every score
+__global__ __launch_bounds__(256) void attention_bias_kernel(const float* __restrict__ bias, int64_t n, float* __restrict__ out) {
+  const int64_t i = block_of() * 256 + threadIdx.x;
+  if (i >= n) return;
+  const float v = bias[i];
+  out[i] = v <= kHidden ? -__builtin_inff() : v * kLog2e;
+}
+
+// dbias[h][t]: what the blocks of 32 queries of all batch entries have on diagonal t, in their order.
+struct AlongArgs {
+  const float* along;
+  int64_t stride;
+  int64_t batch;
+  int heads, queries, keys, tall, rows, waves;     // queries of a workgroup, rows of a tile, waves
+  bool causal;
+  float* out;
+};
+__global__ __launch_bounds__(1024) void attention_along_kernel(AlongArgs p) {
+  __shared__ float shared[16][64];
+  const int distances = p.queries + p.keys - 1, t = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6, h = blockIdx.y;
+  const int blocks = (p.queries + 31) / 32, tiles = (p.queries + p.tall - 1) / p.tall;
+  float sum = 0.0f;
+  if (t < distances) {
+    // the blocks whose diagonals t is among: of block k they are t + 32 (k + 1) - queries, from 0 on
+    for (int64_t n = wave; n < p.batch * blocks; n += 16) {
+      const int64_t b = n / blocks;
+      const int k = (int)(n - b * blocks), at = t + 32 * (k + 1) - p.queries, tile = 32 * k / p.tall;
+      const int last = tile * p.tall + p.tall - 1 < p.queries ? tile * p.tall + p.tall - 1 : p.queries - 1;
+      int to = last + p.keys - p.queries + 1;
+      to = !p.causal || to > p.keys ? p.keys : to < 0 ? 0 : to;
+      if (at >= 0 && at < (to + p.rows - 1) / p.rows * p.rows + 32)
+        sum += p.along[((b * p.heads + h) * tiles * p.waves + k) * p.stride + at];
+    }
+  }
+  shared[wave][threadIdx.x & 63] = sum;
+  __syncthreads();
+  if (wave == 0 && t < distances) {
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; w++) sum += shared[w][threadIdx.x];
+    p.out[(int64_t)h * distances + t] = sum;
+  }
+}
+
+// ---- the relative position bias by buckets ----
+constexpr int kMostBuckets = GACT_MAX_BUCKETS;
+struct Buckets {
+  int near, steps, per;       // buckets of one distance each, buckets behind them, and both together: those of one direction
+  bool both;
+  int32_t border[kMostBuckets];      // the least distance of bucket near + k
+  __device__ __forceinline__ int of(int d) const {       // key - query
+    const int away = both ? (d < 0 ? -d : d) : d < 0 ? -d : 0, side = both && d > 0 ? per : 0;
+    if (away < near) return side + away;
+    int low = 0, high = steps;       // border[low] <= away < border[high]
+    while (high - low > 1) {
+      const int middle = (low + high) / 2;
+      (border[middle] <= away ? low : high) = middle;
+    }
+    return side + near + low;
+  }
+};
+// A thread has a distance and eight heads, whose values lie side by side in the table.  64 heads of 32767 distances: bound by the stores.
+template <typename T>
+__global__ __launch_bounds__(256) void position_bias_kernel(const T* __restrict__ table, int heads, int keys, int distances, Buckets buckets,
+                                                            float* __restrict__ out) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= distances) return;
+  const T* const row = table + (int64_t)buckets.of(t - (keys - 1)) * heads;
+  const int first = blockIdx.y * 8;
+#pragma unroll
+  for (int h = 0; h < 8; h++)
+    if (first + h < heads) out[(int64_t)(first + h) * distances + t] = (float)row[first + h];
+}
+// A bucket's distances are neighbours: a workgroup adds up one bucket of one head, always in the same order
+template <typename T>
+__global__ __launch_bounds__(256) void position_bias_backward_kernel(const float* __restrict__ grad, int heads, int queries, int keys, Buckets buckets,
+                                                                     T* __restrict__ d_table) {
+  __shared__ float shared[4];
+  const int bucket = blockIdx.x, h = blockIdx.y, side = buckets.both && bucket >= buckets.per, n = bucket - (side ? buckets.per : 0);
+  const int distances = queries + keys - 1;
+  // distances from `low` to below `high` on this side of the query
+  const int low = n < buckets.near ? n : buckets.border[n - buckets.near];
+  const int high = n < buckets.near ? n + 1 < buckets.near ? n + 1 : buckets.border[0] : n + 1 < buckets.per ? buckets.border[n + 1 - buckets.near] : 0x40000000;
+  int begin = side ? keys - 1 + (low > 1 ? low : 1) : keys - high, end = side ? (high > queries ? distances : keys - 1 + high) : keys - low;
+  if (!buckets.both && n == 0) end = distances;       // keys behind the query
+  if (begin < 0) begin = 0;
+  if (end > distances) end = distances;
+  const float* const row = grad + (int64_t)h * distances;
+  float sum[4] = {};
+  int t = begin + threadIdx.x;
+  for (; t + 3 * 256 < end; t += 4 * 256)
+#pragma unroll
+    for (int u = 0; u < 4; u++) sum[u] += row[t + u * 256];
+  for (; t < end; t += 256) sum[0] += row[t];
+  const float all = over_lanes<Sum, 64>((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = all;
+  __syncthreads();
+  if (threadIdx.x == 0) d_table[(int64_t)bucket * heads + h] = rounded<T>((shared[0] + shared[1]) + (shared[2] + shared[3]));
+}
+
+// ---- host side ----
+constexpr int kComputeUnits = 256;
+inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+inline int64_t esz(int dtype) { return dtype == GACT_F32 ? 4 : 2; }
+
+bool sizes_fit(const gact_attention* a) {
+  if (!known(a->dtype) || a->batch < 0 || a->queries < 0 || a->keys < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads) return false;
+  if (a->queries > GACT_ATTENTION_MAX_LENGTH || a->keys > GACT_ATTENTION_MAX_LENGTH || a->heads > 65535 || a->batch > 0x7fffffff) return false;
+  return a->width >= 1 && a->width <= GACT_ATTENTION_MAX_WIDTH && a->scale > 0.0f && a->scale < __builtin_inff();
+}
+int64_t distances(const gact_attention* a) { return a->queries + a->keys > 0 ? a->queries + a->keys - 1 : 0; }
+// whole 16-byte pieces, and rows that the kernels' offsets reach.  GACT_OK where nothing of it is read
+int check_rows(const gact_attention* a, const gact_rows* r, int64_t heads, int64_t rows) {
+  if (!r) return GACT_EINVAL;
+  if (a->batch == 0 || rows == 0) return GACT_OK;
+  const int64_t e = esz(a->dtype);
+  if (!r->p || r->batch < 0 || r->head < 0 || (rows > 1 && r->row < a->width)) return GACT_EINVAL;
+  if (!aligned16(r->p) || a->width * e % 16 || (rows > 1 && r->row * e % 16) || (a->batch > 1 && r->batch * e % 16) || (heads > 1 && r->head * e % 16))
+    return GACT_EALIGN;
+  return rows > 1 && r->row * e > GACT_ATTENTION_MAX_STRIDE ? GACT_EINVAL : GACT_OK;
+}
+// (a single row may have any stride)
+Side side_of(const gact_attention* a, const gact_rows* r, int64_t rows) {
+  const int64_t e = esz(a->dtype);
+  return r ? Side{(const char*)r->p, r->batch * e, r->head * e, (rows > 1 ? r->row : a->width) * e} : Side{nullptr, 0, 0, 0};
+}
+int check_all(const gact_attention* a) {
+  if (!a || !sizes_fit(a)) return GACT_EINVAL;
+  if ((a->mask && a->mask_stride < 0) || (a->bias && a->heads * distances(a) > ((int64_t)1 << 40))) return GACT_EINVAL;
+  int rc = check_rows(a, &a->q, a->heads, a->queries);
+  if (rc == GACT_OK) rc = check_rows(a, &a->k, a->kv_heads, a->keys);
+  return rc == GACT_OK ? check_rows(a, &a->v, a->kv_heads, a->keys) : rc;
+}
+
+// How the forward pass is cut.  Few queries: workgroups of 32 rows whose waves take the keys in turn, and splits of the keys until there are two
+// workgroups to a compute unit, each wave with at least two blocks of 32 keys.
+struct ForwardCut {
+  int waves;
+  bool apart;
+  int splits, per_split;
+};
+int waves_of(int64_t rows) { return rows <= 64 ? 2 : 4; }
+int64_t padded_width(const gact_attention* a) { return round_up(a->width, 32); }
+ForwardCut forward_cut(const gact_attention* a) {
+  ForwardCut c{waves_of(a->queries), false, 1, 0};
+  const int64_t group = a->heads / a->kv_heads, rows = group * a->queries;
+  const int64_t blocks = a->batch * a->heads * ((a->queries + c.waves * 32 - 1) / (c.waves * 32));
+  const int64_t units = a->batch * a->kv_heads * ((rows + 31) / 32);
+  c.apart = rows <= 32 || (blocks < kComputeUnits && a->keys >= 256);
+  if (!c.apart || units == 0) return c;
+  c.waves = esz(a->dtype) * padded_width(a) > 256 ? 2 : 4;
+  const int64_t least = c.waves * 64;
+  int64_t splits = 2 * kComputeUnits / units, most = a->keys / least;
+  if (splits > most) splits = most;
+  if (splits < 1) splits = 1;
+  const int64_t per = round_up((a->keys + splits - 1) / splits, c.waves * 32);
+  c.per_split = (int)(per > 0 ? per : c.waves * 32);
+  c.splits = (int)(a->keys > 0 ? (a->keys + c.per_split - 1) / c.per_split : 1);
+  return c;
+}
+int64_t bias_bytes(const gact_attention* a) { return a->bias ? round_up(a->heads * distances(a) * 4, 256) : 0; }
+int64_t split_rows(const gact_attention* a, const ForwardCut& c) {
+  return c.splits > 1 ? a->batch * a->kv_heads * ((a->heads / a->kv_heads * a->queries + 31) / 32) * c.splits * 32 : 0;
+}
+int tile_rows(const gact_attention* a) { return a->dtype == GACT_F32 && a->width > 64 ? 32 : 64; }
+int64_t along_stride(const gact_attention* a) { return round_up(a->keys, tile_rows(a)) + 32; }
+int64_t along_units(const gact_attention* a) {
+  const int waves = waves_of(a->queries);
+  return a->batch * a->heads * ((a->queries + waves * 32 - 1) / (waves * 32)) * waves;
+}
+int64_t delta_bytes(const gact_attention* a) { return round_up(a->batch * a->heads * a->queries * 4, 256); }
+
+AttentionArgs args_of(const gact_attention* a) {
+  AttentionArgs p{};
+  p.q = side_of(a, &a->q, a->queries);
+  p.k = side_of(a, &a->k, a->keys);
+  p.v = side_of(a, &a->v, a->keys);
+  p.mask = a->mask;
+  p.mask_stride = a->mask_stride;
+  p.heads = (int)a->heads;
+  p.kv_heads = (int)a->kv_heads;
+  p.group = (int)(a->heads / a->kv_heads);
+  p.queries = (int)a->queries;
+  p.keys = (int)a->keys;
+  p.width = (int)a->width;
+  p.causal = a->causal != 0;
+  p.scale = a->scale;
+  p.scale2 = a->scale * kLog2e;
+  p.splits = 1;
+  return p;
+}
+int prepare_bias(const gact_attention* a, AttentionArgs& p, float* to, hipStream_t s) {
+  const int64_t n = a->heads * distances(a);
+  if (!a->bias || n == 0) return GACT_OK;
+  p.bias = to;
+  hipLaunchKernelGGL(attention_bias_kernel, grid_of((n + 255) / 256, 256), dim3(256), 0, s, a->bias, n, to);
+  return launch_status();
+}
+
+template <typename T>
+int with_buckets(const void* table, int64_t buckets, int64_t heads, int64_t queries, int64_t keys, int both, int64_t most, const void* out, T&& f) {
+  const int64_t per = both ? buckets / 2 : buckets, near = per / 2;
+  if (buckets < 2 || buckets > GACT_MAX_BUCKETS || (both && buckets % 2) || per < 2 || heads < 1 || heads > 65535) return GACT_EINVAL;
+  if (queries < 1 || keys < 1 || queries > GACT_ATTENTION_MAX_LENGTH || keys > GACT_ATTENTION_MAX_LENGTH || most <= near || most > GACT_ATTENTION_MAX_LENGTH)
+    return GACT_EINVAL;
+  if (!table || !out) return GACT_EINVAL;
+  Buckets b{};
+  b.near = (int)near;
+  b.steps = (int)(per - near);
+  b.per = (int)per;
+  b.both = both != 0;
+  // the least whole distance n with (n / near)^steps >= (most / near)^k; where that is an equation of whole numbers the logarithm's rounding must not
+  // push it to the next one
+  for (int k = 0; k < b.steps; k++) {
+    const long double x = (long double)near * powl((long double)most / (long double)near, (long double)k / (long double)b.steps);
+    b.border[k] = (int32_t)ceill(x * (1.0L - 1e-13L));
+  }
+  return f(b);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t gact_attention_workspace_bytes(const gact_attention* a) {
+  if (!a || !sizes_fit(a)) return 0;
+  const ForwardCut c = forward_cut(a);
+  return bias_bytes(a) + split_rows(a, c) * (padded_width(a) + 2) * 4;
+}
+
+int gact_attention_forward(const gact_attention* a, const gact_rows* out, float* lse, int8_t* rest, void* workspace, void* stream) {
+  int rc = check_all(a);
+  if (rc == GACT_OK) rc = check_rows(a, out, a->heads, a->queries);
+  if (rc != GACT_OK) return rc;
+  if (a->batch == 0 || a->queries == 0) return GACT_OK;
+  if ((uintptr_t)rest % 8) return GACT_EALIGN;
+  if (gact_attention_workspace_bytes(a) > 0) {
+    if (!workspace) return GACT_EINVAL;
+    if (!aligned16(workspace)) return GACT_EALIGN;
+  }
+  fresh_launch();
+  const hipStream_t s = (hipStream_t)stream;
+  AttentionArgs p = args_of(a);
+  p.out = side_of(a, out, a->queries);
+  p.lse = lse;
+  p.rest = rest;
+  rc = prepare_bias(a, p, (float*)workspace, s);
+  if (rc != GACT_OK) return rc;
+  const ForwardCut c = forward_cut(a);
+  p.splits = c.splits;
+  p.per_split = c.per_split;
+  p.part = (float*)((char*)workspace + bias_bytes(a));
+  p.part_stats = p.part + split_rows(a, c) * padded_width(a);
+  return with_type(a->dtype, [&](auto zero) { return attention_forward<decltype(zero)>(p, a->batch, c.waves, c.apart, s); });
+}
+
+int64_t gact_attention_backward_workspace_bytes(const gact_attention* a, int dbias) {
+  if (!a || !sizes_fit(a)) return 0;
+  return bias_bytes(a) + delta_bytes(a) + (dbias ? along_units(a) * along_stride(a) * 4 : 0);
+}
+
+int gact_attention_backward(const gact_attention* a, const gact_rows* out, const float* lse, const int8_t* rest, const gact_rows* d_out,
+                            const gact_rows* dq, const gact_rows* dk, const gact_rows* dv, float* dbias, void* workspace, void* stream) {
+  int rc = check_all(a);
+  if (rc == GACT_OK) rc = check_rows(a, out, a->heads, a->queries);
+  if (rc == GACT_OK) rc = check_rows(a, d_out, a->heads, a->queries);
+  if (rc == GACT_OK && dq) rc = check_rows(a, dq, a->heads, a->queries);
+  if (rc == GACT_OK && dk) rc = check_rows(a, dk, a->kv_heads, a->keys);
+  if (rc == GACT_OK && dv) rc = check_rows(a, dv, a->kv_heads, a->keys);
+  if (rc != GACT_OK) return rc;
+  if (dbias && !a->bias) return GACT_EINVAL;
+  const bool some = a->batch > 0 && a->queries > 0;
+  if (some && !lse) return GACT_EINVAL;
+  if ((uintptr_t)rest % 8) return GACT_EALIGN;
+  if (gact_attention_backward_workspace_bytes(a, dbias != nullptr) > 0) {
+    if (!workspace) return GACT_EINVAL;
+    if (!aligned16(workspace)) return GACT_EALIGN;
+  }
+  fresh_launch();
+  const hipStream_t s = (hipStream_t)stream;
+  AttentionArgs p = args_of(a);
+  p.out = side_of(a, out, a->queries);
+  p.d_out = side_of(a, d_out, a->queries);
+  p.dq = side_of(a, dq, a->queries);
+  p.dk = side_of(a, a->keys > 0 ? dk : nullptr, a->keys);
+  p.dv = side_of(a, a->keys > 0 ? dv : nullptr, a->keys);
+  p.lse = const_cast<float*>(lse);
+  p.rest = const_cast<int8_t*>(rest);
+  rc = prepare_bias(a, p, (float*)workspace, s);
+  if (rc != GACT_OK) return rc;
+  p.delta = (float*)((char*)workspace + bias_bytes(a));
+  p.along = dbias ? (float*)((char*)p.delta + delta_bytes(a)) : nullptr;
+  p.along_stride = along_stride(a);
+  const int waves = waves_of(a->queries);
+  if (a->batch > 0) {
+    rc = with_type(a->dtype, [&](auto zero) { return attention_backward<decltype(zero)>(p, a->batch, waves, waves_of(a->keys), s); });
+    if (rc != GACT_OK) return rc;
+  }
+  if (dbias && distances(a) > 0) {
+    const AlongArgs along{p.along, p.along_stride, some ? a->batch : 0, p.heads, p.queries, p.keys, waves * 32, tile_rows(a), waves, p.causal, dbias};
+    hipLaunchKernelGGL(attention_along_kernel, dim3((unsigned)((distances(a) + 63) / 64), (unsigned)a->heads), dim3(1024), 0, s, along);
+    return launch_status();
+  }
+  return GACT_OK;
+}
+
+int gact_position_bias(const void* table, int dtype, int64_t buckets, int64_t heads, int64_t queries, int64_t keys, int both, int64_t max_distance,
+                       float* out, void* stream) {
+  if (!known(dtype)) return GACT_EINVAL;
+  return with_buckets(table, buckets, heads, queries, keys, both, max_distance, out, [&](const Buckets& b) {
+    fresh_launch();
+    return with_type(dtype, [&](auto zero) {
+      using T = decltype(zero);
+      const int distances = (int)(queries + keys - 1);
+      hipLaunchKernelGGL((position_bias_kernel<T>), dim3((unsigned)((distances + 255) / 256), (unsigned)((heads + 7) / 8)), dim3(256), 0,
+                         (hipStream_t)stream, (const T*)table, (int)heads, (int)keys, distances, b, out);
+      return launch_status();
+    });
+  });
+}
+
+int gact_position_bias_backward(const float* grad, int dtype, int64_t buckets, int64_t heads, int64_t queries, int64_t keys, int both,
+                                int64_t max_distance, void* d_table, void* stream) {
+  if (!known(dtype)) return GACT_EINVAL;
+  return with_buckets(grad, buckets, heads, queries, keys, both, max_distance, d_table, [&](const Buckets& b) {
+    fresh_launch();
+    return with_type(dtype, [&](auto zero) {
+      using T = decltype(zero);
+      hipLaunchKernelGGL((position_bias_backward_kernel<T>), dim3((unsigned)buckets, (unsigned)heads), dim3(256), 0, (hipStream_t)stream, grad,
+                         (int)heads, (int)queries, (int)keys, b, (T*)d_table);
+      return launch_status();
+    });
+  });
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-// What the two files of gact_torch.so share.
+// What the files of gact_torch.so share.
 #pragma once
 #include <torch/csrc/python_headers.h>
 
@@ -19,3 +19,5 @@ struct WithoutGil {
 };
 // the layers' functions, which the module takes beside its own
 extern PyMethodDef gact_layer_methods[];
+extern PyMethodDef gact_attention_methods[];
+extern PyMethodDef gact_adamw_methods[];

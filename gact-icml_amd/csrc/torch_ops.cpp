@@ -552,7 +552,8 @@ at::Tensor gact_torch_empty(c10::IntArrayRef shape, at::ScalarType dtype, c10::D
 PyMODINIT_FUNC PyInit_gact_torch(void) {
   static const char built_with[] = "torch " GACT_TORCH_VERSION;   // the build looks for it in the library
   PyObject* const m = PyModule_Create(&module);
-  if (m && (PyModule_AddStringConstant(m, "torch_version", built_with + 6) < 0 || PyModule_AddFunctions(m, gact_layer_methods) < 0)) {
+  if (m && (PyModule_AddStringConstant(m, "torch_version", built_with + 6) < 0 || PyModule_AddFunctions(m, gact_layer_methods) < 0 ||
+            PyModule_AddFunctions(m, gact_attention_methods) < 0 || PyModule_AddFunctions(m, gact_adamw_methods) < 0)) {
     Py_DECREF(m);
     return nullptr;
   }

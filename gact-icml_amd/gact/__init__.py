@@ -6,6 +6,6 @@ The import surface of the reference package (``gact.ops``, ``gact.controller``, 
 mixed-width path.
 """
 from .conf import config, set_adapt_interval, set_optimization_level
-from . import controller, ops
+from . import controller, ops, optim
 
-__all__ = ["config", "controller", "ops", "set_adapt_interval", "set_optimization_level"]
+__all__ = ["config", "controller", "ops", "optim", "set_adapt_interval", "set_optimization_level"]

@@ -83,6 +83,14 @@ SIGNATURES = {
     "gact_product_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64]),
     "gact_product": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
     "gact_checkpoint_product": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "gact_attention_workspace_bytes": (_i64, [_vp]),
+    "gact_attention_forward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "gact_attention_backward_workspace_bytes": (_i64, [_vp, _i32]),
+    "gact_attention_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "gact_position_bias": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i32, _i64, _vp, _vp]),
+    "gact_position_bias_backward": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i32, _i64, _vp, _vp]),
+    "gact_adamw": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp]),
+    "gact_adamw_values": (_i32, [_vp, _i64, _vp, _vp, _vp]),
 }
 
 

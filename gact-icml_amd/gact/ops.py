@@ -12,10 +12,12 @@ import math
 
 import torch
 
+from .attention import op_attention, op_position_bias  # noqa: F401
 from .conf import config
 from .cpp_extension import _abi
 from .cpp_extension import quantization as ext_quantization
 from .layers import Checkpoint, op_checkpoint, op_checkpoint_product, op_layer_norm, op_linear, op_restore  # noqa: F401
+from .optim import AdamWState, op_adamw, op_adamw_state, op_adamw_values  # noqa: F401
 
 
 # the raw HIP stream torch currently launches on for a device (what _abi.stream_of wraps), bound once: these two

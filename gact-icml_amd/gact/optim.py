@@ -1,0 +1,123 @@
+"""AdamW over many tensors at once, with its states in 8 bits or in 32.
+
+States in 8 bits take 2.06 bytes of an element where floats take 8: groups of 256 elements share the largest magnitude of either state, and a code is
+the square root of the first moment or the fourth root of the second, rounded to nearest, so that both moments of a step have the same spacing: 0.8 %
+of the largest next to it, finer below.  A second moment above zero is never rounded to zero.  Rounding is to nearest: steps are repeatable and need no seeds.
+
+``op_adamw`` is one launch for every 72 tensors of a type; parameters and states are changed in place.  Whatever cannot be taken raises a RuntimeError (a
+TypeError where no tensor was given), before anything is launched.
+"""
+import collections
+
+import torch
+
+from .cpp_extension import _abi
+
+# bits 32: float32 moments, scale None; bits 8: int8 and uint8 codes, scale float32 [groups, 2]; the moments in their parameter's shape and layout
+AdamWState = collections.namedtuple("AdamWState", "exp_avg exp_avg_sq scale")
+
+
+def op_adamw_state(param, bits=8):
+    """The state of a parameter before its first step."""
+    if bits not in (8, 32):
+        raise RuntimeError("states have 8 or 32 bits, got %r" % (bits,))
+    kinds = (torch.int8, torch.uint8) if bits == 8 else (torch.float32, torch.float32)
+    moments = [torch.zeros_like(param, dtype=kind, requires_grad=False) for kind in kinds]
+    scale = torch.zeros(-(-param.numel() // 256), 2, dtype=torch.float32, device=param.device) if bits == 8 else None
+    return AdamWState(*moments, scale)
+
+
+def op_adamw(params, grads, states, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    """One step, the step-th from 1 on, of all params: exp_avg = b1 exp_avg + (1 - b1) grad, exp_avg_sq = b2 exp_avg_sq + (1 - b2) grad^2, param =
+    param (1 - lr weight_decay) - lr / (1 - b1^step) exp_avg / (sqrt(exp_avg_sq / (1 - b2^step)) + eps), computed in float32.
+
+    params: leaves, float32, float16 or bfloat16, dense in memory in whatever order of dimensions; grads: of their shapes and types; states: an
+    AdamWState each.  step and lr: numbers, or one int64 and one float32 on the GPU, which the kernels read (a step that is recorded in a graph).
+    A group of 256 elements whose gradient has a NaN or an infinity is not finite any more where its state has 8 bits."""
+    _abi.native().adamw(params, grads, states, step, lr, betas[0], betas[1], eps, weight_decay)
+
+
+def op_adamw_values(states):
+    """(exp_avg, exp_avg_sq): what the codes of states in 8 bits stand for, float32 [elements] each, one state behind the other in their order of
+    memory."""
+    return _abi.native().adamw_values(states)
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's steps (decoupled weight decay) by op_adamw.  bits: 8 or 32, an option of every group of parameters.
+
+    capturable: the count of steps is in device memory and every step adds one to it there, so that a step can be recorded in a graph; run one step
+    before the capture, which makes the states."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=8, capturable=False):
+        if not 0.0 <= float(lr) or not 0.0 <= eps or not 0.0 <= weight_decay or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError("lr, eps and weight_decay must be 0 or more, and the betas from 0 to below 1")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits, capturable=capturable))
+
+    def add_param_group(self, param_group):
+        if param_group.get("bits", self.defaults["bits"]) not in (8, 32):
+            raise ValueError("states have 8 or 32 bits")
+        super().add_param_group(param_group)
+
+    def _begin(self, group, param, counts):
+        """The state of a parameter that has its first step.  Counts on the GPU are shared by the parameters that begin together."""
+        if group["capturable"]:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a parameter's first step cannot be captured: run one step before the capture")
+            if param.device not in counts:
+                counts[param.device] = torch.zeros((), dtype=torch.int64, device=param.device)
+        kept = op_adamw_state(param, group["bits"])
+        self.state[param] = {"step": counts[param.device] if group["capturable"] else 0, "exp_avg": kept.exp_avg, "exp_avg_sq": kept.exp_avg_sq}
+        if kept.scale is not None:
+            self.state[param]["scale"] = kept.scale
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            # parameters whose counts are the same number, or the same tensor
+            together, counts = {}, {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if not self.state[p]:
+                    self._begin(group, p, counts)
+                count = self.state[p]["step"]
+                key = id(count) if isinstance(count, torch.Tensor) else count
+                together.setdefault(key, (count, []))[1].append(p)
+            for count, params in together.values():
+                count += 1      # in place where it is a tensor
+                states = []
+                for p in params:
+                    kept = self.state[p]
+                    kept["step"] = count
+                    states.append((kept["exp_avg"], kept["exp_avg_sq"], kept.get("scale")))
+                op_adamw(params, [p.grad for p in params], states, count, group["lr"], group["betas"], group["eps"], group["weight_decay"])
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """torch's own would turn codes and scales into the parameters' type."""
+        saved = state_dict["state"]
+        super().load_state_dict({**state_dict, "state": {}})
+        numbers = [n for group in state_dict["param_groups"] for n in group["params"]]
+        params = [(group, p) for group in self.param_groups for p in group["params"]]
+        counts = {}
+        for number, (group, p) in zip(numbers, params):
+            if number not in saved:
+                continue
+            held = saved[number]
+            made = op_adamw_state(p, 8 if "scale" in held else 32)
+            kept = {"exp_avg": made.exp_avg, "exp_avg_sq": made.exp_avg_sq}
+            if made.scale is not None:
+                kept["scale"] = made.scale
+            for name, to in kept.items():
+                if held[name].dtype is not to.dtype or held[name].shape != to.shape:
+                    raise ValueError("the saved %s does not belong to its parameter" % name)
+                to.copy_(held[name])
+            step = int(held["step"])
+            if group["capturable"]:
+                step = counts.setdefault((p.device, step), torch.full((), step, dtype=torch.int64, device=p.device))
+            self.state[p] = {"step": step, **kept}

@@ -287,6 +287,81 @@ int gact_product(const void* a, int64_t lda, const void* b, int64_t ldb, int dty
 int gact_checkpoint_product(const void* grad, int64_t ldg, const void* codes, int64_t ldc, const float* scale, const float* mn, int dtype,
                             int64_t rows, int64_t outer, int64_t inner, void* out, void* workspace, void* stream);
 
+/* ---- Attention.  No counterpart in the reference. ----
+ *
+ * s_ij = scale q_i.k_j + bias[j - i + queries - 1], out_i = sum over j of softmax(s_i)_j v_j, for every batch entry and head; head h reads key head
+ * h / (heads / kv_heads).  A key is hidden from a query where its mask byte is 0, where `causal` is set and j > i + keys - queries, and where the
+ * bias is -1e30 or less; a query that sees nothing gets zeros.  What absent keys (mask byte 0) and values hold does not matter; a NaN or infinity of a
+ * key that is hidden in another way may show.
+ *
+ * Rows: [batch, heads, rows, width] of `dtype`, elements from one batch entry, head and row to the next; a row's values lie side by side, in whole
+ * 16-byte pieces, rows at least a row and at most GACT_ATTENTION_MAX_STRIDE bytes apart (GACT_EALIGN for addresses, widths and strides that are no
+ * multiples of 16 bytes).  batch, queries and keys may be 0. */
+#define GACT_ATTENTION_MAX_LENGTH 0x1000000
+#define GACT_ATTENTION_MAX_WIDTH 128
+#define GACT_ATTENTION_MAX_STRIDE 0x1000000
+typedef struct gact_rows {
+  const void* p;
+  int64_t batch, head, row;
+} gact_rows;
+typedef struct gact_attention {
+  int32_t dtype, causal;
+  int64_t batch, heads, kv_heads, queries, keys, width;
+  float scale;          /* above 0 */
+  float reserved;
+  const float* bias;    /* [heads, queries + keys - 1], may be null */
+  const uint8_t* mask;  /* [batch, keys], rows mask_stride bytes apart; may be null */
+  int64_t mask_stride;
+  gact_rows q, k, v;
+} gact_attention;
+/* lse [batch, heads, queries], which the backward pass reads (the logarithm of base 2 of each query's sum; infinite where it sees nothing), and rest
+ * [batch, queries, heads, width], 8-byte aligned, what rounding the result to 16 bits has left out of it, in eight bits each: either may be null, and rest is
+ * not written for GACT_F32.  workspace: gact_attention_workspace_bytes(), 16-byte aligned; may be null where that is 0. */
+int64_t gact_attention_workspace_bytes(const gact_attention* a);
+int gact_attention_forward(const gact_attention* a, const gact_rows* out, float* lse, int8_t* rest, void* workspace, void* stream);
+/* Recomputes the probabilities from q, k and lse; without rest (null) the result counts as it was rounded.  dq, dk, dv and dbias ([heads, queries + keys - 1]) may each be null.  Sums are made in one order:
+ * results are repeatable. */
+int64_t gact_attention_backward_workspace_bytes(const gact_attention* a, int dbias);
+int gact_attention_backward(const gact_attention* a, const gact_rows* out, const float* lse, const int8_t* rest, const gact_rows* d_out,
+                            const gact_rows* dq, const gact_rows* dk, const gact_rows* dv, float* dbias, void* workspace, void* stream);
+
+/* A bias for each head and distance d = key - query, at d + keys - 1 of [heads, queries + keys - 1], out of table [buckets, heads]; and the table's
+ * gradient.  `both`: half of the buckets for d > 0, half for the others; else all for d < 0, and those above in bucket 0.  Of one direction's buckets the
+ * first half has one distance each, bucket k behind them begins where (|d| / half)^(steps) >= (max_distance / half)^k, and the last one has no end.
+ * 2 to GACT_MAX_BUCKETS buckets, two at least to a direction; max_distance above half of a direction's. */
+#define GACT_MAX_BUCKETS 512
+int gact_position_bias(const void* table, int dtype, int64_t buckets, int64_t heads, int64_t queries, int64_t keys, int both, int64_t max_distance,
+                       float* out, void* stream);
+int gact_position_bias_backward(const float* grad, int dtype, int64_t buckets, int64_t heads, int64_t queries, int64_t keys, int both,
+                                int64_t max_distance, void* d_table, void* stream);
+
+/* ---- AdamW over many tensors.  No counterpart in the reference. ----
+ *
+ * m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2, p = p (1 - lr decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps), in
+ * floats; g and p of `dtype`, the betas and 1 - beta rounded to float.  bits 32: m and v are floats.  bits 8: m int8 and v uint8 codes of groups of
+ * 256 elements, the last one shorter, and scale [groups, 2] the largest |m| and v of each; a code c of m stands for c |c| (scale / 127^2), one of v
+ * for c^4 (scale / 255^4), with the quotients and c^4 rounded to float (255^4 to 4228250624).  A value x of m gets the code nearest to the
+ * root of |x| (127^2 / scale), one of v the nearest to its fourth root, and no v above 0 the code 0; a group whose largest |m| is below 1e-30 (v:
+ * 1e-28) has scale and codes 0.  A group with an infinity or NaN is not finite afterwards.
+ * p and g: any address that their type may have; m, v and scale 16-byte aligned.  Tensors must not overlap. */
+typedef struct gact_adamw_tensor {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* scale;
+  int64_t numel;
+} gact_adamw_tensor;
+typedef struct gact_adamw_options {
+  double lr, beta1, beta2, eps, decay;
+  int64_t step;              /* from 1 on */
+  const float* lr_at;        /* device memory: the kernel reads lr, and step, there where these are not null */
+  const int64_t* step_at;
+} gact_adamw_options;
+int gact_adamw(const gact_adamw_tensor* tensors, int64_t count, int dtype, int bits, const gact_adamw_options* options, void* stream);
+/* What the codes of `count` states stand for, one after the other, into m and v (either may be null); p, g unused. */
+int gact_adamw_values(const gact_adamw_tensor* tensors, int64_t count, float* m, float* v, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
