@@ -74,12 +74,12 @@ constexpr int row_of(int e) { return 8 * (e >> 2) + (e & 3); }
 // Rows of DP values (the width rounded up to 32) in LDS, W bytes each.  A row's pieces of 16 bytes are permuted by turn() of its number: the 16 rows of
 // which the product's first operand takes a piece each, and the four rows of which the transposing read takes 64 bytes (of floats: the rows r and r + 4
 // whose 128 bytes go together), lie in different banks.
-template <typename T, int DP>
+template <typename T, int DP, int WAVES = 4>
 struct Tile {
   using Frag = typename Matrix<T>::Frag;
   static constexpr int kEsz = (int)sizeof(T), kWide = DP * kEsz;
   static constexpr int W = kWide <= 64 ? 64 : kWide <= 128 ? 128 : kWide <= 256 ? 256 : 512;
-  static constexpr int kRows = W <= 256 ? 64 : 32;
+  static constexpr int kRows = W <= 128 || (W == 256 && WAVES == 4) ? 64 : 32;      // two tiles of either side fit a compute unit's LDS at least twice
   static constexpr int NC = kWide / 32, ND = DP / 32;
   static constexpr __device__ __forceinline__ uint32_t turn(uint32_t r) {
     const uint32_t a = r & 1, b = (r >> 1) & 1, c = (r >> 2) & 1, d = (r >> 3) & 1;
@@ -267,11 +267,11 @@ __device__ __forceinline__ void store_row(char* row, int8_t* rest, int width, in
 // hidden scores of a block of 32 rows of the tile: the lane sees rows below `seen`, and of those the ones whose bit is set
 __device__ __forceinline__ void hide(f32x16& s, int seen, uint32_t there, int lane) {
   const int g4 = 4 * (lane >> 5);
+  // as a mask of the lane's rows
+  seen -= g4;
+  there = (there >> g4) & (seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1);
 #pragma unroll
-  for (int e = 0; e < 16; e++) {
-    const bool sees = row_of(e) + g4 < seen && (there >> (row_of(e) + g4) & 1);
-    s[e] = sees ? s[e] : -__builtin_inff();
-  }
+  for (int e = 0; e < 16; e++) s[e] = there >> row_of(e) & 1 ? s[e] : -__builtin_inff();
 }
 
 // what the kernels over keys share: which keys of a tile there are.  The bytes of the next tile but one are on their way while a tile is worked on.
@@ -283,13 +283,26 @@ struct Present {
   __device__ __forceinline__ uint64_t answer() const { return mask ? __ballot(byte != 0) : ~0ull; }
 };
 
+// Waves that a SIMD is to hold: with two the compiler has 256 registers, and the products' results stay where the vector instructions reach them; beyond
+// that they pass through the matrix unit's own registers, an instruction each way for every value (a BERT-large layer's forward pass 95 us, 61 without).
+// Where the registers are too few for a kernel's rows, one.
+enum { FORWARD, FORWARD_APART, DQ, DKV };
+template <typename T, int DP>
+constexpr int waves_held(int kernel) {
+  const int wide = DP * (int)sizeof(T);
+  if (kernel == FORWARD) return wide <= 256 ? 2 : 1;
+  if (kernel == FORWARD_APART) return wide <= 128 ? 2 : 1;
+  if (kernel == DQ) return wide <= 256 && DP <= 96 ? 2 : 1;
+  return wide <= 128 ? 2 : 1;
+}
+
 // ---------------------------------------------------------------------------------------------------------------------------------
 // The forward pass.  APART: for few queries the waves of a workgroup have the same 32 rows (the queries of all heads that share a key head), take the
 // keys in turn, each in tiles of its own, and add up at the end; splits of the keys go to workgroups of their own, which join_kernel adds up.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int WAVES, bool APART, bool BIAS>
-__global__ __launch_bounds__(WAVES * 64) void attention_forward_kernel(AttentionArgs p) {
-  using Shape = Tile<T, DP>;
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(waves_held<T, DP>(APART ? FORWARD_APART : FORWARD)))) void attention_forward_kernel(AttentionArgs p) {
+  using Shape = Tile<T, DP, WAVES>;
   using Frag = typename Shape::Frag;
   constexpr int R = APART ? 32 : Shape::kRows, NB = R / 32, W = Shape::W, NC = Shape::NC, ND = Shape::ND;
   constexpr int kTile = R * W, kRing = 4 * kTile, BM = APART ? 32 : WAVES * 32;
@@ -346,7 +359,9 @@ __global__ __launch_bounds__(WAVES * 64) void attention_forward_kernel(Attention
       load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), (int64_t)key - (tile * BM + BM - 1) + p.queries - 1, BM + R - 1, wave, WAVES,
                   biases + (t & 1) * kBias, lane);
   };
-  const float unit2 = BIAS ? 1.0f : p.scale2;      // with a bias the scores are multiplied before it is added
+  // with a bias the scores are multiplied before it is added.  In vector registers: a scalar operand makes the multiplication take twice as long
+  float unit2 = BIAS ? 1.0f : p.scale2, scale2 = p.scale2;
+  asm("" : "+v"(unit2), "+v"(scale2));
   const float* const far = BIAS && APART ? p.bias + (int64_t)head * p.distances() + p.queries - 1 - query : nullptr;
   float most = -__builtin_inff(), total = 0.0f;
   f32x16 acc[ND];
@@ -367,7 +382,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_forward_kernel(Attention
     if (t + 1 < steps) issue(t + 1, next);
     present.ask(begin + (t + 2) * step + lane);
     const int key = begin + t * step;
-    if (key >= some_see) continue;
+    if (key >= some_see || !there) continue;
     const lds_u8* const keys = ring + (t & 1) * 2 * kTile;
     f32x16 s[NB];
 #pragma unroll
@@ -388,7 +403,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_forward_kernel(Attention
             add = far[key + r < p.keys ? key + r : p.keys - 1];
           else
             add = ((const __attribute__((address_space(3))) float*)(biases + (t & 1) * kBias))[r - (wave * 32 + (lane & 31)) + BM - 1];
-          s[n][e] = __builtin_fmaf(s[n][e], p.scale2, add);
+          s[n][e] = __builtin_fmaf(s[n][e], scale2, add);
         }
     }
     const bool edge = key + R > all_see || (p.mask && (R == 64 ? ~there : ~there & 0xffffffffu) != 0);
@@ -530,19 +545,41 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// dq, and do_i.o_i for the other kernel.  With a bias: the sums of ds along the diagonals, of the wave's 32 queries.  A block of 32 keys adds to 63
-// neighbouring diagonals, to which the wave's lanes add in LDS - lanes 0 to 31 and 32 to 63 each in a copy of their own, so that no two lanes add to one
-// sum at a time and the order of additions is always the same.  After a block the first 32 of the diagonals are complete and leave.
+// dq, and do_i.o_i for the other kernel.  With a bias: the sums of ds along the diagonals, for the wave's 32 queries.  Element e of a block of 32 keys is
+// key row_of(e) + 4 g of query l = 16 half + m of the lane (its row of 16 lanes: g and half); its diagonal, key - query, moves by one with either.  Shifted
+// down its row of lanes by row_of(e) mod 16, lane m has the diagonals 16 c - m + 4 g - 16 half of all elements, where c is 0 for what stays in the row,
+// 1 for what leaves it, and one more for the keys from 16 on: three running sums a lane, two additions an element that shift as they add.  After a block
+// the sums of c = 0 and 1 are complete and the one of 2 is the next block's 0.  The four rows' sums, each a sequence along c and -m, meet in LDS.
+// (Additions into LDS by the hardware's atomics, 16 a block: 750 us for 8 x 16 heads of 1000 x 1000 halves where the kernel without them takes 100.)
 // ---------------------------------------------------------------------------------------------------------------------------------
+template <int N>
+__device__ __forceinline__ float shifted(float v) {      // lane m of a row of 16: the value of lane m + N, zero behind the row's end (N < 0: before its beginning)
+  constexpr int kControl = N > 0 ? 0x100 + N : 0x110 - N;
+  const int b = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, b, kControl, 0xf, 0xf, true));
+}
+template <int E = 0>
+__device__ __forceinline__ void add_diagonals(const f32x16& s, float (&sums)[3]) {
+  if constexpr (E < 16) {
+    constexpr int kShift = row_of(E) % 16, kUp = row_of(E) / 16;
+    if constexpr (kShift == 0) {
+      sums[kUp] += s[E];
+    } else {
+      sums[kUp] += shifted<kShift>(s[E]);
+      sums[kUp + 1] += shifted<kShift - 16>(s[E]);
+    }
+    add_diagonals<E + 1>(s, sums);
+  }
+}
 template <typename T, int DP, int WAVES, bool BIAS>
-__global__ __launch_bounds__(WAVES * 64) void attention_dq_kernel(AttentionArgs p) {
-  using Shape = Tile<T, DP>;
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(waves_held<T, DP>(DQ)))) void attention_dq_kernel(AttentionArgs p) {
+  using Shape = Tile<T, DP, WAVES>;
   using Frag = typename Shape::Frag;
   constexpr int R = Shape::kRows, NB = R / 32, W = Shape::W, NC = Shape::NC, ND = Shape::ND, BM = WAVES * 32;
   constexpr int kTile = R * W, kBias = BIAS ? (BM + R + 63) / 64 * 256 : 0;
   using Load = RowsLoad<T, DP, R, WAVES>;
   __shared__ __attribute__((aligned(1024))) uint8_t memory[4 * kTile + 2 * kBias];
-  __shared__ float diagonals[BIAS ? WAVES : 1][2][64];
+  __shared__ float diagonals[BIAS ? WAVES : 1][4][64];      // the last 64 of each row's sequence
   uint32_t w;
   if (!work_of(p.blocks, w)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -603,14 +640,32 @@ __global__ __launch_bounds__(WAVES * 64) void attention_dq_kernel(AttentionArgs 
 #pragma unroll
   for (int d = 0; d < ND; d++) acc[d] = f32x16{};
   typedef __attribute__((address_space(3))) float lds_float;
-  lds_float* const sums = (lds_float*)diagonals[BIAS ? wave : 0][0];
+  lds_float* const sequence = (lds_float*)diagonals[BIAS ? wave : 0][0];
+  float sums[3] = {};
   if constexpr (BIAS) {
-    sums[lane] = 0.0f;
-    sums[64 + lane] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 4; n++) sequence[64 * n + lane] = 0.0f;
   }
+  // block k is done: numbers 32 k to 32 k + 31 of the wave's diagonals, which begin at key 0 and the last query, are complete.  Number y of a row's
+  // sequence, 16 c - m + 15, belongs to number y + 4 g + 16 (1 - half)
+  auto leave = [&](int k, float* to) __attribute__((always_inline)) {
+    const int at = (32 * k + 15 - (lane & 15)) & 63;
+    in_turn();
+    sequence[64 * (lane >> 4) + at] = sums[0];
+    sequence[64 * (lane >> 4) + ((at + 16) & 63)] = sums[1];
+    in_turn();
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 4; n++) sum += sequence[64 * n + ((32 * k + (lane & 31) - 4 * (n >> 1) - 16 * (1 - (n & 1))) & 63)];
+    if (lane < 32) to[32 * k + lane] = sum;
+    sums[0] = sums[2];
+    sums[1] = sums[2] = 0.0f;
+  };
   // of the diagonals of the wave's queries, which begin at key 0 and query first + 31
   float* const along = BIAS && p.along ? p.along + ((bh * (int64_t)p.tiles + tile) * WAVES + wave) * p.along_stride : nullptr;
 
+  float scale2 = p.scale2;
+  asm("" : "+v"(scale2));
   uint64_t there = 0, next = 0;
   present.ask(lane);
   next = present.answer();
@@ -629,7 +684,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_dq_kernel(AttentionArgs 
     const bool edge = key + R > all_see || (p.mask && (R == 64 ? ~there : ~there & 0xffffffffu) != 0);
 #pragma unroll
     for (int n = 0; n < NB; n++) {
-      if (key + 32 * n < some_see) {
+      if (key + 32 * n < some_see && there) {
         f32x16 s = {}, dp = {};
 #pragma unroll
         for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(keys, 32 * n, c, lane), q[c], s);
@@ -641,35 +696,22 @@ __global__ __launch_bounds__(WAVES * 64) void attention_dq_kernel(AttentionArgs 
           float off = -lse;
           if constexpr (BIAS)
             off += ((const lds_float*)(biases + (t & 1) * kBias))[32 * n + row_of(e) + g4 - (wave * 32 + (lane & 31)) + BM - 1];
-          s[e] = __builtin_fmaf(s[e], p.scale2, off);
+          s[e] = __builtin_fmaf(s[e], scale2, off);
         }
         if (edge) hide(s, seen - key - 32 * n, (uint32_t)(there >> (32 * n)), lane);
 #pragma unroll
         for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(s[e]) * (dp[e] - delta);
-        if constexpr (BIAS) {
-          if (along) {
-            in_turn();
-            lds_float* const mine_at = sums + (lane >> 5) * 64 + 31 - (lane & 31) + g4;
-#pragma unroll
-            for (int e = 0; e < 16; e++) __hip_atomic_fetch_add(mine_at + row_of(e), s[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-          }
-        }
+        if constexpr (BIAS)
+          if (along) add_diagonals(s, sums);
         Shape::add(acc, keys, 32 * n, s, lane);
       }
-      if constexpr (BIAS) {
-        if (along) {
-          in_turn();
-          const float a = sums[lane], c = sums[64 + lane];
-          if (lane < 32) along[key + 32 * n + lane] = a + c;
-          sums[(lane + 32) & 63] = lane < 32 ? 0.0f : a;
-          sums[64 + ((lane + 32) & 63)] = lane < 32 ? 0.0f : c;
-        }
-      }
+      if constexpr (BIAS)
+        if (along) leave((key + 32 * n) / 32, along);
     }
   }
   wait_all();
   if constexpr (BIAS)
-    if (along && lane < 32) along[steps * R + lane] = sums[lane] + sums[64 + lane];
+    if (along) leave(steps * NB, along);
   if (own && p.dq.p) store_row<T, ND>((char*)p.dq.at(b, h, query), nullptr, p.width, lane, acc, p.scale);
 }
 
@@ -677,8 +719,8 @@ __global__ __launch_bounds__(WAVES * 64) void attention_dq_kernel(AttentionArgs 
 // dk and dv: a wave has 32 keys, and the queries of all heads that share the key head pass by.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int WAVES, bool BIAS>
-__global__ __launch_bounds__(WAVES * 64) void attention_dkv_kernel(AttentionArgs p) {
-  using Shape = Tile<T, DP>;
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(waves_held<T, DP>(DKV)))) void attention_dkv_kernel(AttentionArgs p) {
+  using Shape = Tile<T, DP, WAVES>;
   using Frag = typename Shape::Frag;
   constexpr int R = Shape::kRows, NB = R / 32, W = Shape::W, NC = Shape::NC, ND = Shape::ND, BM = WAVES * 32;
   constexpr int kTile = R * W, kBias = BIAS ? (BM + R + 63) / 64 * 256 : 0, kStats = 256;
@@ -705,7 +747,11 @@ __global__ __launch_bounds__(WAVES * 64) void attention_dkv_kernel(AttentionArgs
   const int seen_from = p.causal && key > behind ? key - behind : 0;
   const int all_from = p.causal && first + 31 > behind ? first + 31 - behind : 0, some_from = p.causal && first > behind ? first - behind : 0;
   const int begin = (p.causal && tile * BM > behind ? tile * BM - behind : 0) / R * R;
-  const int per_head = begin < p.queries ? (p.queries - begin + R - 1) / R : 0, steps = per_head * p.group;
+  const int per_head = begin < p.queries ? (p.queries - begin + R - 1) / R : 0;
+  // no key of the workgroup's is there: only zeros to store
+  bool some = p.mask == nullptr;
+  for (int n = lane; n < BM && !some; n += 64) some = tile * BM + n < p.keys && p.mask[(int64_t)b * p.mask_stride + tile * BM + n];
+  const int steps = __ballot(some) ? per_head * p.group : 0;
 
   Load load_q, load_dy;
   load_q.set_up(p.q.row, p.width, wave, lane);
@@ -725,6 +771,8 @@ __global__ __launch_bounds__(WAVES * 64) void attention_dkv_kernel(AttentionArgs
 #pragma unroll
   for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
 
+  float scale2 = p.scale2;
+  asm("" : "+v"(scale2));
   if (steps > 0) issue(0);
   for (int t = 0; t < steps; t++) {
     wait_all();
@@ -753,7 +801,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_dkv_kernel(AttentionArgs
           float off = -l[e];
           if constexpr (BIAS)
             off += ((const lds_float*)(biases + (t & 1) * kBias))[wave * 32 + (lane & 31) - (32 * n + row_of(e4) + e + g4) + R - 1];
-          s[e4 + e] = __builtin_fmaf(s[e4 + e], p.scale2, off);
+          s[e4 + e] = __builtin_fmaf(s[e4 + e], scale2, off);
         }
       }
       if (edge) {

@@ -180,7 +180,11 @@ int64_t bias_bytes(const gact_attention* a) { return a->bias ? round_up(a->heads
 int64_t split_rows(const gact_attention* a, const ForwardCut& c) {
   return c.splits > 1 ? a->batch * a->kv_heads * ((a->heads / a->kv_heads * a->queries + 31) / 32) * c.splits * 32 : 0;
 }
-int tile_rows(const gact_attention* a) { return a->dtype == GACT_F32 && a->width > 64 ? 32 : 64; }
+// rows of a tile in the kernel of dq, as Tile has them
+int tile_rows(const gact_attention* a) {
+  const int64_t wide = padded_width(a) * esz(a->dtype);
+  return wide <= 128 || (wide <= 256 && waves_of(a->queries) == 4) ? 64 : 32;
+}
 int64_t along_stride(const gact_attention* a) { return round_up(a->keys, tile_rows(a)) + 32; }
 int64_t along_units(const gact_attention* a) {
   const int waves = waves_of(a->queries);
