@@ -38,6 +38,7 @@ struct AttentionArgs {
   bool causal;
   float scale, scale2;       // and times log2(e)
   uint32_t tiles, blocks;    // of a head, and in all
+  bool by_length;            // see work_of
   int splits, per_split;     // keys of a split, whole blocks of 32
   float* part;               // [tile, split][32, width rounded up]
   float* part_stats;         // [tile, split][32, 2]
@@ -79,7 +80,8 @@ struct Tile {
   using Frag = typename Matrix<T>::Frag;
   static constexpr int kEsz = (int)sizeof(T), kWide = DP * kEsz;
   static constexpr int W = kWide <= 64 ? 64 : kWide <= 128 ? 128 : kWide <= 256 ? 256 : 512;
-  static constexpr int kRows = W <= 128 || (W == 256 && WAVES == 4) ? 64 : 32;      // two tiles of either side fit a compute unit's LDS at least twice
+  // tiles of 64 rows, of which a compute unit's LDS holds two of either side at least twice; of 32 for workgroups of two waves, of which there are more
+  static constexpr int kRows = W <= 256 && WAVES == 4 ? 64 : W == 64 ? 64 : 32;
   static constexpr int NC = kWide / 32, ND = DP / 32;
   static constexpr __device__ __forceinline__ uint32_t turn(uint32_t r) {
     const uint32_t a = r & 1, b = (r >> 1) & 1, c = (r >> 2) & 1, d = (r >> 3) & 1;
@@ -92,15 +94,27 @@ struct Tile {
     const uint32_t r = lane & 31, g = lane >> 5;
     return *(const __attribute__((address_space(3))) Frag*)(tile + first * W + r * W + (((2 * c) ^ g ^ turn(r)) * 16));
   }
+  // 32 rows by 32 columns of results as an operand
+  struct Halves {
+    Frag f[2];
+  };
+  using Packed = std::conditional_t<sizeof(T) == 2, Halves, f32x16>;
+  static __device__ __forceinline__ Packed pack(const f32x16& p) {
+    if constexpr (sizeof(T) == 2) {
+      Packed k;
+#pragma unroll
+      for (int e = 0; e < 16; e++) k.f[e >> 3][e & 7] = rounded<T>(p[e]);
+      return k;
+    } else {
+      return p;
+    }
+  }
   // acc[32 values of the width, 32 columns] += the tile's rows transposed [., 32 rows] times p [32 rows, 32 columns]
-  static __device__ __forceinline__ void add(f32x16 (&acc)[ND], const lds_u8* tile, int first, const f32x16& p, int lane) {
+  static __device__ __forceinline__ void add(f32x16 (&acc)[ND], const lds_u8* tile, int first, const Packed& p, int lane) {
     const uint32_t i = lane & 15, half = (lane >> 4) & 1, g = lane >> 5;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-        Frag b;
-#pragma unroll
-        for (int e = 0; e < 8; e++) b[e] = rounded<T>(p[8 * s + e]);
 #pragma unroll
         for (int d = 0; d < ND; d++) {
           const uint32_t r = 4 * g + (i >> 2), piece = 4 * d + 2 * half + ((i & 3) >> 1);
@@ -109,7 +123,7 @@ struct Tile {
           const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo);
           const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
           const Frag a = __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-          acc[d] = Matrix<T>::run(a, b, acc[d]);
+          acc[d] = Matrix<T>::run(a, p.f[s], acc[d]);
         }
       }
     } else {
@@ -135,6 +149,8 @@ struct RowsLoad {
   using Shape = Tile<T, DP>;
   static constexpr int W = Shape::W, kLoads = ROWS * W / 1024 / WAVES;
   static_assert(kLoads >= 1, "a wave takes at least one load");
+  Window window;
+  int64_t step;
   uint32_t at[kLoads];
   int wave;
   static __device__ __forceinline__ uint32_t row(int wave, int q, int lane) { return ((wave * kLoads + q) * 1024 + lane * 16) / W; }
@@ -146,11 +162,14 @@ struct RowsLoad {
       at[q] = (int)piece * 16 < width * Shape::kEsz ? r * (uint32_t)stride + piece * 16 : kNowhere;
     }
   }
-  // from `base` on, of which `left` rows are there; absent[r]: row r is left out
-  __device__ __forceinline__ void issue(const char* base, int left, int64_t stride, int width, bool some_absent, uint64_t there, lds_u8* to, int lane) const {
-    Window window;
+  // from `base` on, of which `left` rows are there; `tiles` of ROWS rows to a step
+  __device__ __forceinline__ void start(const char* base, int64_t left, int64_t stride, int width, int tiles = 1) {
     window.base = base;
     window.left = left <= 0 ? 0 : (left - 1) * stride + width * Shape::kEsz;
+    step = tiles * ROWS * stride;
+  }
+  // the next tile, without the rows whose bit of `there` is not set
+  __device__ __forceinline__ void next(bool some_absent, uint64_t there, lds_u8* to, int lane) {
     const __amdgpu_buffer_rsrc_t rsrc = window.rsrc();
 #pragma unroll
     for (int q = 0; q < kLoads; q++) {
@@ -158,18 +177,16 @@ struct RowsLoad {
       if (some_absent && !((there >> row(wave, q, lane)) & 1)) from = kNowhere;
       load_to_lds<16>(rsrc, from, to + (wave * kLoads + q) * 1024);
     }
+    window.advance(step);
   }
 };
 
 // `count` floats from `at` on of an array of `size`, 64 to a wave's instruction; zeros where the array ends on either side
-__device__ __forceinline__ void load_floats(const float* base, int64_t size, int64_t at, int count, int turn, int waves, lds_u8* to, int lane) {
-  Window window;
-  window.base = (const char*)base;
-  window.left = size * 4;
-  const __amdgpu_buffer_rsrc_t rsrc = window.rsrc();
+__device__ __forceinline__ void load_floats(const float* base, int size, int at, int count, int turn, int waves, lds_u8* to, int lane) {
+  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, size * 4, 0x00020000);
   for (int l = turn; l * 64 < count; l += waves) {
-    const int64_t from = at + l * 64 + lane;
-    load_to_lds<4>(rsrc, from < 0 || from >= size ? kNowhere : (uint32_t)from * 4, to + l * 256);
+    const uint32_t from = (uint32_t)(at + l * 64 + lane);
+    load_to_lds<4>(rsrc, from < (uint32_t)size ? from * 4 : kNowhere, to + l * 256);
   }
 }
 
@@ -199,11 +216,25 @@ __device__ __forceinline__ float sum_of_both(float v) {
   return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
 }
 
-// Workgroups go to the 8 XCDs in turn: each XCD has a run of consecutive pieces of work, so that the tiles of a head, which read the same rows, share its L2
-__device__ __forceinline__ bool work_of(uint32_t blocks, uint32_t& w) {
-  const uint32_t id = (uint32_t)block_of(), xcd = id % 8, most = blocks / 8, rest = blocks % 8;
-  w = xcd * most + (xcd < rest ? xcd : rest) + id / 8;
-  return id < blocks;
+// Workgroups go to the 8 XCDs in turn: each XCD has a run of consecutive heads, so that the tiles of a head, which read the same rows, share its L2.
+// Where the tiles are of different lengths and the heads fill the XCDs evenly, an XCD takes all heads' longest tiles first: head by head, the last one's
+// long tiles would be left to a few compute units (two prompts of 4096 tokens 405 us, so 330).
+struct Work {
+  uint32_t tile, head;      // the tile's number in that order
+};
+__device__ __forceinline__ bool work_of(const AttentionArgs& p, uint32_t per_tile, Work& work) {
+  const uint32_t id = (uint32_t)block_of(), xcd = id % 8, i = id / 8;
+  if (id >= p.blocks) return false;
+  if (p.by_length) {
+    const uint32_t heads = p.blocks / per_tile / p.tiles / 8;
+    work.tile = i / heads;
+    work.head = xcd * heads + i % heads;
+  } else {
+    const uint32_t most = p.blocks / 8, rest = p.blocks % 8, w = xcd * most + (xcd < rest ? xcd : rest) + i;
+    work.tile = w % (p.tiles * per_tile);
+    work.head = w / (p.tiles * per_tile);
+  }
+  return true;
 }
 
 // pieces 2c and 2c + 1 of one row, from memory
@@ -264,6 +295,13 @@ __device__ __forceinline__ void store_row(char* row, int8_t* rest, int width, in
     }
 }
 
+__device__ __forceinline__ float most_of(const f32x16& s) {
+  float m = __builtin_fmaxf(s[0], s[1]);
+#pragma unroll
+  for (int e = 2; e < 16; e += 2) m = __builtin_fmaxf(m, __builtin_fmaxf(s[e], s[e + 1]));
+  return m;
+}
+
 // hidden scores of a block of 32 rows of the tile: the lane sees rows below `seen`, and of those the ones whose bit is set
 __device__ __forceinline__ void hide(f32x16& s, int seen, uint32_t there, int lane) {
   const int g4 = 4 * (lane >> 5);
@@ -279,7 +317,9 @@ struct Present {
   const uint8_t* mask;
   int keys;
   uint32_t byte = 0;
-  __device__ __forceinline__ void ask(int key) { byte = mask && key < keys ? mask[key] : 0; }
+  __device__ __forceinline__ void ask(int key) {
+    if (mask) byte = key < keys ? mask[key] : 0;
+  }
   __device__ __forceinline__ uint64_t answer() const { return mask ? __ballot(byte != 0) : ~0ull; }
 };
 
@@ -309,16 +349,15 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   constexpr int kBias = BIAS && !APART ? (BM + R + 63) / 64 * 256 : 0;
   using Load = RowsLoad<T, DP, R, APART ? 1 : WAVES>;
   __shared__ __attribute__((aligned(1024))) uint8_t memory[(APART ? WAVES : 1) * kRing + 2 * kBias];
-  uint32_t w;
-  if (!work_of(p.blocks, w)) return;
+  Work work;
+  if (!work_of(p, APART ? p.splits : 1, work)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   lds_u8* const ring = (lds_u8*)memory + (APART ? wave * kRing : 0);
   lds_u8* const biases = (lds_u8*)memory + (APART ? WAVES : 1) * kRing;
 
-  const int split = APART ? (int)(w % p.splits) : 0;
-  const uint32_t unit = APART ? w / p.splits : w;
-  const int tile = (int)(p.causal ? p.tiles - 1 - unit % p.tiles : unit % p.tiles);      // the longest first
-  const uint32_t bh = unit / p.tiles;
+  const int split = APART ? (int)(work.tile % p.splits) : 0;
+  const int turn = APART ? work.tile / p.splits : work.tile, tile = p.causal ? p.tiles - 1 - turn : turn;      // the longest first
+  const uint32_t bh = work.head;
   const int heads = APART ? p.kv_heads : p.heads, b = bh / heads, h = bh % heads;
   const int kv = APART ? h : h / p.group;
   // the lane's query; behind the last one: that one, of which nothing is stored
@@ -350,20 +389,21 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   load_k.set_up(p.k.row, p.width, APART ? 0 : wave, lane);
   load_v.set_up(p.v.row, p.width, APART ? 0 : wave, lane);
   Present present{p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.keys};
+  load_k.start(p.k.at(b, kv, begin), p.keys - begin, p.k.row, p.width, APART ? WAVES : 1);
+  load_v.start(p.v.at(b, kv, begin), p.keys - begin, p.v.row, p.width, APART ? WAVES : 1);
   auto issue = [&](int t, uint64_t there) __attribute__((always_inline)) {
-    const int key = begin + t * step;
     lds_u8* const at = ring + (t & 1) * 2 * kTile;
-    load_k.issue(p.k.at(b, kv, key), p.keys - key, p.k.row, p.width, false, there, at, lane);
-    load_v.issue(p.v.at(b, kv, key), p.keys - key, p.v.row, p.width, p.mask != nullptr, there, at + kTile, lane);      // what is absent may be a NaN
+    load_k.next(false, there, at, lane);
+    load_v.next(p.mask != nullptr, there, at + kTile, lane);      // what is absent may be a NaN
     if constexpr (kBias > 0)
-      load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), (int64_t)key - (tile * BM + BM - 1) + p.queries - 1, BM + R - 1, wave, WAVES,
+      load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), begin + t * step - (tile * BM + BM - 1) + p.queries - 1, BM + R - 1, wave, WAVES,
                   biases + (t & 1) * kBias, lane);
   };
   // with a bias the scores are multiplied before it is added.  In vector registers: a scalar operand makes the multiplication take twice as long
   float unit2 = BIAS ? 1.0f : p.scale2, scale2 = p.scale2;
   asm("" : "+v"(unit2), "+v"(scale2));
   const float* const far = BIAS && APART ? p.bias + (int64_t)head * p.distances() + p.queries - 1 - query : nullptr;
-  float most = -__builtin_inff(), total = 0.0f;
+  float most = -__builtin_inff(), limit = most, off = 0.0f, total = 0.0f;
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; d++) acc[d] = f32x16{};
@@ -384,17 +424,16 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     const int key = begin + t * step;
     if (key >= some_see || !there) continue;
     const lds_u8* const keys = ring + (t & 1) * 2 * kTile;
-    f32x16 s[NB];
+    const bool edge = key + R > all_see || (p.mask && (R == 64 ? ~there : ~there & 0xffffffffu) != 0);
+    auto scores = [&](int n) __attribute__((always_inline)) {
+      f32x16 s = {};
 #pragma unroll
-    for (int n = 0; n < NB; n++) {
-      s[n] = f32x16{};
-#pragma unroll
-      for (int c = 0; c < NC; c++) s[n] = Matrix<T>::run(Shape::direct(keys, 32 * n, c, lane), q[c], s[n]);
-    }
-    if constexpr (BIAS) {
-      const int g4 = 4 * (lane >> 5);
-#pragma unroll
-      for (int n = 0; n < NB; n++)
+      for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(keys, 32 * n, c, lane), q[c], s);
+      return s;
+    };
+    auto add_bias = [&](int n, f32x16& s) __attribute__((always_inline)) {
+      if constexpr (BIAS) {
+        const int g4 = 4 * (lane >> 5);
 #pragma unroll
         for (int e = 0; e < 16; e++) {
           const int r = 32 * n + row_of(e) + g4;
@@ -403,38 +442,42 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
             add = far[key + r < p.keys ? key + r : p.keys - 1];
           else
             add = ((const __attribute__((address_space(3))) float*)(biases + (t & 1) * kBias))[r - (wave * 32 + (lane & 31)) + BM - 1];
-          s[n][e] = __builtin_fmaf(s[n][e], scale2, add);
+          s[e] = __builtin_fmaf(s[e], scale2, add);
         }
+      }
+    };
+    f32x16 s[NB];
+#pragma unroll
+    for (int n = 0; n < NB; n++) s[n] = scores(n);
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      add_bias(n, s[n]);
+      if (edge) hide(s[n], seen - key - 32 * n, (uint32_t)(there >> (32 * n)), lane);
     }
-    const bool edge = key + R > all_see || (p.mask && (R == 64 ? ~there : ~there & 0xffffffffu) != 0);
-    if (edge) {
+    float m = most_of(s[0]);
 #pragma unroll
-      for (int n = 0; n < NB; n++) hide(s[n], seen - key - 32 * n, (uint32_t)(there >> (32 * n)), lane);
-    }
-    float m = -__builtin_inff();
-#pragma unroll
-    for (int n = 0; n < NB; n++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) m = __builtin_fmaxf(m, s[n][e]);
-    m = most_of_both(m);
+    for (int n = 1; n < NB; n++) m = __builtin_fmaxf(m, most_of(s[n]));
     // the maximum follows when it is left behind by 2^8, which probabilities of every type hold: mostly in the first tile alone
-    if (__ballot(m > most + 8.0f / unit2)) {
-      m = __builtin_fmaxf(m, most);
+    if (__ballot(m > limit)) {
+      m = __builtin_fmaxf(most_of_both(m), most);
       const float factor = m > most ? __builtin_amdgcn_exp2f((most - m) * unit2) : 1.0f;
       most = m;
+      off = m == -__builtin_inff() ? 0.0f : m * unit2;
+      limit = m + 8.0f / unit2;
       total *= factor;
 #pragma unroll
       for (int d = 0; d < ND; d++) acc[d] *= factor;
     }
-    const float off = most == -__builtin_inff() ? 0.0f : most * unit2;
 #pragma unroll
     for (int n = 0; n < NB; n++) {
+      float sum[2] = {};
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         s[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], unit2, -off));
-        total += s[n][e];
+        sum[e & 1] += s[n][e];
       }
-      Shape::add(acc, keys + kTile, 32 * n, s[n], lane);
+      total += sum[0] + sum[1];
+      Shape::add(acc, keys + kTile, 32 * n, Shape::pack(s[n]), lane);
     }
   }
   wait_all();
@@ -473,7 +516,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     }
     const bool whole = p.splits == 1;
     const float scale = !whole ? 1.0f : total > 0.0f ? 1.0f / total : total;
-    const int64_t place = ((int64_t)unit * p.splits + split) * 32 + (lane & 31);
+    const int64_t place = (((int64_t)bh * p.tiles + tile) * p.splits + split) * 32 + (lane & 31);
     char* const row = (char*)p.out.at(b, head, query);
 #pragma unroll
     for (int n = 0; n < kShare; n += 4) {
@@ -512,11 +555,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p) {
   const int rows = p.group * p.queries, row = (int)(at % rows), lane = threadIdx.x % kLanes, down = threadIdx.x / kLanes;
   const int64_t bh = at / rows;
   if (bh >= (int64_t)(p.blocks / p.splits / p.tiles)) return;
-  const int tile = row / 32;
-  const uint32_t unit = (uint32_t)(bh * p.tiles + (p.causal ? p.tiles - 1 - tile : tile));
-  const int64_t first = (int64_t)unit * p.splits * 32 + row % 32;
+  const int64_t first = (bh * p.tiles + row / 32) * p.splits * 32 + row % 32;
+  __shared__ float mosts[4];
   float most = -__builtin_inff();
-  for (int s = 0; s < p.splits; s++) most = __builtin_fmaxf(most, p.part_stats[(first + 32 * (int64_t)s) * 2]);
+  for (int s = threadIdx.x; s < p.splits; s += 256) most = __builtin_fmaxf(most, p.part_stats[(first + 32 * (int64_t)s) * 2]);
+  most = over_lanes<Most, 64>(most);
+  if ((threadIdx.x & 63) == 0) mosts[threadIdx.x >> 6] = most;
+  __syncthreads();
+  most = __builtin_fmaxf(__builtin_fmaxf(mosts[0], mosts[1]), __builtin_fmaxf(mosts[2], mosts[3]));
   f32x4 sum = {};
   float total = 0.0f;
   if (down < kDown) {
@@ -580,13 +626,13 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   using Load = RowsLoad<T, DP, R, WAVES>;
   __shared__ __attribute__((aligned(1024))) uint8_t memory[4 * kTile + 2 * kBias];
   __shared__ float diagonals[BIAS ? WAVES : 1][4][64];      // the last 64 of each row's sequence
-  uint32_t w;
-  if (!work_of(p.blocks, w)) return;
+  Work work;
+  if (!work_of(p, 1, work)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   lds_u8* const ring = (lds_u8*)memory;
   lds_u8* const biases = ring + 4 * kTile;
-  const int tile = (int)(p.causal ? p.tiles - 1 - w % p.tiles : w % p.tiles);
-  const uint32_t bh = w / p.tiles;
+  const int tile = p.causal ? p.tiles - 1 - work.tile : work.tile;
+  const uint32_t bh = work.head;
   const int b = bh / p.heads, h = bh % p.heads, kv = h / p.group;
   const int first = tile * BM + wave * 32, mine = first + (lane & 31), last = tile * BM + BM - 1;
   const bool own = mine < p.queries;
@@ -627,14 +673,14 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   load_k.set_up(p.k.row, p.width, wave, lane);
   load_v.set_up(p.v.row, p.width, wave, lane);
   Present present{p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.keys};
+  load_k.start(p.k.at(b, kv, 0), p.keys, p.k.row, p.width);
+  load_v.start(p.v.at(b, kv, 0), p.keys, p.v.row, p.width);
   auto issue = [&](int t, uint64_t there) __attribute__((always_inline)) {
-    const int key = t * R;
     lds_u8* const to = ring + (t & 1) * 2 * kTile;
-    load_k.issue(p.k.at(b, kv, key), p.keys - key, p.k.row, p.width, p.mask != nullptr, there, to, lane);
-    load_v.issue(p.v.at(b, kv, key), p.keys - key, p.v.row, p.width, p.mask != nullptr, there, to + kTile, lane);
+    load_k.next(p.mask != nullptr, there, to, lane);
+    load_v.next(p.mask != nullptr, there, to + kTile, lane);
     if constexpr (BIAS)
-      load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), (int64_t)key - last + p.queries - 1, BM + R - 1, wave, WAVES,
-                  biases + (t & 1) * kBias, lane);
+      load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), t * R - last + p.queries - 1, BM + R - 1, wave, WAVES, biases + (t & 1) * kBias, lane);
   };
   f32x16 acc[ND];
 #pragma unroll
@@ -682,31 +728,35 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     const int key = t * R;
     const lds_u8* const keys = ring + (t & 1) * 2 * kTile;
     const bool edge = key + R > all_see || (p.mask && (R == 64 ? ~there : ~there & 0xffffffffu) != 0);
+    auto product = [&](const lds_u8* rows, int n, const Frag (&own)[NC]) __attribute__((always_inline)) {
+      f32x16 s = {};
+#pragma unroll
+      for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(rows, 32 * n, c, lane), own[c], s);
+      return s;
+    };
+    // ds of a block from its scores and dp; `hidden`: with some of them hidden
+    auto gradient = [&](int n, f32x16 s, const f32x16& dp, bool hidden) __attribute__((always_inline)) {
+      const int g4 = 4 * (lane >> 5);
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        float off = -lse;
+        if constexpr (BIAS)
+          off += ((const lds_float*)(biases + (t & 1) * kBias))[32 * n + row_of(e) + g4 - (wave * 32 + (lane & 31)) + BM - 1];
+        s[e] = __builtin_fmaf(s[e], scale2, off);
+      }
+      if (hidden) hide(s, seen - key - 32 * n, (uint32_t)(there >> (32 * n)), lane);
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(s[e]) * (dp[e] - delta);
+      if constexpr (BIAS)
+        if (along) add_diagonals(s, sums);
+      return s;
+    };
 #pragma unroll
     for (int n = 0; n < NB; n++) {
-      if (key + 32 * n < some_see && there) {
-        f32x16 s = {}, dp = {};
-#pragma unroll
-        for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(keys, 32 * n, c, lane), q[c], s);
-#pragma unroll
-        for (int c = 0; c < NC; c++) dp = Matrix<T>::run(Shape::direct(keys + kTile, 32 * n, c, lane), dy[c], dp);
-        const int g4 = 4 * (lane >> 5);
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          float off = -lse;
-          if constexpr (BIAS)
-            off += ((const lds_float*)(biases + (t & 1) * kBias))[32 * n + row_of(e) + g4 - (wave * 32 + (lane & 31)) + BM - 1];
-          s[e] = __builtin_fmaf(s[e], scale2, off);
-        }
-        if (edge) hide(s, seen - key - 32 * n, (uint32_t)(there >> (32 * n)), lane);
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(s[e]) * (dp[e] - delta);
-        if constexpr (BIAS)
-          if (along) add_diagonals(s, sums);
-        Shape::add(acc, keys, 32 * n, s, lane);
-      }
+      if (key + 32 * n < some_see && there)
+        Shape::add(acc, keys, 32 * n, Shape::pack(gradient(n, product(keys, n, q), product(keys + kTile, n, dy), edge)), lane);
       if constexpr (BIAS)
-        if (along) leave((key + 32 * n) / 32, along);
+        if (along) leave(key / 32 + n, along);
     }
   }
   wait_all();
@@ -728,14 +778,14 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   typedef __attribute__((address_space(3))) float lds_float;
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
   __shared__ __attribute__((aligned(1024))) uint8_t memory[4 * kTile + 4 * kStats + 2 * kBias];
-  uint32_t w;
-  if (!work_of(p.blocks, w)) return;
+  Work work;
+  if (!work_of(p, 1, work)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   lds_u8* const ring = (lds_u8*)memory;
   lds_u8* const stats = ring + 4 * kTile;
   lds_u8* const biases = stats + 4 * kStats;
-  const int tile = (int)(w % p.tiles);
-  const uint32_t bh = w / p.tiles;
+  const int tile = work.tile;
+  const uint32_t bh = work.head;
   const int b = bh / p.kv_heads, kv = bh % p.kv_heads;
   const int first = tile * BM + wave * 32, key = first + (lane & 31);
   const bool own = key < p.keys && (!p.mask || p.mask[(int64_t)b * p.mask_stride + key]);
@@ -756,16 +806,25 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   Load load_q, load_dy;
   load_q.set_up(p.q.row, p.width, wave, lane);
   load_dy.set_up(p.d_out.row, p.width, wave, lane);
+  // the next tile to load: of head `head`, from query `ahead` on
+  int head = kv * p.group, ahead = begin;
+  const float* stat = nullptr;
   auto issue = [&](int t) __attribute__((always_inline)) {
-    const int head = kv * p.group + t / per_head, query = begin + t % per_head * R;
+    if (ahead >= p.queries || t == 0) {
+      if (t) head++;
+      ahead = begin;
+      load_q.start(p.q.at(b, head, begin), p.queries - begin, p.q.row, p.width);
+      load_dy.start(p.d_out.at(b, head, begin), p.queries - begin, p.d_out.row, p.width);
+      stat = (wave ? p.delta : p.lse) + ((int64_t)b * p.heads + head) * p.queries;
+    }
     lds_u8* const to = ring + (t & 1) * 2 * kTile;
-    load_q.issue(p.q.at(b, head, query), p.queries - query, p.q.row, p.width, false, 0, to, lane);
-    load_dy.issue(p.d_out.at(b, head, query), p.queries - query, p.d_out.row, p.width, false, 0, to + kTile, lane);
-    const int64_t at = ((int64_t)b * p.heads + head) * p.queries;
-    if (wave < 2) load_floats((wave ? p.delta : p.lse) + at, p.queries, query, R, 0, 1, stats + (2 * (t & 1) + wave) * kStats, lane);
+    load_q.next(false, 0, to, lane);
+    load_dy.next(false, 0, to + kTile, lane);
+    if (wave < 2) load_floats(stat, p.queries, ahead, R, 0, 1, stats + (2 * (t & 1) + wave) * kStats, lane);
     if constexpr (BIAS)
-      load_floats(p.bias + (int64_t)head * p.distances(), p.distances(), (int64_t)tile * BM - (query + R - 1) + p.queries - 1, BM + R - 1, wave, WAVES,
+      load_floats(p.bias + (int64_t)head * p.distances(), p.distances(), tile * BM - (ahead + R - 1) + p.queries - 1, BM + R - 1, wave, WAVES,
                   biases + (t & 1) * kBias, lane);
+    ahead += R;
   };
   f32x16 dk[ND], dv[ND];
 #pragma unroll
@@ -773,25 +832,28 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
 
   float scale2 = p.scale2;
   asm("" : "+v"(scale2));
+  int now = begin;
   if (steps > 0) issue(0);
   for (int t = 0; t < steps; t++) {
     wait_all();
     meet();
     __builtin_amdgcn_sched_barrier(0);
     if (t + 1 < steps) issue(t + 1);
-    const int query = begin + t % per_head * R;
+    const int query = now;
+    now += R;
+    if (now >= p.queries) now = begin;
     const lds_u8* const rows = ring + (t & 1) * 2 * kTile;
     const lds_float* const lse = (const lds_float*)(stats + 2 * (t & 1) * kStats);
     const lds_float* const delta = (const lds_float*)(stats + (2 * (t & 1) + 1) * kStats);
     const bool edge = query < all_from || query + R > p.queries;
+    auto product = [&](const lds_u8* from, int n, const Frag (&own)[NC]) __attribute__((always_inline)) {
+      f32x16 s = {};
 #pragma unroll
-    for (int n = 0; n < NB; n++) {
-      if (query + 32 * n + 31 < some_from || query + 32 * n >= p.queries) continue;
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(rows, 32 * n, c, lane), k[c], s);
-#pragma unroll
-      for (int c = 0; c < NC; c++) dp = Matrix<T>::run(Shape::direct(rows + kTile, 32 * n, c, lane), v[c], dp);
+      for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(from, 32 * n, c, lane), own[c], s);
+      return s;
+    };
+    // a block's scores to probabilities, and dp to ds
+    auto gradient = [&](int n, f32x16& s, f32x16& dp, bool hidden) __attribute__((always_inline)) {
       const int g4 = 4 * (lane >> 5);
 #pragma unroll
       for (int e4 = 0; e4 < 16; e4 += 4) {
@@ -804,12 +866,10 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
           s[e4 + e] = __builtin_fmaf(s[e4 + e], scale2, off);
         }
       }
-      if (edge) {
+      if (hidden) {
+        const int from = seen_from - query - 32 * n - g4, to = p.queries - query - 32 * n - g4;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const int i = query + 32 * n + row_of(e) + g4;
-          s[e] = i >= seen_from && i < p.queries ? s[e] : -__builtin_inff();
-        }
+        for (int e = 0; e < 16; e++) s[e] = row_of(e) >= from && row_of(e) < to ? s[e] : -__builtin_inff();
       }
 #pragma unroll
       for (int e4 = 0; e4 < 16; e4 += 4) {
@@ -820,8 +880,14 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
           dp[e4 + e] = s[e4 + e] * (dp[e4 + e] - x[e]);
         }
       }
-      Shape::add(dv, rows + kTile, 32 * n, s, lane);
-      Shape::add(dk, rows, 32 * n, dp, lane);
+    };
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+      if (query + 32 * n + 31 < some_from || query + 32 * n >= p.queries) continue;
+      f32x16 s = product(rows, n, k), dp = product(rows + kTile, n, v);
+      gradient(n, s, dp, edge);
+      Shape::add(dv, rows + kTile, 32 * n, Shape::pack(s), lane);
+      Shape::add(dk, rows, 32 * n, Shape::pack(dp), lane);
     }
   }
   wait_all();
@@ -869,6 +935,7 @@ int attention_forward(AttentionArgs p, int64_t batch, int waves, bool apart, hip
     const int64_t tall = apart ? 32 : waves * 32, tiles = (rows + tall - 1) / tall, blocks = heads * tiles * (apart ? p.splits : 1);
     p.tiles = (uint32_t)tiles;
     p.blocks = (uint32_t)blocks;
+    p.by_length = p.causal && !apart && heads % 8 == 0;
     if (apart) {
       const int rc = p.bias ? launch(attention_forward_kernel<T, DP, A, true, true>, blocks, A * 64, p, s)
                             : launch(attention_forward_kernel<T, DP, A, true, false>, blocks, A * 64, p, s);
@@ -889,6 +956,7 @@ int attention_backward(AttentionArgs p, int64_t batch, int waves_dq, int waves_d
       const int64_t tiles = (rows + waves * 32 - 1) / (waves * 32);
       p.tiles = (uint32_t)tiles;
       p.blocks = (uint32_t)(heads * tiles);
+      p.by_length = p.causal && heads % 8 == 0;
       return heads * tiles;
     };
     const int64_t blocks = shape(batch * p.heads, p.queries, waves_dq);

@@ -37,18 +37,26 @@ __global__ __launch_bounds__(1024) void attention_along_kernel(AlongArgs p) {
   __shared__ float shared[16][64];
   const int distances = p.queries + p.keys - 1, t = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6, h = blockIdx.y;
   const int blocks = (p.queries + 31) / 32, tiles = (p.queries + p.tall - 1) / p.tall;
+  // a wave has every 16th block of queries of the batch entries in turn; diagonal t is number t + 32 (k + 1) - queries of block k, from 0 on
   float sum = 0.0f;
-  if (t < distances) {
-    // the blocks whose diagonals t is among: of block k they are t + 32 (k + 1) - queries, from 0 on
-    for (int64_t n = wave; n < p.batch * blocks; n += 16) {
-      const int64_t b = n / blocks;
-      const int k = (int)(n - b * blocks), at = t + 32 * (k + 1) - p.queries, tile = 32 * k / p.tall;
-      const int last = tile * p.tall + p.tall - 1 < p.queries ? tile * p.tall + p.tall - 1 : p.queries - 1;
-      int to = last + p.keys - p.queries + 1;
-      to = !p.causal || to > p.keys ? p.keys : to < 0 ? 0 : to;
-      if (at >= 0 && at < (to + p.rows - 1) / p.rows * p.rows + 32)
-        sum += p.along[((b * p.heads + h) * tiles * p.waves + k) * p.stride + at];
+  for (int k = wave; k < blocks; k += 16) {
+    const int at = t + 32 * (k + 1) - p.queries, tile = 32 * k / p.tall;
+    const int last = tile * p.tall + p.tall - 1 < p.queries ? tile * p.tall + p.tall - 1 : p.queries - 1;
+    int to = last + p.keys - p.queries + 1;
+    to = !p.causal || to > p.keys ? p.keys : to < 0 ? 0 : to;
+    if (t >= distances || at < 0 || at >= (to + p.rows - 1) / p.rows * p.rows + 32) continue;
+    const float* from = p.along + ((int64_t)h * tiles * p.waves + k) * p.stride + at;
+    const int64_t apart = (int64_t)p.heads * tiles * p.waves * p.stride;
+    int64_t b = 0;
+    for (; b + 8 <= p.batch; b += 8) {      // eight loads on their way at a time
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) v[u] = from[u * apart];
+#pragma unroll
+      for (int u = 0; u < 8; u++) sum += v[u];
+      from += 8 * apart;
     }
+    for (; b < p.batch; b++, from += apart) sum += *from;
   }
   shared[wave][threadIdx.x & 63] = sum;
   __syncthreads();
@@ -183,7 +191,7 @@ int64_t split_rows(const gact_attention* a, const ForwardCut& c) {
 // rows of a tile in the kernel of dq, as Tile has them
 int tile_rows(const gact_attention* a) {
   const int64_t wide = padded_width(a) * esz(a->dtype);
-  return wide <= 128 || (wide <= 256 && waves_of(a->queries) == 4) ? 64 : 32;
+  return (wide <= 256 && waves_of(a->queries) == 4) || wide <= 64 ? 64 : 32;
 }
 int64_t along_stride(const gact_attention* a) { return round_up(a->keys, tile_rows(a)) + 32; }
 int64_t along_units(const gact_attention* a) {
