@@ -303,7 +303,9 @@ __device__ __forceinline__ float most_of(const f32x16& s) {
 }
 
 // hidden scores of a block of 32 rows of the tile: the lane sees rows below `seen`, and of those the ones whose bit is set
+// (the empty statement keeps the branch around it: without one the compiler makes the selections for every block)
 __device__ __forceinline__ void hide(f32x16& s, int seen, uint32_t there, int lane) {
+  asm volatile("");
   const int g4 = 4 * (lane >> 5);
   // as a mask of the lane's rows
   seen -= g4;
@@ -867,6 +869,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
         }
       }
       if (hidden) {
+        asm volatile("");
         const int from = seen_from - query - 32 * n - g4, to = p.queries - query - 32 * n - g4;
 #pragma unroll
         for (int e = 0; e < 16; e++) s[e] = row_of(e) >= from && row_of(e) < to ? s[e] : -__builtin_inff();
