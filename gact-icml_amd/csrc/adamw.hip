@@ -78,7 +78,6 @@ __device__ __forceinline__ float nearest_fourth_root(float w) {
   if (reaches(w, c + 0.5f)) c += 1.0f;
   return c;
 }
-__device__ __forceinline__ uint32_t byte_of(uint32_t w, int e) { return (w >> (8 * e)) & 0xff; }
 // what a code stands for
 __device__ __forceinline__ float first_of(uint32_t code, float unit) {
   const float c = (float)(int8_t)code;
@@ -89,14 +88,129 @@ __device__ __forceinline__ float second_of(uint32_t code, float unit) {
   return square * square * unit;
 }
 
-// m and v of eight elements, and the step; sums with the product rounded together with them
+// m, v and p of an element after the step; sums with the product rounded together with them
 __device__ __forceinline__ void advance(const Rates& r, float g, float& m, float& v, float& p) {
   m = __builtin_fmaf(m, r.beta1, g * r.rest1);
   v = __builtin_fmaf(v, r.beta2, g * g * r.rest2);
   p = __builtin_fmaf(-r.step, m / __builtin_fmaf(sqrtf(v), r.root, r.eps), p * r.keep);
 }
 
-// 32 lanes have a group, eight elements each.  Bound by memory: 16 bytes an element of floats with states in 8 bits, 28 with states in floats.
+// N neighbouring elements, of which `left` are there; WHOLE: all of them, at a multiple of their size
+template <typename T, int N>
+struct Piece {
+  typedef T V __attribute__((ext_vector_type(N)));
+  typedef T Loose __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  template <bool WHOLE>
+  static __device__ __forceinline__ V load(const T* p, int64_t left) {
+    V v = {};
+    if (WHOLE) return *(const V*)p;
+    if (left >= N) return *(const Loose*)p;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+      if (e < left) v[e] = p[e];
+    return v;
+  }
+  template <bool WHOLE>
+  static __device__ __forceinline__ void store(T* p, int64_t left, V v) {
+    if (WHOLE) {
+      *(V*)p = v;
+    } else if (left >= N) {
+      *(Loose*)p = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; e++)
+        if (e < left) p[e] = v[e];
+    }
+  }
+};
+
+// 32 lanes have a group, eight elements each.  Bound by memory.  States in 8 bits: the eight lie side by side (302 million floats 890 us, 5.4 TB/s; four of
+// either half of the group, so that an instruction loads and stores whole lines of floats but codes by four, 1060).  States in floats: four of either half
+// (75 million bfloat16 values 311 us, 5.3 TB/s, eight side by side the same).  Nontemporal loads and stores, and fewer workgroups to a compute unit, change
+// nothing or cost 3 %.
+template <typename T, bool CODES, bool WHOLE>
+__device__ __forceinline__ void step_group(const gact_adamw_tensor& t, const Rates& r, int64_t group, int64_t left_over) {
+  constexpr int N = CODES ? 8 : 4, kPieces = kVec / N;
+  const int lane = threadIdx.x % kLanes;
+  const int64_t begin = group * kGroup;
+  typename Piece<T, N>::V p[kPieces], g[kPieces];
+  typename Piece<uint8_t, N>::V cm[kPieces], cv[kPieces];
+  typename Piece<float, N>::V fm[kPieces], fv[kPieces];
+  f32x2 unit = {};
+  int64_t at[kPieces], left[kPieces];
+#pragma unroll
+  for (int k = 0; k < kPieces; k++) {
+    const int col = k * (kGroup / kPieces) + lane * N;
+    at[k] = begin + col;
+    left[k] = left_over - col;
+    p[k] = Piece<T, N>::template load<WHOLE>((const T*)t.p + at[k], left[k]);
+    g[k] = Piece<T, N>::template load<WHOLE>((const T*)t.g + at[k], left[k]);
+    if constexpr (CODES) {
+      cm[k] = Piece<uint8_t, N>::template load<WHOLE>((const uint8_t*)t.m + at[k], left[k]);
+      cv[k] = Piece<uint8_t, N>::template load<WHOLE>((const uint8_t*)t.v + at[k], left[k]);
+    } else {
+      fm[k] = Piece<float, N>::template load<WHOLE>((const float*)t.m + at[k], left[k]);
+      fv[k] = Piece<float, N>::template load<WHOLE>((const float*)t.v + at[k], left[k]);
+    }
+  }
+  if constexpr (CODES) {
+    if (WHOLE || left_over > 0) unit = *(const f32x2*)(t.scale + 2 * group);
+    unit = f32x2{unit[0] / kSquare, unit[1] / kFourth};
+  }
+  float most_m = 0.0f, most_v = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kPieces; k++)
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      float m, v, x = (float)p[k][e];
+      if constexpr (CODES) {
+        m = first_of(cm[k][e], unit[0]);
+        v = second_of(cv[k][e], unit[1]);
+      } else {
+        m = fm[k][e];
+        v = fv[k][e];
+      }
+      advance(r, (float)g[k][e], m, v, x);
+      p[k][e] = rounded<T>(x);
+      fm[k][e] = m;
+      fv[k][e] = v;
+      if (CODES && (WHOLE || e < left[k])) {
+        most_m = MostBits::of(most_m, __builtin_fabsf(m));
+        most_v = MostBits::of(most_v, __builtin_fabsf(v));
+      }
+    }
+#pragma unroll
+  for (int k = 0; k < kPieces; k++) Piece<T, N>::template store<WHOLE>((T*)t.p + at[k], left[k], p[k]);
+  if constexpr (!CODES) {
+#pragma unroll
+    for (int k = 0; k < kPieces; k++) {
+      Piece<float, N>::template store<WHOLE>((float*)t.m + at[k], left[k], fm[k]);
+      Piece<float, N>::template store<WHOLE>((float*)t.v + at[k], left[k], fv[k]);
+    }
+    return;
+  }
+  most_m = over_lanes<MostBits, kLanes>(most_m);
+  most_v = over_lanes<MostBits, kLanes>(most_v);
+  if (most_m < kLeastM) most_m = 0.0f;
+  if (most_v < kLeastV) most_v = 0.0f;
+  const float inv_m = most_m == 0.0f ? 0.0f : kSquare / most_m, inv_v = most_v == 0.0f ? 0.0f : kFourth / most_v;
+#pragma unroll
+  for (int k = 0; k < kPieces; k++) {
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const float c = nearest_root(__builtin_fabsf(fm[k][e]) * inv_m);
+      float f = nearest_fourth_root(fv[k][e] * inv_v);
+      if (fv[k][e] > 0.0f && most_v > 0.0f && f < 1.0f) f = 1.0f;
+      const int code = c > 0.0f ? (int)c : 0;      // a NaN becomes 0
+      cm[k][e] = (uint8_t)(fm[k][e] < 0.0f ? -code : code);
+      cv[k][e] = (uint8_t)(f > 0.0f ? (uint32_t)f : 0u);
+    }
+    Piece<uint8_t, N>::template store<WHOLE>((uint8_t*)t.m + at[k], left[k], cm[k]);
+    Piece<uint8_t, N>::template store<WHOLE>((uint8_t*)t.v + at[k], left[k], cv[k]);
+  }
+  if (lane == 0 && (WHOLE || left_over > 0)) *(f32x2*)(t.scale + 2 * group) = f32x2{most_m, most_v};
+}
+
 template <typename T, bool CODES>
 __global__ __launch_bounds__(256) void adamw_kernel(Tensors a, Step step) {
   __shared__ Rates made;
@@ -111,137 +225,43 @@ __global__ __launch_bounds__(256) void adamw_kernel(Tensors a, Step step) {
   if (block >= a.first[a.count]) return;
   const int which = __builtin_amdgcn_readfirstlane(tensor_of(a, block));
   const gact_adamw_tensor& t = a.t[which];
-  const int64_t group = (int64_t)(block - a.first[which]) * (256 / kLanes) + threadIdx.x / kLanes, at = group * kGroup + threadIdx.x % kLanes * kVec;
-  const int64_t left = t.numel - at;
-  T* const p = (T*)t.p + at;
-  const T* const g = (const T*)t.g + at;
-  const bool whole = (((uintptr_t)t.p | (uintptr_t)t.g) & 15) == 0 && left >= kVec;
-  float x[kVec], d[kVec], m[kVec], v[kVec];
-  if (whole) {
-    load8(p, x);
-    load8(g, d);
-  } else {
-    load_cols<T, false>(p, left, x);
-    load_cols<T, false>(g, left, d);
-  }
-  if constexpr (CODES) {
-    uint8_t* const mc = (uint8_t*)t.m + at;
-    uint8_t* const vc = (uint8_t*)t.v + at;
-    u32x2 cm = {}, cv = {};
-    f32x2 unit = {};
-    if (left >= kVec) {
-      cm = *(const u32x2*)mc;
-      cv = *(const u32x2*)vc;
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; e++)
-        if (e < left) {
-          cm[e >> 2] |= (uint32_t)mc[e] << (8 * (e & 3));
-          cv[e >> 2] |= (uint32_t)vc[e] << (8 * (e & 3));
-        }
-    }
-    if (group * kGroup < t.numel) unit = *(const f32x2*)(t.scale + 2 * group);
-    unit = f32x2{unit[0] / kSquare, unit[1] / kFourth};
-    float most_m = 0.0f, most_v = 0.0f;
-#pragma unroll
-    for (int e = 0; e < kVec; e++) {
-      m[e] = first_of(byte_of(cm[e >> 2], e & 3), unit[0]);
-      v[e] = second_of(byte_of(cv[e >> 2], e & 3), unit[1]);
-      advance(r, d[e], m[e], v[e], x[e]);
-      if (e < left) {
-        most_m = MostBits::of(most_m, __builtin_fabsf(m[e]));
-        most_v = MostBits::of(most_v, __builtin_fabsf(v[e]));
-      }
-    }
-    most_m = over_lanes<MostBits, kLanes>(most_m);
-    most_v = over_lanes<MostBits, kLanes>(most_v);
-    if (most_m < kLeastM) most_m = 0.0f;
-    if (most_v < kLeastV) most_v = 0.0f;
-    const float inv_m = most_m == 0.0f ? 0.0f : kSquare / most_m, inv_v = most_v == 0.0f ? 0.0f : kFourth / most_v;
-    cm = u32x2{};
-    cv = u32x2{};
-#pragma unroll
-    for (int e = 0; e < kVec; e++) {
-      const float c = nearest_root(__builtin_fabsf(m[e]) * inv_m);
-      float f = nearest_fourth_root(v[e] * inv_v);
-      if (v[e] > 0.0f && most_v > 0.0f && f < 1.0f) f = 1.0f;
-      const int code = c > 0.0f ? (int)c : 0;      // a NaN becomes 0
-      cm[e >> 2] |= ((uint32_t)(m[e] < 0.0f ? -code : code) & 0xff) << (8 * (e & 3));
-      cv[e >> 2] |= (f > 0.0f ? (uint32_t)f & 0xff : 0) << (8 * (e & 3));
-    }
-    if (left >= kVec) {
-      *(u32x2*)mc = cm;
-      *(u32x2*)vc = cv;
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; e++)
-        if (e < left) {
-          mc[e] = (uint8_t)byte_of(cm[e >> 2], e & 3);
-          vc[e] = (uint8_t)byte_of(cv[e >> 2], e & 3);
-        }
-    }
-    if (threadIdx.x % kLanes == 0 && left > 0) *(f32x2*)(t.scale + 2 * group) = f32x2{most_m, most_v};
-  } else {
-    float* const mf = (float*)t.m + at;
-    float* const vf = (float*)t.v + at;
-    if (left >= kVec) {
-      load8(mf, m);
-      load8(vf, v);
-    } else {
-      load_cols<float, false>(mf, left, m);
-      load_cols<float, false>(vf, left, v);
-    }
-#pragma unroll
-    for (int e = 0; e < kVec; e++) advance(r, d[e], m[e], v[e], x[e]);
-    if (left >= kVec) {
-      store8(mf, m);
-      store8(vf, v);
-    } else {
-      store_cols<float, false>(mf, left, m);
-      store_cols<float, false>(vf, left, v);
-    }
-  }
+  const int64_t first = (int64_t)(block - a.first[which]) * (256 / kLanes), group = first + threadIdx.x / kLanes;
+  // the block's groups are whole and lie at multiples of 16 bytes
+  const bool whole = (((uintptr_t)t.p | (uintptr_t)t.g) & 15) == 0 && (first + 256 / kLanes) * kGroup <= t.numel;
   if (whole)
-    store8(p, x);
+    step_group<T, CODES, true>(t, r, group, t.numel - group * kGroup);
   else
-    store_cols<T, false>(p, left, x);
+    step_group<T, CODES, false>(t, r, group, t.numel - group * kGroup);
 }
 
-// the same lanes; t.p and t.g: where a tensor's values go
+// What codes stand for: one of the moments to a block (blockIdx.z), four elements of either half of a group to a lane, so that an instruction stores whole
+// lines; t.p and t.g: where a tensor's values go.  302 million elements 496 us (6.1 TB/s); eight side by side and both moments in turn 703.
 __global__ __launch_bounds__(256) void adamw_values_kernel(Tensors a) {
   const uint32_t block = (uint32_t)block_of();
   if (block >= a.first[a.count]) return;
   const int which = __builtin_amdgcn_readfirstlane(tensor_of(a, block));
   const gact_adamw_tensor& t = a.t[which];
-  const int64_t group = (int64_t)(block - a.first[which]) * (256 / kLanes) + threadIdx.x / kLanes, at = group * kGroup + threadIdx.x % kLanes * kVec;
-  const int64_t left = t.numel - at;
-  if (left <= 0) return;
-  const f32x2 scale = *(const f32x2*)(t.scale + 2 * group);
-  auto one = [&](const uint8_t* codes, float* to, auto value) __attribute__((always_inline)) {
-    if (!to) return;
-    float x[kVec];
-    u32x2 c = {};
-    if (left >= kVec) {
-      c = *(const u32x2*)(codes + at);
-    } else {
+  const bool second = blockIdx.z == 1;
+  float* const to = (float*)(second ? const_cast<void*>(t.g) : t.p);
+  const uint8_t* const codes = (const uint8_t*)(second ? t.v : t.m);
+  if (!to) return;
+  const int64_t group = (int64_t)(block - a.first[which]) * (256 / kLanes) + threadIdx.x / kLanes;
+  const int64_t at = group * kGroup + threadIdx.x % kLanes * 4, left = t.numel - at;
+  typedef Piece<uint8_t, 4> Codes;
+  const Codes::V c[2] = {Codes::load<false>(codes + at, left), Codes::load<false>(codes + at + kGroup / 2, left - kGroup / 2)};
+  const float unit = (group * kGroup < t.numel ? t.scale[2 * group + second] : 0.0f) / (second ? kFourth : kSquare);
 #pragma unroll
-      for (int e = 0; e < kVec; e++)
-        if (e < left) c[e >> 2] |= (uint32_t)codes[at + e] << (8 * (e & 3));
-    }
+  for (int k = 0; k < 2; k++) {
+    f32x4 x;
 #pragma unroll
-    for (int e = 0; e < kVec; e++) x[e] = value(byte_of(c[e >> 2], e & 3));
-    if (((uintptr_t)to & 15) == 0 && left >= kVec)
-      store8(to + at, x);
-    else
-      store_cols<float, false>(to + at, left, x);
-  };
-  one((const uint8_t*)t.m, (float*)t.p, [&](uint32_t c) { return first_of(c, scale[0] / kSquare); });
-  one((const uint8_t*)t.v, (float*)const_cast<void*>(t.g), [&](uint32_t c) { return second_of(c, scale[1] / kFourth); });
+    for (int e = 0; e < 4; e++) x[e] = second ? second_of(c[k][e], unit) : first_of(c[k][e], unit);
+    Piece<float, 4>::store<false>(to + at + k * (kGroup / 2), left - k * (kGroup / 2), x);
+  }
 }
 
 // `run` for each launch's worth of the tensors that have elements
 template <typename F>
-int in_launches(const gact_adamw_tensor* tensors, int64_t count, F&& run) {
+int in_launches(const gact_adamw_tensor* tensors, int64_t count, int groups, F&& run) {
   Tensors a;
   a.count = 0;
   a.first[0] = 0;
@@ -252,7 +272,7 @@ int in_launches(const gact_adamw_tensor* tensors, int64_t count, F&& run) {
       a.count = 0;
     }
     if (i == count || tensors[i].numel == 0) continue;
-    const int64_t blocks = (tensors[i].numel + 8 * kGroup - 1) / (8 * kGroup);
+    const int64_t blocks = (tensors[i].numel + groups * kGroup - 1) / (groups * kGroup);
     // a launch counts its blocks in 31 bits; a tensor of as many goes on its own
     if (a.count && a.first[a.count] + blocks > 0x7fffffff) {
       const int rc = run(a);
@@ -293,7 +313,7 @@ int gact_adamw(const gact_adamw_tensor* tensors, int64_t count, int dtype, int b
   }
   fresh_launch();
   const Step step{o, rates_of(o, o.lr, (double)(o.step_at ? 1 : o.step))};
-  return in_launches(tensors, count, [&](const Tensors& a) {
+  return in_launches(tensors, count, 256 / kLanes, [&](const Tensors& a) {
     return with_type(dtype, [&](auto zero) {
       using T = decltype(zero);
       auto kernel = bits == 8 ? adamw_kernel<T, true> : adamw_kernel<T, false>;
@@ -311,13 +331,15 @@ int gact_adamw_values(const gact_adamw_tensor* tensors, int64_t count, float* m,
   }
   fresh_launch();
   int64_t next = 0;      // the launches' tensors are the list's, in order, without the empty ones
-  return in_launches(tensors, count, [&](Tensors& a) {
+  return in_launches(tensors, count, 256 / kLanes, [&](Tensors& a) {
     for (int i = 0; i < a.count; i++) {
       a.t[i].p = m ? m + next : nullptr;
       a.t[i].g = v ? v + next : nullptr;
       next += a.t[i].numel;
     }
-    hipLaunchKernelGGL(adamw_values_kernel, grid_of(a.first[a.count], 256), dim3(256), 0, (hipStream_t)stream, a);
+    dim3 grid = grid_of(a.first[a.count], 256);
+    grid.z = 2;
+    hipLaunchKernelGGL(adamw_values_kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
     return launch_status();
   });
 }
