@@ -109,8 +109,39 @@ struct Tile {
       return p;
     }
   }
-  // acc[32 values of the width, 32 columns] += the tile's rows transposed [., 32 rows] times p [32 rows, 32 columns]
-  static __device__ __forceinline__ void add(f32x16 (&acc)[ND], const lds_u8* tile, int first, const Packed& p, int lane) {
+  // what rounding p has left out
+  static __device__ __forceinline__ Packed rest(const f32x16& p, const Packed& k) {
+    f32x16 r = {};
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) r[e] = p[e] - (float)k.f[e >> 3][e & 7];
+    }
+    return pack(r);
+  }
+  // the sum of what a lane has of it
+  static __device__ __forceinline__ float sum(const Packed& p) {
+    float s[2] = {};
+    if constexpr (sizeof(T) == 2) {
+      typedef T T2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        [[maybe_unused]] const T2 v = {p.f[e >> 3][e & 7], p.f[e >> 3][(e & 7) + 1]}, one = {(T)1.0f, (T)1.0f};
+#ifdef __HIP_DEVICE_COMPILE__
+        if constexpr (std::is_same<T, bf16>::value)
+          s[(e >> 1) & 1] = __builtin_amdgcn_fdot2_f32_bf16(v, one, s[(e >> 1) & 1], false);
+        else
+          s[(e >> 1) & 1] = __builtin_amdgcn_fdot2(v, one, s[(e >> 1) & 1], false);
+#endif
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e & 1] += p[e];
+    }
+    return s[0] + s[1];
+  }
+  // acc[32 values of the width, 32 columns] += the tile's rows transposed [., 32 rows] times p [32 rows, 32 columns]; and times `more`
+  template <bool TWICE = false>
+  static __device__ __forceinline__ void add(f32x16 (&acc)[ND], const lds_u8* tile, int first, const Packed& p, int lane, const Packed* more = nullptr) {
     const uint32_t i = lane & 15, half = (lane >> 4) & 1, g = lane >> 5;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -124,6 +155,7 @@ struct Tile {
           const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
           const Frag a = __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
           acc[d] = Matrix<T>::run(a, p.f[s], acc[d]);
+          if constexpr (TWICE) acc[d] = Matrix<T>::run(a, more->f[s], acc[d]);
         }
       }
     } else {
@@ -249,7 +281,7 @@ __device__ __forceinline__ void own_row(const char* row, bool there, int width, 
 }
 // What a result of 16 bits leaves out of a float, in eight bits: at most half a step, 2^-8 (bfloat16) or 2^-11 of the value's power of two, in 127ths.
 // ds_ij = p_ij (do_i.v_j - do_i.o_i) is a difference of nearly equal numbers where one key has most of the probability: with o as it was rounded
-// dq and dk were off by 0.0040 of their norm (bfloat16, scores of deviation 2) where the other roundings leave 0.0024; a byte of each o is what that takes.
+// dq and dk were off by 0.0040 of their norm (bfloat16, scores of deviation 2) where the other roundings leave 0.0025; a byte of each o is what that takes.
 template <typename T>
 struct Rest {
   static constexpr bool kept = sizeof(T) == 2;
@@ -472,14 +504,12 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     }
 #pragma unroll
     for (int n = 0; n < NB; n++) {
-      float sum[2] = {};
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        s[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], unit2, -off));
-        sum[e & 1] += s[n][e];
-      }
-      total += sum[0] + sum[1];
-      Shape::add(acc, keys + kTile, 32 * n, Shape::pack(s[n]), lane);
+      for (int e = 0; e < 16; e++) s[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], unit2, -off));
+      // the sum is of the probabilities as they enter the product: where one key has nearly all of a query's, its rounding cancels in the quotient
+      const typename Shape::Packed k = Shape::pack(s[n]);
+      total += Shape::sum(k);
+      Shape::add(acc, keys + kTile, 32 * n, k, lane);
     }
   }
   wait_all();
@@ -755,8 +785,19 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     };
 #pragma unroll
     for (int n = 0; n < NB; n++) {
-      if (key + 32 * n < some_see && there)
-        Shape::add(acc, keys, 32 * n, Shape::pack(gradient(n, product(keys, n, q), product(keys + kTile, n, dy), edge)), lane);
+      if (key + 32 * n < some_see && there) {
+        const f32x16 ds = gradient(n, product(keys, n, q), product(keys + kTile, n, dy), edge);
+        const typename Shape::Packed k = Shape::pack(ds);
+        if constexpr (sizeof(T) == 2) {
+          // A query's ds add up to zero, and few of them are large: their roundings do not average out as dk's do.  What they leave out makes a product of
+          // its own (bfloat16, dq 0.0029 of its norm off without and 0.0021 with it, of which 0.0017 is the result's rounding; a BERT-large layer's
+          // 73 us become 85)
+          const typename Shape::Packed more = Shape::rest(ds, k);
+          Shape::template add<true>(acc, keys, 32 * n, k, lane, &more);
+        } else {
+          Shape::add(acc, keys, 32 * n, k, lane);
+        }
+      }
       if constexpr (BIAS)
         if (along) leave(key / 32 + n, along);
     }
