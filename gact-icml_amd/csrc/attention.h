@@ -39,9 +39,11 @@ struct AttentionArgs {
   float scale, scale2;       // and times log2(e)
   uint32_t tiles, blocks;    // of a head, and in all
   bool by_length;            // see work_of
-  int splits, per_split;     // keys of a split, whole blocks of 32
-  float* part;               // [tile, split][32, width rounded up]
-  float* part_stats;         // [tile, split][32, 2]
+  int splits, per_split;     // of the other side; keys of a split, whole blocks of 32 (in the backward pass whole tiles)
+  // the forward pass: [tile, split][32, width rounded up], and [tile, split][32, 2]; dq: [split][head, row of its tiles][width rounded up]; dk and dv the
+  // same, one behind the other
+  float* part;
+  float* part_stats;
   // keys that query i sees
   __device__ __forceinline__ int seen(int i) const {
     const int n = i + keys - queries + 1;
@@ -332,6 +334,18 @@ __device__ __forceinline__ float most_of(const f32x16& s) {
 #pragma unroll
   for (int e = 2; e < 16; e += 2) m = __builtin_fmaxf(m, __builtin_fmaxf(s[e], s[e + 1]));
   return m;
+}
+
+// the same of a split, to be added up and multiplied later
+template <int DP, int ND>
+__device__ __forceinline__ void store_part(float* row, int width, int lane, const f32x16 (&acc)[ND]) {
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int col = 32 * d + row_of(e) + 4 * (lane >> 5);
+      if (col < width) *(f32x4*)(row + col) = f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
+    }
 }
 
 // hidden scores of a block of 32 rows of the tile: the lane sees rows below `seen`, and of those the ones whose bit is set
@@ -659,11 +673,11 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   __shared__ __attribute__((aligned(1024))) uint8_t memory[4 * kTile + 2 * kBias];
   __shared__ float diagonals[BIAS ? WAVES : 1][4][64];      // the last 64 of each row's sequence
   Work work;
-  if (!work_of(p, 1, work)) return;
+  if (!work_of(p, p.splits, work)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   lds_u8* const ring = (lds_u8*)memory;
   lds_u8* const biases = ring + 4 * kTile;
-  const int tile = p.causal ? p.tiles - 1 - work.tile : work.tile;
+  const int split = work.tile % p.splits, turn = work.tile / p.splits, tile = p.causal ? p.tiles - 1 - turn : turn;
   const uint32_t bh = work.head;
   const int b = bh / p.heads, h = bh % p.heads, kv = h / p.group;
   const int first = tile * BM + wave * 32, mine = first + (lane & 31), last = tile * BM + BM - 1;
@@ -694,25 +708,27 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       }
     }
     delta = sum_of_both(delta);
-    if (own && lane < 32) p.delta[at] = delta;
+    if (own && lane < 32 && split == 0) p.delta[at] = delta;
   }
   const int seen = p.seen(query);
   const int all_see = p.seen(first < p.queries ? first : p.queries - 1), some_see = p.seen(first + 31 < p.queries ? first + 31 : p.queries - 1);
-  const int to = p.seen(last < p.queries ? last : p.queries - 1);
-  const int steps = to > 0 ? (to + R - 1) / R : 0;
+  const int from = split * p.per_split;
+  int to = p.seen(last < p.queries ? last : p.queries - 1);
+  if (p.splits > 1 && from + p.per_split < to) to = from + p.per_split;
+  const int steps = to > from ? (to - from + R - 1) / R : 0;
 
   Load load_k, load_v;
   load_k.set_up(p.k.row, p.width, wave, lane);
   load_v.set_up(p.v.row, p.width, wave, lane);
   Present present{p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.keys};
-  load_k.start(p.k.at(b, kv, 0), p.keys, p.k.row, p.width);
-  load_v.start(p.v.at(b, kv, 0), p.keys, p.v.row, p.width);
+  load_k.start(p.k.at(b, kv, from), p.keys - from, p.k.row, p.width);
+  load_v.start(p.v.at(b, kv, from), p.keys - from, p.v.row, p.width);
   auto issue = [&](int t, uint64_t there) __attribute__((always_inline)) {
     lds_u8* const to = ring + (t & 1) * 2 * kTile;
     load_k.next(p.mask != nullptr, there, to, lane);
     load_v.next(p.mask != nullptr, there, to + kTile, lane);
     if constexpr (BIAS)
-      load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), t * R - last + p.queries - 1, BM + R - 1, wave, WAVES, biases + (t & 1) * kBias, lane);
+      load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), from + t * R - last + p.queries - 1, BM + R - 1, wave, WAVES, biases + (t & 1) * kBias, lane);
   };
   f32x16 acc[ND];
 #pragma unroll
@@ -724,7 +740,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
 #pragma unroll
     for (int n = 0; n < 4; n++) sequence[64 * n + lane] = 0.0f;
   }
-  // block k is done: numbers 32 k to 32 k + 31 of the wave's diagonals, which begin at key 0 and the last query, are complete.  Number y of a row's
+  // block k is done: numbers 32 k to 32 k + 31 of the wave's diagonals, which begin at the first key and the last query, are complete.  Number y of a row's
   // sequence, 16 c - m + 15, belongs to number y + 4 g + 16 (1 - half)
   auto leave = [&](int k, float* to) __attribute__((always_inline)) {
     const int at = (32 * k + 15 - (lane & 15)) & 63;
@@ -739,16 +755,16 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     sums[0] = sums[2];
     sums[1] = sums[2] = 0.0f;
   };
-  // of the diagonals of the wave's queries, which begin at key 0 and query first + 31
-  float* const along = BIAS && p.along ? p.along + ((bh * (int64_t)p.tiles + tile) * WAVES + wave) * p.along_stride : nullptr;
+  // of the diagonals of the wave's queries, which begin at the split's first key and query first + 31
+  float* const along = BIAS && p.along ? p.along + (((bh * (int64_t)p.tiles + tile) * WAVES + wave) * p.splits + split) * p.along_stride : nullptr;
 
   float scale2 = p.scale2;
   asm("" : "+v"(scale2));
   uint64_t there = 0, next = 0;
-  present.ask(lane);
+  present.ask(from + lane);
   next = present.answer();
   if (steps > 0) issue(0, next);
-  present.ask(R + lane);
+  present.ask(from + R + lane);
   for (int t = 0; t < steps; t++) {
     wait_all();
     meet();
@@ -756,8 +772,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     there = next;
     next = present.answer();
     if (t + 1 < steps) issue(t + 1, next);
-    present.ask((t + 2) * R + lane);
-    const int key = t * R;
+    present.ask(from + (t + 2) * R + lane);
+    const int key = from + t * R;
     const lds_u8* const keys = ring + (t & 1) * 2 * kTile;
     const bool edge = key + R > all_see || (p.mask && (R == 64 ? ~there : ~there & 0xffffffffu) != 0);
     auto product = [&](const lds_u8* rows, int n, const Frag (&own)[NC]) __attribute__((always_inline)) {
@@ -799,13 +815,17 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
         }
       }
       if constexpr (BIAS)
-        if (along) leave(key / 32 + n, along);
+        if (along) leave(t * NB + n, along);
     }
   }
   wait_all();
   if constexpr (BIAS)
     if (along) leave(steps * NB, along);
-  if (own && p.dq.p) store_row<T, ND>((char*)p.dq.at(b, h, query), nullptr, p.width, lane, acc, p.scale);
+  if (!own || !p.dq.p) return;
+  if (p.splits > 1)
+    store_part<DP, ND>(p.part + (((int64_t)split * (p.blocks / p.splits / p.tiles) + bh) * p.tiles * BM + mine) * DP, p.width, lane, acc);
+  else
+    store_row<T, ND>((char*)p.dq.at(b, h, query), nullptr, p.width, lane, acc, p.scale);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -822,12 +842,12 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
   __shared__ __attribute__((aligned(1024))) uint8_t memory[4 * kTile + 4 * kStats + 2 * kBias];
   Work work;
-  if (!work_of(p, 1, work)) return;
+  if (!work_of(p, p.splits, work)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   lds_u8* const ring = (lds_u8*)memory;
   lds_u8* const stats = ring + 4 * kTile;
   lds_u8* const biases = stats + 4 * kStats;
-  const int tile = work.tile;
+  const int split = work.tile % p.splits, tile = work.tile / p.splits;
   const uint32_t bh = work.head;
   const int b = bh / p.kv_heads, kv = bh % p.kv_heads;
   const int first = tile * BM + wave * 32, key = first + (lane & 31);
@@ -844,20 +864,29 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   // no key of the workgroup's is there: only zeros to store
   bool some = p.mask == nullptr;
   for (int n = lane; n < BM && !some; n += 64) some = tile * BM + n < p.keys && p.mask[(int64_t)b * p.mask_stride + tile * BM + n];
-  const int steps = __ballot(some) ? per_head * p.group : 0;
+  // the split's share of the tiles of queries of all heads, one after the other
+  const int all_steps = __ballot(some) ? per_head * p.group : 0;
+  const int first_step = (int)((int64_t)all_steps * split / p.splits), steps = (int)((int64_t)all_steps * (split + 1) / p.splits) - first_step;
 
   Load load_q, load_dy;
   load_q.set_up(p.q.row, p.width, wave, lane);
   load_dy.set_up(p.d_out.row, p.width, wave, lane);
   // the next tile to load: of head `head`, from query `ahead` on
   int head = kv * p.group, ahead = begin;
+  if (steps > 0) {
+    head += first_step / per_head;
+    ahead += first_step % per_head * R;
+  }
+  int now = ahead;
   const float* stat = nullptr;
   auto issue = [&](int t) __attribute__((always_inline)) {
     if (ahead >= p.queries || t == 0) {
-      if (t) head++;
-      ahead = begin;
-      load_q.start(p.q.at(b, head, begin), p.queries - begin, p.q.row, p.width);
-      load_dy.start(p.d_out.at(b, head, begin), p.queries - begin, p.d_out.row, p.width);
+      if (t) {
+        head++;
+        ahead = begin;
+      }
+      load_q.start(p.q.at(b, head, ahead), p.queries - ahead, p.q.row, p.width);
+      load_dy.start(p.d_out.at(b, head, ahead), p.queries - ahead, p.d_out.row, p.width);
       stat = (wave ? p.delta : p.lse) + ((int64_t)b * p.heads + head) * p.queries;
     }
     lds_u8* const to = ring + (t & 1) * 2 * kTile;
@@ -875,7 +904,6 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
 
   float scale2 = p.scale2;
   asm("" : "+v"(scale2));
-  int now = begin;
   if (steps > 0) issue(0);
   for (int t = 0; t < steps; t++) {
     wait_all();
@@ -942,8 +970,44 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
 #pragma unroll
     for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
   }
+  if (p.splits > 1) {
+    const int64_t heads = p.blocks / p.splits / p.tiles, row = ((split * heads + bh) * p.tiles * BM + key) * DP;
+    if (p.dk.p) store_part<DP, ND>(p.part + row, p.width, lane, dk);
+    if (p.dv.p) store_part<DP, ND>(p.part + p.splits * heads * p.tiles * BM * DP + row, p.width, lane, dv);
+    return;
+  }
   if (p.dk.p) store_row<T, ND>((char*)p.dk.at(b, kv, key), nullptr, p.width, lane, dk, p.scale * there);
   if (p.dv.p) store_row<T, ND>((char*)p.dv.at(b, kv, key), nullptr, p.width, lane, dv, there);
+}
+
+// out = factor times the sum of the splits' rows, in their order; which of two outputs: blockIdx.z.  Four columns to a lane.
+struct PartRows {
+  const float* part[2];
+  Side out[2];
+  float factor[2];
+  int64_t rows;              // of all heads
+  int heads, length, padded, splits, width;
+};
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attention_add_kernel(PartRows p) {
+  constexpr int kLanes = DP / 4, kDown = 256 / kLanes;
+  const int lane = threadIdx.x % kLanes, down = threadIdx.x / kLanes;
+  const int64_t row = block_of() * kDown + down;
+  if (down >= kDown || row >= p.rows || lane * 4 >= p.width) return;
+  const int64_t bh = row / p.length, n = row - bh * p.length, apart = p.rows / p.length * p.padded * DP;
+  const int z = blockIdx.z;
+  const float* from = p.part[z] + (bh * p.padded + n) * DP + lane * 4;
+  f32x4 sum = {};
+  int k = 0;
+  for (; k + 4 <= p.splits; k += 4) {
+    f32x4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) v[u] = *(const f32x4*)(from + (k + u) * apart);
+#pragma unroll
+    for (int u = 0; u < 4; u++) sum += v[u];
+  }
+  for (; k < p.splits; k++) sum += *(const f32x4*)(from + k * apart);
+  store4<T>((char*)p.out[z].at(bh / p.heads, bh % p.heads, n), nullptr, lane * 4, sum * p.factor[z]);
 }
 
 // ---- launches ----
@@ -992,27 +1056,58 @@ int attention_forward(AttentionArgs p, int64_t batch, int waves, bool apart, hip
                   : launch(attention_forward_kernel<T, DP, 4, false, false>, blocks, 256, p, s);
   });
 }
+template <typename T, int DP>
+int add_parts(const PartRows& p, int outputs, hipStream_t s) {
+  constexpr int kDown = 256 / (DP / 4);
+  const int64_t blocks = (p.rows + kDown - 1) / kDown;
+  if (!blocks_fit(blocks)) return GACT_ELIMIT;
+  dim3 grid = grid_of(blocks, 256);
+  grid.z = outputs;
+  hipLaunchKernelGGL((attention_add_kernel<T, DP>), grid, dim3(256), 0, s, p);
+  return launch_status();
+}
+// how a kernel of the backward pass is cut: waves of a workgroup, splits of the other side, keys of a split
+struct BackwardCut {
+  int waves, splits, per_split;
+};
 template <typename T>
-int attention_backward(AttentionArgs p, int64_t batch, int waves_dq, int waves_dkv, hipStream_t s) {
+int attention_backward(AttentionArgs p, int64_t batch, BackwardCut for_dq, BackwardCut for_dkv, hipStream_t s) {
   return with_width(p.width, [&](auto width) {
     constexpr int DP = decltype(width)::value;
-    auto shape = [&](int64_t heads, int64_t rows, int waves) {
-      const int64_t tiles = (rows + waves * 32 - 1) / (waves * 32);
+    auto shape = [&](int64_t heads, int64_t rows, const BackwardCut& cut) {
+      const int64_t tiles = (rows + cut.waves * 32 - 1) / (cut.waves * 32);
+      p.splits = cut.splits;
+      p.per_split = cut.per_split;
       p.tiles = (uint32_t)tiles;
-      p.blocks = (uint32_t)(heads * tiles);
+      p.blocks = (uint32_t)(heads * tiles * cut.splits);
       p.by_length = p.causal && heads % 8 == 0;
-      return heads * tiles;
+      return heads * tiles * cut.splits;
     };
-    const int64_t blocks = shape(batch * p.heads, p.queries, waves_dq);
+    const int64_t blocks = shape(batch * p.heads, p.queries, for_dq);
     int rc;
-    if (waves_dq == 2)
+    if (for_dq.waves == 2)
       rc = p.bias ? launch(attention_dq_kernel<T, DP, 2, true>, blocks, 128, p, s) : launch(attention_dq_kernel<T, DP, 2, false>, blocks, 128, p, s);
     else
       rc = p.bias ? launch(attention_dq_kernel<T, DP, 4, true>, blocks, 256, p, s) : launch(attention_dq_kernel<T, DP, 4, false>, blocks, 256, p, s);
+    if (rc == GACT_OK && for_dq.splits > 1 && p.dq.p && blocks > 0) {
+      const int padded = (int)p.tiles * for_dq.waves * 32;
+      rc = add_parts<T, DP>(PartRows{{p.part, nullptr}, {p.dq, p.dq}, {p.scale, 0.0f}, batch * p.heads * p.queries, p.heads, p.queries, padded, p.splits, p.width}, 1, s);
+    }
     if (rc != GACT_OK || !(p.dk.p || p.dv.p)) return rc;
-    const int64_t others = shape(batch * p.kv_heads, p.keys, waves_dkv);
-    if (waves_dkv == 2)
-      return p.bias ? launch(attention_dkv_kernel<T, DP, 2, true>, others, 128, p, s) : launch(attention_dkv_kernel<T, DP, 2, false>, others, 128, p, s);
-    return p.bias ? launch(attention_dkv_kernel<T, DP, 4, true>, others, 256, p, s) : launch(attention_dkv_kernel<T, DP, 4, false>, others, 256, p, s);
+    const int64_t others = shape(batch * p.kv_heads, p.keys, for_dkv);
+    if (for_dkv.waves == 2)
+      rc = p.bias ? launch(attention_dkv_kernel<T, DP, 2, true>, others, 128, p, s) : launch(attention_dkv_kernel<T, DP, 2, false>, others, 128, p, s);
+    else
+      rc = p.bias ? launch(attention_dkv_kernel<T, DP, 4, true>, others, 256, p, s) : launch(attention_dkv_kernel<T, DP, 4, false>, others, 256, p, s);
+    if (rc != GACT_OK || for_dkv.splits == 1 || others == 0) return rc;
+    const int padded = (int)p.tiles * for_dkv.waves * 32;
+    const float* const of_v = p.part + (int64_t)p.splits * batch * p.kv_heads * padded * DP;
+    PartRows rows{{p.part, of_v}, {p.dk, p.dv}, {p.scale, 1.0f}, batch * p.kv_heads * p.keys, p.kv_heads, p.keys, padded, p.splits, p.width};
+    if (!p.dk.p) {      // dv alone
+      rows.part[0] = of_v;
+      rows.out[0] = p.dv;
+      rows.factor[0] = 1.0f;
+    }
+    return add_parts<T, DP>(rows, p.dk.p && p.dv.p ? 2 : 1, s);
   });
 }

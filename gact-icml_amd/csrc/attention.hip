@@ -6,9 +6,9 @@
 extern template int attention_forward<float>(AttentionArgs, int64_t, int, bool, hipStream_t);
 extern template int attention_forward<f16>(AttentionArgs, int64_t, int, bool, hipStream_t);
 extern template int attention_forward<bf16>(AttentionArgs, int64_t, int, bool, hipStream_t);
-extern template int attention_backward<float>(AttentionArgs, int64_t, int, int, hipStream_t);
-extern template int attention_backward<f16>(AttentionArgs, int64_t, int, int, hipStream_t);
-extern template int attention_backward<bf16>(AttentionArgs, int64_t, int, int, hipStream_t);
+extern template int attention_backward<float>(AttentionArgs, int64_t, BackwardCut, BackwardCut, hipStream_t);
+extern template int attention_backward<f16>(AttentionArgs, int64_t, BackwardCut, BackwardCut, hipStream_t);
+extern template int attention_backward<bf16>(AttentionArgs, int64_t, BackwardCut, BackwardCut, hipStream_t);
 
 namespace {
 
@@ -29,7 +29,7 @@ struct AlongArgs {
   const float* along;
   int64_t stride;
   int64_t batch;
-  int heads, queries, keys, tall, rows, waves;     // queries of a workgroup, rows of a tile, waves
+  int heads, queries, keys, tall, rows, waves, splits, per_split;     // queries of a workgroup, rows of a tile, waves
   bool causal;
   float* out;
 };
@@ -37,16 +37,19 @@ __global__ __launch_bounds__(1024) void attention_along_kernel(AlongArgs p) {
   __shared__ float shared[16][64];
   const int distances = p.queries + p.keys - 1, t = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6, h = blockIdx.y;
   const int blocks = (p.queries + 31) / 32, tiles = (p.queries + p.tall - 1) / p.tall;
-  // a wave has every 16th block of queries of the batch entries in turn; diagonal t is number t + 32 (k + 1) - queries of block k, from 0 on
+  // a wave has every 16th of the blocks of queries and the splits of their keys, for the batch entries in turn; diagonal t is number
+  // t + 32 (k + 1) - queries of block k from its first key on
   float sum = 0.0f;
-  for (int k = wave; k < blocks; k += 16) {
-    const int at = t + 32 * (k + 1) - p.queries, tile = 32 * k / p.tall;
+  for (int n = wave; n < blocks * p.splits; n += 16) {
+    const int k = n / p.splits, from_key = n % p.splits * p.per_split, tile = 32 * k / p.tall;
     const int last = tile * p.tall + p.tall - 1 < p.queries ? tile * p.tall + p.tall - 1 : p.queries - 1;
     int to = last + p.keys - p.queries + 1;
-    to = !p.causal || to > p.keys ? p.keys : to < 0 ? 0 : to;
-    if (t >= distances || at < 0 || at >= (to + p.rows - 1) / p.rows * p.rows + 32) continue;
-    const float* from = p.along + ((int64_t)h * tiles * p.waves + k) * p.stride + at;
-    const int64_t apart = (int64_t)p.heads * tiles * p.waves * p.stride;
+    to = !p.causal || to > p.keys ? p.keys : to;
+    if (p.splits > 1 && to > from_key + p.per_split) to = from_key + p.per_split;
+    const int at = t + 32 * (k + 1) - p.queries - from_key, there = to > from_key ? (to - from_key + p.rows - 1) / p.rows * p.rows : 0;
+    if (t >= distances || at < 0 || at >= there + 32) continue;
+    const float* from = p.along + (((int64_t)h * tiles * p.waves + k) * p.splits + n % p.splits) * p.stride + at;
+    const int64_t apart = (int64_t)p.heads * tiles * p.waves * p.splits * p.stride;
     int64_t b = 0;
     for (; b + 8 <= p.batch; b += 8) {      // eight loads on their way at a time
       float v[8];
@@ -188,15 +191,48 @@ int64_t bias_bytes(const gact_attention* a) { return a->bias ? round_up(a->heads
 int64_t split_rows(const gact_attention* a, const ForwardCut& c) {
   return c.splits > 1 ? a->batch * a->kv_heads * ((a->heads / a->kv_heads * a->queries + 31) / 32) * c.splits * 32 : 0;
 }
-// rows of a tile in the kernel of dq, as Tile has them
-int tile_rows(const gact_attention* a) {
+// rows of a tile in the backward pass, as Tile has them
+int tile_rows(const gact_attention* a, int waves) {
   const int64_t wide = padded_width(a) * esz(a->dtype);
-  return (wide <= 256 && waves_of(a->queries) == 4) || wide <= 64 ? 64 : 32;
+  return (wide <= 256 && waves == 4) || wide <= 64 ? 64 : 32;
 }
-int64_t along_stride(const gact_attention* a) { return round_up(a->keys, tile_rows(a)) + 32; }
-int64_t along_units(const gact_attention* a) {
-  const int waves = waves_of(a->queries);
-  return a->batch * a->heads * ((a->queries + waves * 32 - 1) / (waves * 32)) * waves;
+// How the backward pass is cut: where the tiles are fewer than the compute units, splits of the other side until there are two workgroups to each, with two
+// tiles at least to a split; the splits' sums are floats that a kernel of its own adds up.
+int splits_of(int64_t blocks, int64_t steps) {
+  if (blocks == 0 || blocks >= kComputeUnits) return 1;
+  int64_t splits = 2 * kComputeUnits / blocks;
+  if (splits > steps / 2) splits = steps / 2;
+  return splits < 1 ? 1 : (int)splits;
+}
+BackwardCut dq_cut(const gact_attention* a) {
+  BackwardCut c{waves_of(a->queries), 1, 0};
+  const int64_t rows = tile_rows(a, c.waves), steps = (a->keys + rows - 1) / rows;
+  const int64_t blocks = a->batch * a->heads * ((a->queries + c.waves * 32 - 1) / (c.waves * 32));
+  c.splits = splits_of(blocks, steps);
+  c.per_split = (int)(((steps + c.splits - 1) / c.splits) * rows);
+  if (c.per_split > 0) c.splits = (int)((a->keys + c.per_split - 1) / c.per_split);
+  if (c.splits < 1) c.splits = 1;
+  return c;
+}
+BackwardCut dkv_cut(const gact_attention* a) {
+  BackwardCut c{waves_of(a->keys), 1, 0};
+  const int64_t rows = tile_rows(a, c.waves), steps = (a->queries + rows - 1) / rows * (a->heads / a->kv_heads);
+  c.splits = splits_of(a->batch * a->kv_heads * ((a->keys + c.waves * 32 - 1) / (c.waves * 32)), steps);
+  return c;
+}
+int64_t along_stride(const gact_attention* a, const BackwardCut& c) {
+  return (c.splits > 1 ? c.per_split : round_up(a->keys, tile_rows(a, c.waves))) + 32;
+}
+int64_t along_bytes(const gact_attention* a, const BackwardCut& c) {
+  return a->batch * a->heads * ((a->queries + c.waves * 32 - 1) / (c.waves * 32)) * c.waves * c.splits * along_stride(a, c) * 4;
+}
+int64_t part_bytes(const gact_attention* a, const BackwardCut& c, int64_t heads, int64_t rows, int outputs) {
+  return c.splits > 1 ? a->batch * heads * round_up(rows, c.waves * 32) * padded_width(a) * 4 * c.splits * outputs : 0;
+}
+// both kernels' sums have the same place, one after the other
+int64_t parts_bytes(const gact_attention* a) {
+  const int64_t q = part_bytes(a, dq_cut(a), a->heads, a->queries, 1), k = part_bytes(a, dkv_cut(a), a->kv_heads, a->keys, 2);
+  return q > k ? q : k;
 }
 int64_t delta_bytes(const gact_attention* a) { return round_up(a->batch * a->heads * a->queries * 4, 256); }
 
@@ -286,7 +322,7 @@ int gact_attention_forward(const gact_attention* a, const gact_rows* out, float*
 
 int64_t gact_attention_backward_workspace_bytes(const gact_attention* a, int dbias) {
   if (!a || !sizes_fit(a)) return 0;
-  return bias_bytes(a) + delta_bytes(a) + (dbias ? along_units(a) * along_stride(a) * 4 : 0);
+  return bias_bytes(a) + delta_bytes(a) + parts_bytes(a) + (dbias ? along_bytes(a, dq_cut(a)) : 0);
 }
 
 int gact_attention_backward(const gact_attention* a, const gact_rows* out, const float* lse, const int8_t* rest, const gact_rows* d_out,
@@ -319,15 +355,17 @@ int gact_attention_backward(const gact_attention* a, const gact_rows* out, const
   rc = prepare_bias(a, p, (float*)workspace, s);
   if (rc != GACT_OK) return rc;
   p.delta = (float*)((char*)workspace + bias_bytes(a));
-  p.along = dbias ? (float*)((char*)p.delta + delta_bytes(a)) : nullptr;
-  p.along_stride = along_stride(a);
-  const int waves = waves_of(a->queries);
+  p.part = (float*)((char*)p.delta + delta_bytes(a));
+  const BackwardCut for_dq = dq_cut(a), for_dkv = dkv_cut(a);
+  p.along = dbias ? (float*)((char*)p.part + parts_bytes(a)) : nullptr;
+  p.along_stride = along_stride(a, for_dq);
   if (a->batch > 0) {
-    rc = with_type(a->dtype, [&](auto zero) { return attention_backward<decltype(zero)>(p, a->batch, waves, waves_of(a->keys), s); });
+    rc = with_type(a->dtype, [&](auto zero) { return attention_backward<decltype(zero)>(p, a->batch, for_dq, for_dkv, s); });
     if (rc != GACT_OK) return rc;
   }
   if (dbias && distances(a) > 0) {
-    const AlongArgs along{p.along, p.along_stride, some ? a->batch : 0, p.heads, p.queries, p.keys, waves * 32, tile_rows(a), waves, p.causal, dbias};
+    const AlongArgs along{p.along, p.along_stride, some ? a->batch : 0, p.heads, p.queries, p.keys, for_dq.waves * 32, tile_rows(a, for_dq.waves), for_dq.waves,
+                          for_dq.splits, for_dq.per_split, p.causal, dbias};
     hipLaunchKernelGGL(attention_along_kernel, dim3((unsigned)((distances(a) + 63) / 64), (unsigned)a->heads), dim3(1024), 0, s, along);
     return launch_status();
   }

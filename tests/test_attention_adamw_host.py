@@ -81,8 +81,10 @@ def test_attention_workspaces_are_sized():
                     bias = -(-4 * (queries + keys - 1) * 4 // 256) * 256
                     assert forward(**kind) >= bias and (forward(**kind) - bias) <= (1 << 31)
                     delta = -(-batch * 4 * queries * 4 // 256) * 256
-                    assert backward(**kind) == bias + delta
-                    assert backward(1, **kind) >= bias + delta + batch * 4 * (-(-queries // 32)) * (keys + 31) * 4
+                    # floats of few tiles' splits: for dq, or for dk and dv, at most two workgroups' rows to each of 256 compute units
+                    parts = backward(**kind) - bias - delta
+                    assert parts == 0 if batch == 200 and keys > 1 else 0 <= parts <= 2 * 512 * 128 * 64 * 4
+                    assert backward(1, **kind) >= bias + delta + parts + batch * 4 * (-(-queries // 32)) * (keys + 31) * 4
 
 
 def test_position_bias_refuses_before_it_touches_the_gpu():

@@ -75,6 +75,16 @@ def test_few_queries_train(shape, dtype):
     check(q, k, v, dy, bias, mask, True)
 
 
+# few tiles, with the keys and the queries cut into splits whose sums are added afterwards
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("shape", [(1, 1, 1, 700, 900, 64), (1, 4, 1, 333, 1100, 128), (2, 2, 2, 1500, 130, 40), (1, 2, 2, 130, 2049, 96), (1, 1, 1, 1025, 513, 32),
+                                   (3, 4, 2, 40, 650, 77)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", ["plain", "causal", "mask", "all"])
+def test_gradients_of_few_tiles(shape, kind, dtype):
+    q, k, v, dy, bias, mask = inputs(*shape, dtype, kind == "all", kind in ("mask", "all"))
+    check(q, k, v, dy, bias, mask, kind in ("causal", "all"))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 def test_queries_that_see_nothing(dtype):
     q, k, v, dy, bias, _ = inputs(3, 2, 2, 70, 40, 64, dtype, True)

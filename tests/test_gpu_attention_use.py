@@ -195,8 +195,9 @@ def test_memory_that_is_kept():
     torch.cuda.reset_peak_memory_stats()
     before = torch.cuda.memory_allocated()
     torch.autograd.grad(y.sum(), [q, k, v])
-    # three gradients, that of the sum as a dense tensor, one float per query
-    assert torch.cuda.max_memory_allocated() - before <= 6 * y.numel() * 4 + (1 << 20)
+    # three gradients, that of the sum as a dense tensor, one float per query; floats of dk and dv from the 8 splits (two tiles of 64 queries each) of the
+    # 32 tiles of 128 keys, which are fewer than the compute units
+    assert torch.cuda.max_memory_allocated() - before <= (6 + 2 * 8) * y.numel() * 4 + (1 << 20)
 
 
 # ---- autocast, modes, captures ----
