@@ -348,6 +348,41 @@ __device__ __forceinline__ void store_part(float* row, int width, int lane, cons
     }
 }
 
+// do_i . o_i of the lane's row, which two lanes share, with what the rounding of o has left out
+template <typename T, int NC>
+__device__ __forceinline__ float delta_of(const typename Matrix<T>::Frag (&o)[NC], const typename Matrix<T>::Frag (&dy)[NC], const int8_t* rest, int width, int lane) {
+  float delta = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; c++) {
+    u32x2 code = {};
+    const int piece = 2 * c + (lane >> 5);
+    if constexpr (Rest<T>::kept)
+      if (rest && piece * 8 < width) code = *(const u32x2*)(rest + piece * 8);
+#pragma unroll
+    for (int e = 0; e < 16 / (int)sizeof(T); e++) {
+      float exact = (float)o[c][e];
+      if constexpr (Rest<T>::kept)
+        if (rest) exact = Rest<T>::add(o[c][e], code[e >> 2] >> (8 * (e & 3)));
+      delta = __builtin_fmaf(exact, (float)dy[c][e], delta);
+    }
+  }
+  return sum_of_both(delta);
+}
+// dq of a block of keys.  A query's ds add up to zero, and few of them are large: their roundings do not average out as dk's do.  What they leave out makes
+// a product of its own (bfloat16, dq 0.0029 of its norm off without and 0.0021 with it, of which 0.0017 is the result's rounding; a BERT-large layer's
+// 73 us become 85)
+template <typename T, int DP, int WAVES>
+__device__ __forceinline__ void add_ds(f32x16 (&acc)[DP / 32], const lds_u8* keys, int first, const f32x16& ds, int lane) {
+  using Shape = Tile<T, DP, WAVES>;
+  const typename Shape::Packed k = Shape::pack(ds);
+  if constexpr (sizeof(T) == 2) {
+    const typename Shape::Packed more = Shape::rest(ds, k);
+    Shape::template add<true>(acc, keys, first, k, lane, &more);
+  } else {
+    Shape::add(acc, keys, first, k, lane);
+  }
+}
+
 // hidden scores of a block of 32 rows of the tile: the lane sees rows below `seen`, and of those the ones whose bit is set
 // (the empty statement keeps the branch around it: without one the compiler makes the selections for every block)
 __device__ __forceinline__ void hide(f32x16& s, int seen, uint32_t there, int lane) {
@@ -374,7 +409,7 @@ struct Present {
 // Waves that a SIMD is to hold: with two the compiler has 256 registers, and the products' results stay where the vector instructions reach them; beyond
 // that they pass through the matrix unit's own registers, an instruction each way for every value (a BERT-large layer's forward pass 95 us, 61 without).
 // Where the registers are too few for a kernel's rows, one.
-enum { FORWARD, FORWARD_APART, DQ, DKV };
+enum { FORWARD, FORWARD_APART, DQ, DKV, SHORT };
 template <typename T, int DP>
 constexpr int waves_held(int kernel) {
   const int wide = DP * (int)sizeof(T);
@@ -688,26 +723,11 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   own_row<T, NC>(p.d_out.at(b, h, query), own, p.width, lane, dy);
   const int64_t at = ((int64_t)b * p.heads + h) * p.queries + query;
   const float lse = own ? p.lse[at] : __builtin_inff();
-  float delta = 0.0f;
+  float delta;
   {
     Frag o[NC];
     own_row<T, NC>(p.out.at(b, h, query), own, p.width, lane, o);
-    const int8_t* const rest = p.rest_at(b, h, query);
-#pragma unroll
-    for (int c = 0; c < NC; c++) {
-      u32x2 code = {};
-      const int piece = 2 * c + (lane >> 5);
-      if constexpr (Rest<T>::kept)
-        if (rest && piece * 8 < p.width) code = *(const u32x2*)(rest + piece * 8);
-#pragma unroll
-      for (int e = 0; e < 16 / (int)sizeof(T); e++) {
-        float exact = (float)o[c][e];
-        if constexpr (Rest<T>::kept)
-          if (rest) exact = Rest<T>::add(o[c][e], code[e >> 2] >> (8 * (e & 3)));
-        delta = __builtin_fmaf(exact, (float)dy[c][e], delta);
-      }
-    }
-    delta = sum_of_both(delta);
+    delta = delta_of<T, NC>(o, dy, p.rest_at(b, h, query), p.width, lane);
     if (own && lane < 32 && split == 0) p.delta[at] = delta;
   }
   const int seen = p.seen(query);
@@ -803,16 +823,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     for (int n = 0; n < NB; n++) {
       if (key + 32 * n < some_see && there) {
         const f32x16 ds = gradient(n, product(keys, n, q), product(keys + kTile, n, dy), edge);
-        const typename Shape::Packed k = Shape::pack(ds);
-        if constexpr (sizeof(T) == 2) {
-          // A query's ds add up to zero, and few of them are large: their roundings do not average out as dk's do.  What they leave out makes a product of
-          // its own (bfloat16, dq 0.0029 of its norm off without and 0.0021 with it, of which 0.0017 is the result's rounding; a BERT-large layer's
-          // 73 us become 85)
-          const typename Shape::Packed more = Shape::rest(ds, k);
-          Shape::template add<true>(acc, keys, 32 * n, k, lane, &more);
-        } else {
-          Shape::add(acc, keys, 32 * n, k, lane);
-        }
+        add_ds<T, DP, WAVES>(acc, keys, 32 * n, ds, lane);
       }
       if constexpr (BIAS)
         if (along) leave(t * NB + n, along);
@@ -980,6 +991,156 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   if (p.dv.p) store_row<T, ND>((char*)p.dv.at(b, kv, key), nullptr, p.width, lane, dv, there);
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------
+// dq, dk and dv of sequences of up to 64 queries and keys in one pass: a workgroup has a key head and takes the heads that share it one after the other.
+// Five products instead of the seven of two kernels, and every operand read once: dk's and dv's leave ds with a key to a lane, which passes through LDS, in
+// the place of the queries and of dy, to become a query to a lane for dq.  24576 heads of 49 tokens of width 32: 420 us in floats, 575 in two kernels, and
+// 218 and 282 in bfloat16; 6144 of 64 tokens, width 64: 133 and 182.  The matrix unit is busy for half the time (the products of 64 x 64 take 205 us of the
+// 420); the rest goes to the loads and the four meetings of two waves that three workgroups beside each other do not cover.
+// ---------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+constexpr bool kShortFits = DP * sizeof(T) <= 256;
+template <typename T, int DP>
+__global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<T, DP>(SHORT)))) void attention_short_kernel(AttentionArgs p) {
+  using Shape = Tile<T, DP, 2>;
+  using Frag = typename Shape::Frag;
+  constexpr int R = 64, W = Shape::W, NC = Shape::NC, ND = Shape::ND;
+  constexpr int kTile = R * W, kRow = (R + 4) * 4, kDs = R * kRow, kShared = 2 * kTile > kDs ? 2 * kTile : kDs;
+  using Load = RowsLoad<T, DP, R, 2>;
+  typedef __attribute__((address_space(3))) float lds_float;
+  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+  __shared__ __attribute__((aligned(1024))) uint8_t memory[kTile + kShared + 2 * R * 4];
+  Work work;
+  if (!work_of(p, 1, work)) return;
+  const int thread = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  lds_u8* const keys = (lds_u8*)memory;
+  lds_u8* const queries = keys + kTile;
+  lds_float* const lse = (lds_float*)(queries + kShared);
+  lds_float* const deltas = lse + R;
+  const int b = work.head / p.kv_heads, kv = work.head % p.kv_heads;
+  const int first = wave * 32;
+  int lane = thread, mine = first + (lane & 31);      // the lane's key, and its query
+  Load load;
+  load.set_up(p.k.row, p.width, wave, lane);
+  Present present{p.mask ? p.mask + (int64_t)b * p.mask_stride : nullptr, p.keys};
+  present.ask(lane);
+  const uint64_t there = present.answer();
+  load.start(p.k.at(b, kv, 0), p.keys, p.k.row, p.width);
+  load.next(p.mask != nullptr, there, keys, lane);
+  const bool own = mine < p.keys && (there >> mine & 1);
+  Frag k[NC], v[NC];
+  own_row<T, NC>(p.v.at(b, kv, mine), own, p.width, lane, v);
+  const int behind = p.keys - p.queries;
+  const int seen_from = p.causal && mine > behind ? mine - behind : 0;
+  const int all_from = p.causal && first + 31 > behind ? first + 31 - behind : 0, some_from = p.causal && first > behind ? first - behind : 0;
+  // keys that the wave's queries see
+  const int some_see = first < p.queries ? p.seen(first + 31 < p.queries ? first + 31 : p.queries - 1) : 0;
+  const bool all_own = __ballot(own) == ~0ull;
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
+  float scale2 = p.scale2;
+  asm("" : "+v"(scale2));
+  for (int g = 0; g < p.group; g++) {
+    const int head = kv * p.group + g;
+    if (g) meet();
+    // addresses anew for each head: kept, they would take more registers than there are for three waves
+    lane = thread;
+    asm volatile("" : "+v"(lane));
+    mine = first + (lane & 31);
+    const int g4 = 4 * (lane >> 5);
+    // ds: rows of 64 keys, 16 bytes apart, so that neighbouring rows' pieces lie in different banks
+    lds_u8* const ds_of_key = queries + g4 * kRow + mine * 4;
+    const lds_u8* const ds_of_query = queries + mine * kRow + g4 * 4;
+    load.set_up(p.q.row, p.width, wave, lane);
+    load.start(p.q.at(b, head, 0), p.queries, p.q.row, p.width);
+    load.next(false, 0, queries, lane);
+    load.set_up(p.d_out.row, p.width, wave, lane);
+    load.start(p.d_out.at(b, head, 0), p.queries, p.d_out.row, p.width);
+    load.next(false, 0, queries + kTile, lane);
+    const int64_t at = ((int64_t)b * p.heads + head) * p.queries;
+    if (wave == 0) load_floats(p.lse + at, p.queries, 0, R, 0, 1, (lds_u8*)lse, lane);
+    {
+      Frag o[NC], dy[NC];
+      own_row<T, NC>(p.out.at(b, head, mine), mine < p.queries, p.width, lane, o);
+      wait_all();
+      meet();
+#pragma unroll
+      for (int c = 0; c < NC; c++) dy[c] = Shape::direct(queries + kTile, first, c, lane);
+      const float delta = delta_of<T, NC>(o, dy, mine < p.queries ? p.rest_at(b, head, mine) : nullptr, p.width, lane);
+      if (lane < 32) deltas[mine] = delta;
+    }
+    if (g == 0) {
+#pragma unroll
+      for (int c = 0; c < NC; c++) k[c] = Shape::direct(keys, first, c, lane);
+    }
+    meet();
+    f32x16 ds[2] = {};
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      if (32 * n + 31 < some_from || 32 * n >= p.queries || first >= p.keys) continue;
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(queries, 32 * n, c, lane), k[c], s);
+#pragma unroll
+      for (int c = 0; c < NC; c++) dp = Matrix<T>::run(Shape::direct(queries + kTile, 32 * n, c, lane), v[c], dp);
+#pragma unroll
+      for (int e4 = 0; e4 < 16; e4 += 4) {
+        const f32x4 l = *(const lds_f32x4*)(lse + 32 * n + row_of(e4) + g4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[e4 + e] = __builtin_fmaf(s[e4 + e], scale2, -l[e]);
+      }
+      if (32 * n < all_from || 32 * n + 32 > p.queries || !all_own) {
+        int from = seen_from - 32 * n - g4, to = own ? p.queries - 32 * n - g4 : -64;
+        asm volatile("" : "+v"(from), "+v"(to));      // compared anew for each head: what the comparisons leave would fill the scalar registers
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = row_of(e) >= from && row_of(e) < to ? s[e] : -__builtin_inff();
+      }
+#pragma unroll
+      for (int e4 = 0; e4 < 16; e4 += 4) {
+        const f32x4 x = *(const lds_f32x4*)(deltas + 32 * n + row_of(e4) + g4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          s[e4 + e] = __builtin_amdgcn_exp2f(s[e4 + e]);
+          ds[n][e4 + e] = s[e4 + e] * (dp[e4 + e] - x[e]);
+        }
+      }
+      Shape::add(dv, queries + kTile, 32 * n, Shape::pack(s), lane);
+      Shape::add(dk, queries, 32 * n, Shape::pack(ds[n]), lane);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    meet();
+#pragma unroll
+    for (int n = 0; n < 2; n++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) *(lds_float*)(ds_of_key + (32 * n + row_of(e)) * kRow) = ds[n][e];
+    meet();
+    f32x16 dq[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) dq[d] = f32x16{};
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      if (32 * n >= some_see) continue;
+      f32x16 x;
+#pragma unroll
+      for (int e4 = 0; e4 < 16; e4 += 4) {
+        const f32x4 part = *(const lds_f32x4*)(ds_of_query + (32 * n + row_of(e4)) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e4 + e] = part[e];
+      }
+      add_ds<T, DP, 2>(dq, keys, 32 * n, x, lane);
+    }
+    if (mine < p.queries && p.dq.p) store_row<T, ND>((char*)p.dq.at(b, head, mine), nullptr, p.width, lane, dq, p.scale);
+  }
+  if (mine >= p.keys) return;
+  if (!own) {
+#pragma unroll
+    for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
+  }
+  if (p.dk.p) store_row<T, ND>((char*)p.dk.at(b, kv, mine), nullptr, p.width, lane, dk, p.scale);
+  if (p.dv.p) store_row<T, ND>((char*)p.dv.at(b, kv, mine), nullptr, p.width, lane, dv, 1.0f);
+}
+
 // out = factor times the sum of the splits' rows, in their order; which of two outputs: blockIdx.z.  Four columns to a lane.
 struct PartRows {
   const float* part[2];
@@ -1070,6 +1231,11 @@ int add_parts(const PartRows& p, int outputs, hipStream_t s) {
 struct BackwardCut {
   int waves, splits, per_split;
 };
+// Heads that share keys pass one after the other: with few workgroups that takes longer than two kernels that split them (4 workgroups of 16 heads of 50
+// tokens 86 us, and 18; 256 of 4 heads of 4 tokens 20 and 17; 4096 of 4 heads of 32 tokens 139 and 145)
+inline bool sequences_are_short(const AttentionArgs& p, int64_t batch) {
+  return p.queries <= 64 && p.keys <= 64 && !p.bias && (p.group == 1 || batch * p.kv_heads >= 512);
+}
 template <typename T>
 int attention_backward(AttentionArgs p, int64_t batch, BackwardCut for_dq, BackwardCut for_dkv, hipStream_t s) {
   return with_width(p.width, [&](auto width) {
@@ -1083,6 +1249,8 @@ int attention_backward(AttentionArgs p, int64_t batch, BackwardCut for_dq, Backw
       p.by_length = p.causal && heads % 8 == 0;
       return heads * tiles * cut.splits;
     };
+    if constexpr (kShortFits<T, DP>)
+      if (sequences_are_short(p, batch)) return launch(attention_short_kernel<T, DP>, shape(batch * p.kv_heads, 1, BackwardCut{2, 1, 0}), 128, p, s);
     const int64_t blocks = shape(batch * p.heads, p.queries, for_dq);
     int rc;
     if (for_dq.waves == 2)

@@ -75,6 +75,16 @@ def test_few_queries_train(shape, dtype):
     check(q, k, v, dy, bias, mask, True)
 
 
+# up to 64 queries and keys, of one head or of several that share its keys
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("shape", [(2, 3, 3, 64, 64, 64), (3, 6, 2, 40, 64, 64), (2, 4, 1, 64, 17, 80), (1, 2, 2, 5, 60, 32), (2, 8, 1, 33, 33, 128), (30, 3, 3, 49, 49, 32),
+                                   (1, 4, 2, 31, 33, 100), (256, 4, 2, 33, 35, 40), (520, 3, 1, 5, 64, 128)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", ["plain", "causal", "mask", "both"])
+def test_short_sequences(shape, kind, dtype):
+    q, k, v, dy, bias, mask = inputs(*shape, dtype, False, kind in ("mask", "both"))
+    check(q, k, v, dy, bias, mask, kind in ("causal", "both"))
+
+
 # few tiles, with the keys and the queries cut into splits whose sums are added afterwards
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("shape", [(1, 1, 1, 700, 900, 64), (1, 4, 1, 333, 1100, 128), (2, 2, 2, 1500, 130, 40), (1, 2, 2, 130, 2049, 96), (1, 1, 1, 1025, 513, 32),
