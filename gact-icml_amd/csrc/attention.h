@@ -368,9 +368,9 @@ __device__ __forceinline__ float delta_of(const typename Matrix<T>::Frag (&o)[NC
   }
   return sum_of_both(delta);
 }
-// dq of a block of keys.  A query's ds add up to zero, and few of them are large: their roundings do not average out as dk's do.  What they leave out makes
-// a product of its own (bfloat16, dq 0.0029 of its norm off without and 0.0021 with it, of which 0.0017 is the result's rounding; a BERT-large layer's
-// 73 us become 85)
+// A block's ds into dq or dk.  A row's ds add up to zero, or nearly, and few of them are large: their roundings do not average out.  What they leave out
+// makes a product of its own (bfloat16, a BERT-large layer: dq 0.0029 of its norm off without and 0.0021 with it, dk 0.0025 and 0.0019, of which 0.0017 is
+// the result's rounding; dq 73 us and 84, dk and dv 91 and 105)
 template <typename T, int DP, int WAVES>
 __device__ __forceinline__ void add_ds(f32x16 (&acc)[DP / 32], const lds_u8* keys, int first, const f32x16& ds, int lane) {
   using Shape = Tile<T, DP, WAVES>;
@@ -558,7 +558,16 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       // the sum is of the probabilities as they enter the product: where one key has nearly all of a query's, its rounding cancels in the quotient
       const typename Shape::Packed k = Shape::pack(s[n]);
       total += Shape::sum(k);
-      Shape::add(acc, keys + kTile, 32 * n, k, lane);
+      if constexpr (BIAS && sizeof(T) == 2) {
+        // A bias's gradient adds up many ds, and those of a query are all off by what do_i . o_i is: with the probabilities' roundings in o a table's
+        // gradient was up to 0.00035 of its norm off (float16, 8 x 1000 tokens) where its own rounding leaves 0.0002, which is all that is left of it now;
+        // 71 us become 94
+        const typename Shape::Packed more = Shape::rest(s[n], k);
+        total += Shape::sum(more);
+        Shape::template add<true>(acc, keys + kTile, 32 * n, k, lane, &more);
+      } else {
+        Shape::add(acc, keys + kTile, 32 * n, k, lane);
+      }
     }
   }
   wait_all();
@@ -970,7 +979,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       f32x16 s = product(rows, n, k), dp = product(rows + kTile, n, v);
       gradient(n, s, dp, edge);
       Shape::add(dv, rows + kTile, 32 * n, Shape::pack(s), lane);
-      Shape::add(dk, rows, 32 * n, Shape::pack(dp), lane);
+      add_ds<T, DP, WAVES>(dk, rows, 32 * n, dp, lane);
     }
   }
   wait_all();
@@ -1106,7 +1115,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
         }
       }
       Shape::add(dv, queries + kTile, 32 * n, Shape::pack(s), lane);
-      Shape::add(dk, queries, 32 * n, Shape::pack(ds[n]), lane);
+      add_ds<T, DP, 2>(dk, queries, 32 * n, ds[n], lane);
       __builtin_amdgcn_sched_barrier(0);
     }
     meet();
