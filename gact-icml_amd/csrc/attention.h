@@ -421,7 +421,10 @@ constexpr int waves_held(int kernel) {
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // The forward pass.  APART: for few queries the waves of a workgroup have the same 32 rows (the queries of all heads that share a key head), take the
-// keys in turn, each in tiles of its own, and add up at the end; splits of the keys go to workgroups of their own, which join_kernel adds up.
+// keys in turn, each in tiles of its own, and add up at the end; splits of the keys go to workgroups of their own, which the joining kernels add up.
+// Bound by the vector instructions between its two products, of which a score takes nine and an exponential: 32 x 16 heads of 512 tokens, width 64, bfloat16
+// 61 us (564 TFLOP/s), 2 x 32 causal heads of 4096, width 128, 305 (900), where the products alone would take 14 and 110 at the instructions' peak.  One token
+// behind 65537 keys of 8 heads, width 128: 43 us, 6.3 TB/s, which is what memory gives.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int WAVES, bool APART, bool BIAS>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(waves_held<T, DP>(APART ? FORWARD_APART : FORWARD)))) void attention_forward_kernel(AttentionArgs p) {
@@ -635,17 +638,66 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   }
 }
 
-// The splits' results as one: a workgroup has a row, its lanes the width, its waves the splits.
+// The splits' results as one.
+struct Joined {
+  int64_t first;      // its place in split 0 of its tile
+  int b, head, query;
+};
+__device__ __forceinline__ bool row_to_join(const AttentionArgs& p, int64_t at, Joined& j) {
+  const int rows = p.group * p.queries, row = (int)(at % rows);
+  const int64_t bh = at / rows;
+  if (bh >= (int64_t)(p.blocks / p.splits / p.tiles)) return false;
+  j = Joined{(bh * p.tiles + row / 32) * p.splits * 32 + row % 32, (int)(bh / p.kv_heads), (int)(bh % p.kv_heads) * p.group + row / p.queries, row % p.queries};
+  return true;
+}
+template <typename T>
+__device__ __forceinline__ void store_joined(const AttentionArgs& p, const Joined& j, int lane, f32x4 sum, float total, float most) {
+  sum *= total > 0.0f ? 1.0f / total : total;
+  if (lane * 4 < p.width) store4<T>((char*)p.out.at(j.b, j.head, j.query), p.rest_at(j.b, j.head, j.query), lane * 4, sum);
+  if (p.lse && lane == 0) p.lse[((int64_t)j.b * p.heads + j.head) * p.queries + j.query] = total == 0.0f ? __builtin_inff() : most + __builtin_amdgcn_logf(total);
+}
+// Few of them: DP / 4 lanes have a row (8 heads of 512 tokens, two splits: 4 us, 7.5 with the kernel below; with up to eight splits this way 5.9 where the
+// other takes 4.2)
+constexpr int kFewSplits = 4;
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attention_join_few_kernel(AttentionArgs p) {
+  constexpr int kLanes = DP / 4, kDown = 256 / kLanes;
+  const int lane = threadIdx.x % kLanes, down = threadIdx.x / kLanes;
+  Joined j;
+  if (down >= kDown || !row_to_join(p, block_of() * kDown + down, j)) return;
+  f32x2 stat[kFewSplits];
+  f32x4 part[kFewSplits];
+#pragma unroll
+  for (int s = 0; s < kFewSplits; s++) {      // all on their way at once
+    const int64_t place = j.first + 32 * (int64_t)(s < p.splits ? s : 0);
+    stat[s] = *(const f32x2*)(p.part_stats + place * 2);
+    if (lane * 4 < p.width) part[s] = *(const f32x4*)(p.part + place * DP + lane * 4);
+  }
+  float most = stat[0][0];
+#pragma unroll
+  for (int s = 1; s < kFewSplits; s++) most = __builtin_fmaxf(most, stat[s][0]);
+  f32x4 sum = {};
+  float total = 0.0f;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; s++) {
+    if (s >= p.splits) break;
+    const float factor = stat[s][0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(stat[s][0] - most);
+    total = __builtin_fmaf(stat[s][1], factor, total);
+    sum += part[s] * factor;
+  }
+  store_joined<T>(p, j, lane, sum, total, most);
+}
+// Many: a workgroup has a row, its lanes the width, its waves the splits.  Latency: a launch, and three loads one after the other (32 rows, 32 splits of
+// width 128: 5 us)
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p) {
   constexpr int kLanes = DP / 4, kDown = 256 / kLanes;
   __shared__ f32x4 sums[kDown][kLanes];
   __shared__ float totals[kDown];
-  const int64_t at = block_of();
-  const int rows = p.group * p.queries, row = (int)(at % rows), lane = threadIdx.x % kLanes, down = threadIdx.x / kLanes;
-  const int64_t bh = at / rows;
-  if (bh >= (int64_t)(p.blocks / p.splits / p.tiles)) return;
-  const int64_t first = (bh * p.tiles + row / 32) * p.splits * 32 + row % 32;
+  const int lane = threadIdx.x % kLanes, down = threadIdx.x / kLanes;
+  Joined j;
+  if (!row_to_join(p, block_of(), j)) return;
+  const int64_t first = j.first;
   __shared__ float mosts[4];
   float most = -__builtin_inff();
   for (int s = threadIdx.x; s < p.splits; s += 256) most = __builtin_fmaxf(most, p.part_stats[(first + 32 * (int64_t)s) * 2]);
@@ -674,10 +726,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p) {
     sum += sums[d][lane];
     total += totals[d];
   }
-  const int b = (int)(bh / p.kv_heads), head = (int)(bh % p.kv_heads) * p.group + row / p.queries, query = row % p.queries;
-  sum *= total > 0.0f ? 1.0f / total : total;
-  if (lane * 4 < p.width) store4<T>((char*)p.out.at(b, head, query), p.rest_at(b, head, query), lane * 4, sum);
-  if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + head) * p.queries + query] = total == 0.0f ? __builtin_inff() : most + __builtin_amdgcn_logf(total);
+  store_joined<T>(p, j, lane, sum, total, most);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -686,6 +735,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p) {
 // down its row of lanes by row_of(e) mod 16, lane m has the diagonals 16 c - m + 4 g - 16 half of all elements, where c is 0 for what stays in the row,
 // 1 for what leaves it, and one more for the keys from 16 on: three running sums a lane, two additions an element that shift as they add.  After a block
 // the sums of c = 0 and 1 are complete and the one of 2 is the next block's 0.  The four rows' sums, each a sequence along c and -m, meet in LDS.
+// Three products, and two of 16-bit types for what rounding leaves out; bound as the forward pass is: 32 x 16 heads of 512 tokens, width 64, bfloat16 85 us;
+// 8 x 16 of 1000, halves, with a bias 121, of which the diagonals take 30.
 // (Additions into LDS by the hardware's atomics, 16 a block: 750 us for 8 x 16 heads of 1000 x 1000 halves where the kernel without them takes 100.)
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int N>
@@ -849,7 +900,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// dk and dv: a wave has 32 keys, and the queries of all heads that share the key head pass by.
+// dk and dv: a wave has 32 keys, and the queries of all heads that share the key head pass by.  No sums through atomics: a result has the same bits every
+// time, for seven products in two kernels where one with atomics for dq would make five.  32 x 16 heads of 512 tokens, width 64, bfloat16: 105 us, bound as
+// the forward pass is.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int WAVES, bool BIAS>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(waves_held<T, DP>(DKV)))) void attention_dkv_kernel(AttentionArgs p) {
@@ -1217,7 +1270,10 @@ int attention_forward(AttentionArgs p, int64_t batch, int waves, bool apart, hip
     if (apart) {
       const int rc = p.bias ? launch(attention_forward_kernel<T, DP, A, true, true>, blocks, A * 64, p, s)
                             : launch(attention_forward_kernel<T, DP, A, true, false>, blocks, A * 64, p, s);
-      return rc != GACT_OK || p.splits == 1 ? rc : launch(attention_join_kernel<T, DP>, heads * rows, 256, p, s);
+      if (rc != GACT_OK || p.splits == 1) return rc;
+      constexpr int kDown = 256 / (DP / 4);
+      if (p.splits <= kFewSplits) return launch(attention_join_few_kernel<T, DP>, (heads * rows + kDown - 1) / kDown, 256, p, s);
+      return launch(attention_join_kernel<T, DP>, heads * rows, 256, p, s);
     }
     if (waves == 2)
       return p.bias ? launch(attention_forward_kernel<T, DP, 2, false, true>, blocks, 128, p, s)

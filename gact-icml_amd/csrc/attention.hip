@@ -161,8 +161,11 @@ int check_all(const gact_attention* a) {
   return rc == GACT_OK ? check_rows(a, &a->v, a->kv_heads, a->keys) : rc;
 }
 
-// How the forward pass is cut.  Few queries: workgroups of 32 rows whose waves take the keys in turn, and splits of the keys until there are two
-// workgroups to a compute unit, each wave with at least two blocks of 32 keys.
+// How the forward pass is cut.  Workgroups of two waves for up to 64 queries (24576 heads of 49 floats' tokens 179 us, with four 334; 1024 heads of 40
+// tokens 7.2 and 8.5).  Few queries: workgroups of 32 rows whose waves take the keys in turn, and splits of the keys until there is a workgroup to a compute
+// unit (32 heads' token on 8 key heads of 65537 keys 47 us, with twice the splits 52, in tiles 1728), each wave with at least two blocks of 32 keys (8 heads'
+// token behind 2048 keys 9.2 us, with four blocks 10.6).  The same for more queries where their tiles are fewer than the compute units (4 heads of 4096
+// tokens 36 us, in tiles 74; 12 of 2048 33 and 40), but not above (24 of 2048, width 128: 76 us in 384 tiles, 136 so).
 struct ForwardCut {
   int waves;
   bool apart;
@@ -179,7 +182,7 @@ ForwardCut forward_cut(const gact_attention* a) {
   if (!c.apart || units == 0) return c;
   c.waves = esz(a->dtype) * padded_width(a) > 256 ? 2 : 4;
   const int64_t least = c.waves * 64;
-  int64_t splits = 2 * kComputeUnits / units, most = a->keys / least;
+  int64_t splits = kComputeUnits / units, most = a->keys / least;
   if (splits > most) splits = most;
   if (splits < 1) splits = 1;
   const int64_t per = round_up((a->keys + splits - 1) / splits, c.waves * 32);
