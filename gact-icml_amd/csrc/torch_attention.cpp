@@ -95,11 +95,15 @@ struct AttentionBackward : public Node {
   bool has_bias = false, has_mask = false;
   // hooks for saved tensors may give back other values: probabilities from these and sums from those that were given would be no probabilities
   bool again_forward = false;
+  // The bias of a call under hooks, which do not get it: in codes of few bits the values that hide a key would leave nothing of the others.
+  at::Tensor held_bias;
+  int64_t bias_version = 0;
   bool released = false;
   std::string name() const override { return "OpAttentionBackward"; }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
     for (SavedVariable* v : {&query, &key, &value, &bias, &mask, &result, &lse, &rest}) give_up(*v);
+    held_bias.reset();
     released = true;
   }
   variable_list apply(variable_list&& grads) override {
@@ -113,7 +117,10 @@ struct AttentionBackward : public Node {
     const at::Tensor k = again(key, dtype, {c.batch, c.kv_heads, c.keys, c.width}, dy, false);
     const at::Tensor v = again(value, dtype, {c.batch, c.kv_heads, c.keys, c.width}, dy, false);
     at::Tensor b, m, y, l, r;
-    if (has_bias) b = again(bias, at::kFloat, {c.heads, c.distances()}, dy, false);
+    if (held_bias.defined()) {
+      TORCH_CHECK(held_bias._version() == bias_version, "the bias has been modified by an inplace operation since op_attention was given it");
+      b = held_bias;
+    } else if (has_bias) b = again(bias, at::kFloat, {c.heads, c.distances()}, dy, false);
     if (has_mask) m = again(mask, at::kBool, {c.batch, c.keys}, dy, false);
     if (!again_forward) {
       y = result.unpack(shared_from_this());
@@ -210,7 +217,13 @@ at::Tensor attention(const at::Tensor& q_given, const at::Tensor& k_given, const
     node->query = SavedVariable(q, false);
     node->key = SavedVariable(k, false);
     node->value = SavedVariable(v, false);
-    if (bias) node->bias = SavedVariable(*bias, false);
+    if (bias && hooked) {
+      TORCH_CHECK(!bias->is_inference(), "Inference tensors cannot be saved for backward. To work around you can make a clone to get a normal tensor and use it in autograd.");
+      node->held_bias = bias->detach();
+      node->bias_version = bias->_version();
+    } else if (bias) {
+      node->bias = SavedVariable(*bias, false);
+    }
     if (mask) node->mask = SavedVariable(*mask, false);
     torch::autograd::set_history(y, node);
     if (!hooked) {

@@ -25,8 +25,8 @@ def op_attention(query, key, value, bias=None, mask=None, causal=False, scale=No
     A query that nothing is left for gets zeros, and gives none of its gradient to anyone.
 
     The result lies in memory as [batch, queries, heads, width], so that its transpose(1, 2) is a projection's contiguous input.  Under hooks for saved
-    tensors (the Controller's) query, key and value are all that is saved, and the backward pass runs the forward pass again on what the hooks give
-    back: the gradients are exactly those of these values.  Under autocast it runs in autocast's type, the bias in float32."""
+    tensors (the Controller's) query, key and value, and a mask, are all that they get; the bias is held as it is, and the backward pass runs the forward
+    pass again on what the hooks give back: the gradients are exactly those of these values.  Under autocast it runs in autocast's type, the bias in float32."""
     autocast = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None
     return _abi.native().attention(query, key, value, bias, mask, causal, scale, autocast)
 

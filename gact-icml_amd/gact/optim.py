@@ -89,13 +89,15 @@ class AdamW(torch.optim.Optimizer):
                 key = id(count) if isinstance(count, torch.Tensor) else count
                 together.setdefault(key, (count, []))[1].append(p)
             for count, params in together.values():
+                states = [(kept["exp_avg"], kept["exp_avg_sq"], kept.get("scale")) for kept in map(self.state.__getitem__, params)]
                 count += 1      # in place where it is a tensor
-                states = []
+                try:
+                    op_adamw(params, [p.grad for p in params], states, count, group["lr"], group["betas"], group["eps"], group["weight_decay"])
+                except Exception:
+                    count -= 1      # a step that was refused has not been made
+                    raise
                 for p in params:
-                    kept = self.state[p]
-                    kept["step"] = count
-                    states.append((kept["exp_avg"], kept["exp_avg_sq"], kept.get("scale")))
-                op_adamw(params, [p.grad for p in params], states, count, group["lr"], group["betas"], group["eps"], group["weight_decay"])
+                    self.state[p]["step"] = count
         return loss
 
     def load_state_dict(self, state_dict):
@@ -104,7 +106,7 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict({**state_dict, "state": {}})
         numbers = [n for group in state_dict["param_groups"] for n in group["params"]]
         params = [(group, p) for group in self.param_groups for p in group["params"]]
-        counts = {}
+        counts = {}      # a group's own: each adds to its counts by itself
         for number, (group, p) in zip(numbers, params):
             if number not in saved:
                 continue
@@ -119,5 +121,5 @@ class AdamW(torch.optim.Optimizer):
                 to.copy_(held[name])
             step = int(held["step"])
             if group["capturable"]:
-                step = counts.setdefault((p.device, step), torch.full((), step, dtype=torch.int64, device=p.device))
+                step = counts.setdefault((id(group), p.device, step), torch.full((), step, dtype=torch.int64, device=p.device))
             self.state[p] = {"step": step, **kept}

@@ -154,3 +154,24 @@ def test_optimizer_checks_its_options():
         with pytest.raises(ValueError):
             optim.AdamW([p], **bad)
     optim.AdamW([p]).step()      # no gradient, nothing to do
+
+
+def test_optimizer_groups_count_their_steps_by_themselves():
+    """Counts in device memory are added to in place: two groups that were loaded with the same count must not share it."""
+    params = [torch.nn.Parameter(torch.zeros(300)) for _ in range(4)]
+    opt = optim.AdamW([{"params": params[:2]}, {"params": params[2:]}], capturable=True)
+    state = opt.state_dict()
+    moments = {n: {"step": torch.tensor(5), **ops.op_adamw_state(p)._asdict()} for n, p in enumerate(params)}
+    opt.load_state_dict({**state, "state": moments})
+    a, b, c, d = (opt.state[p]["step"] for p in params)
+    assert a is b and c is d and a is not c and int(a) == int(c) == 5
+
+
+def test_optimizer_does_not_count_a_step_that_was_refused():
+    for capturable in (False, True):
+        p = torch.nn.Parameter(torch.zeros(300))
+        opt = optim.AdamW([p], capturable=capturable)
+        p.grad = torch.zeros(300)
+        with pytest.raises(RuntimeError):        # not on a GPU
+            opt.step()
+        assert int(opt.state[p].get("step", 0)) == 0

@@ -144,7 +144,7 @@ def test_under_hooks_the_gradients_are_those_of_what_the_hooks_give_back():
 
     with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
         y = ops.op_attention(q, k, v, bias)
-    assert [tuple(t.shape) for t in saved] == [(2, 4, 96, 64)] * 3 + [(4, 191)]        # neither the result nor sums
+    assert [tuple(t.shape) for t in saved] == [(2, 4, 96, 64)] * 3        # neither the result nor sums, nor the bias
     got = torch.autograd.grad(y, [q, k, v], dy)
     moved = [(t.detach() * 1.0625).requires_grad_() for t in (q, k, v)]
     want = torch.autograd.grad(ops.op_attention(*moved, bias), moved, dy)
@@ -182,6 +182,44 @@ def test_under_the_controller(bit):
     assert torch.isfinite(got).all() and 0.2 * want.norm() <= got.norm() <= 5 * want.norm()
     if bit == 8:
         assert (got - want).norm() <= 0.05 * want.norm()
+
+
+@pytest.mark.parametrize("hidden", [-math.inf, torch.finfo(torch.float32).min, -1e30])
+def test_under_the_controller_a_bias_hides_what_it_hid(hidden):
+    config.auto_prec, config.bit, config.compress_bool_masks = False, 8, True
+    torch.manual_seed(0)
+    model = torch.nn.Linear(64, 192).cuda()
+    bias = normal(4, 119, seed=2)
+    bias[:, 70:] = hidden        # keys more than ten behind the query
+    bias.requires_grad_()
+    mask = torch.rand(4, 60, generator=torch.Generator().manual_seed(3)).cuda() < 0.8
+    controller = Controller(model)
+    x, dy = normal(4, 60, 64), normal(4, 60, 64, seed=1)
+
+    def run():
+        q, k, v = model(x).view(4, 60, 3, 4, 16).permute(2, 0, 3, 1, 4)
+        y = ops.op_attention(2 * q, k, v, bias, mask).transpose(1, 2).reshape(4, 60, 64)
+        return torch.autograd.grad((y * dy).sum(), [model.weight, bias])
+
+    want = run()
+    controller.install_hook()
+    got = run()
+    controller.uninstall_hook()
+    # codes of 8 bits: steps of 1/255 of a group's range, which is some six deviations, of three factors
+    for a, b in zip(got, want):
+        assert (a - b).norm() <= 0.05 * b.norm()
+    assert (got[1][:, 70:] == 0).all()
+
+
+def test_a_bias_that_changes_before_the_backward_pass_is_refused():
+    q, k, v = (normal(1, 2, 40, 32, seed=s).requires_grad_() for s in range(3))
+    bias = normal(2, 79, seed=3)
+    for hooks in (torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t), torch.enable_grad()):
+        with hooks:
+            y = ops.op_attention(q, k, v, bias)
+        bias.add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
 
 
 def test_memory_that_is_kept():
