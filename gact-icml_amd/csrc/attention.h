@@ -1203,7 +1203,8 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
   if (p.dv.p) store_row<T, ND>((char*)p.dv.at(b, kv, mine), nullptr, p.width, lane, dv, 1.0f);
 }
 
-// out = factor times the sum of the splits' rows, in their order; which of two outputs: blockIdx.z.  Four columns to a lane.
+// out = factor times the sum of the splits' rows, in their order; which of two outputs: blockIdx.z.  Four columns to a lane, four loads on their way.  Latency:
+// 3 x 6 heads of 197 queries of width 72, 6 splits, 4 us; dq, dk and dv of 4096 rows of width 128, 8 splits (50 MB), 10.7 in two launches.
 struct PartRows {
   const float* part[2];
   Side out[2];

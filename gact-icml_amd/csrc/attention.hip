@@ -24,7 +24,8 @@ __global__ __launch_bounds__(256) void attention_bias_kernel(const float* __rest
   out[i] = v <= kHidden ? -__builtin_inff() : v * kLog2e;
 }
 
-// dbias[h][t]: what the blocks of 32 queries of all batch entries have on diagonal t, in their order.
+// dbias[h][t]: what the blocks of 32 queries of all batch entries have on diagonal t, in their order.  Bound by what the caches give of its one use of every
+// float: 8 x 16 heads of 1000 x 1000 (17 MB) 7 us; with the loads one after the other 24.
 struct AlongArgs {
   const float* along;
   int64_t stride;
@@ -88,7 +89,8 @@ struct Buckets {
     return side + near + low;
   }
 };
-// A thread has a distance and eight heads, whose values lie side by side in the table.  64 heads of 32767 distances: bound by the stores.
+// A thread has a distance and eight heads, whose values lie side by side in the table.  64 heads of 32767 distances (8.4 MB) 5.9 us, 12 of 393 2.8: start and
+// end of a launch and the search for the bucket.
 template <typename T>
 __global__ __launch_bounds__(256) void position_bias_kernel(const T* __restrict__ table, int heads, int keys, int distances, Buckets buckets,
                                                             float* __restrict__ out) {
@@ -100,7 +102,8 @@ __global__ __launch_bounds__(256) void position_bias_kernel(const T* __restrict_
   for (int h = 0; h < 8; h++)
     if (first + h < heads) out[(int64_t)(first + h) * distances + t] = (float)row[first + h];
 }
-// A bucket's distances are neighbours: a workgroup adds up one bucket of one head, always in the same order
+// A bucket's distances are neighbours: a workgroup adds up one bucket of one head, always in the same order.  64 heads of 32767 distances 7.7 us, of which
+// the largest bucket's workgroups, 65 KB each, are the last; 12 of 393 2.6.
 template <typename T>
 __global__ __launch_bounds__(256) void position_bias_backward_kernel(const float* __restrict__ grad, int heads, int queries, int keys, Buckets buckets,
                                                                      T* __restrict__ d_table) {
