@@ -277,6 +277,19 @@ def test_the_same_bits_every_time():
             assert all(torch.equal(a, b) for a, b in zip(first, all_of))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("shape", [(2, 2, 2, 50, 60, 64), (1, 4, 2, 700, 900, 64), (2, 16, 16, 1100, 1030, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_some_of_the_gradients(shape, dtype):
+    """A single kernel, splits of either side, and neither: a gradient is the same whichever others are wanted."""
+    q, k, v, dy, bias, mask = inputs(*shape, dtype, False, True)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    y = ops.op_attention(*leaves, None, mask, True)
+    want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    for some in ([0], [1], [2], [0, 2], [1, 2], [2, 0]):
+        got = torch.autograd.grad(y, [leaves[n] for n in some], dy, retain_graph=True)
+        assert all(torch.equal(g, want[n]) for g, n in zip(got, some))
+
+
 def test_only_the_gradients_that_are_asked_for():
     q, k, v, dy, bias, mask = inputs(2, 4, 2, 100, 100, 64, torch.bfloat16, True)
     leaves = [t.requires_grad_() for t in (q, k, v, bias)]
