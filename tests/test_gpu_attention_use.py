@@ -311,6 +311,39 @@ def test_graphs_are_captured_and_replayed():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_a_bias_and_short_sequences_train_in_graphs():
+    """The table's gradient from a backward pass in splits, and sequences that one kernel takes, replayed with other values and the eager pass in between."""
+    q, k, v, dy = (normal(1, 2, 700, 64, dtype=torch.float16, seed=n) for n in range(4))
+    table = normal(32, 2, dtype=torch.float16, seed=4)
+    short = [normal(40, 3, 49, 32, seed=n) for n in range(4)]
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, table)]
+        y = ops.op_attention(*leaves[:3], ops.op_position_bias(leaves[3], 700, 700), None, True)
+        return [t.detach() for t in [y] + list(torch.autograd.grad(y, leaves, dy)) + train(*short)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        graphs.append((graph, out))
+    for turn in range(4):
+        for t in [q, k, v, dy, table] + short:
+            t.mul_(0.9).add_(0.01 * turn)
+        for graph, out in graphs:
+            graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
     q = normal(1, 2, 40, 32).requires_grad_()
     alive = ops.op_attention(q, q, q)
