@@ -27,7 +27,7 @@ struct Side {
 struct AttentionArgs {
   Side q, k, v, out, d_out, dq, dk, dv;
   float* lse;                // [batch, heads, queries]; infinite for a query that sees nothing
-  float* delta;              // the same: do_i.o_i
+  float* delta;              // the same: -do_i.o_i, with which the sums of do_i.v_j begin
   int8_t* rest;              // [batch, queries, heads, width]: what rounding o to T has left out, see Rest; may be null
   const float* bias;         // [heads, queries + keys - 1], times log2(e)
   const uint8_t* mask;       // [batch, keys]
@@ -114,7 +114,15 @@ struct Tile {
   // what rounding p has left out
   static __device__ __forceinline__ Packed rest(const f32x16& p, const Packed& k) {
     f32x16 r = {};
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (std::is_same<T, bf16>::value) {
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {      // out of the pairs as they are: left to itself the compiler rounds every value again, on its own
+        uint32_t w = __builtin_bit_cast(u32x4, k.f[e >> 3])[(e & 7) / 2];
+        asm("" : "+v"(w));
+        r[e] = p[e] - __builtin_bit_cast(float, w << 16);
+        r[e + 1] = p[e + 1] - __builtin_bit_cast(float, w & 0xffff0000u);
+      }
+    } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int e = 0; e < 16; e++) r[e] = p[e] - (float)k.f[e >> 3][e & 7];
     }
@@ -370,7 +378,7 @@ __device__ __forceinline__ float delta_of(const typename Matrix<T>::Frag (&o)[NC
 }
 // A block's ds into dq or dk.  A row's ds add up to zero, or nearly, and few of them are large: their roundings do not average out.  What they leave out
 // makes a product of its own (bfloat16, a BERT-large layer: dq 0.0029 of its norm off without and 0.0021 with it, dk 0.0025 and 0.0019, of which 0.0017 is
-// the result's rounding; dq 73 us and 84, dk and dv 91 and 105)
+// the result's rounding; 12 us of 80, and 13 of 101)
 template <typename T, int DP, int WAVES>
 __device__ __forceinline__ void add_ds(f32x16 (&acc)[DP / 32], const lds_u8* keys, int first, const f32x16& ds, int lane) {
   using Shape = Tile<T, DP, WAVES>;
@@ -735,8 +743,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p) {
 // down its row of lanes by row_of(e) mod 16, lane m has the diagonals 16 c - m + 4 g - 16 half of all elements, where c is 0 for what stays in the row,
 // 1 for what leaves it, and one more for the keys from 16 on: three running sums a lane, two additions an element that shift as they add.  After a block
 // the sums of c = 0 and 1 are complete and the one of 2 is the next block's 0.  The four rows' sums, each a sequence along c and -m, meet in LDS.
-// Three products, and two of 16-bit types for what rounding leaves out; bound as the forward pass is: 32 x 16 heads of 512 tokens, width 64, bfloat16 85 us;
-// 8 x 16 of 1000, halves, with a bias 121, of which the diagonals take 30.
+// Three products, and two of 16-bit types for what rounding leaves out; bound as the forward pass is: 32 x 16 heads of 512 tokens, width 64, bfloat16 80 us;
+// 8 x 16 of 1000, halves, with a bias 116, of which the diagonals take 30.
 // (Additions into LDS by the hardware's atomics, 16 a block: 750 us for 8 x 16 heads of 1000 x 1000 halves where the kernel without them takes 100.)
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <int N>
@@ -788,7 +796,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     Frag o[NC];
     own_row<T, NC>(p.out.at(b, h, query), own, p.width, lane, o);
     delta = delta_of<T, NC>(o, dy, p.rest_at(b, h, query), p.width, lane);
-    if (own && lane < 32 && split == 0) p.delta[at] = delta;
+    if (own && lane < 32 && split == 0) p.delta[at] = -delta;
   }
   const int seen = p.seen(query);
   const int all_see = p.seen(first < p.queries ? first : p.queries - 1), some_see = p.seen(first + 31 < p.queries ? first + 31 : p.queries - 1);
@@ -840,6 +848,14 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
 
   float scale2 = p.scale2;
   asm("" : "+v"(scale2));
+  // what the sums of do_i.v_j begin with, in registers of its own; floats have none to spare, and their instructions take far longer than a subtraction
+  constexpr bool kBegin = sizeof(T) == 2;
+  f32x16 minus = {};
+  if constexpr (kBegin) {
+#pragma unroll
+    for (int e = 0; e < 16; e++) minus[e] = -delta;
+    asm("" : "+v"(minus));
+  }
   uint64_t there = 0, next = 0;
   present.ask(from + lane);
   next = present.answer();
@@ -856,13 +872,12 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     const int key = from + t * R;
     const lds_u8* const keys = ring + (t & 1) * 2 * kTile;
     const bool edge = key + R > all_see || (p.mask && (R == 64 ? ~there : ~there & 0xffffffffu) != 0);
-    auto product = [&](const lds_u8* rows, int n, const Frag (&own)[NC]) __attribute__((always_inline)) {
-      f32x16 s = {};
+    auto product = [&](const lds_u8* rows, int n, const Frag (&own)[NC], f32x16 s) __attribute__((always_inline)) {
 #pragma unroll
       for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(rows, 32 * n, c, lane), own[c], s);
       return s;
     };
-    // ds of a block from its scores and dp; `hidden`: with some of them hidden
+    // ds of a block from its scores and do.v - do.o; `hidden`: with some of them hidden
     auto gradient = [&](int n, f32x16 s, const f32x16& dp, bool hidden) __attribute__((always_inline)) {
       const int g4 = 4 * (lane >> 5);
 #pragma unroll
@@ -874,7 +889,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       }
       if (hidden) hide(s, seen - key - 32 * n, (uint32_t)(there >> (32 * n)), lane);
 #pragma unroll
-      for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(s[e]) * (dp[e] - delta);
+      for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(s[e]) * (kBegin ? dp[e] : dp[e] - delta);
       if constexpr (BIAS)
         if (along) add_diagonals(s, sums);
       return s;
@@ -882,7 +897,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
 #pragma unroll
     for (int n = 0; n < NB; n++) {
       if (key + 32 * n < some_see && there) {
-        const f32x16 ds = gradient(n, product(keys, n, q), product(keys + kTile, n, dy), edge);
+        const f32x16 ds = gradient(n, product(keys, n, q, f32x16{}), product(keys + kTile, n, dy, minus), edge);
         add_ds<T, DP, WAVES>(acc, keys, 32 * n, ds, lane);
       }
       if constexpr (BIAS)
@@ -901,8 +916,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // dk and dv: a wave has 32 keys, and the queries of all heads that share the key head pass by.  No sums through atomics: a result has the same bits every
-// time, for seven products in two kernels where one with atomics for dq would make five.  32 x 16 heads of 512 tokens, width 64, bfloat16: 105 us, bound as
-// the forward pass is.
+// time, for seven products in two kernels where one with atomics for dq would make five.  32 x 16 heads of 512 tokens, width 64, bfloat16: 101 us, bound as
+// the forward pass is; nothing that is loaded at the beginning waits for the mask (2 us).
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int WAVES, bool BIAS>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(waves_held<T, DP>(DKV)))) void attention_dkv_kernel(AttentionArgs p) {
@@ -924,29 +939,33 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   const uint32_t bh = work.head;
   const int b = bh / p.kv_heads, kv = bh % p.kv_heads;
   const int first = tile * BM + wave * 32, key = first + (lane & 31);
-  const bool own = key < p.keys && (!p.mask || p.mask[(int64_t)b * p.mask_stride + key]);
+  // which of the workgroup's keys there are, two bytes to a lane.  Nothing that is loaded waits for it
+  uint32_t present[BM / 64];
+#pragma unroll
+  for (int n = 0; n < BM / 64; n++) {
+    const int at = tile * BM + 64 * n + lane;
+    present[n] = at < p.keys;
+    if (p.mask && at < p.keys) present[n] = p.mask[(int64_t)b * p.mask_stride + at];
+  }
   Frag k[NC], v[NC];
-  own_row<T, NC>(p.k.at(b, kv, key), own, p.width, lane, k);
-  own_row<T, NC>(p.v.at(b, kv, key), own, p.width, lane, v);
+  own_row<T, NC>(p.k.at(b, kv, key), key < p.keys, p.width, lane, k);
+  own_row<T, NC>(p.v.at(b, kv, key), key < p.keys, p.width, lane, v);
   // queries from `seen_from` on see the lane's key
   const int behind = p.keys - p.queries;
   const int seen_from = p.causal && key > behind ? key - behind : 0;
   const int all_from = p.causal && first + 31 > behind ? first + 31 - behind : 0, some_from = p.causal && first > behind ? first - behind : 0;
   const int begin = (p.causal && tile * BM > behind ? tile * BM - behind : 0) / R * R;
   const int per_head = begin < p.queries ? (p.queries - begin + R - 1) / R : 0;
-  // no key of the workgroup's is there: only zeros to store
-  bool some = p.mask == nullptr;
-  for (int n = lane; n < BM && !some; n += 64) some = tile * BM + n < p.keys && p.mask[(int64_t)b * p.mask_stride + tile * BM + n];
   // the split's share of the tiles of queries of all heads, one after the other
-  const int all_steps = __ballot(some) ? per_head * p.group : 0;
-  const int first_step = (int)((int64_t)all_steps * split / p.splits), steps = (int)((int64_t)all_steps * (split + 1) / p.splits) - first_step;
+  const int all_steps = per_head * p.group;
+  const int first_step = (int)((int64_t)all_steps * split / p.splits), planned = (int)((int64_t)all_steps * (split + 1) / p.splits) - first_step;
 
   Load load_q, load_dy;
   load_q.set_up(p.q.row, p.width, wave, lane);
   load_dy.set_up(p.d_out.row, p.width, wave, lane);
   // the next tile to load: of head `head`, from query `ahead` on
   int head = kv * p.group, ahead = begin;
-  if (steps > 0) {
+  if (planned > 0) {
     head += first_step / per_head;
     ahead += first_step % per_head * R;
   }
@@ -977,7 +996,19 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
 
   float scale2 = p.scale2;
   asm("" : "+v"(scale2));
-  if (steps > 0) issue(0);
+  if (planned > 0) issue(0);
+  bool own = false, some = false;
+#pragma unroll
+  for (int n = 0; n < BM / 64; n++) {
+    const uint64_t keys = __ballot(present[n] != 0);
+    some |= keys != 0;
+    if (wave / 2 == n) own = keys >> (wave % 2 * 32 + (lane & 31)) & 1;
+  }
+  if (!own) {
+#pragma unroll
+    for (int c = 0; c < NC; c++) k[c] = v[c] = Frag{};
+  }
+  const int steps = some ? planned : 0;      // no key of the workgroup's is there: only zeros to store
   for (int t = 0; t < steps; t++) {
     wait_all();
     meet();
@@ -990,13 +1021,23 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     const lds_float* const lse = (const lds_float*)(stats + 2 * (t & 1) * kStats);
     const lds_float* const delta = (const lds_float*)(stats + (2 * (t & 1) + 1) * kStats);
     const bool edge = query < all_from || query + R > p.queries;
-    auto product = [&](const lds_u8* from, int n, const Frag (&own)[NC]) __attribute__((always_inline)) {
-      f32x16 s = {};
+    auto product = [&](const lds_u8* from, int n, const Frag (&own)[NC], f32x16 s) __attribute__((always_inline)) {
 #pragma unroll
       for (int c = 0; c < NC; c++) s = Matrix<T>::run(Shape::direct(from, 32 * n, c, lane), own[c], s);
       return s;
     };
-    // a block's scores to probabilities, and dp to ds
+    // what the sums of do_i.v_j of a block begin with
+    auto minus = [&](int n) __attribute__((always_inline)) {
+      f32x16 x;
+#pragma unroll
+      for (int e4 = 0; e4 < 16; e4 += 4) {
+        const f32x4 part = *(const lds_f32x4*)(delta + 32 * n + row_of(e4) + 4 * (lane >> 5));
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e4 + e] = part[e];
+      }
+      return x;
+    };
+    // a block's scores to probabilities, and do.v - do.o to ds
     auto gradient = [&](int n, f32x16& s, f32x16& dp, bool hidden) __attribute__((always_inline)) {
       const int g4 = 4 * (lane >> 5);
 #pragma unroll
@@ -1017,19 +1058,15 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
         for (int e = 0; e < 16; e++) s[e] = row_of(e) >= from && row_of(e) < to ? s[e] : -__builtin_inff();
       }
 #pragma unroll
-      for (int e4 = 0; e4 < 16; e4 += 4) {
-        const f32x4 x = *(const lds_f32x4*)(delta + 32 * n + row_of(e4) + g4);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          s[e4 + e] = __builtin_amdgcn_exp2f(s[e4 + e]);
-          dp[e4 + e] = s[e4 + e] * (dp[e4 + e] - x[e]);
-        }
+      for (int e = 0; e < 16; e++) {
+        s[e] = __builtin_amdgcn_exp2f(s[e]);
+        dp[e] *= s[e];
       }
     };
 #pragma unroll
     for (int n = 0; n < NB; n++) {
       if (query + 32 * n + 31 < some_from || query + 32 * n >= p.queries) continue;
-      f32x16 s = product(rows, n, k), dp = product(rows + kTile, n, v);
+      f32x16 s = product(rows, n, k, f32x16{}), dp = product(rows + kTile, n, v, minus(n));
       gradient(n, s, dp, edge);
       Shape::add(dv, rows + kTile, 32 * n, Shape::pack(s), lane);
       add_ds<T, DP, WAVES>(dk, rows, 32 * n, dp, lane);
