@@ -337,11 +337,13 @@ __device__ __forceinline__ void store_row(char* row, int8_t* rest, int width, in
     }
 }
 
-__device__ __forceinline__ float most_of(const f32x16& s) {
-  float m = __builtin_fmaxf(s[0], s[1]);
+// The largest of them, as the middle one of each two and `top`, infinity: a maximum of two would have every product's result made a quiet NaN first, if it
+// is one, in an instruction of its own
+__device__ __forceinline__ float most_of(const f32x16& s, float top) {
+  float m[2] = {__builtin_amdgcn_fmed3f(s[0], s[1], top), __builtin_amdgcn_fmed3f(s[2], s[3], top)};
 #pragma unroll
-  for (int e = 2; e < 16; e += 2) m = __builtin_fmaxf(m, __builtin_fmaxf(s[e], s[e + 1]));
-  return m;
+  for (int e = 4; e < 16; e++) m[e & 1] = __builtin_amdgcn_fmed3f(m[e & 1], s[e], top);
+  return __builtin_amdgcn_fmed3f(m[0], m[1], top);
 }
 
 // the same of a split, to be added up and multiplied later
@@ -495,7 +497,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   };
   // with a bias the scores are multiplied before it is added.  In vector registers: a scalar operand makes the multiplication take twice as long
   float unit2 = BIAS ? 1.0f : p.scale2, scale2 = p.scale2;
-  asm("" : "+v"(unit2), "+v"(scale2));
+  float top = __builtin_inff();
+  asm("" : "+v"(unit2), "+v"(scale2), "+v"(top));
   const float* const far = BIAS && APART ? p.bias + (int64_t)head * p.distances() + p.queries - 1 - query : nullptr;
   float most = -__builtin_inff(), limit = most, off = 0.0f, total = 0.0f;
   f32x16 acc[ND];
@@ -548,9 +551,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       add_bias(n, s[n]);
       if (edge) hide(s[n], seen - key - 32 * n, (uint32_t)(there >> (32 * n)), lane);
     }
-    float m = most_of(s[0]);
+    float m = most_of(s[0], top);
 #pragma unroll
-    for (int n = 1; n < NB; n++) m = __builtin_fmaxf(m, most_of(s[n]));
+    for (int n = 1; n < NB; n++) m = __builtin_amdgcn_fmed3f(m, most_of(s[n], top), top);
     // the maximum follows when it is left behind by 2^8, which probabilities of every type hold: mostly in the first tile alone
     if (__ballot(m > limit)) {
       m = __builtin_fmaxf(most_of_both(m), most);
