@@ -38,10 +38,11 @@ __global__ __launch_bounds__(1024) void attention_along_kernel(AlongArgs p) {
   __shared__ float shared[16][64];
   const int distances = p.queries + p.keys - 1, t = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6, h = blockIdx.y;
   const int blocks = (p.queries + 31) / 32, tiles = (p.queries + p.tall - 1) / p.tall;
-  // a wave has every 16th of the blocks of queries and the splits of their keys, for the batch entries in turn; diagonal t is number
-  // t + 32 (k + 1) - queries of block k from its first key on
+  // a wave has every 16th of the blocks of queries and the splits of their keys, for the batch entries in turn, or, where there are fewer than 16, one of
+  // them for every few batch entries (492 heads of 54 tokens 8 us, with one wave at work 22); diagonal t is number t + 32 (k + 1) - queries of block k from its first key on
   float sum = 0.0f;
-  for (int n = wave; n < blocks * p.splits; n += 16) {
+  const int units = blocks * p.splits, shares = units < 16 ? 16 / (units > 0 ? units : 1) : 1;
+  for (int n = wave / shares; n < units; n += 16 / shares) {
     const int k = n / p.splits, from_key = n % p.splits * p.per_split, tile = 32 * k / p.tall;
     const int last = tile * p.tall + p.tall - 1 < p.queries ? tile * p.tall + p.tall - 1 : p.queries - 1;
     int to = last + p.keys - p.queries + 1;
@@ -50,9 +51,11 @@ __global__ __launch_bounds__(1024) void attention_along_kernel(AlongArgs p) {
     const int at = t + 32 * (k + 1) - p.queries - from_key, there = to > from_key ? (to - from_key + p.rows - 1) / p.rows * p.rows : 0;
     if (t >= distances || at < 0 || at >= there + 32) continue;
     const float* from = p.along + (((int64_t)h * tiles * p.waves + k) * p.splits + n % p.splits) * p.stride + at;
-    const int64_t apart = (int64_t)p.heads * tiles * p.waves * p.splits * p.stride;
+    const int64_t entry = (int64_t)p.heads * tiles * p.waves * p.splits * p.stride, apart = shares * entry;
+    const int64_t share = wave % shares, entries = (p.batch + shares - 1 - share) / shares;
+    from += share * entry;
     int64_t b = 0;
-    for (; b + 8 <= p.batch; b += 8) {      // eight loads on their way at a time
+    for (; b + 8 <= entries; b += 8) {      // eight loads on their way at a time
       float v[8];
 #pragma unroll
       for (int u = 0; u < 8; u++) v[u] = from[u * apart];
@@ -60,7 +63,7 @@ __global__ __launch_bounds__(1024) void attention_along_kernel(AlongArgs p) {
       for (int u = 0; u < 8; u++) sum += v[u];
       from += 8 * apart;
     }
-    for (; b < p.batch; b++, from += apart) sum += *from;
+    for (; b < entries; b++, from += apart) sum += *from;
   }
   shared[wave][threadIdx.x & 63] = sum;
   __syncthreads();

@@ -85,6 +85,15 @@ def test_short_sequences(shape, kind, dtype):
     check(q, k, v, dy, bias, mask, kind in ("causal", "both"))
 
 
+# the batch entries' diagonals are added up by several waves where there are few blocks of queries
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("shape", [(37, 2, 2, 20, 24, 64), (300, 1, 1, 54, 54, 128), (21, 2, 1, 100, 40, 32), (9, 2, 2, 230, 70, 32)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", ["bias", "all"])
+def test_biases_of_many_batch_entries(shape, kind, dtype):
+    q, k, v, dy, bias, mask = inputs(*shape, dtype, True, kind == "all")
+    check(q, k, v, dy, bias, mask, kind == "all")
+
+
 # few tiles, with the keys and the queries cut into splits whose sums are added afterwards
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("shape", [(1, 1, 1, 700, 900, 64), (1, 4, 1, 333, 1100, 128), (2, 2, 2, 1500, 130, 40), (1, 2, 2, 130, 2049, 96), (1, 1, 1, 1025, 513, 32),
