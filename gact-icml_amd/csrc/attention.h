@@ -432,8 +432,9 @@ constexpr int waves_held(int kernel) {
 // ---------------------------------------------------------------------------------------------------------------------------------
 // The forward pass.  APART: for few queries the waves of a workgroup have the same 32 rows (the queries of all heads that share a key head), take the
 // keys in turn, each in tiles of its own, and add up at the end; splits of the keys go to workgroups of their own, which the joining kernels add up.
-// Bound by the vector instructions between its two products, of which a score takes nine and an exponential: 32 x 16 heads of 512 tokens, width 64, bfloat16
-// 61 us (564 TFLOP/s), 2 x 32 causal heads of 4096, width 128, 305 (900), where the products alone would take 14 and 110 at the instructions' peak.  One token
+// Bound by the vector instructions between its two products, of which a score takes four and an exponential, and which the products of a SIMD's two waves
+// hardly overlap: 32 x 16 heads of 512 tokens, width 64, bfloat16 59 us (582 TFLOP/s; the SIMDs are at them for 72 of 108 thousand cycles, at the products for
+// 22), 2 x 32 causal heads of 4096, width 128, 305 (900), where the products alone would take 14 and 110 at the instructions' peak.  One token
 // behind 65537 keys of 8 heads, width 128: 43 us, 6.3 TB/s, which is what memory gives.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int WAVES, bool APART, bool BIAS>
