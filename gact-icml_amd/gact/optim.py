@@ -47,12 +47,18 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's steps (decoupled weight decay) by op_adamw.  bits: 8 or 32, an option of every group of parameters.
 
     capturable: the count of steps is in device memory and every step adds one to it there, so that a step can be recorded in a graph; run one step
-    before the capture, which makes the states."""
+    before the capture, which makes the states.  Parameters that begin together, or are loaded with the same count, share it until a step finds only some
+    of them with a gradient; those of a recorded step go on together, and a step of some of them is refused, as the graph would count for all."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, bits=8, capturable=False):
         if not 0.0 <= float(lr) or not 0.0 <= eps or not 0.0 <= weight_decay or not all(0.0 <= b < 1.0 for b in betas):
             raise ValueError("lr, eps and weight_decay must be 0 or more, and the betas from 0 to below 1")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, bits=bits, capturable=capturable))
+        self._recorded = {}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._recorded = {}      # a copy's counts are its own
 
     def add_param_group(self, param_group):
         if param_group.get("bits", self.defaults["bits"]) not in (8, 32):
@@ -71,12 +77,28 @@ class AdamW(torch.optim.Optimizer):
         if kept.scale is not None:
             self.state[param]["scale"] = kept.scale
 
+    def _divide(self, work):
+        """The counts of a step's work: one on the GPU that parameters without a gradient hold as well is divided.  -> whether the step is recorded"""
+        if not any(isinstance(count, torch.Tensor) for _, count, _ in work):
+            return False
+        capturing = torch.cuda.is_current_stream_capturing()
+        holders = collections.Counter(id(kept["step"]) for kept in self.state.values() if "step" in kept)
+        for n, (group, count, params) in enumerate(work):
+            if not isinstance(count, torch.Tensor) or holders[id(count)] == len(params):
+                continue
+            if capturing or id(count) in self._recorded:
+                raise RuntimeError("a parameter that is counted together with others in a recorded step is without a gradient: give all of them "
+                                   "gradients, or load the state anew")
+            work[n] = (group, count.clone(), params)
+        return capturing
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        work = []
         for group in self.param_groups:
             # parameters whose counts are the same number, or the same tensor
             together, counts = {}, {}
@@ -87,23 +109,28 @@ class AdamW(torch.optim.Optimizer):
                     self._begin(group, p, counts)
                 count = self.state[p]["step"]
                 key = id(count) if isinstance(count, torch.Tensor) else count
-                together.setdefault(key, (count, []))[1].append(p)
-            for count, params in together.values():
-                states = [(kept["exp_avg"], kept["exp_avg_sq"], kept.get("scale")) for kept in map(self.state.__getitem__, params)]
-                count += 1      # in place where it is a tensor
-                try:
-                    op_adamw(params, [p.grad for p in params], states, count, group["lr"], group["betas"], group["eps"], group["weight_decay"])
-                except Exception:
-                    count -= 1      # a step that was refused has not been made
-                    raise
-                for p in params:
-                    self.state[p]["step"] = count
+                together.setdefault(key, (group, count, []))[2].append(p)
+            work.extend(together.values())
+        capturing = self._divide(work)
+        for group, count, params in work:
+            states = [(kept["exp_avg"], kept["exp_avg_sq"], kept.get("scale")) for kept in map(self.state.__getitem__, params)]
+            count += 1      # in place where it is a tensor
+            try:
+                op_adamw(params, [p.grad for p in params], states, count, group["lr"], group["betas"], group["eps"], group["weight_decay"])
+            except Exception:
+                count -= 1      # a step that was refused has not been made
+                raise
+            for p in params:
+                self.state[p]["step"] = count
+            if capturing and isinstance(count, torch.Tensor):
+                self._recorded[id(count)] = count
         return loss
 
     def load_state_dict(self, state_dict):
         """torch's own would turn codes and scales into the parameters' type."""
         saved = state_dict["state"]
         super().load_state_dict({**state_dict, "state": {}})
+        self._recorded = {}
         numbers = [n for group in state_dict["param_groups"] for n in group["params"]]
         params = [(group, p) for group in self.param_groups for p in group["params"]]
         counts = {}      # a group's own: each adds to its counts by itself

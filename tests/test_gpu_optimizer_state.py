@@ -1,0 +1,60 @@
+"""gact.optim.AdamW on the GPU: parameters that miss gradients, and states that go from one optimizer to another."""
+import pytest
+import torch
+
+import gact
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(*shape, dtype=torch.float32, seed=0):
+    g = torch.Generator().manual_seed(seed + 7919 * sum(shape))
+    return torch.randn(*shape, generator=g).to(dtype).cuda()
+
+
+def leaves(sizes, dtype=torch.float32):
+    return [normal(*s, dtype=dtype, seed=n).requires_grad_() for n, s in enumerate(sizes)]
+
+
+def test_counts_on_the_gpu_skip_parameters_without_gradients():
+    sizes = [(300,), (7, 41), (1000,)]
+    ours, theirs = leaves(sizes), leaves(sizes)
+    opts = [gact.optim.AdamW(p, lr=1e-2, bits=32, capturable=c) for p, c in ((ours, True), (theirs, False))]
+    for turn, some in enumerate([(0, 1, 2), (0,), (0,), (0, 2), (0, 1, 2), (1,), (0, 1, 2)]):
+        for params in (ours, theirs):
+            for n, p in enumerate(params):
+                p.grad = normal(*sizes[n], seed=10 * turn + n) if n in some else None
+        for opt in opts:
+            opt.step()
+        for p, q in zip(ours, theirs):
+            # the corrections are of the GPU's power function there and of the host's here: a unit in the last place of the step, or of the parameter
+            assert (p - q).abs().max() <= 2.0 ** -22 * (q.abs().max() + 1e-2 * 8)
+            assert int(opts[0].state[p]["step"]) == opts[1].state[q]["step"]
+    assert [opts[1].state[q]["step"] for q in theirs] == [6, 4, 4]
+
+
+def test_a_recorded_step_counts_for_all_that_it_has():
+    params, same = leaves([(300,), (50,)]), leaves([(300,), (50,)])
+    opt, other = gact.optim.AdamW(params, capturable=True), gact.optim.AdamW(same)
+    for p, q in zip(params, same):
+        p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(stream)
+    other.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for turn in range(3):
+        graph.replay()
+        other.step()
+    kept, params[1].grad = params[1].grad, None
+    with pytest.raises(RuntimeError, match="without a gradient"):
+        opt.step()
+    params[1].grad = kept
+    opt.step()
+    other.step()
+    for p, q in zip(params, same):
+        assert int(opt.state[p]["step"]) == other.state[q]["step"] == 5 and (p - q).abs().max() <= 2.0 ** -21

@@ -1,0 +1,83 @@
+"""What gact.optim.AdamW keeps of its parameters and loads, without a GPU: the step itself is replaced by one that notes the counts it is given."""
+import copy
+
+import pytest
+import torch
+
+from gact import optim
+
+
+@pytest.fixture
+def counts(monkeypatch):
+    """{parameter: the count of its last step}; a step on the CPU that changes nothing."""
+    seen = {}
+
+    def step(params, grads, states, count, *rest):
+        for p in params:
+            seen[p] = int(count)
+
+    monkeypatch.setattr(optim, "op_adamw", step)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return seen
+
+
+def parameters(n):
+    return [torch.nn.Parameter(torch.zeros(300)) for _ in range(n)]
+
+
+def step_with(opt, params, some):
+    for p in params:
+        p.grad = torch.zeros(300) if p in some else None
+    opt.step()
+
+
+@pytest.mark.parametrize("loaded", [False, True], ids=["begun", "loaded"])
+def test_a_parameter_without_a_gradient_is_not_counted(counts, loaded):
+    """Whether counts are numbers or in device memory, where parameters that begin together, or are loaded with the same number, share one."""
+    held = {}
+    for capturable in (False, True):
+        a, b, c = params = parameters(3)
+        opt = optim.AdamW(params, capturable=capturable)
+        step_with(opt, params, {a, b, c})
+        if loaded:
+            fresh = optim.AdamW(params, capturable=capturable)
+            fresh.load_state_dict(copy.deepcopy(opt.state_dict()))
+            opt = fresh
+        order = [{a}, {a, c}, {a}, {a, b}, {b, c}, {a, b, c}, {a, b, c}, {c}, {a, b, c}]
+        want = {p: 1 for p in params}
+        for some in order:
+            step_with(opt, params, some)
+            for p in some:
+                want[p] += 1
+                assert counts[p] == want[p]
+            assert [int(opt.state[p]["step"]) for p in params] == [want[p] for p in params]
+        held[capturable] = [counts[p] for p in params]
+        if capturable:      # those that go on together share a count as long as they do
+            together = optim.AdamW(params, capturable=True)
+            step_with(together, params, {a, b, c})
+            step_with(together, params, {a, b})
+            step_with(together, params, {a, b})
+            assert together.state[a]["step"] is together.state[b]["step"] is not together.state[c]["step"]
+    assert held[False] == held[True]
+
+
+def test_a_count_that_a_graph_adds_to_is_not_divided(counts, monkeypatch):
+    """A recorded step adds to the tensor that it was recorded with, for all parameters that it stepped."""
+    a, b, c = params = parameters(3)
+    opt = optim.AdamW([{"params": [a, b]}, {"params": [c]}], capturable=True)
+    step_with(opt, params, {a, b, c})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="without a gradient"):
+        step_with(opt, params, {a})
+    step_with(opt, params, {a, b})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    with pytest.raises(RuntimeError, match="without a gradient"):
+        step_with(opt, params, {b})
+    assert [int(opt.state[p]["step"]) for p in params] == [2, 2, 1]
+    step_with(opt, params, {c})
+    step_with(opt, params, {a, b})
+    assert [int(opt.state[p]["step"]) for p in params] == [3, 3, 2]
+    # a loaded state has counts of its own, which no graph adds to
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    step_with(opt, params, {b})
+    assert [int(opt.state[p]["step"]) for p in params] == [3, 4, 2]
