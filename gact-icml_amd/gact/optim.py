@@ -43,6 +43,11 @@ def op_adamw_values(states):
     return _abi.native().adamw_values(states)
 
 
+def _order(t):
+    """What the order of a dense tensor's elements in memory goes by."""
+    return [stride for size, stride in zip(t.shape, t.stride()) if size > 1]
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's steps (decoupled weight decay) by op_adamw.  bits: 8 or 32, an option of every group of parameters.
 
@@ -127,7 +132,8 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """torch's own would turn codes and scales into the parameters' type."""
+        """torch's own would turn codes and scales into the parameters' type.  States in 8 bits belong to the layout that their parameter had; those in
+        32 bits are loaded into any."""
         saved = state_dict["state"]
         super().load_state_dict({**state_dict, "state": {}})
         self._recorded = {}
@@ -145,6 +151,9 @@ class AdamW(torch.optim.Optimizer):
             for name, to in kept.items():
                 if held[name].dtype is not to.dtype or held[name].shape != to.shape:
                     raise ValueError("the saved %s does not belong to its parameter" % name)
+                if made.scale is not None and _order(held[name]) != _order(to):
+                    raise ValueError("the saved %s is in another order of memory than its parameter, and its codes' scales go by that order: give the "
+                                     "parameter the layout that it had" % name)
                 to.copy_(held[name])
             step = int(held["step"])
             if group["capturable"]:

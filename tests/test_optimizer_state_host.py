@@ -81,3 +81,40 @@ def test_a_count_that_a_graph_adds_to_is_not_divided(counts, monkeypatch):
     opt.load_state_dict(copy.deepcopy(opt.state_dict()))
     step_with(opt, params, {b})
     assert [int(opt.state[p]["step"]) for p in params] == [3, 4, 2]
+
+
+def a_state(p, bits, seed=0):
+    """A parameter's state with something in it."""
+    kept = {k: v for k, v in optim.op_adamw_state(p, bits)._asdict().items() if v is not None}
+    g = torch.Generator().manual_seed(seed)
+    for name, t in kept.items():
+        t.copy_(torch.randint(0, 128, t.shape, generator=g))
+    return {"step": 5, **kept}
+
+
+def saved(opt, states):
+    return {**opt.state_dict(), "state": dict(enumerate(states))}
+
+
+def test_codes_in_another_order_of_memory_are_refused():
+    """A group of codes is 256 neighbours in memory, and its scale theirs."""
+    last = torch.zeros(8, 3, 5, 5).to(memory_format=torch.channels_last)
+    first = torch.zeros(8, 3, 5, 5)
+    for given, to in ((last, first), (first, last), (torch.zeros(40, 30).t(), torch.zeros(30, 40))):
+        opt = optim.AdamW([torch.nn.Parameter(to)])
+        with pytest.raises(ValueError, match="order of memory"):
+            opt.load_state_dict(saved(opt, [a_state(given, 8)]))
+        # floats stand for themselves
+        opt = optim.AdamW([torch.nn.Parameter(to)], bits=32)
+        state = a_state(given, 32)
+        opt.load_state_dict(saved(opt, [state]))
+        for name in ("exp_avg", "exp_avg_sq"):
+            kept = opt.state[opt.param_groups[0]["params"][0]][name]
+            assert torch.equal(kept, state[name]) and kept.stride() == to.stride()
+    # the same order, whatever the strides of single rows are
+    for given, to in ((last, last), (first, first), (torch.zeros(1, 5, 1).as_strided((1, 5, 1), (7, 1, 3)), torch.zeros(1, 5, 1))):
+        opt = optim.AdamW([torch.nn.Parameter(to)])
+        state = a_state(given, 8)
+        opt.load_state_dict(saved(opt, [state]))
+        kept = opt.state[opt.param_groups[0]["params"][0]]
+        assert all(torch.equal(kept[name], state[name]) for name in ("exp_avg", "exp_avg_sq", "scale"))
