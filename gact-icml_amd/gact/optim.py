@@ -135,27 +135,33 @@ class AdamW(torch.optim.Optimizer):
         """torch's own would turn codes and scales into the parameters' type.  States in 8 bits belong to the layout that their parameter had; those in
         32 bits are loaded into any."""
         saved = state_dict["state"]
+        numbers = [n for group in state_dict["param_groups"] for n in group["params"]]
+        # everything that may be refused is looked at before anything is changed
+        states = {p: self._loaded(p, saved[n]) for n, p in zip(numbers, (p for group in self.param_groups for p in group["params"])) if saved.get(n)}
         super().load_state_dict({**state_dict, "state": {}})
         self._recorded = {}
-        numbers = [n for group in state_dict["param_groups"] for n in group["params"]]
-        params = [(group, p) for group in self.param_groups for p in group["params"]]
-        counts = {}      # a group's own: each adds to its counts by itself
-        for number, (group, p) in zip(numbers, params):
-            if number not in saved:
-                continue
-            held = saved[number]
-            made = op_adamw_state(p, 8 if "scale" in held else 32)
-            kept = {"exp_avg": made.exp_avg, "exp_avg_sq": made.exp_avg_sq}
-            if made.scale is not None:
-                kept["scale"] = made.scale
-            for name, to in kept.items():
-                if held[name].dtype is not to.dtype or held[name].shape != to.shape:
-                    raise ValueError("the saved %s does not belong to its parameter" % name)
-                if made.scale is not None and _order(held[name]) != _order(to):
-                    raise ValueError("the saved %s is in another order of memory than its parameter, and its codes' scales go by that order: give the "
-                                     "parameter the layout that it had" % name)
-                to.copy_(held[name])
-            step = int(held["step"])
-            if group["capturable"]:
-                step = counts.setdefault((id(group), p.device, step), torch.full((), step, dtype=torch.int64, device=p.device))
-            self.state[p] = {"step": step, **kept}
+        for group in self.param_groups:
+            counts = {}      # a group's own: each adds to its counts by itself
+            for p in group["params"]:
+                if p not in states:
+                    continue
+                step = states[p]["step"]
+                if group["capturable"]:
+                    step = counts.setdefault((p.device, step), torch.full((), step, dtype=torch.int64, device=p.device))
+                self.state[p] = {**states[p], "step": step}
+
+    @staticmethod
+    def _loaded(p, held):
+        """A parameter's state as it was saved, on its device."""
+        bits = 8 if "scale" in held else 32
+        made = {name: t for name, t in op_adamw_state(p, bits)._asdict().items() if t is not None}
+        for name, to in made.items():
+            if name not in held or held[name].dtype is not to.dtype or held[name].shape != to.shape:
+                raise ValueError("the saved %s does not belong to its parameter" % name)
+            if bits == 8 and _order(held[name]) != _order(to):
+                raise ValueError("the saved %s is in another order of memory than its parameter, and its codes' scales go by that order: give the "
+                                 "parameter the layout that it had" % name)
+            to.copy_(held[name])
+        if "step" not in held:
+            raise ValueError("the saved state has no step")
+        return {"step": int(held["step"]), **made}

@@ -118,3 +118,30 @@ def test_codes_in_another_order_of_memory_are_refused():
         opt.load_state_dict(saved(opt, [state]))
         kept = opt.state[opt.param_groups[0]["params"][0]]
         assert all(torch.equal(kept[name], state[name]) for name in ("exp_avg", "exp_avg_sq", "scale"))
+
+
+def test_a_refused_load_leaves_everything_as_it_was(counts):
+    params = parameters(2)
+    opt = optim.AdamW(params, lr=0.5)
+    step_with(opt, params, set(params))
+    kept = {p: dict(opt.state[p]) for p in params}
+    good = [a_state(p, 8) for p in params]
+    short = {**good[1], "exp_avg": torch.zeros(299, dtype=torch.int8)}
+    other = {**good[1], "exp_avg_sq": torch.zeros(300, dtype=torch.int8)}
+    for states in ([good[0], short], [good[0], other], [good[0], {"step": 5, "momentum_buffer": torch.zeros(300)}], [good[0], {"exp_avg": good[1]["exp_avg"]}]):
+        given = saved(opt, states)
+        given["param_groups"] = [{**given["param_groups"][0], "lr": 0.25}]
+        with pytest.raises(ValueError):
+            opt.load_state_dict(given)
+        assert opt.param_groups[0]["lr"] == 0.5 and list(opt.state) == params
+        for p in params:
+            assert all(opt.state[p][name] is t for name, t in kept[p].items()) and opt.state[p]["step"] == 1
+    given = saved(opt, good)
+    given["param_groups"] = given["param_groups"] * 2
+    with pytest.raises(ValueError):
+        opt.load_state_dict(given)
+    assert list(opt.state) == params
+    # of some of the parameters; an entry may be empty, as one whose first step was refused is
+    for states in (good[:1], [good[0], {}]):
+        opt.load_state_dict(saved(opt, states))
+        assert opt.state[params[0]]["step"] == 5 and not opt.state[params[1]]
