@@ -133,13 +133,24 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch's own would turn codes and scales into the parameters' type.  States in 8 bits belong to the layout that their parameter had; those in
-        32 bits are loaded into any."""
+        32 bits are loaded into any.  A checkpoint of torch.optim.AdamW's is one of states in 32 bits; options of its groups that make other steps
+        (amsgrad, maximize) are refused, and those that it lacks stay as they are."""
         saved = state_dict["state"]
+        for group in state_dict["param_groups"]:
+            other = [name for name in ("amsgrad", "maximize") if group.get(name)]
+            if group.get("weight_decay") and not group.get("decoupled_weight_decay", True):
+                other.append("weight decay in the gradient")
+            if other:
+                raise ValueError("the saved optimizer's steps are other ones: %s" % ", ".join(other))
         numbers = [n for group in state_dict["param_groups"] for n in group["params"]]
         # everything that may be refused is looked at before anything is changed
         states = {p: self._loaded(p, saved[n]) for n, p in zip(numbers, (p for group in self.param_groups for p in group["params"])) if saved.get(n)}
+        options = [{name: group[name] for name in self.defaults if name in group} for group in self.param_groups]
         super().load_state_dict({**state_dict, "state": {}})
         self._recorded = {}
+        for group, had in zip(self.param_groups, options):      # torch's groups have no bits
+            for name, value in had.items():
+                group.setdefault(name, value)
         for group in self.param_groups:
             counts = {}      # a group's own: each adds to its counts by itself
             for p in group["params"]:

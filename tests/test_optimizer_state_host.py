@@ -145,3 +145,45 @@ def test_a_refused_load_leaves_everything_as_it_was(counts):
     for states in (good[:1], [good[0], {}]):
         opt.load_state_dict(saved(opt, states))
         assert opt.state[params[0]]["step"] == 5 and not opt.state[params[1]]
+
+
+def test_a_checkpoint_of_torchs_adamw_is_loaded(counts):
+    params = parameters(3)
+    theirs = torch.optim.AdamW(params[:2], lr=0.125, betas=(0.5, 0.75), weight_decay=0.25)
+    for p in params:
+        p.grad = torch.ones(300)
+    theirs.step()
+    theirs.step()
+    given = copy.deepcopy(theirs.state_dict())
+    for bits in (8, 32):
+        opt = optim.AdamW(params[:2], bits=bits)
+        opt.load_state_dict(given)
+        group = opt.param_groups[0]
+        assert group["lr"] == 0.125 and group["betas"] == (0.5, 0.75) and group["weight_decay"] == 0.25 and group["bits"] == bits and not group["capturable"]
+        assert opt.state[params[0]]["step"] == 2 and torch.equal(opt.state[params[1]]["exp_avg"], given["state"][1]["exp_avg"])
+        # a parameter that comes later has the group's bits
+        group["params"].append(params[2])
+        opt.step()
+        assert counts[params[0]] == 3 and counts[params[2]] == 1
+        assert opt.state[params[2]]["exp_avg"].dtype is (torch.int8 if bits == 8 else torch.float32)
+    # what was saved before an option existed
+    given["param_groups"][0].pop("capturable")
+    opt = optim.AdamW(params[:2])
+    opt.load_state_dict({**given, "state": {}})
+    assert opt.param_groups[0]["capturable"] is False
+    step_with(opt, params, set(params))
+
+
+@pytest.mark.parametrize("option", [dict(amsgrad=True), dict(maximize=True)], ids=lambda o: next(iter(o)))
+def test_a_checkpoint_of_other_steps_is_refused(option):
+    """Options that change what a step is, and that this optimizer does not have, are not passed over."""
+    params = parameters(2)
+    theirs = torch.optim.AdamW(params, **option)
+    opt = optim.AdamW(params)
+    with pytest.raises(ValueError, match=next(iter(option))):
+        opt.load_state_dict(theirs.state_dict())
+    other = torch.optim.Adam(params, weight_decay=0.1).state_dict()
+    other["param_groups"][0]["decoupled_weight_decay"] = False
+    with pytest.raises(ValueError, match="decay"):
+        opt.load_state_dict(other)
+    assert "amsgrad" not in opt.param_groups[0]
