@@ -49,7 +49,8 @@ def _order(t):
 
 
 class AdamW(torch.optim.Optimizer):
-    """torch.optim.AdamW's steps (decoupled weight decay) by op_adamw.  bits: 8 or 32, an option of every group of parameters.
+    """torch.optim.AdamW's steps (decoupled weight decay) by op_adamw.  bits: 8 or 32, an option of every group of parameters.  lr: a number, a tensor on the
+    CPU, which is read at every step, or one float32 on the GPU, which the kernels read.
 
     capturable: the count of steps is in device memory and every step adds one to it there, so that a step can be recorded in a graph; run one step
     before the capture, which makes the states.  Parameters that begin together, or are loaded with the same count, share it until a step finds only some
@@ -119,9 +120,12 @@ class AdamW(torch.optim.Optimizer):
         capturing = self._divide(work)
         for group, count, params in work:
             states = [(kept["exp_avg"], kept["exp_avg_sq"], kept.get("scale")) for kept in map(self.state.__getitem__, params)]
+            lr = group["lr"]
+            if isinstance(lr, torch.Tensor) and lr.device.type == "cpu":
+                lr = float(lr)
             count += 1      # in place where it is a tensor
             try:
-                op_adamw(params, [p.grad for p in params], states, count, group["lr"], group["betas"], group["eps"], group["weight_decay"])
+                op_adamw(params, [p.grad for p in params], states, count, lr, group["betas"], group["eps"], group["weight_decay"])
             except Exception:
                 count -= 1      # a step that was refused has not been made
                 raise

@@ -58,3 +58,39 @@ def test_a_recorded_step_counts_for_all_that_it_has():
     other.step()
     for p, q in zip(params, same):
         assert int(opt.state[p]["step"]) == other.state[q]["step"] == 5 and (p - q).abs().max() <= 2.0 ** -21
+
+
+def test_a_rate_on_the_cpu_is_a_number():
+    params, same = leaves([(300,), (50, 3)]), leaves([(300,), (50, 3)])
+    opt, other = gact.optim.AdamW(params, lr=torch.tensor(0.01)), gact.optim.AdamW(same, lr=float(torch.tensor(0.01)))
+    for p, q in zip(params, same):
+        p.grad, q.grad = normal(*p.shape, seed=5), normal(*p.shape, seed=5)
+    for turn in range(3):
+        opt.step()
+        other.step()
+        assert all(torch.equal(p, q) for p, q in zip(params, same))
+        opt.param_groups[0]["lr"].mul_(0.5)
+        other.param_groups[0]["lr"] *= 0.5
+
+
+def test_torchs_checkpoint_goes_on_as_torch_does():
+    sizes = [(300,), (50, 3)]
+    params, same = leaves(sizes), leaves(sizes)
+    theirs = torch.optim.AdamW(params, lr=1e-2)
+    for turn in range(2):
+        for n, p in enumerate(params):
+            p.grad = normal(*sizes[n], seed=turn)
+        theirs.step()
+    with torch.no_grad():
+        for p, q in zip(params, same):
+            q.copy_(p)
+    opt = gact.optim.AdamW(same, bits=8)
+    opt.load_state_dict(theirs.state_dict())
+    for n, (p, q) in enumerate(zip(params, same)):
+        p.grad = normal(*sizes[n], seed=9)
+        q.grad = p.grad.clone()
+    theirs.step()
+    opt.step()
+    # one step from the same state: a few roundings in another order
+    for p, q in zip(params, same):
+        assert (p - q).abs().max() <= 16 * 2.0 ** -24 * (p.abs().max() + 1e-2)

@@ -187,3 +187,20 @@ def test_a_checkpoint_of_other_steps_is_refused(option):
     with pytest.raises(ValueError, match="decay"):
         opt.load_state_dict(other)
     assert "amsgrad" not in opt.param_groups[0]
+
+
+def test_a_rate_that_is_a_tensor_on_the_cpu(monkeypatch):
+    """A number like any other; one on the GPU goes to the kernels as it is."""
+    rates = []
+    monkeypatch.setattr(optim, "op_adamw", lambda params, grads, states, count, lr, *rest: rates.append(lr))
+    p = parameters(1)[0]
+    p.grad = torch.zeros(300)
+    opt = optim.AdamW([p], lr=torch.tensor(0.125))
+    opt.step()
+    opt.param_groups[0]["lr"].mul_(2)
+    opt.step()
+    opt.param_groups[0]["lr"] = 0.5
+    opt.step()
+    assert rates == [0.125, 0.25, 0.5] and not any(isinstance(r, torch.Tensor) for r in rates)
+    with pytest.raises(ValueError):
+        optim.AdamW([p], lr=torch.tensor(-1.0))
