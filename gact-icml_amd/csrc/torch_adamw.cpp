@@ -116,6 +116,8 @@ void step_all(std::vector<One>& all, const NumberAt<int64_t>& step, const Number
   std::vector<Range> ranges;
   for (One& o : all) {
     if (o.p.numel() == 0) continue;
+    for (const at::Tensor* t : {&step.at, &lr.at})
+      TORCH_CHECK(!t->defined() || t->device() == o.p.device(), "step and lr, where they are tensors, must be on the parameters' device");
     kinds[{o.p.device().index(), dtype_code(o.p.scalar_type()), o.state.codes() ? 8 : 32}].push_back(&o);
     add_range(ranges, o.p, true);
     add_range(ranges, o.state.m, true);
@@ -126,8 +128,6 @@ void step_all(std::vector<One>& all, const NumberAt<int64_t>& step, const Number
   refuse_overlaps(ranges);
   for (const auto& kind : kinds) {
     const Place at(kind.second[0]->p);
-    for (const at::Tensor* t : {&step.at, &lr.at})
-      TORCH_CHECK(!t->defined() || t->device() == at.device, "step and lr, where they are tensors, must be on the parameters' device");
     options.step = step.value;
     options.lr = lr.value;
     options.step_at = (const int64_t*)in(step.at);

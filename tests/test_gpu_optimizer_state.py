@@ -94,3 +94,13 @@ def test_torchs_checkpoint_goes_on_as_torch_does():
     # one step from the same state: a few roundings in another order
     for p, q in zip(params, same):
         assert (p - q).abs().max() <= 16 * 2.0 ** -24 * (p.abs().max() + 1e-2)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="two devices")
+def test_counts_on_another_device_are_refused_before_anything_runs():
+    params = [torch.ones(300, device="cuda:%d" % n) for n in range(2)]
+    step = torch.ones((), dtype=torch.int64, device="cuda:0")
+    grads = [torch.ones_like(p) for p in params]
+    with pytest.raises(RuntimeError, match="parameters' device"):
+        gact.ops.op_adamw(params, grads, [gact.ops.op_adamw_state(p) for p in params], step)
+    assert all((p == 1).all() for p in params)
