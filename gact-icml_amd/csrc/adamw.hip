@@ -2,7 +2,8 @@
 //
 // 8 bits: groups of 256 elements share the largest magnitude of either state.  The first moment's codes are spaced by the square, the second's by the
 // fourth power, so that sqrt(v), by which the step is divided, has the same spacing as m: a step of 0.8 % next to the largest, and values down to
-// (1/255)^4 of the largest of v.  A v above zero never becomes zero, which would blow its step up.
+// (1/255)^4 of the largest of v.  A v above zero never becomes zero, which would blow its step up: of a group whose largest is too small to divide by, the
+// codes are those beside kLeastV, so that a v of 1e-45 still stands for (1/255)^4 of it.
 #include <math.h>
 
 #include "device.h"
@@ -192,7 +193,7 @@ __device__ __forceinline__ void step_group(const gact_adamw_tensor& t, const Rat
   most_m = over_lanes<MostBits, kLanes>(most_m);
   most_v = over_lanes<MostBits, kLanes>(most_v);
   if (most_m < kLeastM) most_m = 0.0f;
-  if (most_v < kLeastV) most_v = 0.0f;
+  if (most_v > 0.0f && most_v < kLeastV) most_v = kLeastV;      // zero, the first moment would be divided by eps alone
   const float inv_m = most_m == 0.0f ? 0.0f : kSquare / most_m, inv_v = most_v == 0.0f ? 0.0f : kFourth / most_v;
 #pragma unroll
   for (int k = 0; k < kPieces; k++) {

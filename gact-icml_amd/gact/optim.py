@@ -2,7 +2,8 @@
 
 States in 8 bits take 2.06 bytes of an element where floats take 8: groups of 256 elements share the largest magnitude of either state, and a code is
 the square root of the first moment or the fourth root of the second, rounded to nearest, so that both moments of a step have the same spacing: 0.8 %
-of the largest next to it, finer below.  A second moment above zero is never rounded to zero.  Rounding is to nearest: steps are repeatable and need no seeds.
+of the largest next to it, finer below.  A second moment above zero is never rounded to zero, and a group's largest one is held as 1e-28 at least; a
+group whose largest first moment is below 1e-30 has zeros.  Rounding is to nearest: steps are repeatable and need no seeds.
 
 ``op_adamw`` is one launch for every 72 tensors of a type; parameters and states are changed in place.  Whatever cannot be taken raises a RuntimeError (a
 TypeError where no tensor was given), before anything is launched.

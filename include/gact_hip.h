@@ -341,8 +341,8 @@ int gact_position_bias_backward(const float* grad, int dtype, int64_t buckets, i
  * floats; g and p of `dtype`, the betas and 1 - beta rounded to float.  bits 32: m and v are floats.  bits 8: m int8 and v uint8 codes of groups of
  * 256 elements, the last one shorter, and scale [groups, 2] the largest |m| and v of each; a code c of m stands for c |c| (scale / 127^2), one of v
  * for c^4 (scale / 255^4), with the quotients and c^4 rounded to float (255^4 to 4228250624).  A value x of m gets the code nearest to the
- * root of |x| (127^2 / scale), one of v the nearest to its fourth root, and no v above 0 the code 0; a group whose largest |m| is below 1e-30 (v:
- * 1e-28) has scale and codes 0.  A group with an infinity or NaN is not finite afterwards.
+ * root of |x| (127^2 / scale), one of v the nearest to its fourth root, and no v above 0 the code 0; a group whose largest |m| is below 1e-30
+ * has scale and codes 0, one whose largest v is above 0 and below 1e-28 the scale 1e-28.  A group with an infinity or NaN is not finite afterwards.
  * p and g: any address that their type may have; m, v and scale 16-byte aligned.  Tensors must not overlap. */
 typedef struct gact_adamw_tensor {
   void* p;

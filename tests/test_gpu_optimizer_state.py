@@ -104,3 +104,28 @@ def test_counts_on_another_device_are_refused_before_anything_runs():
     with pytest.raises(RuntimeError, match="parameters' device"):
         gact.ops.op_adamw(params, grads, [gact.ops.op_adamw_state(p) for p in params], step)
     assert all((p == 1).all() for p in params)
+
+
+def test_second_moments_next_to_nothing_are_kept():
+    """Gradients whose squares are too small for a group's largest to be divided by, then none: with eps 0 a second moment lost would make the step infinite."""
+    lr, betas = 1e-2, (0.9, 0.999)
+    sizes = [10.0 ** -n for n in range(12, 18)]
+    p = torch.zeros(256 * len(sizes), device="cuda")
+    g = torch.tensor(sizes, device="cuda").repeat_interleave(256)
+    for dtype in (torch.float32, torch.bfloat16):
+        at, grad = p.to(dtype), g.to(dtype)
+        state = gact.ops.op_adamw_state(at)
+        m, v = torch.zeros_like(g).double(), torch.zeros_like(g).double()
+        for step in range(1, 8):
+            if step == 2:
+                grad = torch.zeros_like(grad)
+            before = at.clone()
+            gact.ops.op_adamw([at], [grad], [state], step, lr, betas, 0.0, 0.0)
+            m, v = betas[0] * m + (1 - betas[0]) * grad.double(), betas[1] * v + (1 - betas[1]) * grad.double() ** 2
+            want = lr * (m / (1 - betas[0] ** step)) / (v / (1 - betas[1] ** step)).sqrt()
+            moved = (before.double() - at.double()).abs()
+            # a code c for a value between c - 1/2 and c + 1/2 is off by (1 + 1 / (2 c))^2 in the second moment's root; c is 1 or more.  The first moment's
+            # one code is a group's largest, and exact
+            assert torch.isfinite(at).all() and state.exp_avg_sq.min() >= 1
+            close_to = 2.0 ** -8 * at.double().abs() if dtype is torch.bfloat16 else 1e-6
+            assert (moved <= 2.25 * 1.01 * want + close_to).all() and (moved >= want / 2.25 / 1.01 - close_to).all()
