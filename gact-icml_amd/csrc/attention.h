@@ -111,6 +111,28 @@ struct Tile {
       return p;
     }
   }
+  // `up` times it, and what rounding that has left out; up: a power of two, so that what is left out is exact before it is rounded itself
+  static __device__ __forceinline__ Packed pack_up(const f32x16& p, float up) {
+    Packed k;
+#pragma unroll
+    for (int e = 0; e < 16; e++) k.f[e >> 3][e & 7] = (T)(p[e] * up);
+    return k;
+  }
+  static __device__ __forceinline__ Packed rest_up(const f32x16& p, float up, const Packed& k) {
+    Packed r;
+#pragma unroll
+    for (int e = 0; e < 16; e++) r.f[e >> 3][e & 7] = (T)__builtin_fmaf(p[e], up, -(float)k.f[e >> 3][e & 7]);
+    return r;
+  }
+  // whether one of them is 2 or more, an infinity or no number, in float16
+  static __device__ __forceinline__ bool some_large(const Packed& k) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int w = 0; w < 4; w++) any |= __builtin_bit_cast(u32x4, k.f[h])[w];
+    return (any & 0x40004000u) != 0;
+  }
   // what rounding p has left out
   static __device__ __forceinline__ Packed rest(const f32x16& p, const Packed& k) {
     f32x16 r = {};
@@ -149,27 +171,43 @@ struct Tile {
     }
     return s[0] + s[1];
   }
+  // the tile's rows transposed, as the first operand of a product of 32 values of the width by 32 columns, whose depth is the rows
+  struct Turned {
+    Frag f[2][ND];
+  };
+  static __device__ __forceinline__ Frag turned(const lds_u8* tile, int first, int s, int d, int lane) {
+    const uint32_t i = lane & 15, half = (lane >> 4) & 1, g = lane >> 5;
+    const uint32_t r = 4 * g + (i >> 2), piece = 4 * d + 2 * half + ((i & 3) >> 1);
+    const lds_u8* lo = tile + (first + 16 * s) * W + r * W + ((piece ^ turn(r)) * 16) + (i & 1) * 8;
+    const lds_u8* hi = tile + (first + 16 * s) * W + (r + 8) * W + ((piece ^ turn(r + 8)) * 16) + (i & 1) * 8;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
+    return __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  static __device__ __forceinline__ Turned turned(const lds_u8* tile, int first, int lane) {
+    Turned t;
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int d = 0; d < ND; d++) t.f[s][d] = turned(tile, first, s, d, lane);
+    return t;
+  }
   // acc[32 values of the width, 32 columns] += the tile's rows transposed [., 32 rows] times p [32 rows, 32 columns]; and times `more`
   template <bool TWICE = false>
   static __device__ __forceinline__ void add(f32x16 (&acc)[ND], const lds_u8* tile, int first, const Packed& p, int lane, const Packed* more = nullptr) {
-    const uint32_t i = lane & 15, half = (lane >> 4) & 1, g = lane >> 5;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int s = 0; s < 2; s++) {
 #pragma unroll
         for (int d = 0; d < ND; d++) {
-          const uint32_t r = 4 * g + (i >> 2), piece = 4 * d + 2 * half + ((i & 3) >> 1);
-          const lds_u8* lo = tile + (first + 16 * s) * W + r * W + ((piece ^ turn(r)) * 16) + (i & 1) * 8;
-          const lds_u8* hi = tile + (first + 16 * s) * W + (r + 8) * W + ((piece ^ turn(r + 8)) * 16) + (i & 1) * 8;
-          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo);
-          const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
-          const Frag a = __builtin_bit_cast(Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+          const Frag a = turned(tile, first, s, d, lane);
           acc[d] = Matrix<T>::run(a, p.f[s], acc[d]);
           if constexpr (TWICE) acc[d] = Matrix<T>::run(a, more->f[s], acc[d]);
         }
       }
     } else {
       // the addresses anew each time, beside products of 64 cycles: kept from one block to the next they would take more registers than there are
+      const uint32_t g = lane >> 5;
       uint32_t l = lane & 31;
       asm volatile("" : "+v"(l));
 #pragma unroll
@@ -346,15 +384,15 @@ __device__ __forceinline__ float most_of(const f32x16& s, float top) {
   return __builtin_amdgcn_fmed3f(m[0], m[1], top);
 }
 
-// the same of a split, to be added up and multiplied later
+// the same of a split, to be added up and multiplied later; `down`: what takes it to the others' scale
 template <int DP, int ND>
-__device__ __forceinline__ void store_part(float* row, int width, int lane, const f32x16 (&acc)[ND]) {
+__device__ __forceinline__ void store_part(float* row, int width, int lane, const f32x16 (&acc)[ND], float down) {
 #pragma unroll
   for (int d = 0; d < ND; d++)
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
       const int col = 32 * d + row_of(e) + 4 * (lane >> 5);
-      if (col < width) *(f32x4*)(row + col) = f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
+      if (col < width) *(f32x4*)(row + col) = f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]} * down;
     }
 }
 
@@ -381,15 +419,62 @@ __device__ __forceinline__ float delta_of(const typename Matrix<T>::Frag (&o)[NC
 // A block's ds into dq or dk.  A row's ds add up to zero, or nearly, and few of them are large: their roundings do not average out.  What they leave out
 // makes a product of its own (bfloat16, a BERT-large layer: dq 0.0029 of its norm off without and 0.0021 with it, dk 0.0025 and 0.0019, of which 0.0017 is
 // the result's rounding; 12 us of 80, and 13 of 101)
+//
+// A float16 has nothing below 2^-25, and ds is about dy / keys: with dy of 1e-3 and 4096 keys dq was 0.0053 of its norm off where the result's rounding
+// is 0.0007, with 1e-4 0.053 (0.0066), and behind 65536 keys dv was 0.0007 (0.0002), whose probabilities are below 2^-14.  So in float16 the probabilities of
+// dv are multiplied by 2^15, and ds by `up`, a power of two for each row of dq or dk, which the lane and the one 32 further on share: 2^15, until a product
+// reaches 2, then the one that takes the largest so far to 1/8, and what has been added up follows.  A ds is so off by 2^-22 of the row's largest or by
+// 2^-40, and what is left is the result's own rounding.  In a block that changes nothing it is an OR of the pairs, half an instruction a score
+// (32 x 16 heads of 512 tokens, width 64, float16: dq 105 -> 106 us, dk and dv 109 -> 113; 2 x 16 causal heads on 4 of 2048 tokens, width 128, where one
+// wave has a SIMD and waits at the branch: 98 -> 108 and 109 -> 121; both blocks of a tile behind one branch were no faster).
+template <typename T>
+struct Up {
+  static constexpr bool kept = std::is_same<T, f16>::value;
+  static constexpr float kMost = 32768.0f;
+  // 1 / up
+  static __device__ __forceinline__ float down(float up) { return kept ? __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, up)) : 1.0f; }
+  template <typename Shape>
+  static __device__ __forceinline__ typename Shape::Packed probabilities(const f32x16& p) {
+    if constexpr (kept) return Shape::pack_up(p, kMost);
+    else return Shape::pack(p);
+  }
+  static constexpr float kDown = kept ? 1.0f / kMost : 1.0f;      // of dv
+};
 template <typename T, int DP, int WAVES>
-__device__ __forceinline__ void add_ds(f32x16 (&acc)[DP / 32], const lds_u8* keys, int first, const f32x16& ds, int lane) {
+__device__ __forceinline__ void add_ds(f32x16 (&acc)[DP / 32], float& up, const lds_u8* keys, int first, const f32x16& ds, int lane) {
   using Shape = Tile<T, DP, WAVES>;
-  const typename Shape::Packed k = Shape::pack(ds);
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (Up<T>::kept) {
+    // what the product reads is on its way before the branch
+    const typename Shape::Turned rows = Shape::turned(keys, first, lane);
+    typename Shape::Packed k = Shape::pack_up(ds, up);
+    if (__builtin_expect(__ballot(Shape::some_large(k)) != 0, 0)) {
+      float most = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; e++) most = __builtin_fmaxf(most, __builtin_fabsf(ds[e]));
+      most = most_of_both(most);
+      const uint32_t power = __builtin_bit_cast(uint32_t, most) >> 23;
+      // a row's own products alone move it, so that its bits are the same whatever rows it shares the wave with; an infinity does not, whose result is none
+      // either way
+      const bool moves = (float)(T)(most * up) >= 2.0f && power < 255;
+      const float fits = moves ? __builtin_bit_cast(float, (power < 250 ? 251 - power : 1) << 23) : up, factor = fits * Up<T>::down(up);
+      up = fits;
+      // through a product of zeros: read by a vector instruction themselves, wide rows' sums would be moved from the matrix unit's registers to the vector
+      // instructions' and back for every block
+#pragma unroll
+      for (int d = 0; d < DP / 32; d++) acc[d] = Matrix<T>::run({}, {}, acc[d]) * factor;
+      k = Shape::pack_up(ds, up);
+    }
+    const typename Shape::Packed more = Shape::rest_up(ds, up, k);
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int d = 0; d < DP / 32; d++) acc[d] = Matrix<T>::run(rows.f[s][d], more.f[s], Matrix<T>::run(rows.f[s][d], k.f[s], acc[d]));
+  } else if constexpr (sizeof(T) == 2) {
+    const typename Shape::Packed k = Shape::pack(ds);
     const typename Shape::Packed more = Shape::rest(ds, k);
     Shape::template add<true>(acc, keys, first, k, lane, &more);
   } else {
-    Shape::add(acc, keys, first, k, lane);
+    Shape::add(acc, keys, first, Shape::pack(ds), lane);
   }
 }
 
@@ -823,6 +908,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), from + t * R - last + p.queries - 1, BM + R - 1, wave, WAVES, biases + (t & 1) * kBias, lane);
   };
   f32x16 acc[ND];
+  float up = Up<T>::kMost;
 #pragma unroll
   for (int d = 0; d < ND; d++) acc[d] = f32x16{};
   typedef __attribute__((address_space(3))) float lds_float;
@@ -902,7 +988,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     for (int n = 0; n < NB; n++) {
       if (key + 32 * n < some_see && there) {
         const f32x16 ds = gradient(n, product(keys, n, q, f32x16{}), product(keys + kTile, n, dy, minus), edge);
-        add_ds<T, DP, WAVES>(acc, keys, 32 * n, ds, lane);
+        add_ds<T, DP, WAVES>(acc, up, keys, 32 * n, ds, lane);
       }
       if constexpr (BIAS)
         if (along) leave(t * NB + n, along);
@@ -913,9 +999,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     if (along) leave(steps * NB, along);
   if (!own || !p.dq.p) return;
   if (p.splits > 1)
-    store_part<DP, ND>(p.part + (((int64_t)split * (p.blocks / p.splits / p.tiles) + bh) * p.tiles * BM + mine) * DP, p.width, lane, acc);
+    store_part<DP, ND>(p.part + (((int64_t)split * (p.blocks / p.splits / p.tiles) + bh) * p.tiles * BM + mine) * DP, p.width, lane, acc, Up<T>::down(up));
   else
-    store_row<T, ND>((char*)p.dq.at(b, h, query), nullptr, p.width, lane, acc, p.scale);
+    store_row<T, ND>((char*)p.dq.at(b, h, query), nullptr, p.width, lane, acc, p.scale * Up<T>::down(up));
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -995,6 +1081,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     ahead += R;
   };
   f32x16 dk[ND], dv[ND];
+  float up = Up<T>::kMost;
 #pragma unroll
   for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
 
@@ -1072,8 +1159,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       if (query + 32 * n + 31 < some_from || query + 32 * n >= p.queries) continue;
       f32x16 s = product(rows, n, k, f32x16{}), dp = product(rows + kTile, n, v, minus(n));
       gradient(n, s, dp, edge);
-      Shape::add(dv, rows + kTile, 32 * n, Shape::pack(s), lane);
-      add_ds<T, DP, WAVES>(dk, rows, 32 * n, dp, lane);
+      Shape::add(dv, rows + kTile, 32 * n, Up<T>::template probabilities<Shape>(s), lane);
+      add_ds<T, DP, WAVES>(dk, up, rows, 32 * n, dp, lane);
     }
   }
   wait_all();
@@ -1086,12 +1173,12 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   }
   if (p.splits > 1) {
     const int64_t heads = p.blocks / p.splits / p.tiles, row = ((split * heads + bh) * p.tiles * BM + key) * DP;
-    if (p.dk.p) store_part<DP, ND>(p.part + row, p.width, lane, dk);
-    if (p.dv.p) store_part<DP, ND>(p.part + p.splits * heads * p.tiles * BM * DP + row, p.width, lane, dv);
+    if (p.dk.p) store_part<DP, ND>(p.part + row, p.width, lane, dk, Up<T>::down(up));
+    if (p.dv.p) store_part<DP, ND>(p.part + p.splits * heads * p.tiles * BM * DP + row, p.width, lane, dv, Up<T>::kDown);
     return;
   }
-  if (p.dk.p) store_row<T, ND>((char*)p.dk.at(b, kv, key), nullptr, p.width, lane, dk, p.scale * there);
-  if (p.dv.p) store_row<T, ND>((char*)p.dv.at(b, kv, key), nullptr, p.width, lane, dv, there);
+  if (p.dk.p) store_row<T, ND>((char*)p.dk.at(b, kv, key), nullptr, p.width, lane, dk, p.scale * Up<T>::down(up) * there);
+  if (p.dv.p) store_row<T, ND>((char*)p.dv.at(b, kv, key), nullptr, p.width, lane, dv, Up<T>::kDown * there);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -1140,6 +1227,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
   const int some_see = first < p.queries ? p.seen(first + 31 < p.queries ? first + 31 : p.queries - 1) : 0;
   const bool all_own = __ballot(own) == ~0ull;
   f32x16 dk[ND], dv[ND];
+  float up = Up<T>::kMost;
 #pragma unroll
   for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
   float scale2 = p.scale2;
@@ -1208,8 +1296,8 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
           ds[n][e4 + e] = s[e4 + e] * (dp[e4 + e] - x[e]);
         }
       }
-      Shape::add(dv, queries + kTile, 32 * n, Shape::pack(s), lane);
-      add_ds<T, DP, 2>(dk, queries, 32 * n, ds[n], lane);
+      Shape::add(dv, queries + kTile, 32 * n, Up<T>::template probabilities<Shape>(s), lane);
+      add_ds<T, DP, 2>(dk, up, queries, 32 * n, ds[n], lane);
       __builtin_amdgcn_sched_barrier(0);
     }
     meet();
@@ -1219,6 +1307,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
       for (int e = 0; e < 16; e++) *(lds_float*)(ds_of_key + (32 * n + row_of(e)) * kRow) = ds[n][e];
     meet();
     f32x16 dq[ND];
+    float dq_up = Up<T>::kMost;
 #pragma unroll
     for (int d = 0; d < ND; d++) dq[d] = f32x16{};
 #pragma unroll
@@ -1231,17 +1320,17 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
 #pragma unroll
         for (int e = 0; e < 4; e++) x[e4 + e] = part[e];
       }
-      add_ds<T, DP, 2>(dq, keys, 32 * n, x, lane);
+      add_ds<T, DP, 2>(dq, dq_up, keys, 32 * n, x, lane);
     }
-    if (mine < p.queries && p.dq.p) store_row<T, ND>((char*)p.dq.at(b, head, mine), nullptr, p.width, lane, dq, p.scale);
+    if (mine < p.queries && p.dq.p) store_row<T, ND>((char*)p.dq.at(b, head, mine), nullptr, p.width, lane, dq, p.scale * Up<T>::down(dq_up));
   }
   if (mine >= p.keys) return;
   if (!own) {
 #pragma unroll
     for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
   }
-  if (p.dk.p) store_row<T, ND>((char*)p.dk.at(b, kv, mine), nullptr, p.width, lane, dk, p.scale);
-  if (p.dv.p) store_row<T, ND>((char*)p.dv.at(b, kv, mine), nullptr, p.width, lane, dv, 1.0f);
+  if (p.dk.p) store_row<T, ND>((char*)p.dk.at(b, kv, mine), nullptr, p.width, lane, dk, p.scale * Up<T>::down(up));
+  if (p.dv.p) store_row<T, ND>((char*)p.dv.at(b, kv, mine), nullptr, p.width, lane, dv, Up<T>::kDown);
 }
 
 // out = factor times the sum of the splits' rows, in their order; which of two outputs: blockIdx.z.  Four columns to a lane, four loads on their way.  Latency:
