@@ -422,17 +422,21 @@ __device__ __forceinline__ float delta_of(const typename Matrix<T>::Frag (&o)[NC
 //
 // A float16 has nothing below 2^-25, and ds is about dy / keys: with dy of 1e-3 and 4096 keys dq was 0.0053 of its norm off where the result's rounding
 // is 0.0007, with 1e-4 0.053 (0.0066), and behind 65536 keys dv was 0.0007 (0.0002), whose probabilities are below 2^-14.  So in float16 the probabilities of
-// dv are multiplied by 2^15, and ds by `up`, a power of two for each row of dq or dk, which the lane and the one 32 further on share: 2^15, until a product
-// reaches 2, then the one that takes the largest so far to 1/8, and what has been added up follows.  A ds is so off by 2^-22 of the row's largest or by
-// 2^-40, and what is left is the result's own rounding.  In a block that changes nothing it is an OR of the pairs, half an instruction a score
-// (32 x 16 heads of 512 tokens, width 64, float16: dq 105 -> 106 us, dk and dv 109 -> 113; 2 x 16 causal heads on 4 of 2048 tokens, width 128, where one
-// wave has a SIMD and waits at the branch: 98 -> 108 and 109 -> 121; both blocks of a tile behind one branch were no faster).
+// dv are multiplied by 2^15, and ds by `up`, a power of two for each row of dq or dk, which the lane and the one 32 further on share: the one that takes
+// the largest of its first block to 1/64, 2^15 at most, and, where a product reaches 2, the one that does so with that; what has been added up follows.  A
+// ds is so off by 2^-19 of the row's largest or by 2^-40, and what is left is the result's own rounding.  It begins as infinity, with which every product
+// is too large, and in a block that changes nothing it is an OR of the pairs, half an instruction a score (the largest of them all, with a limit of 2^15
+// and so hardly a change, takes longer: 8 instructions of 16 scores instead of 4).  32 x 16 heads of 512 tokens, width 64, float16: dq 104 us as without
+// it, dk and dv 109 -> 113; 8 x 16 of 1000 with a bias: 113 as without, 107 -> 118; 2 x 16 causal heads on 4 of 2048 tokens, width 128, where one wave has a
+// SIMD and waits at the branch: 98 -> 102 and 109 -> 118 (both blocks of a tile behind one branch: no faster).
 template <typename T>
 struct Up {
   static constexpr bool kept = std::is_same<T, f16>::value;
-  static constexpr float kMost = 32768.0f;
-  // 1 / up
-  static __device__ __forceinline__ float down(float up) { return kept ? __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, up)) : 1.0f; }
+  static constexpr float kMost = 32768.0f, kBegin = __builtin_inff();
+  // 1 / up; of a row without a block: of nothing
+  static __device__ __forceinline__ float down(float up) {
+    return kept ? __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, __builtin_fminf(up, kMost))) : 1.0f;
+  }
   template <typename Shape>
   static __device__ __forceinline__ typename Shape::Packed probabilities(const f32x16& p) {
     if constexpr (kept) return Shape::pack_up(p, kMost);
@@ -453,11 +457,12 @@ __device__ __forceinline__ void add_ds(f32x16 (&acc)[DP / 32], float& up, const 
       for (int e = 0; e < 16; e++) most = __builtin_fmaxf(most, __builtin_fabsf(ds[e]));
       most = most_of_both(most);
       const uint32_t power = __builtin_bit_cast(uint32_t, most) >> 23;
-      // a row's own products alone move it, so that its bits are the same whatever rows it shares the wave with; an infinity does not, whose result is none
-      // either way
-      const bool moves = (float)(T)(most * up) >= 2.0f && power < 255;
-      const float fits = moves ? __builtin_bit_cast(float, (power < 250 ? 251 - power : 1) << 23) : up, factor = fits * Up<T>::down(up);
-      up = fits;
+      // what takes the largest to 1/64 and above; an infinity, whose row's result is none either way, has none
+      const float fits = __builtin_fminf(power < 247 ? __builtin_bit_cast(float, (248 - power) << 23) : power < 255 ? 0x1p-126f : Up<T>::kMost, Up<T>::kMost);
+      // a row's own products alone move it, so that its bits are the same whatever rows it shares the wave with
+      const bool moves = up == Up<T>::kBegin || ((float)(T)(most * up) >= 2.0f && power < 255);
+      const float factor = moves ? fits * Up<T>::down(up) : 1.0f;
+      up = moves ? fits : up;
       // through a product of zeros: read by a vector instruction themselves, wide rows' sums would be moved from the matrix unit's registers to the vector
       // instructions' and back for every block
 #pragma unroll
@@ -908,7 +913,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), from + t * R - last + p.queries - 1, BM + R - 1, wave, WAVES, biases + (t & 1) * kBias, lane);
   };
   f32x16 acc[ND];
-  float up = Up<T>::kMost;
+  float up = Up<T>::kBegin;
 #pragma unroll
   for (int d = 0; d < ND; d++) acc[d] = f32x16{};
   typedef __attribute__((address_space(3))) float lds_float;
@@ -1081,7 +1086,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     ahead += R;
   };
   f32x16 dk[ND], dv[ND];
-  float up = Up<T>::kMost;
+  float up = Up<T>::kBegin;
 #pragma unroll
   for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
 
@@ -1227,7 +1232,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
   const int some_see = first < p.queries ? p.seen(first + 31 < p.queries ? first + 31 : p.queries - 1) : 0;
   const bool all_own = __ballot(own) == ~0ull;
   f32x16 dk[ND], dv[ND];
-  float up = Up<T>::kMost;
+  float up = Up<T>::kBegin;
 #pragma unroll
   for (int d = 0; d < ND; d++) dk[d] = dv[d] = f32x16{};
   float scale2 = p.scale2;
@@ -1307,7 +1312,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
       for (int e = 0; e < 16; e++) *(lds_float*)(ds_of_key + (32 * n + row_of(e)) * kRow) = ds[n][e];
     meet();
     f32x16 dq[ND];
-    float dq_up = Up<T>::kMost;
+    float dq_up = Up<T>::kBegin;
 #pragma unroll
     for (int d = 0; d < ND; d++) dq[d] = f32x16{};
 #pragma unroll

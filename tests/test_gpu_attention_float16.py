@@ -2,7 +2,7 @@
 of the results themselves.
 
 Results are compared by their norms with 64 bits.  A result's rounding is half a step at most, 2^-11 of it or 2^-25.  What else there is of dq and dk: ds as a
-pair of float16 numbers, off by 2^-22 of a row's largest or 2^-40; the byte of each o, 2^-19 of do.o; probabilities from scores in 32 bits, 2^-19: of
+pair of float16 numbers, off by 2^-19 of a row's largest or 2^-40; the byte of each o, 2^-19 of do.o; probabilities from scores in 32 bits, 2^-19: of
 each ds, together below 2^-17.  A row of dq adds up ds of either sign whose sizes are those of the sum times the root of their number at most, whose
 deviation from the mean of k is of order one: 2^-13 of the norm is four times more than that for the widest cancellation here (16).  dv is a
 product of probabilities rounded to float16, each off by 2^-11 of itself with a sign of its own."""
