@@ -586,6 +586,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       load_floats(p.bias + (int64_t)h * p.distances(), p.distances(), begin + t * step - (tile * BM + BM - 1) + p.queries - 1, BM + R - 1, wave, WAVES,
                   biases + (t & 1) * kBias, lane);
   };
+  // In float16 the probabilities are multiplied by 2^7, which 2^8, the most that one of them is before the maximum follows, leaves room for: unscaled, 100000 keys of
+  // 2^-19 beside one of 1 are subnormal numbers, off by 2^-6 each, and the result by 0.004.  Sums and lse follow.
+  constexpr float kUp = std::is_same<T, f16>::value ? 7.0f : 0.0f;
   // with a bias the scores are multiplied before it is added.  In vector registers: a scalar operand makes the multiplication take twice as long
   float unit2 = BIAS ? 1.0f : p.scale2, scale2 = p.scale2;
   float top = __builtin_inff();
@@ -650,7 +653,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
       m = __builtin_fmaxf(most_of_both(m), most);
       const float factor = m > most ? __builtin_amdgcn_exp2f((most - m) * unit2) : 1.0f;
       most = m;
-      off = m == -__builtin_inff() ? 0.0f : m * unit2;
+      off = m == -__builtin_inff() ? 0.0f : m * unit2 - kUp;
       limit = m + 8.0f / unit2;
       total *= factor;
 #pragma unroll
@@ -678,7 +681,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   wait_all();
 
   total = sum_of_both(total);
-  most = most == -__builtin_inff() ? most : most * unit2;
+  most = most == -__builtin_inff() ? most : most * unit2 - kUp;
   if constexpr (!APART) {
     if (!own) return;
     store_row<T, ND>((char*)p.out.at(b, head, query), p.rest_at(b, head, query), p.width, lane, acc, total > 0.0f ? 1.0f / total : total);

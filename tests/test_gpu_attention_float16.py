@@ -127,3 +127,24 @@ def test_an_infinite_gradient_stays_in_its_row(shape):
         dv[0, 1, :, 3] = want[2][0, 1, :, 3]
         off = (dv[0, 1] - want[2][0, 1]).double()
         assert torch.equal(dv[0, 0], want[2][0, 0]) and torch.isfinite(off).all() and off.abs().max() == 0
+
+
+@pytest.mark.parametrize("keys,below", [(100000, 32.49), (20000, 8.49), (1000000, 300.49)])
+@pytest.mark.parametrize("shape", [(300, 33), (1, 1), (2, 300)], ids=["tiles", "one", "few"])
+def test_many_small_probabilities_beside_a_large_one(shape, keys, below):
+    """One key's score is so far above all others' that their probabilities, unnormalised, lie between two of float16's subnormal numbers; together they count.
+    Each is off by 2^-32 of the largest at most, which one is 1 or more: keys times that of the sum, and of the values' sizes."""
+    heads, queries = shape
+    q, k = torch.zeros(1, heads, queries, 64, dtype=HALF, device="cuda"), torch.zeros(1, 1, keys, 64, dtype=HALF, device="cuda")
+    v = torch.full_like(k, -1.0)
+    q[..., 0], k[0, 0, 0, 0], v[0, 0, 0] = 1.0, 13.0, 1.0
+    apart = math.log(2.0 ** 24 / below)
+    bias = torch.zeros(heads, queries + keys - 1, device="cuda")
+    others = (keys - 1) * math.exp(-13.0 * (scale := torch.tensor(apart / 13.0).item()))
+    want = (1 - others) / (1 + others)
+    for given in (None, bias):
+        with torch.no_grad():
+            y = ops.op_attention(q, k, v, given, scale=scale).double()
+        # the result's rounding, and the exponents' in 32 bits
+        off = 2.0 ** -11 * abs(want) + 2 * keys * 2.0 ** -32 + 2.0 ** -17
+        assert (y - want).abs().max() <= off, (float((y - want).abs().max()), off)
