@@ -141,7 +141,7 @@ inline int64_t esz(int dtype) { return dtype == GACT_F32 ? 4 : 2; }
 bool sizes_fit(const gact_attention* a) {
   if (!known(a->dtype) || a->batch < 0 || a->queries < 0 || a->keys < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads) return false;
   if (a->queries > GACT_ATTENTION_MAX_LENGTH || a->keys > GACT_ATTENTION_MAX_LENGTH || a->heads > 65535 || a->batch > 0x7fffffff) return false;
-  return a->width >= 1 && a->width <= GACT_ATTENTION_MAX_WIDTH && a->scale > 0.0f && a->scale < __builtin_inff();
+  return a->width >= 1 && a->width <= GACT_ATTENTION_MAX_WIDTH && a->scale > 0.0f && a->scale * kLog2e < __builtin_inff();
 }
 int64_t distances(const gact_attention* a) { return a->queries + a->keys > 0 ? a->queries + a->keys - 1 : 0; }
 // whole 16-byte pieces, and rows that the kernels' offsets reach.  GACT_OK where nothing of it is read

@@ -175,7 +175,7 @@ at::Tensor attention(const at::Tensor& q_given, const at::Tensor& k_given, const
   TORCH_CHECK(q_given.size(2) <= GACT_ATTENTION_MAX_LENGTH && k_given.size(2) <= GACT_ATTENTION_MAX_LENGTH, "attention takes up to ",
               GACT_ATTENTION_MAX_LENGTH, " queries and keys");
   const double scale = scale_given ? *scale_given : 1.0 / std::sqrt((double)width);
-  TORCH_CHECK((float)scale > 0.0f && std::isfinite((float)scale), "scale must be a positive number");
+  TORCH_CHECK((float)scale > 0.0f && std::isfinite((float)scale * 1.44269504f), "scale must be a positive number below 2.3e38");
   const int64_t distances = std::max<int64_t>(q_given.size(2) + k_given.size(2) - 1, 0);
   if (b_given) {
     TORCH_CHECK(autocast || b_given->scalar_type() == at::kFloat, "The type of bias is not correct!");

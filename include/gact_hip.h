@@ -307,7 +307,7 @@ typedef struct gact_rows {
 typedef struct gact_attention {
   int32_t dtype, causal;
   int64_t batch, heads, kv_heads, queries, keys, width;
-  float scale;          /* above 0 */
+  float scale;          /* above 0; times log2(e) a float */
   float reserved;
   const float* bias;    /* [heads, queries + keys - 1], may be null */
   const uint8_t* mask;  /* [batch, keys], rows mask_stride bytes apart; may be null */
