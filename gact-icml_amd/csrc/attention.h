@@ -36,6 +36,7 @@ struct AttentionArgs {
   int64_t along_stride;
   int heads, kv_heads, group, queries, keys, width;
   bool causal;
+  bool blind;                // there may be queries that see nothing
   float scale, scale2;       // and times log2(e)
   uint32_t tiles, blocks;    // of a head, and in all
   bool by_length;            // see work_of
@@ -234,12 +235,13 @@ struct RowsLoad {
   uint32_t at[kLoads];
   int wave;
   static __device__ __forceinline__ uint32_t row(int wave, int q, int lane) { return ((wave * kLoads + q) * 1024 + lane * 16) / W; }
-  __device__ __forceinline__ void set_up(int64_t stride, int width, int w, int lane) {
+  // (rows before `from` become zero as well)
+  __device__ __forceinline__ void set_up(int64_t stride, int width, int w, int lane, int from = 0) {
     wave = w;
 #pragma unroll
     for (int q = 0; q < kLoads; q++) {
       const uint32_t r = row(w, q, lane), piece = ((lane * 16 % W) / 16) ^ Shape::turn(r);
-      at[q] = (int)piece * 16 < width * Shape::kEsz ? r * (uint32_t)stride + piece * 16 : kNowhere;
+      at[q] = (int)piece * 16 < width * Shape::kEsz && (int)r >= from ? r * (uint32_t)stride + piece * 16 : kNowhere;
     }
   }
   // from `base` on, of which `left` rows are there; `tiles` of ROWS rows to a step
@@ -493,6 +495,19 @@ __device__ __forceinline__ void hide(f32x16& s, int seen, uint32_t there, int la
   there = (there >> g4) & (seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1);
 #pragma unroll
   for (int e = 0; e < 16; e++) s[e] = there >> row_of(e) & 1 ? s[e] : -__builtin_inff();
+}
+
+// The gradients of queries that see nothing are nobody's, whatever they are: zeros take their place in a tile, where a NaN times a probability of zero
+// would be one.  A wave clears every WAVES-th row.  -> whether there are any, which all waves find alike
+template <int W, int ROWS, int WAVES>
+__device__ __forceinline__ bool clear_blind(lds_u8* tile, const __attribute__((address_space(3))) float* lse, int wave, int lane) {
+  const uint64_t all = __ballot(lse[lane & (ROWS - 1)] == __builtin_inff()), none = ROWS < 64 ? all & 0xffffffffu : all;
+  if (__builtin_expect(none == 0, 1)) return false;
+  for (uint64_t left = none; left; left &= left - 1) {
+    const int r = __builtin_ctzll(left);
+    if (r % WAVES == wave && lane * 16 < W) *(__attribute__((address_space(3))) u32x4*)(tile + r * W + lane * 16) = u32x4{};
+  }
+  return true;
 }
 
 // what the kernels over keys share: which keys of a tile there are.  The bytes of the next tile but one are on their way while a tile is worked on.
@@ -888,6 +903,11 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
   own_row<T, NC>(p.d_out.at(b, h, query), own, p.width, lane, dy);
   const int64_t at = ((int64_t)b * p.heads + h) * p.queries + query;
   const float lse = own ? p.lse[at] : __builtin_inff();
+  if (p.blind && __ballot(lse == __builtin_inff())) {
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+      if (lse == __builtin_inff()) dy[c] = Frag{};
+  }
   float delta;
   {
     Frag o[NC];
@@ -1119,6 +1139,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(wave
     const lds_u8* const rows = ring + (t & 1) * 2 * kTile;
     const lds_float* const lse = (const lds_float*)(stats + 2 * (t & 1) * kStats);
     const lds_float* const delta = (const lds_float*)(stats + (2 * (t & 1) + 1) * kStats);
+    // (with a mask alone a query that sees nothing is one of a batch entry without keys, which has no steps)
+    if (BIAS || (p.causal && p.blind))
+      if (clear_blind<W, R, WAVES>(ring + (t & 1) * 2 * kTile + kTile, lse, wave, lane)) meet();
     const bool edge = query < all_from || query + R > p.queries;
     auto product = [&](const lds_u8* from, int n, const Frag (&own)[NC], f32x16 s) __attribute__((always_inline)) {
 #pragma unroll
@@ -1234,6 +1257,10 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
   // keys that the wave's queries see
   const int some_see = first < p.queries ? p.seen(first + 31 < p.queries ? first + 31 : p.queries - 1) : 0;
   const bool all_own = __ballot(own) == ~0ull;
+  // queries before it see nothing, and zeros take the place of their gradients, which are nobody's
+  const uint64_t keys_there = p.keys < 64 ? there & ((1ull << p.keys) - 1) : there;
+  const int first_key = keys_there ? __builtin_ctzll(keys_there) : 0;
+  const int sees_from = !keys_there ? 64 : p.causal && first_key > behind ? first_key - behind : 0;
   f32x16 dk[ND], dv[ND];
   float up = Up<T>::kBegin;
 #pragma unroll
@@ -1254,7 +1281,7 @@ __global__ __launch_bounds__(128) __attribute__((amdgpu_waves_per_eu(waves_held<
     load.set_up(p.q.row, p.width, wave, lane);
     load.start(p.q.at(b, head, 0), p.queries, p.q.row, p.width);
     load.next(false, 0, queries, lane);
-    load.set_up(p.d_out.row, p.width, wave, lane);
+    load.set_up(p.d_out.row, p.width, wave, lane, sees_from);
     load.start(p.d_out.at(b, head, 0), p.queries, p.d_out.row, p.width);
     load.next(false, 0, queries + kTile, lane);
     const int64_t at = ((int64_t)b * p.heads + head) * p.queries;

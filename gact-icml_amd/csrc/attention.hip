@@ -263,6 +263,7 @@ AttentionArgs args_of(const gact_attention* a) {
   p.keys = (int)a->keys;
   p.width = (int)a->width;
   p.causal = a->causal != 0;
+  p.blind = a->bias || a->mask || (p.causal && a->queries > a->keys);
   p.scale = a->scale;
   p.scale2 = a->scale * kLog2e;
   p.splits = 1;

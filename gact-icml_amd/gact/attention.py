@@ -22,7 +22,7 @@ def op_attention(query, key, value, bias=None, mask=None, causal=False, scale=No
     bias: float32 [heads, queries + keys - 1], added at j - i + queries - 1 (op_position_bias makes one); values of -1e30 or less hide the key.
     mask: bool [batch, keys], which keys are there.  What absent keys and values hold does not matter.
     causal: query i sees the keys up to i + keys - queries: the last query sees all of them.  A NaN of a key that is hidden in this way may show.
-    A query that nothing is left for gets zeros, and gives none of its gradient to anyone.
+    A query that nothing is left for gets zeros, and gives none of its gradient to anyone, NaN and infinity included.
 
     The result lies in memory as [batch, queries, heads, width], so that its transpose(1, 2) is a projection's contiguous input.  Under hooks for saved
     tensors (the Controller's) query, key and value, and a mask, are all that they get; the bias is held as it is, and the backward pass runs the forward
