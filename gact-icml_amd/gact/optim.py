@@ -172,7 +172,8 @@ class AdamW(torch.optim.Optimizer):
         bits = 8 if "scale" in held else 32
         made = {name: t for name, t in op_adamw_state(p, bits)._asdict().items() if t is not None}
         for name, to in made.items():
-            if name not in held or held[name].dtype is not to.dtype or held[name].shape != to.shape:
+            fits = name in held and (held[name].dtype is to.dtype or bits == 32 and held[name].is_floating_point()) and held[name].shape == to.shape
+            if not fits:
                 raise ValueError("the saved %s does not belong to its parameter" % name)
             if bits == 8 and _order(held[name]) != _order(to):
                 raise ValueError("the saved %s is in another order of memory than its parameter, and its codes' scales go by that order: give the "

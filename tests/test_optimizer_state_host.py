@@ -204,3 +204,23 @@ def test_a_rate_that_is_a_tensor_on_the_cpu(monkeypatch):
     assert rates == [0.125, 0.25, 0.5] and not any(isinstance(r, torch.Tensor) for r in rates)
     with pytest.raises(ValueError):
         optim.AdamW([p], lr=torch.tensor(-1.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_a_checkpoint_with_moments_of_another_type_is_loaded(dtype):
+    """torch's moments have their parameter's type; here they are float32, whatever that is."""
+    p = torch.nn.Parameter(torch.zeros(300, dtype=dtype))
+    theirs = torch.optim.AdamW([p])
+    p.grad = torch.ones(300, dtype=dtype) * 0.3
+    theirs.step()
+    given = theirs.state_dict()
+    opt = optim.AdamW([p], bits=32)
+    opt.load_state_dict(given)
+    for name in ("exp_avg", "exp_avg_sq"):
+        kept = opt.state[p][name]
+        assert kept.dtype is torch.float32 and torch.equal(kept, given["state"][0][name].float())
+    # codes are not floats of another type
+    state = a_state(torch.zeros(300), 32)
+    state["exp_avg"] = state["exp_avg"].to(torch.int8)
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.load_state_dict(saved(opt, [state]))
