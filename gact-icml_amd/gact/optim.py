@@ -93,7 +93,10 @@ class AdamW(torch.optim.Optimizer):
         for n, (group, count, params) in enumerate(work):
             if not isinstance(count, torch.Tensor) or holders[id(count)] == len(params):
                 continue
-            if capturing or id(count) in self._recorded:
+            if capturing:
+                raise RuntimeError("a parameter that is counted together with others is without a gradient: run a step of those that have one before "
+                                   "the capture")
+            if id(count) in self._recorded:
                 raise RuntimeError("a parameter that is counted together with others in a recorded step is without a gradient: give all of them "
                                    "gradients, or load the state anew")
             work[n] = (group, count.clone(), params)
