@@ -427,10 +427,11 @@ __device__ __forceinline__ float delta_of(const typename Matrix<T>::Frag (&o)[NC
 // dv are multiplied by 2^15, and ds by `up`, a power of two for each row of dq or dk, which the lane and the one 32 further on share: the one that takes
 // the largest of its first block to 1/64, 2^15 at most, and, where a product reaches 2, the one that does so with that; what has been added up follows.  A
 // ds is so off by 2^-19 of the row's largest or by 2^-40, and what is left is the result's own rounding.  It begins as infinity, with which every product
-// is too large, and in a block that changes nothing it is an OR of the pairs, half an instruction a score (the largest of them all, with a limit of 2^15
-// and so hardly a change, takes longer: 8 instructions of 16 scores instead of 4).  32 x 16 heads of 512 tokens, width 64, float16: dq 104 us as without
-// it, dk and dv 109 -> 113; 8 x 16 of 1000 with a bias: 113 as without, 107 -> 118; 2 x 16 causal heads on 4 of 2048 tokens, width 128, where one wave has a
-// SIMD and waits at the branch: 98 -> 102 and 109 -> 118 (both blocks of a tile behind one branch: no faster).
+// is too large, and in a block that changes nothing it is an OR of the pairs, a third of an instruction a score (the sum of their squares, with a limit of
+// 2^15 and so hardly a change, takes as long where rows change and 2 % longer where they do not).  32 x 16 heads of 512 tokens, width 64, float16: dq 104 us as without
+// it, dk and dv 109 -> 113; 8 x 16 of 1000 with a bias: 113 as without, 107 -> 118, and where some channels are larger, so that the largest grows along a
+// row, 117 -> 123 and 111 -> 124; 2 x 16 causal heads on 4 of 2048 tokens, width 128, where one wave has a SIMD and waits at the branch: 98 -> 102 and
+// 109 -> 118 (both blocks of a tile behind one branch: no faster).
 template <typename T>
 struct Up {
   static constexpr bool kept = std::is_same<T, f16>::value;
@@ -538,8 +539,9 @@ constexpr int waves_held(int kernel) {
 // The forward pass.  APART: for few queries the waves of a workgroup have the same 32 rows (the queries of all heads that share a key head), take the
 // keys in turn, each in tiles of its own, and add up at the end; splits of the keys go to workgroups of their own, which the joining kernels add up.
 // Bound by the vector instructions between its two products, of which a score takes four and an exponential, and which the products of a SIMD's two waves
-// hardly overlap: 32 x 16 heads of 512 tokens, width 64, bfloat16 59 us (582 TFLOP/s; the SIMDs are at them for 72 of 108 thousand cycles, at the products for
-// 22), 2 x 32 causal heads of 4096, width 128, 305 (900), where the products alone would take 14 and 110 at the instructions' peak.  One token
+// hardly overlap: 32 x 16 heads of 512 tokens, width 64, bfloat16, of which a mask leaves 0.69 of the tiles, 59 us (400 TFLOP/s of those; the SIMDs are at the
+// vector instructions for 72 of 108 thousand cycles, at the products for 22), 2 x 32 causal heads of 4096, width 128, 305 (900), where the products alone would
+// take 10 and 110 at the instructions' peak.  One token
 // behind 65537 keys of 8 heads, width 128: 43 us, 6.3 TB/s, which is what memory gives.
 // ---------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int DP, int WAVES, bool APART, bool BIAS>

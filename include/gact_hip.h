@@ -291,8 +291,8 @@ int gact_checkpoint_product(const void* grad, int64_t ldg, const void* codes, in
  *
  * s_ij = scale q_i.k_j + bias[j - i + queries - 1], out_i = sum over j of softmax(s_i)_j v_j, for every batch entry and head; head h reads key head
  * h / (heads / kv_heads).  A key is hidden from a query where its mask byte is 0, where `causal` is set and j > i + keys - queries, and where the
- * bias is -1e30 or less; a query that sees nothing gets zeros, and its gradient, whatever it is, is nobody's.  What absent keys (mask byte 0) and values hold does not matter; a NaN or infinity of a
- * key that is hidden in another way may show.
+ * bias is -1e30 or less; a query that sees nothing gets zeros, and its gradient, whatever it is, is nobody's.  What absent keys (mask byte 0) and
+ * values hold does not matter; a NaN or infinity of a key that is hidden in another way may show.
  *
  * Rows: [batch, heads, rows, width] of `dtype`, elements from one batch entry, head and row to the next; a row's values lie side by side, in whole
  * 16-byte pieces, rows at least a row and at most GACT_ATTENTION_MAX_STRIDE bytes apart (GACT_EALIGN for addresses, widths and strides that are no

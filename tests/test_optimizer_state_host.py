@@ -1,5 +1,6 @@
 """What gact.optim.AdamW keeps of its parameters and loads, without a GPU: the step itself is replaced by one that notes the counts it is given."""
 import copy
+import pickle
 
 import pytest
 import torch
@@ -224,3 +225,15 @@ def test_a_checkpoint_with_moments_of_another_type_is_loaded(dtype):
     state["exp_avg"] = state["exp_avg"].to(torch.int8)
     with pytest.raises(ValueError, match="exp_avg"):
         opt.load_state_dict(saved(opt, [state]))
+
+
+def test_copies_of_an_optimizer_count_by_themselves(counts):
+    params = parameters(2)
+    opt = optim.AdamW(params, capturable=True)
+    step_with(opt, params, set(params))
+    for twin in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        held = twin.param_groups[0]["params"]
+        assert twin.state[held[0]]["step"] is twin.state[held[1]]["step"] is not opt.state[params[0]]["step"]
+        step_with(twin, held, {held[0]})
+        assert [int(twin.state[p]["step"]) for p in held] == [2, 1]
+    assert [int(opt.state[p]["step"]) for p in params] == [1, 1]
